@@ -92,6 +92,18 @@ int q38_set_decode_split(q38_ctx *ctx, int tokens);
  */
 int q38_kv_create(q38_ctx *ctx, int n_slots, int max_pages, int max_seqs, int max_tokens_per_seq,
                   q38_kv **out);
+/* The same cache with rows of another type: F32 (ggml type 0, q38_kv_create's),
+ * F16 (1), BF16 (30) or Q8_K (15); other types fail with -1.  Every row is
+ * rounded to the type once, when it is stored -- F16 and BF16 to nearest even
+ * (F16: magnitudes from 65520 on become infinity), Q8_K one block of the
+ * format per kv head (256 values share a scale), with the quants and scale of
+ * q38_quantize_q8_k for finite values -- and every call below reads the values
+ * that the stored rows stand for: a token appended by q38_attn_decode or
+ * q38_full_core attends to its own row as it is stored.  A page takes 64 KiB
+ * per slot for K and V together in 16 bits and 32.5 KiB in Q8_K, against
+ * 128 KiB in F32.  No counterpart in the reference (its cache is f32). */
+int q38_kv_create_typed(q38_ctx *ctx, int ggml_type, int n_slots, int max_pages, int max_seqs,
+                        int max_tokens_per_seq, q38_kv **out);
 int q38_kv_destroy(q38_kv *kv);
 /* Pages not held by any sequence. */
 int q38_kv_free_pages(q38_kv *kv, int *n_free);
@@ -137,6 +149,26 @@ int q38_kv_set_prefill_cache(q38_kv *kv, int enable);
 
 /* Gather positions pos0..pos0+n_tokens-1 back into rows [n_tokens][1024]. */
 int q38_kv_read(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, float *d_k, float *d_v);
+
+/* A ragged batch's raw key and value rows into layer `layer`'s slot (the k
+ * RMSNorm, RoPE and append of ops.rs:844-866, for many tokens of many
+ * sequences): sequence seq_ids[b] takes n_tokens[b] rows (0: none) at
+ * positions pos0[b].., the batch's rows packed in order in d_key and d_value
+ * ([rows][1024], 16-byte aligned).  Each kv head of a key row is RMSNormed
+ * with d_k_norm ([256], 16-byte aligned; eps 1e-6) and rotated at its
+ * position, then stored, as the value row is, in the cache's type; the result
+ * equals q38_attn_pre's k rows stored with q38_kv_write, bit for bit.
+ * Sequence ids must be distinct; pages are reserved as needed.  At most 2^27
+ * rows a call. */
+int q38_kv_append(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
+                  const int32_t *n_tokens, const float *d_k_norm, const float *d_key, const float *d_value);
+
+/* The stored rows of a ragged batch back (q38_kv_read for many sequences, e.g.
+ * to hand a prompt's cache to another context): rows packed in order in d_k
+ * and d_v (16-byte aligned), as f32 (ggml_type 0), or, for an F16 or BF16
+ * cache and that ggml_type, in 16 bits as they are stored. */
+int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
+                  const int32_t *n_tokens, int ggml_type, void *d_k, void *d_v);
 
 /* --------------------------------------------------------- full attention */
 
@@ -205,8 +237,9 @@ int q38_attn_pre(q38_ctx *ctx, int n_tokens, int pos0, const float *d_q_norm, co
 /*
  * Prefill of one sequence (batch_full_attention, ops.rs:1153-1172, which runs
  * full_core for tokens base_pos .. base_pos+n_tokens-1 in order): stores the
- * n_tokens rows of d_k / d_v ([n][1024], post-norm, post-RoPE) at base_pos..,
- * then token t attends causally over positions 0..base_pos+t.
+ * n_tokens rows of d_k / d_v ([n][1024], post-norm, post-RoPE) at base_pos..
+ * (both NULL: q38_kv_append or q38_kv_write has stored them already), then
+ * token t attends causally over positions 0..base_pos+t.
  * d_q, d_gate (nullable), d_out: [n_tokens][24][256].
  */
 int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens, const float *d_q,
@@ -338,6 +371,24 @@ int q38_q8k_bytes(int n_tokens, int width, size_t *bytes);
  * round-to-nearest-even of x * (-127/m) capped at 127; all-zero blocks give
  * zeros.  Bit-exact with the reference. */
 int q38_quantize_q8_k(q38_ctx *ctx, int n_tokens, int width, const float *d_x, void *d_q8k);
+
+/* The f32 values that a device Q8_K buffer stands for (quant times its block's
+ * scale): d_x [n_tokens][width], both pointers 16-byte aligned. */
+int q38_dequantize_q8_k(q38_ctx *ctx, int n_tokens, int width, const void *d_q8k, float *d_x);
+
+/* The residual's addition and the layer norm before a layer's projections
+ * (accumulate, ops.rs:547-560; rmsnorm, ops.rs:476-498; quantize_input,
+ * ops.rs:617-620), for n_tokens rows of `width` floats in one launch:
+ *   h = d_x + d_residual (d_residual NULL: h = d_x)
+ *   y = h * (1 / sqrt(mean(h^2) + 1e-6)) * d_weight    (f64 sum of squares)
+ * d_sum receives h, d_y receives y, d_q8k the Q8_K rows of y (as
+ * q38_quantize_q8_k of y, bit for bit, for finite y); each may be NULL, not
+ * all three.  d_q8k needs a width that is a multiple of 256 and 16-byte
+ * alignment; any width >= 1 does without.  d_sum or d_y may be d_x or
+ * d_residual itself (the residual stream updated in place), and no buffer
+ * else may overlap an output.  It allocates nothing and may be captured. */
+int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, const float *d_residual,
+                     const float *d_weight, float *d_sum, float *d_y, void *d_q8k);
 
 /* tensor_gemv_q8_k / tensor_gemm_q8_k (src/kernel/tensor.rs:1131-1173,
  * :1217-1270) for every weight type the reference projects on this path:

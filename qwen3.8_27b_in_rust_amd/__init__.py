@@ -30,6 +30,8 @@ LIN_QK_HEADS, LIN_V_HEADS, LIN_HEAD_DIM = 16, 48, 128
 LIN_QK_DIM, LIN_V_DIM, LIN_QKV_DIM = 2048, 6144, 10240
 LIN_STATE_FLOATS = LIN_V_HEADS * LIN_HEAD_DIM * LIN_HEAD_DIM
 PAGE_TOKENS = 16
+# ggml type ids of a KV cache's rows
+GGML_F32, GGML_F16, GGML_Q8_K, GGML_BF16 = 0, 1, 15, 30
 NOALLOC_SCRATCH_BYTES = 16 << 20  # Q38_NOALLOC_SCRATCH_BYTES of include/q38_attn.h
 
 
@@ -73,6 +75,9 @@ _SIGNATURES = {
     "q38_device_copy": (c_int, [_P, _P, _P, c_size_t]),
     "q38_device_noop": (c_int, [_P]),
     "q38_kv_create": (c_int, [_P, c_int, c_int, c_int, c_int, POINTER(c_void_p)]),
+    "q38_kv_create_typed": (c_int, [_P, c_int, c_int, c_int, c_int, c_int, POINTER(c_void_p)]),
+    "q38_kv_append": (c_int, [_P, c_int, c_int, _I32P, _I32P, _I32P, _P, _P, _P]),
+    "q38_kv_gather": (c_int, [_P, c_int, c_int, _I32P, _I32P, _I32P, c_int, _P, _P]),
     "q38_kv_destroy": (c_int, [_P]),
     "q38_kv_free_pages": (c_int, [_P, POINTER(c_int)]),
     "q38_kv_set_prefill_cache": (c_int, [_P, c_int]),
@@ -100,6 +105,8 @@ _SIGNATURES = {
     "q38_decode_graph_destroy": (c_int, [_P]),
     "q38_q8k_bytes": (c_int, [c_int, c_int, POINTER(c_size_t)]),
     "q38_quantize_q8_k": (c_int, [_P, c_int, c_int, _P, _P]),
+    "q38_dequantize_q8_k": (c_int, [_P, c_int, c_int, _P, _P]),
+    "q38_add_rms_norm": (c_int, [_P, c_int, c_int, _P, _P, _P, _P, _P, _P]),
     "q38_gemv_q8_k": (c_int, [_P, c_int, c_int, c_int, _P, _P, c_int, _P]),
     "q38_gemv_f32": (c_int, [_P, c_int, c_int, c_int, _P, _P, c_int, _P]),
     "q38_gemv_q8_k_multi": (c_int, [_P, c_int, c_int, _I32P, c_int, POINTER(c_void_p), _P, c_int,
@@ -322,6 +329,14 @@ class Context:
     def quantize_q8_k(self, n_tokens, width, x, q8k):
         _check(lib().q38_quantize_q8_k(self.handle, n_tokens, width, _ptr(x), _ptr(q8k)), "q38_quantize_q8_k")
 
+    def dequantize_q8_k(self, n_tokens, width, q8k, x):
+        _check(lib().q38_dequantize_q8_k(self.handle, n_tokens, width, _ptr(q8k), _ptr(x)), "q38_dequantize_q8_k")
+
+    def add_rms_norm(self, n_tokens, width, x, weight, residual=None, sum_out=None, y=None, q8k=None):
+        """h = x (+ residual) and its RMSNorm: h to sum_out, the norm to y, its Q8_K rows to q8k."""
+        _check(lib().q38_add_rms_norm(self.handle, n_tokens, width, _ptr(x), _ptr(residual), _ptr(weight), _ptr(sum_out),
+                                      _ptr(y), _ptr(q8k)), "q38_add_rms_norm")
+
     def gemv_f32(self, ggml_type, rows, width, weights, x, n_tokens, out):
         _check(lib().q38_gemv_f32(self.handle, ggml_type, rows, width, _ptr(weights), _ptr(x), n_tokens, _ptr(out)),
                "q38_gemv_f32")
@@ -357,14 +372,21 @@ def _ptr(x):
     return int(x)
 
 
-class KVCache:
-    """Paged device KV cache (q38_kv_*)."""
+def _same_length(*lists) -> int:
+    if len({len(x) for x in lists}) != 1:
+        raise Q38Error("sequence ids, positions and counts differ in number")
+    return len(lists[0])
 
-    def __init__(self, ctx: Context, n_slots: int, max_pages: int, max_seqs: int, max_tokens_per_seq: int):
+
+class KVCache:
+    """Paged device KV cache (q38_kv_*) of F32, F16, BF16 or Q8_K rows."""
+
+    def __init__(self, ctx: Context, n_slots: int, max_pages: int, max_seqs: int, max_tokens_per_seq: int,
+                 ggml_type: int = GGML_F32):
         self.ctx = ctx
         h = c_void_p()
-        _check(lib().q38_kv_create(ctx.handle, n_slots, max_pages, max_seqs, max_tokens_per_seq,
-                                   ctypes.byref(h)), "q38_kv_create")
+        _check(lib().q38_kv_create_typed(ctx.handle, ggml_type, n_slots, max_pages, max_seqs, max_tokens_per_seq,
+                                         ctypes.byref(h)), "q38_kv_create_typed")
         self.handle = h.value
 
     def close(self) -> None:
@@ -413,6 +435,18 @@ class KVCache:
         _check(lib().q38_kv_read(self.handle, layer, seq, pos0, n_tokens, _ptr(d_k), _ptr(d_v)),
                "q38_kv_read")
 
+    def append(self, layer, seq_ids, pos0, n_tokens, k_norm, key, value):
+        """Raw rows of a ragged batch: keys normed and rotated, then both stored."""
+        n = _same_length(seq_ids, pos0, n_tokens)
+        _check(lib().q38_kv_append(self.handle, layer, n, _i32(seq_ids), _i32(pos0), _i32(n_tokens), _ptr(k_norm),
+                                   _ptr(key), _ptr(value)), "q38_kv_append")
+
+    def gather(self, layer, seq_ids, pos0, n_tokens, d_k, d_v, ggml_type=GGML_F32):
+        """The stored rows of a ragged batch, as f32 or in the cache's own 16-bit type."""
+        n = _same_length(seq_ids, pos0, n_tokens)
+        _check(lib().q38_kv_gather(self.handle, layer, n, _i32(seq_ids), _i32(pos0), _i32(n_tokens), ggml_type,
+                                   _ptr(d_k), _ptr(d_v)), "q38_kv_gather")
+
     def attn_decode(self, layer, seq_ids, positions, q, out, k_new=None, v_new=None, gate=None):
         n = len(seq_ids)
         _check(lib().q38_attn_decode(self.handle, layer, n, _i32(seq_ids), _i32(positions), _ptr(q),
@@ -438,6 +472,7 @@ class KVCache:
         return DecodeGraph(self, seq_ids, positions, calls)
 
     def attn_prefill(self, layer, seq, base_pos, n_tokens, q, k, v, out, gate=None):
+        """k and v None: the rows are in the cache already."""
         _check(lib().q38_attn_prefill(self.handle, layer, seq, base_pos, n_tokens, _ptr(q), _ptr(k), _ptr(v),
                                       _ptr(gate), _ptr(out)), "q38_attn_prefill")
 

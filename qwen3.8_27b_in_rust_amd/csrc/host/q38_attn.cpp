@@ -122,6 +122,21 @@ constexpr GemvType kGemv[] = {
     {Q38_GGML_IQ1_M, "q38_gemv_q8k_iq1m", "q38_gemm_q8k_iq1m", "q38_gemm_ks_q8k_iq1m", "q38_gemm_ks16_q8k_iq1m", "q38_gemm_ks4_q8k_iq1m", nullptr, 1, 2048 * 8, 0.0, 0.0},
 };
 constexpr int kGemvTypes = (int)(sizeof(kGemv) / sizeof(kGemv[0]));
+/* Row types of a KV cache: the bytes of a page's block (one kv head's 16
+ * tokens), and the suffix of the kernels that read and write it.  Index 0 is
+ * the f32 cache. */
+struct KvType {
+    int ggml_type;
+    size_t block_bytes;
+    const char *suffix;
+};
+constexpr KvType kKvTypes[] = {
+    {Q38_GGML_F32, Q38_KV_BLOCK_F32, "f32"},
+    {Q38_GGML_F16, Q38_KV_BLOCK_16, "f16"},
+    {Q38_GGML_BF16, Q38_KV_BLOCK_16, "bf16"},
+    {Q38_GGML_Q8_K, Q38_KV_BLOCK_Q8, "q8k"},
+};
+constexpr int kKvTypeCount = (int)(sizeof(kKvTypes) / sizeof(kKvTypes[0]));
 /* The split-block GEMM's grid: at least this many workgroups (fewer: the
  * GEMV), at most this many per CU (more: the 128 x 64 tiles) */
 constexpr long kGemmKsMinTiles = 64;
@@ -155,6 +170,16 @@ struct q38_ctx {
     hipFunction_t f_decode_split_pre_one = nullptr;
     hipFunction_t f_decode_merge = nullptr;
     hipFunction_t f_kv_copy = nullptr;
+    hipModule_t mod_rows = nullptr;
+    hipFunction_t f_kv_append[kKvTypeCount] = {};  /* by kKvTypes index */
+    hipFunction_t f_kv_gather[kKvTypeCount] = {};
+    hipFunction_t f_kv_gather_16 = nullptr;        /* 16-bit rows as they are stored */
+    hipFunction_t f_kv_split_typed[kKvTypeCount] = {}; /* from index 1 on */
+    hipModule_t mod_norm = nullptr;
+    hipFunction_t f_add_rms_norm = nullptr;
+    hipFunction_t f_dequantize_q8k = nullptr;
+    hipModule_t mod_typed = nullptr;
+    hipFunction_t f_decode_typed[kKvTypeCount][2] = {}; /* from index 1 on; [1]: the pre step fused */
     hipFunction_t f_attn_pre = nullptr;
     hipFunction_t f_gdn_decode = nullptr;
     hipFunction_t f_gdn_pre = nullptr;
@@ -252,6 +277,7 @@ struct q38_ctx {
 
 struct q38_kv {
     q38_ctx *ctx = nullptr;
+    int type = 0; /* kKvTypes index of the cached rows */
     int n_slots = 0;
     int max_pages = 0;
     int max_seqs = 0;
@@ -303,9 +329,13 @@ struct q38_kv {
         }
     }
 
-    size_t slot_floats() const { return (size_t)max_pages * Q38_PAGE_FLOATS; }
-    float *kslot(int slot) const { return kpool + (size_t)slot * slot_floats(); }
-    float *vslot(int slot) const { return vpool + (size_t)slot * slot_floats(); }
+    /* a slot's pages; a typed cache's kernels read them as bytes */
+    size_t slot_bytes() const { return (size_t)max_pages * Q38_ATTN_KV_HEADS * kKvTypes[type].block_bytes; }
+    float *slot_of_pool(float *pool, int slot) const {
+        return reinterpret_cast<float *>(reinterpret_cast<char *>(pool) + (size_t)slot * slot_bytes());
+    }
+    float *kslot(int slot) const { return slot_of_pool(kpool, slot); }
+    float *vslot(int slot) const { return slot_of_pool(vpool, slot); }
 
     int check_seq(int seq) const {
         if (seq < 0 || seq >= max_seqs || !seq_live[seq]) return fail("sequence %d does not exist", seq);
@@ -440,6 +470,23 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
      * exactly Q38_DECODE_WAVES waves */
     if (ctx->decode_block != 64 * Q38_DECODE_WAVES)
         return fail("decode kernel has block size %d, expected %d", ctx->decode_block, 64 * Q38_DECODE_WAVES);
+    const std::string p_norm = dir + "/norm.hsaco";
+    Q38_HIP(hipModuleLoad(&ctx->mod_norm, p_norm.c_str()));
+    Q38_HIP(hipModuleGetFunction(&ctx->f_add_rms_norm, ctx->mod_norm, "q38_add_rms_norm"));
+    Q38_HIP(hipModuleGetFunction(&ctx->f_dequantize_q8k, ctx->mod_norm, "q38_dequantize_q8k"));
+    const std::string p_rows = dir + "/kv_rows.hsaco", p_typed = dir + "/attn_decode_typed.hsaco";
+    Q38_HIP(hipModuleLoad(&ctx->mod_rows, p_rows.c_str()));
+    Q38_HIP(hipModuleLoad(&ctx->mod_typed, p_typed.c_str()));
+    Q38_HIP(hipModuleGetFunction(&ctx->f_kv_gather_16, ctx->mod_rows, "q38_kv_gather_16"));
+    for (int i = 0; i < kKvTypeCount; ++i) {
+        const std::string ty = kKvTypes[i].suffix;
+        Q38_HIP(hipModuleGetFunction(&ctx->f_kv_append[i], ctx->mod_rows, ("q38_kv_append_" + ty).c_str()));
+        Q38_HIP(hipModuleGetFunction(&ctx->f_kv_gather[i], ctx->mod_rows, ("q38_kv_gather_" + ty).c_str()));
+        if (i == 0) continue;
+        Q38_HIP(hipModuleGetFunction(&ctx->f_kv_split_typed[i], ctx->mod_prefill, ("q38_kv_split_mfma_" + ty).c_str()));
+        Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed[i][0], ctx->mod_typed, ("q38_attn_decode_" + ty).c_str()));
+        Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed[i][1], ctx->mod_typed, ("q38_attn_decode_" + ty + "_pre").c_str()));
+    }
     const std::string p_proj = dir + "/proj.hsaco";
     Q38_HIP(hipModuleLoad(&ctx->mod_proj, p_proj.c_str()));
     Q38_HIP(hipModuleGetFunction(&ctx->f_quantize_q8k, ctx->mod_proj, "q38_quantize_q8k"));
@@ -505,6 +552,9 @@ int q38_ctx_destroy(q38_ctx *ctx) {
     if (ctx->work) (void)hipFree(ctx->work);
     if (ctx->arrivals) (void)hipFree(ctx->arrivals);
     if (ctx->mod_decode) (void)hipModuleUnload(ctx->mod_decode);
+    if (ctx->mod_norm) (void)hipModuleUnload(ctx->mod_norm);
+    if (ctx->mod_rows) (void)hipModuleUnload(ctx->mod_rows);
+    if (ctx->mod_typed) (void)hipModuleUnload(ctx->mod_typed);
     if (ctx->mod_gdn) (void)hipModuleUnload(ctx->mod_gdn);
     if (ctx->mod_prefill) (void)hipModuleUnload(ctx->mod_prefill);
     if (ctx->mod_gdn_chunk) (void)hipModuleUnload(ctx->mod_gdn_chunk);
@@ -693,6 +743,17 @@ int q38_kernel_timer_start(q38_ctx *ctx, const char *kernel_name, int max_launch
     else if (name == "q38_gdn_chunk_scan") f = ctx->f_chunk_scan;
     else if (name == "q38_gdn_post") f = ctx->f_gdn_post;
     else {
+        for (int i = 0; i < kKvTypeCount; ++i) {
+            const std::string ty = kKvTypes[i].suffix;
+            if (name == "q38_kv_append_" + ty) f = ctx->f_kv_append[i];
+            if (name == "q38_kv_gather_" + ty) f = ctx->f_kv_gather[i];
+            if (i > 0 && name == "q38_kv_split_mfma_" + ty) f = ctx->f_kv_split_typed[i];
+            if (i > 0 && name == "q38_attn_decode_" + ty) f = ctx->f_decode_typed[i][0];
+            if (i > 0 && name == "q38_attn_decode_" + ty + "_pre") f = ctx->f_decode_typed[i][1];
+        }
+        if (name == "q38_add_rms_norm") f = ctx->f_add_rms_norm;
+        if (name == "q38_dequantize_q8k") f = ctx->f_dequantize_q8k;
+        if (name == "q38_kv_gather_16") f = ctx->f_kv_gather_16;
         for (int i = 0; i < kGemvTypes; ++i) {
             if (name == kGemv[i].kernel) f = ctx->f_gemv_q8k[i];
             if (kGemv[i].gemm_kernel != nullptr && name == kGemv[i].gemm_kernel) f = ctx->f_gemm[i];
@@ -733,8 +794,17 @@ int q38_kernel_timer_stop(q38_ctx *ctx, float *total_ms, int *launches) {
 
 int q38_kv_create(q38_ctx *ctx, int n_slots, int max_pages, int max_seqs, int max_tokens_per_seq,
                   q38_kv **out) {
+    return q38_kv_create_typed(ctx, Q38_GGML_F32, n_slots, max_pages, max_seqs, max_tokens_per_seq, out);
+}
+
+int q38_kv_create_typed(q38_ctx *ctx, int ggml_type, int n_slots, int max_pages, int max_seqs, int max_tokens_per_seq,
+                        q38_kv **out) {
     if (ctx == nullptr || out == nullptr) return fail("NULL argument");
     *out = nullptr;
+    int type = -1;
+    for (int i = 0; i < kKvTypeCount; ++i)
+        if (kKvTypes[i].ggml_type == ggml_type) type = i;
+    if (type < 0) return fail("a KV cache holds F32 (0), F16 (1), BF16 (30) or Q8_K (15) rows, not type %d", ggml_type);
     if (n_slots < 1 || n_slots > 17) return fail("n_slots %d outside 1..17", n_slots);
     if (max_pages < 1 || max_seqs < 1 || max_tokens_per_seq < 1)
         return fail("max_pages, max_seqs and max_tokens_per_seq must be positive");
@@ -743,11 +813,12 @@ int q38_kv_create(q38_ctx *ctx, int n_slots, int max_pages, int max_seqs, int ma
                     (long)Q38_MAX_SPLITS * Q38_MAX_SPLIT_TOKENS);
     std::unique_ptr<q38_kv> kv(new q38_kv);
     kv->ctx = ctx;
+    kv->type = type;
     kv->n_slots = n_slots;
     kv->max_pages = max_pages;
     kv->max_seqs = max_seqs;
     kv->pt_stride = (max_tokens_per_seq + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS;
-    const size_t pool_bytes = (size_t)n_slots * max_pages * Q38_PAGE_FLOATS * sizeof(float);
+    const size_t pool_bytes = (size_t)n_slots * kv->slot_bytes();
     Q38_HIP(hipSetDevice(ctx->device));
     Q38_HIP(hipMalloc(&kv->kpool, pool_bytes));
     if (hipMalloc(&kv->vpool, pool_bytes) != hipSuccess) {
@@ -878,6 +949,87 @@ int q38_seq_capacity(q38_kv *kv, int seq, int *n_tokens) {
     return 0;
 }
 
+namespace {
+
+/* Rows most that one append or gather moves (f32 rows of half a terabyte):
+ * row counts and the grid stay within 32 bits. */
+constexpr long kMaxRows = 1L << 27;
+
+/* Every check of a ragged batch of rows, with nothing changed: sequence b's
+ * rows are positions pos0[b] .. pos0[b] + n_tokens[b] - 1.  An append names
+ * each sequence once and finds pages for the whole batch; a gather finds
+ * every position reserved. */
+int validate_rows(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0, const int32_t *n_tokens,
+                  bool appends, int *slot, long *n_rows) {
+    if (kv->slot_of(layer, slot)) return -1;
+    if (n_seq < 0) return fail("negative n_seq");
+    if (n_seq > 0 && (seq_ids == nullptr || pos0 == nullptr || n_tokens == nullptr))
+        return fail("NULL seq_ids/positions/counts");
+    std::vector<char> seen(appends ? kv->max_seqs : 0, 0);
+    long pages_needed = 0;
+    *n_rows = 0;
+    for (int b = 0; b < n_seq; ++b) {
+        const int s = seq_ids[b];
+        if (kv->check_seq(s)) return -1;
+        if (pos0[b] < 0 || n_tokens[b] < 0) return fail("negative position or count");
+        const long end = (long)pos0[b] + n_tokens[b];
+        if (end > (long)kv->pt_stride * Q38_PAGE_TOKENS)
+            return fail("positions %d..%ld are past the context limit %d", pos0[b], end - 1,
+                        kv->pt_stride * Q38_PAGE_TOKENS);
+        if (appends) {
+            if (seen[s]) return fail("sequence %d appears twice", s);
+            seen[s] = 1;
+        }
+        if (n_tokens[b] == 0) continue;
+        const long need = (end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS;
+        if (appends)
+            pages_needed += std::max<long>(0, need - kv->seq_pages[s]);
+        else if (need > kv->seq_pages[s])
+            return fail("positions %d..%ld are not reserved", pos0[b], end - 1);
+        *n_rows += n_tokens[b];
+    }
+    if (*n_rows > kMaxRows) return fail("%ld rows: at most %ld a call", *n_rows, kMaxRows);
+    if (pages_needed > (long)kv->free_pages.size())
+        return fail("KV pool exhausted: the batch needs %ld more pages, %zu free", pages_needed, kv->free_pages.size());
+    return 0;
+}
+
+/* Moves a validated batch whose pages are reserved, in launches of up to
+ * Q38_MAX_BATCH sequences; rows of `elem_bytes` a value. */
+int launch_rows(q38_kv *kv, hipFunction_t f, int slot, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
+                const int32_t *n_tokens, void *d_k, void *d_v, size_t elem_bytes, const float *d_k_norm) {
+    size_t row = 0;
+    for (int b = 0; b < n_seq;) {
+        q38_kv_rows_args a;
+        memset(&a, 0, sizeof(a));
+        a.kpool = kv->kslot(slot);
+        a.vpool = kv->vslot(slot);
+        a.page_table = kv->d_page_table;
+        a.k_rows = static_cast<char *>(d_k) + row * Q38_ATTN_KV_DIM * elem_bytes;
+        a.v_rows = static_cast<char *>(d_v) + row * Q38_ATTN_KV_DIM * elem_bytes;
+        a.k_norm = d_k_norm;
+        a.theta_scale = kv->ctx->rope_theta_scale;
+        a.pt_stride = kv->pt_stride;
+        int n = 0;
+        for (; b < n_seq && n < Q38_MAX_BATCH; ++b) {
+            if (n_tokens[b] == 0) continue;
+            a.seq[n] = seq_ids[b];
+            a.pos0[n] = pos0[b];
+            a.row_base[n + 1] = a.row_base[n] + n_tokens[b];
+            const int first = pos0[b] / Q38_PAGE_TOKENS, last = (pos0[b] + n_tokens[b] - 1) / Q38_PAGE_TOKENS;
+            a.page_base[n + 1] = a.page_base[n] + last - first + 1;
+            ++n;
+        }
+        if (n == 0) break;
+        a.n_seq = n;
+        if (kv->ctx->launch(f, (unsigned)a.page_base[n], 2, 1, 256, &a)) return -1;
+        row += (size_t)a.row_base[n];
+    }
+    return 0;
+}
+
+}  // namespace
+
 static int kv_copy(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, float *d_k, float *d_v,
                    int to_pages) {
     if (kv == nullptr) return fail("kv is NULL");
@@ -893,6 +1045,9 @@ static int kv_copy(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, float
     } else if (pos0 + n_tokens > kv->seq_pages[seq] * Q38_PAGE_TOKENS) {
         return fail("positions %d..%d are not reserved", pos0, pos0 + n_tokens - 1);
     }
+    if (kv->type != 0)
+        return launch_rows(kv, to_pages ? kv->ctx->f_kv_append[kv->type] : kv->ctx->f_kv_gather[kv->type], slot, 1, &seq,
+                           &pos0, &n_tokens, d_k, d_v, sizeof(float), nullptr);
     q38_kv_copy_args a;
     memset(&a, 0, sizeof(a));
     a.kpool = kv->kslot(slot);
@@ -915,6 +1070,43 @@ int q38_kv_write(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, const f
 
 int q38_kv_read(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, float *d_k, float *d_v) {
     return kv_copy(kv, layer, seq, pos0, n_tokens, d_k, d_v, 0);
+}
+
+int q38_kv_append(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
+                  const int32_t *n_tokens, const float *d_k_norm, const float *d_key, const float *d_value) {
+    if (kv == nullptr) return fail("kv is NULL");
+    int slot = 0;
+    long n_rows = 0;
+    if (validate_rows(kv, layer, n_seq, seq_ids, pos0, n_tokens, true, &slot, &n_rows)) return -1;
+    if (n_rows == 0) return 0;
+    if (!d_k_norm || !d_key || !d_value) return fail("NULL argument");
+    if (((uintptr_t)d_k_norm | (uintptr_t)d_key | (uintptr_t)d_value) % 16 != 0)
+        return fail("d_k_norm, d_key and d_value must be 16-byte aligned");
+    for (int b = 0; b < n_seq; ++b) {
+        if (n_tokens[b] == 0) continue;
+        if (kv->reserve(seq_ids[b], pos0[b] + n_tokens[b])) return -1;
+        kv->images_from(seq_ids[b], slot, pos0[b]);
+    }
+    return launch_rows(kv, kv->ctx->f_kv_append[kv->type], slot, n_seq, seq_ids, pos0, n_tokens,
+                       const_cast<float *>(d_key), const_cast<float *>(d_value), sizeof(float), d_k_norm);
+}
+
+int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
+                  const int32_t *n_tokens, int ggml_type, void *d_k, void *d_v) {
+    if (kv == nullptr) return fail("kv is NULL");
+    int slot = 0;
+    long n_rows = 0;
+    if (validate_rows(kv, layer, n_seq, seq_ids, pos0, n_tokens, false, &slot, &n_rows)) return -1;
+    const int own = kKvTypes[kv->type].ggml_type;
+    const bool as_stored = ggml_type == own && (own == Q38_GGML_F16 || own == Q38_GGML_BF16);
+    if (!as_stored && ggml_type != Q38_GGML_F32)
+        return fail("rows of a cache of type %d come as F32 (0)%s, not as type %d", own,
+                    own == Q38_GGML_F16 || own == Q38_GGML_BF16 ? " or as they are stored" : "", ggml_type);
+    if (n_rows == 0) return 0;
+    if (!d_k || !d_v) return fail("NULL argument");
+    if (((uintptr_t)d_k | (uintptr_t)d_v) % 16 != 0) return fail("d_k and d_v must be 16-byte aligned");
+    return launch_rows(kv, as_stored ? kv->ctx->f_kv_gather_16 : kv->ctx->f_kv_gather[kv->type], slot, n_seq, seq_ids,
+                       pos0, n_tokens, d_k, d_v, as_stored ? 2 : sizeof(float), nullptr);
 }
 
 /* ------------------------------------------------------------ attention decode */
@@ -1046,7 +1238,7 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
     /* up to 256 splits, each split's first two page ids ride in the launch
      * arguments (from the host mirror of the page table), so the kernel's
      * first row loads wait on no page-table load */
-    const bool arg_pages = arg_pages_choice < 0 ? total <= Q38_HEAD_PAGE_SPLITS : arg_pages_choice > 0;
+    const bool arg_pages = kv->type == 0 && (arg_pages_choice < 0 ? total <= Q38_HEAD_PAGE_SPLITS : arg_pages_choice > 0);
     if (arg_pages) {
         if (total > Q38_HEAD_PAGE_SPLITS)
             return fail("%d splits: at most %d carry their page ids in the arguments", total, Q38_HEAD_PAGE_SPLITS);
@@ -1073,6 +1265,7 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
     L->f = pre != nullptr ? (one ? ctx->f_decode_split_pre_one
                                  : arg_pages ? ctx->f_decode_split_pre : ctx->f_decode_split_pre_many)
                           : (one ? ctx->f_decode_split_one : arg_pages ? ctx->f_decode_split : ctx->f_decode_split_many);
+    if (kv->type != 0) L->f = ctx->f_decode_typed[kv->type][pre != nullptr ? 1 : 0];
     L->grid_x = (unsigned)total;
     q38_merge_args &m = L->m;
     memset(&m, 0, sizeof(m));
@@ -1679,7 +1872,8 @@ int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     if (kv == nullptr) return fail("kv is NULL");
     if (n_tokens < 0 || base_pos < 0) return fail("negative count or position");
     if (n_tokens == 0) return 0;
-    if (!d_q || !d_k || !d_v || !d_out) return fail("NULL argument");
+    if (!d_q || !d_out) return fail("NULL argument");
+    if ((d_k == nullptr) != (d_v == nullptr)) return fail("d_k and d_v go together");
     if (kv->check_seq(seq)) return -1;
     int slot = 0;
     if (kv->slot_of(layer, &slot)) return -1;
@@ -1688,6 +1882,7 @@ int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
         return fail("positions %d..%ld are past the context limit %d", base_pos, end - 1,
                     kv->pt_stride * Q38_PAGE_TOKENS);
     const long need = (end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS - kv->seq_pages[seq];
+    if (d_k == nullptr && need > 0) return fail("positions %d..%ld are not reserved", base_pos, end - 1);
     if (need > (long)kv->free_pages.size())
         return fail("KV pool exhausted: need %ld pages, %zu free", need, kv->free_pages.size());
     q38_ctx *ctx = kv->ctx;
@@ -1753,12 +1948,12 @@ int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     a.part_ml = a.part_o + part_rows * Q38_ATTN_HEAD_DIM;
     /* append the prompt's rows (reserves pages; the blocks from base_pos on
      * are no longer valid images) */
-    if (q38_kv_write(kv, layer, seq, base_pos, n_tokens, d_k, d_v)) return -1;
+    if (d_k != nullptr && q38_kv_write(kv, layer, seq, base_pos, n_tokens, d_k, d_v)) return -1;
     /* the K/V blocks without a valid image split once into bf16 hi/lo
      * images, then the attention kernel */
     a.kb0 = im != nullptr ? std::min(im->valid, a.n_kblocks) : 0;
     if (a.kb0 < a.n_kblocks &&
-        ctx->launch(ctx->f_kv_split, a.n_kblocks - a.kb0, Q38_ATTN_KV_HEADS, 1, 256, &a))
+        ctx->launch(kv->type == 0 ? ctx->f_kv_split : ctx->f_kv_split_typed[kv->type], a.n_kblocks - a.kb0, Q38_ATTN_KV_HEADS, 1, 256, &a))
         return -1;
     /* the blocks every key of which is now in the cache stay valid */
     if (im != nullptr) im->valid = (int)(end / Q38_PREFILL_KEYS);
@@ -2273,6 +2468,53 @@ int q38_quantize_project_q8_k(q38_ctx *ctx, int ggml_type, int n_mats, const int
                               float *const *d_out) {
     if (d_x == nullptr && n_tokens > 0) return fail("d_x is NULL");
     return gemv_q8k_multi(ctx, ggml_type, n_mats, rows, width, d_weights, d_x, d_q8k, n_tokens, d_out);
+}
+
+int q38_dequantize_q8_k(q38_ctx *ctx, int n_tokens, int width, const void *d_q8k, float *d_x) {
+    if (ctx == nullptr) return fail("ctx is NULL");
+    if (n_tokens < 0) return fail("negative n_tokens");
+    if (width < 1 || width % Q38_Q8K_BLOCK != 0) return fail("width %d is not a positive multiple of 256", width);
+    if (n_tokens == 0) return 0;
+    if (!d_q8k || !d_x) return fail("NULL argument");
+    if (((uintptr_t)d_q8k | (uintptr_t)d_x) % 16 != 0) return fail("d_q8k and d_x must be 16-byte aligned");
+    const size_t groups = ((size_t)n_tokens * width + 1023) / 1024;
+    if (groups > 0xFFFFFFFFull / 256) return fail("%d rows of %d: too many for one call", n_tokens, width);
+    q38_dequantize_args a = {d_q8k, d_x, width, n_tokens};
+    return ctx->launch(ctx->f_dequantize_q8k, (unsigned)groups, 1, 1, 256, &a);
+}
+
+int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, const float *d_residual,
+                     const float *d_weight, float *d_sum, float *d_y, void *d_q8k) {
+    if (ctx == nullptr) return fail("ctx is NULL");
+    if (n_tokens < 0) return fail("negative n_tokens");
+    if (width < 1) return fail("width %d is not positive", width);
+    if (d_q8k != nullptr && width % Q38_Q8K_BLOCK != 0)
+        return fail("Q8_K rows need a width that is a multiple of 256, not %d", width);
+    if (n_tokens == 0) return 0;
+    if (!d_x || !d_weight) return fail("NULL argument");
+    if (!d_sum && !d_y && !d_q8k) return fail("no output given");
+    if ((uintptr_t)d_q8k % 16 != 0) return fail("d_q8k must be 16-byte aligned");
+    if (((uintptr_t)d_x | (uintptr_t)d_residual | (uintptr_t)d_weight | (uintptr_t)d_sum | (uintptr_t)d_y) % 4 != 0)
+        return fail("f32 rows must be 4-byte aligned");
+    /* an output may be one of the inputs' rows themselves: a row is read whole
+     * before any of it is written; overlapping in part it is not */
+    const size_t bytes = (size_t)n_tokens * width * sizeof(float);
+    auto overlaps = [](const void *p, size_t np, const void *q, size_t nq) {
+        return p != nullptr && q != nullptr && (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
+    };
+    const size_t q_bytes = d_q8k != nullptr ? Q38_Q8K_BYTES(n_tokens, width) : 0;
+    for (float *o : {d_sum, d_y}) {
+        for (const float *in : {d_x, d_residual})
+            if (o != in && overlaps(o, bytes, in, bytes)) return fail("an output overlaps an input in part");
+        if (overlaps(o, bytes, d_weight, (size_t)width * sizeof(float))) return fail("an output overlaps the weight");
+        if (overlaps(o, bytes, d_q8k, q_bytes)) return fail("outputs overlap");
+    }
+    if (overlaps(d_sum, bytes, d_y, bytes)) return fail("outputs overlap");
+    if (overlaps(d_q8k, q_bytes, d_x, bytes) || overlaps(d_q8k, q_bytes, d_residual, bytes) ||
+        overlaps(d_q8k, q_bytes, d_weight, (size_t)width * sizeof(float)))
+        return fail("d_q8k overlaps an input");
+    q38_norm_args a = {d_x, d_residual, d_weight, d_sum, d_y, d_q8k, width, n_tokens};
+    return ctx->launch(ctx->f_add_rms_norm, (unsigned)n_tokens, 1, 1, 256, &a);
 }
 
 int q38_gemv_q8_k(q38_ctx *ctx, int ggml_type, int rows, int width, const void *d_weights, const void *d_q8k,

@@ -37,7 +37,7 @@
  *  - the loads of block kb+1's image are issued between the MFMA steps of
  *    block kb, so the direct-to-LDS traffic runs under the matrix work.
  */
-#include "q38_device.h"
+#include "q38_kv_types.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -115,7 +115,9 @@ Q38_DEV const uint4 *image_of(const q38_prefill_args &a, int j, int kb) {
  * the transposed V part is assembled in LDS (a 4-byte write per key pair and
  * dim) and then streamed to the image in 16-byte stores, so neither part is
  * written with scattered small stores. */
-extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma(q38_prefill_args a) {
+namespace {
+template <int T>
+Q38_DEV void kv_split(const q38_prefill_args &a) {
     __shared__ __attribute__((aligned(16))) __bf16 vimg[2][Q38_ATTN_HEAD_DIM][kVRow];
     const int kb = a.kb0 + blockIdx.x;
     const int j = blockIdx.y;
@@ -136,20 +138,32 @@ extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma(q38_prefill_
         return pool + ((size_t)(r < 16 ? pg0 : pg1) * Q38_ATTN_KV_HEADS + j) * Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM +
                (size_t)(kp & 15) * Q38_ATTN_HEAD_DIM;
     };
+    /* typed rows: the block and token of key r */
+    auto block_of = [&](const float *pool, int r) {
+        return q38_kv_block<T>(const_cast<float *>(pool), r < 16 ? pg0 : pg1, j);
+    };
+    auto token_of = [&](int r) { return min(kp0 + r, kmax) & 15; };
     constexpr int kKPer = kKB * Q38_ATTN_HEAD_DIM / 4 / 256;     /* K float4s per thread */
     constexpr int kVPer = kKB / 2 * Q38_ATTN_HEAD_DIM / 4 / 256; /* V key pairs per thread */
     f32x4 kx[kKPer], vx[2 * kVPer];
 #pragma unroll
     for (int m = 0; m < kKPer; ++m) {
         const int i = tid + 256 * m;
-        kx[m] = q38_ld4(row_of(a.kpool, i >> 6) + 4 * (i & 63));
+        if (T == Q38_KV_F32)
+            kx[m] = q38_ld4(row_of(a.kpool, i >> 6) + 4 * (i & 63));
+        else
+            kx[m] = q38_k_load4<T>(block_of(a.kpool, i >> 6), token_of(i >> 6), 4 * (i & 63));
     }
 #pragma unroll
     for (int m = 0; m < kVPer; ++m) {
         const int i = tid + 256 * m;
         const int r = 2 * (i >> 6), c4 = i & 63;
-        vx[2 * m] = q38_ld4(row_of(a.vpool, r) + 4 * c4);
-        vx[2 * m + 1] = q38_ld4(row_of(a.vpool, r + 1) + 4 * c4);
+        if (T == Q38_KV_F32) {
+            vx[2 * m] = q38_ld4(row_of(a.vpool, r) + 4 * c4);
+            vx[2 * m + 1] = q38_ld4(row_of(a.vpool, r + 1) + 4 * c4);
+        } else {
+            q38_v_load4<T>(block_of(a.vpool, r), token_of(r), token_of(r + 1), 4 * c4, vx[2 * m], vx[2 * m + 1]);
+        }
     }
 #pragma unroll
     for (int m = 0; m < kKPer; ++m) {
@@ -179,6 +193,14 @@ extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma(q38_prefill_
     uint4 *dst = reinterpret_cast<uint4 *>(&img->vt[0][0][0]);
     for (int i = tid; i < (int)(sizeof(vimg) / 16); i += 256) dst[i] = src[i];
 }
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma(q38_prefill_args a) { kv_split<Q38_KV_F32>(a); }
+/* The same from typed pages: a block's values as f32, split the same way (a
+ * bf16 row's low parts are zero). */
+extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma_f16(q38_prefill_args a) { kv_split<Q38_KV_F16>(a); }
+extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma_bf16(q38_prefill_args a) { kv_split<Q38_KV_BF16>(a); }
+extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma_q8k(q38_prefill_args a) { kv_split<Q38_KV_Q8>(a); }
 
 extern "C" __global__ __launch_bounds__(kThreads, 1) void q38_attn_prefill_mfma(q38_prefill_args a) {
     __shared__ __attribute__((aligned(16))) Tile tiles[2];

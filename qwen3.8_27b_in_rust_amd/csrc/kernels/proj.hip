@@ -48,12 +48,6 @@ namespace {
  * half (subnormals included; f16 denormals are not flushed). */
 Q38_DEV float q38_f16(uint32_t h) { return (float)__builtin_bit_cast(_Float16, (unsigned short)(h & 0xffffu)); }
 
-/* nearest_int (quant.rs:16-20) */
-Q38_DEV int q38_nearest_int(float v) {
-    const float shifted = v + 12582912.0f;
-    return (int)(__float_as_uint(shifted) & 0x007fffffu) - 0x00400000;
-}
-
 Q38_DEV int q38_sdot4(uint32_t a, uint32_t b, int c) { return __builtin_amdgcn_sdot4((int)a, (int)b, c, false); }
 
 /* Byte i (0..11) of the 12 packed scale bytes held in three words. */

@@ -100,6 +100,12 @@ Q38_DEV f32x4 q38_fma4(float s, f32x4 v, f32x4 acc) {
     return acc;
 }
 
+/* nearest_int (quant.rs:16-20) */
+Q38_DEV int q38_nearest_int(float v) {
+    const float shifted = v + 12582912.0f;
+    return (int)(__float_as_uint(shifted) & 0x007fffffu) - 0x00400000;
+}
+
 /* f64 all-reduce (sum) over each row of 16 lanes, each half-wave and the wave
  * with the DPP and permlane moves of the f32 forms above, a word at a time.
  * A sum by __shfl_xor of doubles is two LDS permutes per step, and the decode

@@ -24,6 +24,12 @@
 /* one page of one layer: [4 kv heads][16 tokens][256] floats, K and V pools apart */
 #define Q38_PAGE_FLOATS (Q38_ATTN_KV_HEADS * Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM)
 
+/* bytes of one kv head's 16 tokens x 256 values in a page, by the cache's type
+ * (Q8_K: quants, then the 16 tokens' f32 scales) */
+#define Q38_KV_BLOCK_F32 (Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM * 4)
+#define Q38_KV_BLOCK_16 (Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM * 2)
+#define Q38_KV_BLOCK_Q8 (Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM + Q38_PAGE_TOKENS * 4)
+
 #define Q38_LIN_QK_HEADS 16
 #define Q38_LIN_V_HEADS 48
 #define Q38_LIN_HEAD_DIM 128
@@ -83,6 +89,28 @@ typedef struct {
     int32_t to_pages; /* 1: rows -> pages (append), 0: pages -> rows (gather) */
     int32_t pad_;
 } q38_kv_copy_args;
+
+/* Rows of a ragged batch to or from the pages of a cache of any type: row
+ * row_base[b] + i is position pos0[b] + i of sequence seq[b].  grid
+ * (page_base[n_seq], 2): workgroup x serves one page of one sequence -- page
+ * pos0[b] / 16 + x - page_base[b] of the sequence b that holds x -- and y = 0
+ * moves K, y = 1 moves V; 256 threads, a wave per kv head. */
+typedef struct {
+    void *kpool;
+    void *vpool;
+    const int32_t *page_table;
+    void *k_rows; /* [rows][1024]: f32, or (gathering only) the cache's 16-bit type */
+    void *v_rows;
+    const float *k_norm; /* append of raw keys: [256] RMSNorm weight; NULL: rows stored as they are */
+    float theta_scale;   /* append of raw keys: RoPE 1e7^(-2/64) in f32 */
+    int32_t pt_stride;
+    int32_t n_seq;
+    int32_t pad_;
+    int32_t seq[Q38_MAX_BATCH];
+    int32_t pos0[Q38_MAX_BATCH];
+    int32_t row_base[Q38_MAX_BATCH + 1];
+    int32_t page_base[Q38_MAX_BATCH + 1];
+} q38_kv_rows_args;
 
 /* q/gate split, q and k RMSNorm, RoPE.  grid (n_tokens, 28): y < 24 is a
  * query head, y >= 24 a kv head. */
@@ -296,6 +324,7 @@ typedef struct {
 #define Q38_GGML_Q8_0 8
 #define Q38_GGML_Q2_K 10
 #define Q38_GGML_Q3_K 11
+#define Q38_GGML_Q8_K 15
 #define Q38_GGML_IQ4_NL 20
 #define Q38_GGML_Q4_K 12
 #define Q38_GGML_Q5_K 13
@@ -322,6 +351,26 @@ typedef struct {
     int32_t width;
     int32_t n_tokens;
 } q38_quantize_args;
+
+/* x + residual, its RMSNorm and the norm's Q8_K form: grid (n_tokens). */
+typedef struct {
+    const float *x;        /* [T][W] */
+    const float *residual; /* [T][W] or NULL */
+    const float *weight;   /* [W] */
+    float *sum;            /* [T][W] x + residual, or NULL */
+    float *y;              /* [T][W] the norm, or NULL */
+    void *q8k;             /* planar Q8_K of the norm, or NULL */
+    int32_t width;
+    int32_t n_tokens;
+} q38_norm_args;
+
+/* Q8_K rows as f32: grid (ceil(T * W / 1024)), 256 threads. */
+typedef struct {
+    const void *q8k;
+    float *out; /* [T][W] */
+    int32_t width;
+    int32_t n_tokens;
+} q38_dequantize_args;
 
 /* K-quant x Q8_K GEMV / GEMM over up to Q38_GEMV_MAX_MATS matrices of one
  * type and width that read the same activations: G = wg_begin[n_mats] row
