@@ -1190,6 +1190,7 @@ struct decode_launch {
     q38_merge_args m;
     hipFunction_t f = nullptr;
     unsigned grid_x = 0;
+    unsigned block = 0;
     bool merge = false;
 };
 
@@ -1265,7 +1266,11 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
     L->f = pre != nullptr ? (one ? ctx->f_decode_split_pre_one
                                  : arg_pages ? ctx->f_decode_split_pre : ctx->f_decode_split_pre_many)
                           : (one ? ctx->f_decode_split_one : arg_pages ? ctx->f_decode_split : ctx->f_decode_split_many);
-    if (kv->type != 0) L->f = ctx->f_decode_typed[kv->type][pre != nullptr ? 1 : 0];
+    L->block = (unsigned)ctx->decode_block;
+    if (kv->type != 0) {
+        L->f = ctx->f_decode_typed[kv->type][pre != nullptr ? 1 : 0];
+        L->block = 64 * Q38_DECODE_TYPED_WAVES;
+    }
     L->grid_x = (unsigned)total;
     q38_merge_args &m = L->m;
     memset(&m, 0, sizeof(m));
@@ -1289,7 +1294,7 @@ int decode_chunk(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
     if (build_decode(kv, slot, n_seq, seq_ids, positions, d_q, d_k_new, d_v_new, d_gate, d_out, plan,
                      plan.work_bytes > 0 ? work : nullptr, pre, -1, &L))
         return -1;
-    if (ctx->launch(L.f, L.grid_x, Q38_ATTN_KV_HEADS, 1, ctx->decode_block, &L.a)) return -1;
+    if (ctx->launch(L.f, L.grid_x, Q38_ATTN_KV_HEADS, 1, L.block, &L.a)) return -1;
     if (L.merge && ctx->launch(ctx->f_decode_merge, n_seq, Q38_ATTN_HEADS, 4, 256, &L.m)) return -1;
     return 0;
 }
@@ -1533,7 +1538,7 @@ struct q38_decode_graph {
             *arg = &k.L.a;
             p->func = reinterpret_cast<void *>(k.L.f);
             p->gridDim = dim3(k.L.grid_x, Q38_ATTN_KV_HEADS, 1);
-            p->blockDim = dim3(kv->ctx->decode_block, 1, 1);
+            p->blockDim = dim3(k.L.block, 1, 1);
         } else {
             *arg = &k.L.m;
             p->func = reinterpret_cast<void *>(kv->ctx->f_decode_merge);

@@ -1,7 +1,34 @@
 /*
  * Full-attention GQA decode over a paged KV cache of 16-bit or 8-bit rows
- * (gfx950, wave64): the same path as over f32 rows (attn_decode.hip; full_core,
- * src/model/ops.rs:813-940), whose cache holds each row rounded to its type.
+ * (gfx950, wave64): the path of attn_decode.hip (full_core,
+ * src/model/ops.rs:813-940) over a cache that holds each row rounded to its
+ * type.
+ *
+ * A workgroup streams one kv head's pages of one context split once for the
+ * group's 6 query heads, a wave per page, and the split's partials are joined
+ * by q38_attn_decode_merge.  Half or a quarter of the f32 bytes come in per
+ * row, and the vector unit no longer keeps up with them (12 multiply-adds a
+ * value and the conversions), so the products run on the matrix unit, in f32
+ * class precision although its operands have 16 bits:
+ *  - S^T = K Q^T, 16 tokens x 16 columns.  A cached value is an operand as it
+ *    stands (an 8-bit quant as a whole number in f16, its row's scale applied
+ *    to the score).  A query is split into parts whose sum it is -- f16 hi and
+ *    lo (22 bits, after a power of two per head brings the largest to 2^9..10,
+ *    clear of f16's ends), or bf16 hi, mid and lo (24 bits) -- and the 6 heads
+ *    fill columns 0-5 with one part and 8-13 with another, so two parts cost
+ *    one product; a rotation of the 16 lanes by 8 adds them up.
+ *  - O = P V, 16 rows x 16 dims.  The lanes that hold a score are those that
+ *    supply its weight as an operand (C's column l % 16, rows 4 (l / 16) + i
+ *    are A's row l % 16, k 4 (l / 16) + i), so the weights never leave their
+ *    registers; they are split like the queries, into rows 0-5 and 8-13.
+ *    8-bit rows: the value's scale goes into its weight, over a power of two
+ *    at or above every scale seen so far, which keeps f16 clear of overflow.
+ *  - softmax in base 2 against a reference per head that is raised (and O and
+ *    the sum rescaled) only when a score passes it by 2^8: weights stay below
+ *    2^15, which f16 holds, and most pages rescale nothing.
+ * A row's position past the sequence's end counts nothing whatever it holds:
+ * its scores are -inf and its values, which a weight of 0 would not keep NaN
+ * out of, are cleared.
  */
 #include "q38_kv_types.h"
 #include "q38_rope.h"
@@ -9,97 +36,449 @@
 /* 1/sqrt(256) (ops.rs:869) times log2(e). */
 #define Q38_SCORE_LOG2 0.09016844005556021f
 
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
 namespace {
+
+constexpr int kWaves = Q38_DECODE_TYPED_WAVES;
+constexpr int kGroup = Q38_ATTN_GROUP;
+/* A head's reference lies kRefBelow under the score that set it, and is
+ * raised once a score passes it by kRefSlack: weights are at most 2^15. */
+constexpr float kRefBelow = 7.0f, kRefSlack = 15.0f;
+
+/* One page of one kv head as a wave holds it. */
+template <int T>
+struct Page {
+    static constexpr int kLoads = T == Q38_KV_Q8 ? 4 : 8; /* 1 KiB loads of each of K and V */
+    q38_u32x4 k[kLoads], v[kLoads];
+    f32x4 ks, vs; /* 8-bit rows: the scales of tokens 4 (lane / 16) .. + 3 */
+};
+
+Q38_DEV q38_u32x4 ld_stream(const char *p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const q38_u32x4 *>(p));
+}
+
+template <int T>
+Q38_DEV void load_page(Page<T> &p, const q38_decode_args &a, int page, int j, int lane) {
+    const char *kb = q38_kv_block<T>(a.kpool, page, j), *vb = q38_kv_block<T>(a.vpool, page, j);
+#pragma unroll
+    for (int i = 0; i < Page<T>::kLoads; ++i) p.k[i] = ld_stream(kb + 1024 * i + 16 * lane);
+    if (T == Q38_KV_Q8) {
+        p.ks = *reinterpret_cast<const f32x4 *>(kb + 4096 + 16 * (lane >> 4));
+        p.vs = *reinterpret_cast<const f32x4 *>(vb + 4096 + 16 * (lane >> 4));
+    }
+#pragma unroll
+    for (int i = 0; i < Page<T>::kLoads; ++i) p.v[i] = ld_stream(vb + 1024 * i + 16 * lane);
+}
+
+/* Two biased bytes of u as two halves: 0x6400 | b is 1024 + b, and 1152 less
+ * is the quant, both exact. */
+template <uint32_t SEL>
+Q38_DEV uint32_t halves_of(uint32_t u) {
+    const f16x2 x = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, SEL));
+    return __builtin_bit_cast(uint32_t, x + f16x2{(_Float16)-1152.0f, (_Float16)-1152.0f});
+}
+
+Q38_DEV float row_ror8(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF, false));
+}
+
+/* The maximum over the four lanes of a column (l, l ^ 16, l ^ 32, l ^ 48). */
+Q38_DEV float column_max(float x) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const q38_halves h = q38_both_halves(x);
+    return fmaxf(h.a, h.b);
+}
+Q38_DEV float column_sum(float x) {
+    x = q38_pair_rows_sum(x);
+    const q38_halves h = q38_both_halves(x);
+    return h.a + h.b;
+}
+
+/* What a wave carries from page to page. */
+struct State {
+    float ref; /* column l % 16's reference, in log2 units */
+    float l;   /* the sum of this lane's weights */
+    float cap; /* 8-bit rows: a power of two at or above every value scale so far */
+    f32x4 o[16]; /* o[n][i]: row 4 (l / 16) + i, dim 16 n + l % 16 */
+};
+
+template <int T>
+Q38_DEV f32x4 mma_k(q38_u32x4 k, q38_u32x4 q, f32x4 c) {
+    if (T == Q38_KV_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+}
+template <int T>
+Q38_DEV f32x4 mma_v(q38_u32x2 p, q38_u32x2 v, f32x4 c) {
+    if (T == Q38_KV_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, p), __builtin_bit_cast(s16x4, v), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, p), __builtin_bit_cast(f16x4, v), c, 0, 0, 0);
+}
+
+Q38_DEV uint32_t pack16(uint16_t lo, uint16_t hi) { return (uint32_t)hi << 16 | lo; }
+
+/* Scores of a page's tokens, the softmax update, the weighted sum of its
+ * values.  valid: tokens of the page that count (16 but for the sequence's
+ * last page). */
+template <int T>
+Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (&q)[8], const q38_u32x4 (*q2)[64], float unscale,
+                       int valid, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+    /* bf16's third part is read from LDS at every page (an index that the
+     * compiler cannot see through keeps it from 32 registers of the loop's) */
+    int ql = lane;
+    if (T == Q38_KV_BF16) asm volatile("" : "+v"(ql));
+    if (T == Q38_KV_Q8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const q38_u32x4 u = p.k[i];
+            const q38_u32x4 a = {halves_of<0x04010400u>(u[0]), halves_of<0x04030402u>(u[0]), halves_of<0x04010400u>(u[1]),
+                                 halves_of<0x04030402u>(u[1])};
+            const q38_u32x4 b = {halves_of<0x04010400u>(u[2]), halves_of<0x04030402u>(u[2]), halves_of<0x04010400u>(u[3]),
+                                 halves_of<0x04030402u>(u[3])};
+            s0 = mma_k<T>(a, q[2 * i], s0);
+            s1 = mma_k<T>(b, q[2 * i + 1], s1);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            f32x4 &s = T == Q38_KV_F16 && (i & 1) ? s1 : s0;
+            s = mma_k<T>(p.k[i], q[i], s);
+            if (T == Q38_KV_BF16) s1 = mma_k<T>(p.k[i], q2[i][ql], s1);
+        }
+    }
+    float s[4];
+    f32x4 ks = p.ks, vs = p.vs;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = s0[i] + s1[i];
+        s[i] = x + row_ror8(x);
+        if (T == Q38_KV_Q8)
+            s[i] *= ks[i] * unscale;
+        else if (T == Q38_KV_F16)
+            s[i] *= unscale;
+        if (valid < 16 && 4 * g + i >= valid) {
+            s[i] = -INFINITY;
+            vs[i] = 0.0f;
+        }
+    }
+    const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    if (__any(mx > st.ref + kRefSlack)) {
+        /* the page's maximum per head; heads that it does not raise keep theirs */
+        const float top = column_max(mx) - kRefBelow;
+        const float ref = fmaxf(st.ref, top);
+        const float f = st.ref == -INFINITY ? 0.0f : q38_exp2(st.ref - ref);
+        st.ref = ref;
+        st.l *= f;
+        float fr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * g + i, 64);
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st.o[n][i] *= fr[i];
+    }
+    float vinv = 1.0f;
+    if (T == Q38_KV_Q8) {
+        /* scales are signed (the largest value is quant -127) */
+        const float big = fmaxf(fmaxf(fabsf(vs[0]), fabsf(vs[1])), fmaxf(fabsf(vs[2]), fabsf(vs[3])));
+        if (__any(big > st.cap)) {
+            const float top = column_max(big);
+            /* the next power of two, not below 2^-100 */
+            const uint32_t e = max((__float_as_uint(top) >> 23) + 1u, 27u);
+            const float cap = __uint_as_float(min(e, 254u) << 23);
+            const float f = st.cap / cap;
+            st.cap = cap;
+#pragma unroll
+            for (int n = 0; n < 16; ++n) st.o[n] *= f;
+        }
+        vinv = 1.0f / st.cap;
+    }
+    float w[4], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = q38_exp2(s[i] - st.ref);
+        sum += w[i];
+        if (T == Q38_KV_Q8) w[i] *= vs[i] * vinv;
+    }
+    st.l += sum;
+
+    /* the weights' parts: rows 0-5 the first (and, in a product of its own,
+     * the third), rows 8-13 the second */
+    q38_u32x2 a0, a1;
+    const bool first = c < 8;
+    if (T == Q38_KV_BF16) {
+        uint32_t x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t hi = __float_as_uint(w[i]) & 0xFFFF0000u;
+            const float r = w[i] - __uint_as_float(hi);
+            const uint32_t mid = __float_as_uint(r) & 0xFFFF0000u;
+            const float lo = r - __uint_as_float(mid);
+            x[i] = first ? hi : mid;
+            y[i] = first ? __float_as_uint(lo) : 0u;
+        }
+        a0 = q38_u32x2{__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+        a1 = q38_u32x2{__builtin_amdgcn_perm(y[1], y[0], 0x07060302u), __builtin_amdgcn_perm(y[3], y[2], 0x07060302u)};
+    } else {
+        uint16_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const _Float16 hi = (_Float16)w[i];
+            const _Float16 lo = (_Float16)(w[i] - (float)hi);
+            x[i] = __builtin_bit_cast(uint16_t, first ? hi : lo);
+        }
+        a0 = q38_u32x2{pack16(x[0], x[1]), pack16(x[2], x[3])};
+    }
+    /* values of tokens that do not count are cleared (8-bit ones are finite) */
+    q38_u32x2 keep = {~0u, ~0u};
+    if (T != Q38_KV_Q8 && valid < 16) {
+        const int n = valid - 4 * g;
+        keep = q38_u32x2{n <= 0 ? 0u : n == 1 ? 0xFFFFu : ~0u, n <= 2 ? 0u : n == 3 ? 0xFFFFu : ~0u};
+    }
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+        q38_u32x2 v;
+        if (T == Q38_KV_Q8) {
+            const uint32_t u = p.v[n >> 2][n & 3];
+            v = q38_u32x2{halves_of<0x04010400u>(u), halves_of<0x04030402u>(u)};
+        } else {
+            v = q38_u32x2{p.v[n >> 1][2 * (n & 1)] & keep[0], p.v[n >> 1][2 * (n & 1) + 1] & keep[1]};
+        }
+        st.o[n] = mma_v<T>(a0, v, st.o[n]);
+        if (T == Q38_KV_BF16) st.o[n] = mma_v<T>(a1, v, st.o[n]);
+    }
+}
 
 template <int T, bool kPre>
 Q38_DEV void decode_typed(const q38_decode_args &a) {
-    __shared__ __attribute__((aligned(16))) float q[Q38_ATTN_GROUP][Q38_ATTN_HEAD_DIM];
-    __shared__ float row[2][Q38_ATTN_HEAD_DIM];
-    __shared__ float p[Q38_ATTN_GROUP][Q38_PAGE_TOKENS];
-    __shared__ float cs[32][2];
-    const int g = blockIdx.x, j = blockIdx.y, tid = threadIdx.x;
+    constexpr int kQSets = T == Q38_KV_BF16 ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) float q_rows[8][Q38_ATTN_HEAD_DIM];
+    __shared__ q38_u32x4 q_frag[kQSets][8][64];
+    __shared__ float q_unscale[8];
+    /* the new token's rows as they are stored: 16-bit values, or biased bytes */
+    __shared__ __attribute__((aligned(16))) uint16_t new_row[2][Q38_ATTN_HEAD_DIM];
+    __shared__ float new_scale[2];
+    __shared__ float rope_cs[kPre ? kWaves : 1][32][2];
+    __shared__ float red_o[kWaves][kGroup][Q38_ATTN_HEAD_DIM];
+    __shared__ float red_m[kWaves][8];
+    __shared__ float red_l[kWaves][8];
+    static_assert(kWaves == 8 && kGroup == 6, "a wave per query head, one for the key and one for the value");
+
+    const int g_split = blockIdx.x, j = blockIdx.y, tid = threadIdx.x;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int b = 0;
-    while (b + 1 < a.n_seq && a.split_base[b + 1] <= g) ++b;
+    while (b + 1 < a.n_seq && a.split_base[b + 1] <= g_split) ++b;
     const int seq = a.seq[b], pos = a.pos[b];
-    const int split = g - a.split_base[b], nsplit = a.split_base[b + 1] - a.split_base[b];
+    const int split = g_split - a.split_base[b], nsplit = a.split_base[b + 1] - a.split_base[b];
     const int t_begin = split * a.split_tokens, t_end = min(pos + 1, t_begin + a.split_tokens);
-    const int32_t *pt = a.page_table + (size_t)seq * a.pt_stride;
-    const int lane = tid & 63, wave = tid >> 6;
+    const int n_pages = (t_end - t_begin + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS;
+    const bool has_pos = t_end == pos + 1;
+
+    /* this wave's page ids, the i-th in lane i: pages wave, wave + 8, ... (64
+     * of them cover the largest split) */
+    static_assert(Q38_MAX_SPLIT_TOKENS <= 64 * kWaves * Q38_PAGE_TOKENS, "a lane per page id");
+    const int32_t *pt = a.page_table + (size_t)seq * a.pt_stride + (t_begin >> 4);
+    const int my_pages = pt[min(wave + kWaves * lane, n_pages - 1)];
+
+    /* the rows that this wave forms: query head `wave`, or the new key or value */
     const int q_stride = kPre ? 2 * Q38_ATTN_HEAD_DIM : Q38_ATTN_HEAD_DIM;
-    const float *qb = a.q + ((size_t)b * Q38_ATTN_HEADS + j * Q38_ATTN_GROUP) * q_stride;
-    if (kPre) {
-        if (tid < 64) q38_rope_table(cs, lane, pos, a.theta_scale);
-        __syncthreads();
+    const bool forms_q = wave < kGroup;
+    const bool forms_new = !forms_q && a.k_new != nullptr && has_pos;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, xw = x;
+    if (forms_q) {
+        x = q38_ld4(a.q + ((size_t)b * Q38_ATTN_HEADS + j * kGroup + wave) * q_stride + 4 * lane);
+        if (kPre) xw = q38_ld4(a.q_norm + 4 * lane);
+    } else if (forms_new) {
+        x = q38_ld4((wave == kGroup ? a.k_new : a.v_new) + (size_t)b * Q38_ATTN_KV_DIM + j * Q38_ATTN_HEAD_DIM + 4 * lane);
+        if (kPre) xw = q38_ld4(a.k_norm + 4 * lane);
     }
-    for (int hh = wave; hh < Q38_ATTN_GROUP; hh += 4) {
-        f32x4 x = q38_ld4(qb + hh * q_stride + 4 * lane);
-        if (kPre) q38_norm_rope4_cs(x, q38_ld4(a.q_norm + 4 * lane), lane, cs);
-        q38_st4(&q[hh][4 * lane], x * Q38_SCORE_LOG2);
+    Page<T> cur;
+    if (wave < n_pages) load_page<T>(cur, a, __builtin_amdgcn_readlane(my_pages, 0), j, lane);
+
+    if (kPre && (forms_q || (forms_new && wave == kGroup))) {
+        q38_rope_table(rope_cs[wave], lane, pos, a.theta_scale);
+        /* the lanes read each other's entries below: LDS serves a wave in
+         * order, the fence keeps the compiler to it */
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        q38_norm_rope4_cs(x, xw, lane, rope_cs[wave]);
     }
-    if (a.k_new != nullptr && t_end == pos + 1 && wave < 2) {
-        /* the new token's row: wave 0 the key, wave 1 the value */
-        const float *src = (wave ? a.v_new : a.k_new) + (size_t)b * Q38_ATTN_KV_DIM + j * Q38_ATTN_HEAD_DIM;
-        f32x4 x = q38_ld4(src + 4 * lane);
-        if (kPre && wave == 0) q38_norm_rope4_cs(x, q38_ld4(a.k_norm + 4 * lane), lane, cs);
-        char *block = q38_kv_block<T>(wave ? a.vpool : a.kpool, pt[pos >> 4], j);
-        const int t = pos & 15;
-        int qv[4];
-        float scale = 0.0f;
-        if (T == Q38_KV_Q8) {
-            q38_wave_q8k(x, qv, scale);
-            if (lane == 0) q38_kv_scales(block)[t] = scale;
+    if (forms_q) {
+        x *= Q38_SCORE_LOG2;
+        if (T != Q38_KV_BF16) {
+            float big = q38_max16(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+            big = column_max(big);
+            /* exponent of the largest, kept where 2^(10 - e) and its inverse are normal */
+            const int e = min(max((int)(__float_as_uint(big) >> 23) - 126, -100), 100);
+            x *= __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+            if (lane == 0) q_unscale[wave] = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
         }
-        for (int c = 0; c < 4; ++c) {
-            const int i = wave ? q38_v_index<T>(t, 4 * lane + c) : q38_k_index<T>(t, 4 * lane + c);
-            if (T == Q38_KV_Q8)
-                reinterpret_cast<uint8_t *>(block)[i] = (uint8_t)(qv[c] + 128);
-            else
-                reinterpret_cast<uint16_t *>(block)[i] = q38_to16<T>(x[c]);
-        }
-        __threadfence();
-    }
-    __syncthreads();
-    float m[Q38_ATTN_GROUP], l[Q38_ATTN_GROUP], o[Q38_ATTN_GROUP];
-    for (int hh = 0; hh < Q38_ATTN_GROUP; ++hh) m[hh] = -INFINITY, l[hh] = o[hh] = 0.0f;
-    for (int tb = t_begin; tb < t_end; tb += Q38_PAGE_TOKENS) {
-        const int page = pt[tb >> 4], n = min(Q38_PAGE_TOKENS, t_end - tb);
-        char *kb = q38_kv_block<T>(a.kpool, page, j), *vb = q38_kv_block<T>(a.vpool, page, j);
-        if (tid < Q38_ATTN_GROUP * Q38_PAGE_TOKENS) {
-            const int hh = tid >> 4, t = tid & 15;
-            float s = 0.0f;
-            if (t < n)
-                for (int d = 0; d < Q38_ATTN_HEAD_DIM; ++d)
-                    s = __builtin_fmaf(q[hh][d], q38_kv_value<T>(kb, q38_k_index<T>(t, d), t), s);
-            p[hh][t] = t < n ? s : -INFINITY;
-        }
-        __syncthreads();
-        for (int hh = 0; hh < Q38_ATTN_GROUP; ++hh) {
-            float mx = m[hh];
-            for (int t = 0; t < n; ++t) mx = fmaxf(mx, p[hh][t]);
-            const float f = q38_exp2(m[hh] - mx);
-            l[hh] *= f;
-            o[hh] *= f;
-            m[hh] = mx;
-            for (int t = 0; t < n; ++t) {
-                const float w = q38_exp2(p[hh][t] - mx);
-                l[hh] += w;
-                o[hh] = __builtin_fmaf(w, q38_kv_value<T>(vb, q38_v_index<T>(t, tid), t), o[hh]);
+        q38_st4(&q_rows[wave][4 * lane], x);
+    } else {
+        q38_st4(&q_rows[wave][4 * lane], f32x4{0.f, 0.f, 0.f, 0.f}); /* columns 6 and 7 */
+        if (lane == 0) q_unscale[wave] = 1.0f;
+        if (forms_new) {
+            const int which = wave - kGroup;
+            char *block = q38_kv_block<T>(which ? a.vpool : a.kpool, pt[(pos - t_begin) >> 4], j);
+            const int t = pos & 15;
+            int qv[4] = {0, 0, 0, 0};
+            float scale = 0.0f;
+            if (T == Q38_KV_Q8) q38_wave_q8k(x, qv, scale);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = 4 * lane + i;
+                const int at = which ? q38_v_index<T>(t, d) : q38_k_index<T>(t, d);
+                if (T == Q38_KV_Q8) {
+                    new_row[which][d] = (uint16_t)(qv[i] + 128);
+                    reinterpret_cast<uint8_t *>(block)[at] = (uint8_t)(qv[i] + 128);
+                } else {
+                    new_row[which][d] = q38_to16<T>(x[i]);
+                    reinterpret_cast<uint16_t *>(block)[at] = q38_to16<T>(x[i]);
+                }
+            }
+            if (T == Q38_KV_Q8 && lane == 0) {
+                new_scale[which] = scale;
+                q38_kv_scales(block)[t] = scale;
             }
         }
-        __syncthreads();
     }
-    for (int hh = 0; hh < Q38_ATTN_GROUP; ++hh) {
-        const int h = j * Q38_ATTN_GROUP + hh;
+    __syncthreads();
+    const int c = lane & 15, g = lane >> 4;
+    {
+        /* operand `wave` of the queries: column c, dims d0 .. d0 + 7 */
+        const int d0 = T == Q38_KV_Q8 ? 64 * (wave >> 1) + 16 * g + 8 * (wave & 1) : 32 * wave + 8 * g;
+        const bool first = c < 8;
+        uint16_t f0[8], f1[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = q_rows[c & 7][d0 + e];
+            if (T == Q38_KV_BF16) {
+                const uint32_t hi = __float_as_uint(v) & 0xFFFF0000u;
+                const float r = v - __uint_as_float(hi);
+                const uint32_t mid = __float_as_uint(r) & 0xFFFF0000u;
+                const float lo = r - __uint_as_float(mid);
+                f0[e] = (uint16_t)((first ? hi : mid) >> 16);
+                f1[e] = first ? (uint16_t)(__float_as_uint(lo) >> 16) : 0;
+            } else {
+                const _Float16 hi = (_Float16)v;
+                const _Float16 lo = (_Float16)(v - (float)hi);
+                f0[e] = __builtin_bit_cast(uint16_t, first ? hi : lo);
+            }
+        }
+        q_frag[0][wave][lane] = q38_u32x4{pack16(f0[0], f0[1]), pack16(f0[2], f0[3]), pack16(f0[4], f0[5]), pack16(f0[6], f0[7])};
+        if (kQSets > 1)
+            q_frag[kQSets - 1][wave][lane] =
+                q38_u32x4{pack16(f1[0], f1[1]), pack16(f1[2], f1[3]), pack16(f1[4], f1[5]), pack16(f1[6], f1[7])};
+    }
+    __syncthreads();
+
+    if (wave < n_pages) {
+        q38_u32x4 q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = q_frag[0][i][lane];
+        const float unscale = q_unscale[c & 7];
+        State st;
+        st.ref = -INFINITY;
+        st.l = 0.0f;
+        st.cap = __uint_as_float(27u << 23); /* 2^-100 */
+#pragma unroll
+        for (int n = 0; n < 16; ++n) st.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = wave; i < n_pages; i += kWaves) {
+            Page<T> next;
+            if (i + kWaves < n_pages) load_page<T>(next, a, __builtin_amdgcn_readlane(my_pages, (i + kWaves) / kWaves), j, lane);
+            int valid = Q38_PAGE_TOKENS;
+            if (i == n_pages - 1) {
+                valid = t_end - t_begin - Q38_PAGE_TOKENS * i;
+                if (has_pos && a.k_new != nullptr) {
+                    /* the new token's rows in place of what the page held */
+                    const int t = valid - 1;
+                    const bool key_lane = c == t, value_lane = g == (t >> 2);
+                    if (T == Q38_KV_Q8) {
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                uint32_t kw = 0;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) kw |= (uint32_t)new_row[0][64 * s + 16 * g + 4 * w + e] << (8 * e);
+                                if (key_lane) cur.k[s][w] = kw;
+                                const uint32_t sh = 8 * (t & 3);
+                                const uint32_t vw = (uint32_t)new_row[1][64 * s + 16 * w + c] << sh;
+                                if (value_lane) cur.v[s][w] = (cur.v[s][w] & ~(255u << sh)) | vw;
+                            }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (value_lane && (t & 3) == e) cur.ks[e] = new_scale[0], cur.vs[e] = new_scale[1];
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < 8; ++s) {
+                            const q38_u32x4 kw = *reinterpret_cast<const q38_u32x4 *>(&new_row[0][32 * s + 8 * g]);
+                            if (key_lane) cur.k[s] = kw;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t sh = 16 * (t & 1);
+                                const uint32_t vw = (uint32_t)new_row[1][32 * s + 16 * h + c] << sh;
+#pragma unroll
+                                for (int w = 0; w < 2; ++w)
+                                    if (value_lane && ((t >> 1) & 1) == w)
+                                        cur.v[s][2 * h + w] = (cur.v[s][2 * h + w] & ~(0xFFFFu << sh)) | vw;
+                            }
+                        }
+                    }
+                }
+            }
+            page_step<T>(st, cur, q, q_frag[kQSets - 1], unscale, valid, lane);
+            cur = next;
+        }
+        /* both parts' rows added (lanes l and l ^ 32), the lower half of the wave
+         * storing the even tiles and the upper half the odd ones */
+        const float l = column_sum(st.l);
+        if (lane < 8) {
+            red_m[wave][lane] = st.ref;
+            red_l[wave][lane] = l;
+        }
+        const bool upper = lane >= 32;
+#pragma unroll
+        for (int n = 0; n < 16; n += 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const q38_halves e = q38_both_halves(st.o[n][i]), o = q38_both_halves(st.o[n + 1][i]);
+                float v = upper ? o.a + o.b : e.a + e.b;
+                if (T == Q38_KV_Q8) v *= st.cap;
+                const int head = 4 * (g & 1) + i;
+                if (head < kGroup) red_o[wave][head][16 * (n + (upper ? 1 : 0)) + c] = v;
+            }
+        }
+    }
+    __syncthreads();
+
+    const int live = min(kWaves, n_pages);
+    for (int i = tid; i < kGroup * Q38_ATTN_HEAD_DIM; i += 64 * kWaves) {
+        const int hh = i >> 8, d = i & 255;
+        float M = -INFINITY;
+        for (int w = 0; w < live; ++w) M = fmaxf(M, red_m[w][hh]);
+        float L = 0.0f, O = 0.0f;
+        for (int w = 0; w < live; ++w) {
+            const float f = red_m[w][hh] == -INFINITY ? 0.0f : q38_exp2(red_m[w][hh] - M);
+            L += red_l[w][hh] * f;
+            O += red_o[w][hh][d] * f;
+        }
+        const int h = j * kGroup + hh;
         if (nsplit == 1) {
-            float r = o[hh] / l[hh];
-            if (a.gate != nullptr)
-                r *= q38_sigmoid(a.gate[((size_t)b * Q38_ATTN_HEADS + h) * a.gate_head_stride + tid]);
-            a.out[(size_t)b * Q38_ATTN_Q_DIM + h * Q38_ATTN_HEAD_DIM + tid] = r;
+            float r = O / L;
+            if (a.gate != nullptr) r *= q38_sigmoid(a.gate[((size_t)b * Q38_ATTN_HEADS + h) * a.gate_head_stride + d]);
+            a.out[(size_t)b * Q38_ATTN_Q_DIM + h * Q38_ATTN_HEAD_DIM + d] = r;
         } else {
-            a.part_o[((size_t)g * Q38_ATTN_HEADS + h) * Q38_ATTN_HEAD_DIM + tid] = o[hh];
-            if (tid == 0) {
-                a.part_ml[((size_t)g * Q38_ATTN_HEADS + h) * 2 + 0] = m[hh];
-                a.part_ml[((size_t)g * Q38_ATTN_HEADS + h) * 2 + 1] = l[hh];
+            a.part_o[((size_t)g_split * Q38_ATTN_HEADS + h) * Q38_ATTN_HEAD_DIM + d] = O;
+            if (d == 0) {
+                a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 0] = M;
+                a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 1] = L;
             }
         }
     }
@@ -107,12 +486,12 @@ Q38_DEV void decode_typed(const q38_decode_args &a) {
 
 }  // namespace
 
-#define Q38_DECODE_KERNELS(name, T)                                                                     \
-    extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_##name(q38_decode_args a) {       \
-        decode_typed<T, false>(a);                                                                      \
-    }                                                                                                   \
-    extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_##name##_pre(q38_decode_args a) { \
-        decode_typed<T, true>(a);                                                                       \
+#define Q38_DECODE_KERNELS(name, T)                                                                                  \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name(q38_decode_args a) {            \
+        decode_typed<T, false>(a);                                                                                   \
+    }                                                                                                                \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name##_pre(q38_decode_args a) {      \
+        decode_typed<T, true>(a);                                                                                    \
     }
 Q38_DECODE_KERNELS(f16, Q38_KV_F16)
 Q38_DECODE_KERNELS(bf16, Q38_KV_BF16)

@@ -42,8 +42,15 @@ def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, gate=None):
     scaling to base 2 and back two roundings more).  A weight is then off by a
     factor exp(+-e), e the largest such error plus 4 u for exp2 and its
     argument's rounding, |s| u; numerator and denominator each by e, and by
-    (n + 16) u for their sums and the splits' rescalings; weights split into
-    parts lose 2^-21 of the largest weight at most.  The gate's sigmoid 8 u."""
+    (n + 16) u for their sums and the splits' rescalings; a weight's parts
+    carry 2^-21 of it or better while they are normal halves.  Below those, a
+    part is rounded to whole steps of 2^-24 (half of one off), and the largest
+    weight of a chain is 2^7 at least (its reference lies at most 7 under its
+    largest score): each weight is off by 2^-32 of the largest at most,
+    whatever its own size, times its value -- for 8-bit rows, whose weight
+    carries the value's scale over a power of two of up to twice the largest
+    scale, times up to twice the largest value.  A term n 2^-31 pmax vmax
+    covers both.  The gate's sigmoid 8 u."""
     u = 2.0 ** -24
     n = k.shape[0]
     out, bound = np.empty((24, 256)), np.empty((24, 256))
@@ -56,7 +63,7 @@ def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, gate=None):
         p /= p.sum()
         out[h] = p @ vv
         e = 2.0 * ((264 * big + 4 + float(np.abs(s).max())) * u) + (n + 16) * u + 2.0 ** -21
-        bound[h] = e * (p @ np.abs(vv)) * 1.01 + 1e-37
+        bound[h] = e * (p @ np.abs(vv)) * 1.01 + n * 2.0 ** -31 * p.max() * np.abs(vv).max() + 1e-37
     if gate is not None:
         sig = 1.0 / (1.0 + np.exp(-gate.reshape(24, 256).astype(np.float64)))
         out, bound = out * sig, bound * sig + 8 * u * np.abs(out * sig)
