@@ -137,6 +137,12 @@ constexpr KvType kKvTypes[] = {
     {Q38_GGML_Q8_K, Q38_KV_BLOCK_Q8, "q8k"},
 };
 constexpr int kKvTypeCount = (int)(sizeof(kKvTypes) / sizeof(kKvTypes[0]));
+/* q38_add_rms_norm's kernels that hold a row in registers: 256 or 1024
+ * threads, 1 .. kNormVectors vectors of 4 values a thread. */
+constexpr int kNormVectors = 5;
+std::string norm_kernel_name(int wide, int v) {
+    return std::string("q38_add_rms_norm_") + (wide ? "1024_" : "256_") + std::to_string(v + 1);
+}
 /* The split-block GEMM's grid: at least this many workgroups (fewer: the
  * GEMV), at most this many per CU (more: the 128 x 64 tiles) */
 constexpr long kGemmKsMinTiles = 64;
@@ -176,7 +182,8 @@ struct q38_ctx {
     hipFunction_t f_kv_gather_16 = nullptr;        /* 16-bit rows as they are stored */
     hipFunction_t f_kv_split_typed[kKvTypeCount] = {}; /* from index 1 on */
     hipModule_t mod_norm = nullptr;
-    hipFunction_t f_add_rms_norm = nullptr;
+    hipFunction_t f_norm[2][kNormVectors] = {}; /* [256 or 1024 threads][vectors a thread - 1] */
+    hipFunction_t f_norm_any = nullptr;
     hipFunction_t f_dequantize_q8k = nullptr;
     hipModule_t mod_typed = nullptr;
     hipFunction_t f_decode_typed[kKvTypeCount][2] = {}; /* from index 1 on; [1]: the pre step fused */
@@ -472,7 +479,10 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
         return fail("decode kernel has block size %d, expected %d", ctx->decode_block, 64 * Q38_DECODE_WAVES);
     const std::string p_norm = dir + "/norm.hsaco";
     Q38_HIP(hipModuleLoad(&ctx->mod_norm, p_norm.c_str()));
-    Q38_HIP(hipModuleGetFunction(&ctx->f_add_rms_norm, ctx->mod_norm, "q38_add_rms_norm"));
+    for (int v = 0; v < kNormVectors; ++v)
+        for (int w = 0; w < 2; ++w)
+            Q38_HIP(hipModuleGetFunction(&ctx->f_norm[w][v], ctx->mod_norm, norm_kernel_name(w, v).c_str()));
+    Q38_HIP(hipModuleGetFunction(&ctx->f_norm_any, ctx->mod_norm, "q38_add_rms_norm_any"));
     Q38_HIP(hipModuleGetFunction(&ctx->f_dequantize_q8k, ctx->mod_norm, "q38_dequantize_q8k"));
     const std::string p_rows = dir + "/kv_rows.hsaco", p_typed = dir + "/attn_decode_typed.hsaco";
     Q38_HIP(hipModuleLoad(&ctx->mod_rows, p_rows.c_str()));
@@ -751,7 +761,10 @@ int q38_kernel_timer_start(q38_ctx *ctx, const char *kernel_name, int max_launch
             if (i > 0 && name == "q38_attn_decode_" + ty) f = ctx->f_decode_typed[i][0];
             if (i > 0 && name == "q38_attn_decode_" + ty + "_pre") f = ctx->f_decode_typed[i][1];
         }
-        if (name == "q38_add_rms_norm") f = ctx->f_add_rms_norm;
+        for (int v = 0; v < kNormVectors; ++v)
+            for (int w = 0; w < 2; ++w)
+                if (name == norm_kernel_name(w, v)) f = ctx->f_norm[w][v];
+        if (name == "q38_add_rms_norm_any") f = ctx->f_norm_any;
         if (name == "q38_dequantize_q8k") f = ctx->f_dequantize_q8k;
         if (name == "q38_kv_gather_16") f = ctx->f_kv_gather_16;
         for (int i = 0; i < kGemvTypes; ++i) {
@@ -2519,7 +2532,19 @@ int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, co
         overlaps(d_q8k, q_bytes, d_weight, (size_t)width * sizeof(float)))
         return fail("d_q8k overlaps an input");
     q38_norm_args a = {d_x, d_residual, d_weight, d_sum, d_y, d_q8k, width, n_tokens};
-    return ctx->launch(ctx->f_add_rms_norm, (unsigned)n_tokens, 1, 1, 256, &a);
+    /* rows of whole 16-byte vectors stay in registers where they fit */
+    const bool vectors = width % 4 == 0 && ((uintptr_t)d_x | (uintptr_t)d_residual | (uintptr_t)d_weight |
+                                            (uintptr_t)d_sum | (uintptr_t)d_y) % 16 == 0;
+    if (!vectors || width > 1024 * 4 * kNormVectors)
+        return ctx->launch(ctx->f_norm_any, (unsigned)n_tokens, 1, 1, 1024, &a);
+    /* up to two rows per CU the chip has waves to spare, and 1024 threads a row
+     * shorten the row's own chain; past that 256 keep more rows in flight and
+     * waste fewer lanes on short ones (rows of 5120, us: 1 row 3.9 against 4.2,
+     * 256 rows 5.3 against 6.1, 1024 rows 15.1 against 14.3; 4096 rows of 1024
+     * 17.3 against 11.7) */
+    const int wide = width > 256 * 4 * kNormVectors || n_tokens <= 2 * ctx->cu_count;
+    const int per = (wide ? 1024 : 256) * 4;
+    return ctx->launch(ctx->f_norm[wide][(width + per - 1) / per - 1], (unsigned)n_tokens, 1, 1, wide ? 1024 : 256, &a);
 }
 
 int q38_gemv_q8_k(q38_ctx *ctx, int ggml_type, int rows, int width, const void *d_weights, const void *d_q8k,

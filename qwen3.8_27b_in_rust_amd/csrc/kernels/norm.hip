@@ -8,61 +8,153 @@
 
 namespace {
 
-Q38_DEV double block_sum_f64(double x, double *part, int waves) {
+/* The sum over the workgroup, the same in every thread. */
+template <int NT>
+Q38_DEV double block_sum_f64(double x, double *part) {
     x = q38_wave_sum_f64(x);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
     __syncthreads();
     double s = 0.0;
-    for (int w = 0; w < waves; ++w) s += part[w];
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) s += part[w];
     return s;
+}
+
+Q38_DEV float norm_scale(double ss, int width) {
+    const float mean = (float)(ss / (double)width);
+    return 1.0f / sqrtf(mean + 1e-6f);
+}
+
+Q38_DEV double square_sum(f32x4 h) {
+    return (double)h.x * (double)h.x + (double)h.y * (double)h.y + (double)h.z * (double)h.z + (double)h.w * (double)h.w;
+}
+
+/* Where a row's Q8_K blocks go. */
+struct Q8kRow {
+    int8_t *quants;
+    int16_t *sums;
+    float *scales;
+};
+Q38_DEV Q8kRow q8k_row(const q38_norm_args &a, int t) {
+    const size_t n = (size_t)a.n_tokens * a.width, row = (size_t)t * a.width;
+    int8_t *base = static_cast<int8_t *>(a.q8k);
+    int16_t *sums = reinterpret_cast<int16_t *>(base + n);
+    return {base + row, sums + row / 16, reinterpret_cast<float *>(sums + n / 16) + row / 256};
+}
+
+/* Block b of a row, held 4 values per lane by a wave. */
+Q38_DEV void store_q8k(const Q8kRow &r, int b, int lane, f32x4 y) {
+    int q[4];
+    float scale;
+    q38_wave_q8k(y, q, scale);
+    reinterpret_cast<uint32_t *>(r.quants)[b * 64 + lane] =
+        (uint32_t)(q[0] & 255) | (uint32_t)(q[1] & 255) << 8 | (uint32_t)(q[2] & 255) << 16 | (uint32_t)(q[3] & 255) << 24;
+    int s = q[0] + q[1] + q[2] + q[3];
+    s += __builtin_amdgcn_update_dpp(0, s, 0xB1, 0xF, 0xF, false);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x4E, 0xF, 0xF, false);
+    if ((lane & 3) == 0) r.sums[b * 16 + (lane >> 2)] = (int16_t)s;
+    if (lane == 0) r.scales[b] = scale;
+}
+
+/* A workgroup of NT threads per row, the row in registers: thread i holds
+ * dims 4 (i + NT v) .. + 3, so a wave's v-th vectors are 256 consecutive dims,
+ * a Q8_K block.  Every load is issued at once and every value read once, so
+ * the kernel runs at the memory's rate: 4096 rows of 5120 with all outputs
+ * (17.14 bytes a value) 67 us, 5.4 TB/s; 1024 rows of 10240 6.7 TB/s; one row
+ * 3.9 us a launch among others, where an empty one takes about as long.  A first
+ * version that read its row twice and value by value took 187 us. */
+template <int NT, int V>
+Q38_DEV void norm_row(const q38_norm_args &a) {
+    __shared__ double part[NT / 64];
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, width = a.width;
+    const size_t row = (size_t)t * width;
+    const bool adds = a.residual != nullptr;
+    f32x4 h[V], r[V], w[V];
+    /* threads past the row load its last vector and leave it out: no load
+     * sits under a branch, so all of them are in flight together */
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int d = min(4 * (tid + NT * v), width - 4);
+        h[v] = q38_ld4(a.x + row + d);
+        w[v] = q38_ld4(a.weight + d);
+    }
+    if (adds) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = q38_ld4(a.residual + row + min(4 * (tid + NT * v), width - 4));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] += r[v];
+    }
+    double ss = 0.0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const double s = square_sum(h[v]);
+        ss += 4 * (tid + NT * v) < width ? s : 0.0;
+    }
+    const float scale = norm_scale(block_sum_f64<NT>(ss, part), width);
+    const Q8kRow q = q8k_row(a, t);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int d = 4 * (tid + NT * v);
+        if (d - 4 * lane >= width) break; /* past the row for the whole wave */
+        const f32x4 y = h[v] * scale * w[v];
+        if (d < width) {
+            if (a.sum != nullptr) q38_st4(a.sum + row + d, h[v]);
+            if (a.y != nullptr) q38_st4(a.y + row + d, y);
+        }
+        /* the width is a multiple of 256: the wave's 256 dims are all there */
+        if (a.q8k != nullptr) store_q8k(q, d >> 8, lane, y);
+        /* one block's quantiser at a time: run together they take registers
+         * that more rows in flight need */
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 }  // namespace
 
-/* grid (n_tokens), 256 threads. */
-extern "C" __global__ __launch_bounds__(256) void q38_add_rms_norm(q38_norm_args a) {
-    __shared__ double part[4];
-    const int t = blockIdx.x, width = a.width;
+#define Q38_NORM_KERNEL(NT, V)                                                                              \
+    extern "C" __global__ __launch_bounds__(NT) void q38_add_rms_norm_##NT##_##V(q38_norm_args a) { norm_row<NT, V>(a); }
+Q38_NORM_KERNEL(256, 1)
+Q38_NORM_KERNEL(256, 2)
+Q38_NORM_KERNEL(256, 3)
+Q38_NORM_KERNEL(256, 4)
+Q38_NORM_KERNEL(256, 5)
+Q38_NORM_KERNEL(1024, 1)
+Q38_NORM_KERNEL(1024, 2)
+Q38_NORM_KERNEL(1024, 3)
+Q38_NORM_KERNEL(1024, 4)
+Q38_NORM_KERNEL(1024, 5)
+
+/* Rows that are not whole aligned vectors, or too long for registers: the row
+ * is read again after its sum (from the cache), value by value. */
+extern "C" __global__ __launch_bounds__(1024) void q38_add_rms_norm_any(q38_norm_args a) {
+    __shared__ double part[16];
+    const int t = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, width = a.width;
     const size_t row = (size_t)t * width;
     double ss = 0.0;
-    for (int d = threadIdx.x; d < width; d += 256) {
+    for (int d = threadIdx.x; d < width; d += 1024) {
         const float h = a.residual != nullptr ? a.x[row + d] + a.residual[row + d] : a.x[row + d];
         ss += (double)h * (double)h;
     }
-    const float mean = (float)(block_sum_f64(ss, part, 4) / (double)width);
-    const float scale = 1.0f / sqrtf(mean + 1e-6f);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int blocks = width / Q38_Q8K_BLOCK;
-    int8_t *quants = static_cast<int8_t *>(a.q8k);
-    int16_t *sums = reinterpret_cast<int16_t *>(quants + (size_t)a.n_tokens * width);
-    float *scales = reinterpret_cast<float *>(sums + (size_t)a.n_tokens * blocks * 16);
-    /* a wave per 256 values, lane l: 4l .. 4l + 3 */
-    for (int b = wave; b * 256 < width; b += 4) {
-        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    const float scale = norm_scale(block_sum_f64<1024>(ss, part), width);
+    const Q8kRow q = q8k_row(a, t);
+    /* a wave per 256 values, lane l: 4l .. 4l + 3.  A thread reads again only
+     * what no other writes, so an output may be an input's own row. */
+    for (int b = wave; b * 256 < width; b += 16) {
+        f32x4 h = {0.f, 0.f, 0.f, 0.f}, y = h;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int d = b * 256 + 4 * lane + c;
-            if (d >= width) continue;
-            const float h = a.residual != nullptr ? a.x[row + d] + a.residual[row + d] : a.x[row + d];
-            y[c] = h * scale * a.weight[d];
-            if (a.sum != nullptr) a.sum[row + d] = h;
-            if (a.y != nullptr) a.y[row + d] = y[c];
+            if (d < width) h[c] = a.residual != nullptr ? a.x[row + d] + a.residual[row + d] : a.x[row + d];
+            if (d < width) y[c] = h[c] * scale * a.weight[d];
         }
-        if (a.q8k == nullptr) continue;
-        int q[4];
-        float qs;
-        q38_wave_q8k(y, q, qs);
-        const size_t k = (size_t)t * blocks + b;
-        int s = 0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            quants[k * 256 + 4 * lane + c] = (int8_t)q[c];
-            s += q[c];
+            const int d = b * 256 + 4 * lane + c;
+            if (a.sum != nullptr && d < width) a.sum[row + d] = h[c];
+            if (a.y != nullptr && d < width) a.y[row + d] = y[c];
         }
-        s += __builtin_amdgcn_update_dpp(0, s, 0xB1, 0xF, 0xF, false);
-        s += __builtin_amdgcn_update_dpp(0, s, 0x4E, 0xF, 0xF, false);
-        if ((lane & 3) == 0) sums[k * 16 + (lane >> 2)] = (int16_t)s;
-        if (lane == 0) scales[k] = qs;
+        if (a.q8k != nullptr) store_q8k(q, b, lane, y);
     }
 }
 
