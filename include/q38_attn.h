@@ -158,7 +158,7 @@ int q38_kv_read(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, float *d
  * with d_k_norm ([256], 16-byte aligned; eps 1e-6) and rotated at its
  * position, then stored, as the value row is, in the cache's type; the result
  * equals q38_attn_pre's k rows stored with q38_kv_write, bit for bit.
- * Sequence ids must be distinct; pages are reserved as needed.  At most 2^27
+ * Sequence ids must be distinct; pages are reserved as needed.  At most 2^25
  * rows a call. */
 int q38_kv_append(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
                   const int32_t *n_tokens, const float *d_k_norm, const float *d_key, const float *d_value);

@@ -26,6 +26,7 @@ extern "C" hipError_t hipExtModuleLaunchKernel(hipFunction_t f, uint32_t globalW
                                                uint32_t flags);
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -964,9 +965,9 @@ int q38_seq_capacity(q38_kv *kv, int seq, int *n_tokens) {
 
 namespace {
 
-/* Rows most that one append or gather moves (f32 rows of half a terabyte):
+/* Rows most that one append or gather moves (f32 rows of 128 GB each for K and V):
  * row counts and the grid stay within 32 bits. */
-constexpr long kMaxRows = 1L << 27;
+constexpr long kMaxRows = 1L << 25;
 
 /* Every check of a ragged batch of rows, with nothing changed: sequence b's
  * rows are positions pos0[b] .. pos0[b] + n_tokens[b] - 1.  An append names
@@ -1035,7 +1036,8 @@ int launch_rows(q38_kv *kv, hipFunction_t f, int slot, int n_seq, const int32_t 
         }
         if (n == 0) break;
         a.n_seq = n;
-        if (kv->ctx->launch(f, (unsigned)a.page_base[n], 2, 1, 256, &a)) return -1;
+        for (int i = n + 1; i < Q38_MAX_BATCH + 8; ++i) a.page_base[i] = INT_MAX;
+        if (kv->ctx->launch(f, (unsigned)a.page_base[n], 2, 1, Q38_KV_ROWS_THREADS, &a)) return -1;
         row += (size_t)a.row_base[n];
     }
     return 0;

@@ -6,13 +6,23 @@
  * are, both converted to the cache's type once.  Gather is the inverse: the
  * values that the rows stand for as f32, or 16-bit rows as they are stored.
  *
- * A workgroup serves one page of one sequence, a wave per kv head; lane l of
- * a wave holds dims 4l .. 4l + 3 of the wave's head.
+ * Both move bytes: 4 KB of f32 a row and half or a quarter of that in the
+ * page.  A workgroup of 16 waves serves one page of one sequence; a wave has
+ * four tokens (a quad) of one kv head, lane l the dims 4l .. 4l + 3 of each.
+ * All its loads go out at once -- 16 waves a workgroup and two workgroups a
+ * CU keep the memory busy -- and the quad's part of the page is put together
+ * in the wave's own LDS, where the page's element order (q38_kv_layout.h)
+ * makes it 16-byte pieces: of one token for K, of all four for V.  The page's
+ * rotation angles are formed once per workgroup.
  */
 #include "q38_kv_types.h"
 #include "q38_rope.h"
 
 namespace {
+
+constexpr int kQuads = Q38_PAGE_TOKENS / 4;
+constexpr int kThreads = 64 * Q38_ATTN_KV_HEADS * kQuads;
+static_assert(kThreads == Q38_KV_ROWS_THREADS, "a wave per head and quad");
 
 struct PageSpan {
     int t0, t1;   /* tokens of the page, [t0, t1) */
@@ -22,8 +32,12 @@ struct PageSpan {
 };
 
 Q38_DEV PageSpan page_span(const q38_kv_rows_args &a, int x) {
+    /* the sequence that holds page x: entries past n_seq are INT_MAX, so eight
+     * are compared at a time, without a chain of dependent scalar loads */
     int b = 0;
-    while (b + 1 < a.n_seq && a.page_base[b + 1] <= x) ++b;
+    for (int i0 = 1; i0 < a.n_seq; i0 += 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b += a.page_base[i0 + i] <= x ? 1 : 0;
     const int first = a.pos0[b], n = a.row_base[b + 1] - a.row_base[b];
     const int lp = (first >> 4) + x - a.page_base[b];
     const int p0 = max(first, lp * Q38_PAGE_TOKENS);
@@ -32,82 +46,351 @@ Q38_DEV PageSpan page_span(const q38_kv_rows_args &a, int x) {
             a.page_table[(size_t)a.seq[b] * a.pt_stride + lp]};
 }
 
+/* LDS of one wave: a quad's elements in page order, 16-bit (2 KiB) or 8-bit. */
+typedef q38_u32x4 Stage[128];
+
+/* The lanes of a wave read what others of it wrote: LDS serves a wave in
+ * order, the fence keeps the compiler to it. */
+Q38_DEV void stage_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+/* Place of (token i of the quad, dim d) in a stage, in elements: the page's
+ * order with the other quads left out. */
 template <int T>
-Q38_DEV void store_row(char *block, bool key, int t, int lane, f32x4 x) {
-    if (T == Q38_KV_Q8) {
-        int q[4];
-        float scale;
-        q38_wave_q8k(x, q, scale);
-        uint8_t *out = reinterpret_cast<uint8_t *>(block);
-        if (lane == 0) q38_kv_scales(block)[t] = scale;
+Q38_DEV int stage_k(int i, int d) {
+    if (T == Q38_KV_Q8) return ((d >> 4) * 4 + i) * 16 + (d & 15);
+    return ((d >> 3) * 4 + i) * 8 + (d & 7);
+}
+template <int T>
+Q38_DEV int stage_v(int i, int d) {
+    if (T == Q38_KV_Q8) return ((d >> 6) * 16 + (d & 15)) * 16 + ((d >> 4) & 3) * 4 + i;
+    return ((d >> 5) * 16 + (d & 15)) * 8 + ((d >> 4) & 1) * 4 + i;
+}
+/* Piece p of a quad's stage in the block, in 16-byte pieces. */
+Q38_DEV int piece_at(bool key, int quad, int p) {
+    return key ? (p >> 2) * 16 + 4 * quad + (p & 3) : (p >> 4) * 64 + quad * 16 + (p & 15);
+}
+
+/* Four tokens' wave-wide sums or maxima at once: each step halves the values a
+ * lane still carries, so that lane l ends with token l % 4's, in 7 operations
+ * where four separate reductions take 24 -- and what follows (a division, a
+ * root) is done once for all four. */
+template <typename V, typename DPP1, typename DPP2, typename DPP4, typename DPP8, typename Join, typename Halves>
+Q38_DEV V quad_reduce(const V (&s)[4], int lane, DPP1 xor1, DPP2 xor2, DPP4 ror4, DPP8 ror8, Join join, Halves across) {
+    const bool b0 = lane & 1, b1 = lane & 2;
+    const V a = join(b0 ? s[1] : s[0], xor1(b0 ? s[0] : s[1]));
+    const V c = join(b0 ? s[3] : s[2], xor1(b0 ? s[2] : s[3]));
+    V r = join(b1 ? c : a, xor2(b1 ? a : c));
+    r = join(r, ror4(r));
+    r = join(r, ror8(r));
+    return across(r);
+}
+Q38_DEV double quad_sum_f64(const double (&s)[4], int lane) {
+    return quad_reduce(
+        s, lane, [](double x) { return q38_dpp_f64<0xB1>(x); }, [](double x) { return q38_dpp_f64<0x4E>(x); },
+        [](double x) { return q38_dpp_f64<0x124>(x); }, [](double x) { return q38_dpp_f64<0x128>(x); },
+        [](double x, double y) { return x + y; },
+        [](double x) {
+            uint64_t b = __builtin_bit_cast(uint64_t, x);
+            auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+            auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+            x = __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+            b = __builtin_bit_cast(uint64_t, x);
+            auto lo2 = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+            auto hi2 = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+            return __builtin_bit_cast(double, (uint64_t)hi2[0] << 32 | lo2[0]) +
+                   __builtin_bit_cast(double, (uint64_t)hi2[1] << 32 | lo2[1]);
+        });
+}
+Q38_DEV float quad_max(const float (&s)[4], int lane) {
+    return quad_reduce(
+        s, lane, [](float x) { return q38_dpp<0xB1>(x); }, [](float x) { return q38_dpp<0x4E>(x); },
+        [](float x) { return q38_dpp<0x124>(x); }, [](float x) { return q38_dpp<0x128>(x); },
+        [](float x, float y) { return fmaxf(x, y); },
+        [](float x) {
+            auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+            x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+            const q38_halves h = q38_both_halves(x);
+            return fmaxf(h.a, h.b);
+        });
+}
+/* Token i's value of one that lane l holds for token l % 4. */
+Q38_DEV float quad_value(float x, int i) {
+    return i == 0 ? q38_dpp<0x00>(x) : i == 1 ? q38_dpp<0x55>(x) : i == 2 ? q38_dpp<0xAA>(x) : q38_dpp<0xFF>(x);
+}
+
+/* RMSNorm and rotation of the quad's keys (q38_norm_rope4_cs, four at once).
+ * Every f32 square is exact in f64, so the fused sum is the plain one. */
+Q38_DEV void norm_rope_quad(f32x4 (&x)[4], f32x4 w, int lane, const float (*cs)[32][2], const int (&t)[4]) {
+    double ss[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int d = 4 * lane + c;
-            out[key ? q38_k_index<T>(t, d) : q38_v_index<T>(t, d)] = (uint8_t)(q[c] + 128);
+    for (int i = 0; i < 4; ++i) {
+        ss[i] = (double)x[i].x * (double)x[i].x;
+#pragma unroll
+        for (int c = 1; c < 4; ++c) ss[i] = __builtin_fma((double)x[i][c], (double)x[i][c], ss[i]);
+    }
+    const float scale = q38_rms_scale_of(quad_sum_f64(ss, lane));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[i] = x[i] * quad_value(scale, i) * w;
+        /* lanes 0-7 hold dims 0 .. 31, lanes 8-15 their partners 32 .. 63 */
+        f32x4 partner;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) partner[c] = q38_dpp<0x128>(x[i][c]);
+        if (lane < 16) {
+            const f32x4 *p = reinterpret_cast<const f32x4 *>(&cs[t[i]][4 * (lane & 7)][0]);
+            const f32x4 p0 = p[0], p1 = p[1];
+            const float cosine[4] = {p0[0], p0[2], p1[0], p1[2]}, sine[4] = {p0[1], p0[3], p1[1], p1[3]};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float own = x[i][c] * cosine[c], other = partner[c] * sine[c];
+                x[i][c] = lane < 8 ? own - other : other + own;
+            }
         }
+    }
+}
+
+/* The quad's Q8_K blocks (q38_wave_q8k, four at once): quants + 128 packed,
+ * and in lane l token l % 4's scale. */
+Q38_DEV float q8k_quad(const f32x4 (&x)[4], int lane, uint32_t (&b)[4]) {
+    float up[4], down[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        up[i] = fmaxf(fmaxf(x[i].x, x[i].y), fmaxf(x[i].z, x[i].w));
+        down[i] = fmaxf(fmaxf(-x[i].x, -x[i].y), fmaxf(-x[i].z, -x[i].w));
+    }
+    const float pos = quad_max(up, lane), neg = quad_max(down, lane);
+    float m = pos > neg ? pos : -neg;
+    if (__any(pos == neg && pos != 0.0f)) {
+        /* the largest size with both signs: the first value of it decides */
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float big = quad_value(pos, i);
+            const f32x4 v = x[i];
+            const bool mine = fabsf(v.x) == big || fabsf(v.y) == big || fabsf(v.z) == big || fabsf(v.w) == big;
+            const float cand = fabsf(v.x) == big ? v.x : fabsf(v.y) == big ? v.y : fabsf(v.z) == big ? v.z : v.w;
+            const uint64_t holders = __ballot(mine);
+            const float at = __uint_as_float(
+                __builtin_amdgcn_readlane(__float_as_uint(cand), holders ? __builtin_ctzll(holders) : 0));
+            if ((lane & 3) == i && pos == neg) m = at;
+        }
+    }
+    const bool zero = pos == 0.0f && neg == 0.0f;
+    const float inverse = zero ? 0.0f : -127.0f / m;
+    const float scale = zero ? 0.0f : 1.0f / inverse;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float inv = quad_value(inverse, i);
+        uint32_t q[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) q[c] = (uint32_t)(min(q38_nearest_int(inv * x[i][c]), 127) + 128);
+        b[i] = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
+    }
+    return scale;
+}
+
+template <int T>
+Q38_DEV void store_quad(char *block, Stage &stage, bool key, int quad, int first, int last, int lane, const f32x4 (&x)[4]) {
+    /* tokens first .. last - 1 of the quad are the batch's */
+    if (T == Q38_KV_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i >= first && i < last)
+                q38_st4(reinterpret_cast<float *>(block) + q38_k_index<T>(4 * quad + i, 4 * lane), x[i]);
         return;
     }
+    uint32_t b[4][T == Q38_KV_Q8 ? 1 : 2]; /* token i's four elements */
+    if (T == Q38_KV_Q8) {
+        uint32_t q[4];
+        const float scale = q8k_quad(x, lane, q);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const int d = 4 * lane + c;
-        const int i = key ? q38_k_index<T>(t, d) : q38_v_index<T>(t, d);
-        if (T == Q38_KV_F32)
-            reinterpret_cast<float *>(block)[i] = x[c];
-        else
-            reinterpret_cast<uint16_t *>(block)[i] = q38_to16<T>(x[c]);
+        for (int i = 0; i < 4; ++i) b[i][0] = q[i];
+        if (lane >= first && lane < last) q38_kv_scales(block)[4 * quad + lane] = scale;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                b[i][T == Q38_KV_Q8 ? 0 : h] =
+                    (uint32_t)q38_to16<T>(x[i][2 * h]) | (uint32_t)q38_to16<T>(x[i][2 * h + 1]) << 16;
+    }
+    constexpr int kPieces = T == Q38_KV_Q8 ? 64 : 128;
+    q38_u32x4 *out = reinterpret_cast<q38_u32x4 *>(block);
+    if (key) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t *at = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(stage) +
+                                                        stage_k<T>(i, 4 * lane) * (T == Q38_KV_Q8 ? 1 : 2));
+            at[0] = b[i][0];
+            if (T != Q38_KV_Q8) at[1] = b[i][T == Q38_KV_Q8 ? 0 : 1];
+        }
+        stage_fence();
+#pragma unroll
+        for (int p = lane; p < kPieces; p += 64)
+            if ((p & 3) >= first && (p & 3) < last) out[piece_at(true, quad, p)] = stage[p];
+        return;
+    }
+    /* the four tokens of each dim side by side */
+    if (first == 0 && last == 4) {
+        if (T == Q38_KV_Q8) {
+            const uint32_t lo = __builtin_amdgcn_perm(b[1][0], b[0][0], 0x05010400u); /* dims 0, 1 of tokens 0, 1 */
+            const uint32_t hi = __builtin_amdgcn_perm(b[1][0], b[0][0], 0x07030602u); /* dims 2, 3 */
+            const uint32_t lo2 = __builtin_amdgcn_perm(b[3][0], b[2][0], 0x05010400u);
+            const uint32_t hi2 = __builtin_amdgcn_perm(b[3][0], b[2][0], 0x07030602u);
+            const uint32_t w[4] = {__builtin_amdgcn_perm(lo2, lo, 0x05040100u), __builtin_amdgcn_perm(lo2, lo, 0x07060302u),
+                                   __builtin_amdgcn_perm(hi2, hi, 0x05040100u), __builtin_amdgcn_perm(hi2, hi, 0x07060302u)};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                *reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(stage) + stage_v<T>(0, 4 * lane + c)) = w[c];
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int h = T == Q38_KV_Q8 ? 0 : c >> 1;
+                const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;
+                q38_u32x2 w = {__builtin_amdgcn_perm(b[1][h], b[0][h], sel), __builtin_amdgcn_perm(b[3][h], b[2][h], sel)};
+                *reinterpret_cast<q38_u32x2 *>(reinterpret_cast<char *>(stage) + 2 * stage_v<T>(0, 4 * lane + c)) = w;
+            }
+        }
+        stage_fence();
+#pragma unroll
+        for (int p = lane; p < kPieces; p += 64) out[piece_at(false, quad, p)] = stage[p];
+        return;
+    }
+    /* a quad that the batch holds in part: its own elements only */
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (i < first || i >= last) continue;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int at = q38_v_index<T>(4 * quad + i, 4 * lane + c);
+            if (T == Q38_KV_Q8)
+                reinterpret_cast<uint8_t *>(block)[at] = (uint8_t)(b[i][0] >> (8 * c));
+            else
+                reinterpret_cast<uint16_t *>(block)[at] = (uint16_t)(b[i][T == Q38_KV_Q8 ? 0 : c >> 1] >> (16 * (c & 1)));
+        }
     }
 }
 
 template <int T>
 Q38_DEV void kv_append(const q38_kv_rows_args &a) {
-    __shared__ float cs[Q38_PAGE_TOKENS][32][2];
+    __shared__ __attribute__((aligned(16))) float cs[Q38_PAGE_TOKENS][32][2];
+    __shared__ Stage stages[T == Q38_KV_F32 ? 1 : kThreads / 64];
     const PageSpan sp = page_span(a, blockIdx.x);
     const bool key = blockIdx.y == 0;
-    const int lane = threadIdx.x & 63, head = threadIdx.x >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int head = wave & 3, quad = wave >> 2;
     const bool turns = key && a.k_norm != nullptr;
+    const int first = max(sp.t0 - 4 * quad, 0), last = min(sp.t1 - 4 * quad, 4);
+    const bool live = first < last;
+    const float *rows = static_cast<const float *>(key ? a.k_rows : a.v_rows) +
+                        (size_t)sp.row0 * Q38_ATTN_KV_DIM + head * Q38_ATTN_HEAD_DIM + 4 * lane;
+    f32x4 x[4], w = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+        /* a token that is not the batch's loads a neighbour's row, and is not stored */
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            x[i] = q38_ld4_stream(rows + (size_t)(4 * quad + min(max(i, first), last - 1) - sp.t0) * Q38_ATTN_KV_DIM);
+        if (turns) w = q38_ld4(a.k_norm + 4 * lane);
+    }
     if (turns) {
         /* the page's angles: a half-wave per token */
-        for (int t = sp.t0 + (int)(threadIdx.x >> 5); t < sp.t1; t += 8)
-            q38_rope_table(cs[t], lane & 31, sp.pos0 + t - sp.t0, a.theta_scale);
+        const int t = tid >> 5;
+        if (t >= sp.t0 && t < sp.t1) q38_rope_table(cs[t], lane & 31, sp.pos0 + t - sp.t0, a.theta_scale);
         __syncthreads();
     }
-    const float *rows = static_cast<const float *>(key ? a.k_rows : a.v_rows);
-    char *block = q38_kv_block<T>(key ? a.kpool : a.vpool, sp.page, head);
-    const f32x4 w = turns ? q38_ld4(a.k_norm + 4 * lane) : f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int t = sp.t0; t < sp.t1; ++t) {
-        f32x4 x = q38_ld4(rows + (size_t)(sp.row0 + t - sp.t0) * Q38_ATTN_KV_DIM + head * Q38_ATTN_HEAD_DIM + 4 * lane);
-        if (turns) q38_norm_rope4_cs(x, w, lane, cs[t]);
-        store_row<T>(block, key, t, lane, x);
+    if (!live) return;
+    if (turns) {
+        int t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = 4 * quad + min(max(i, first), last - 1);
+        norm_rope_quad(x, w, lane, cs, t);
     }
+    store_quad<T>(q38_kv_block<T>(key ? a.kpool : a.vpool, sp.page, head), stages[T == Q38_KV_F32 ? 0 : wave], key, quad,
+                  first, last, lane, x);
 }
 
-template <int T, bool k16>
+/* OUT16: rows in the cache's 16 bits, moved as they are (T is BF16 for both). */
+template <int T, bool OUT16>
 Q38_DEV void kv_gather(const q38_kv_rows_args &a) {
+    __shared__ Stage stages[T == Q38_KV_F32 ? 1 : kThreads / 64];
     const PageSpan sp = page_span(a, blockIdx.x);
     const bool key = blockIdx.y == 0;
-    const int lane = threadIdx.x & 63, head = threadIdx.x >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int head = wave & 3, quad = wave >> 2;
+    const int first = max(sp.t0 - 4 * quad, 0), last = min(sp.t1 - 4 * quad, 4);
+    if (first >= last) return;
     char *block = q38_kv_block<T>(key ? a.kpool : a.vpool, sp.page, head);
+    const size_t row = (size_t)(sp.row0 + 4 * quad - sp.t0) * Q38_ATTN_KV_DIM + head * Q38_ATTN_HEAD_DIM + 4 * lane;
     void *rows = key ? a.k_rows : a.v_rows;
-    for (int t = sp.t0; t < sp.t1; ++t) {
-        const size_t at = (size_t)(sp.row0 + t - sp.t0) * Q38_ATTN_KV_DIM + head * Q38_ATTN_HEAD_DIM + 4 * lane;
+    f32x4 x[4];
+    q38_u32x2 raw[4];
+    if (T == Q38_KV_F32) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int d = 4 * lane + c;
-            const int i = key ? q38_k_index<T>(t, d) : q38_v_index<T>(t, d);
-            if (k16)
-                static_cast<uint16_t *>(rows)[at + c] = reinterpret_cast<const uint16_t *>(block)[i];
-            else
-                static_cast<float *>(rows)[at + c] = q38_kv_value<T>(block, i, t);
+        for (int i = 0; i < 4; ++i)
+            x[i] = q38_ld4(reinterpret_cast<const float *>(block) + q38_k_index<T>(4 * quad + i, 4 * lane));
+    } else {
+        constexpr int kPieces = T == Q38_KV_Q8 ? 64 : 128;
+        q38_u32x4 *stage = stages[T == Q38_KV_F32 ? 0 : wave];
+        const q38_u32x4 *in = reinterpret_cast<const q38_u32x4 *>(block);
+        q38_u32x4 piece[kPieces / 64];
+        f32x4 scale = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kPieces / 64; ++k) piece[k] = in[piece_at(key, quad, lane + 64 * k)];
+        if (T == Q38_KV_Q8) scale = q38_ld4(q38_kv_scales(block) + 4 * quad);
+#pragma unroll
+        for (int k = 0; k < kPieces / 64; ++k) stage[lane + 64 * k] = piece[k];
+        stage_fence();
+        const char *at = reinterpret_cast<const char *>(stage);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t e[4]; /* the token's four elements */
+            if (key) {
+                if (T == Q38_KV_Q8) {
+                    const uint32_t u = *reinterpret_cast<const uint32_t *>(at + stage_k<T>(i, 4 * lane));
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) e[c] = (u >> (8 * c)) & 255u;
+                } else {
+                    const q38_u32x2 u = *reinterpret_cast<const q38_u32x2 *>(at + 2 * stage_k<T>(i, 4 * lane));
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) e[c] = (u[c >> 1] >> (16 * (c & 1))) & 0xFFFFu;
+                }
+            } else {
+                /* the dim's four tokens in one read; the compiler keeps it for all i */
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (T == Q38_KV_Q8) {
+                        const uint32_t u = *reinterpret_cast<const uint32_t *>(at + stage_v<T>(0, 4 * lane + c));
+                        e[c] = (u >> (8 * i)) & 255u;
+                    } else {
+                        const q38_u32x2 u = *reinterpret_cast<const q38_u32x2 *>(at + 2 * stage_v<T>(0, 4 * lane + c));
+                        e[c] = (u[i >> 1] >> (16 * (i & 1))) & 0xFFFFu;
+                    }
+                }
+            }
+            raw[i] = q38_u32x2{e[0] | e[1] << 16, e[2] | e[3] << 16};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                x[i][c] = T == Q38_KV_Q8 ? (float)((int)e[c] - 128) * scale[i] : q38_from16<T>((uint16_t)e[c]);
         }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (i < first || i >= last) continue;
+        if (OUT16)
+            *reinterpret_cast<q38_u32x2 *>(static_cast<uint16_t *>(rows) + row + (size_t)i * Q38_ATTN_KV_DIM) = raw[i];
+        else
+            q38_st4(static_cast<float *>(rows) + row + (size_t)i * Q38_ATTN_KV_DIM, x[i]);
     }
 }
 
 }  // namespace
 
-#define Q38_KV_ROWS_KERNELS(name, T)                                                                        \
-    extern "C" __global__ __launch_bounds__(256) void q38_kv_append_##name(q38_kv_rows_args a) { kv_append<T>(a); } \
-    extern "C" __global__ __launch_bounds__(256) void q38_kv_gather_##name(q38_kv_rows_args a) {            \
-        kv_gather<T, false>(a);                                                                             \
+#define Q38_KV_ROWS_KERNELS(name, T)                                                                             \
+    extern "C" __global__ __launch_bounds__(kThreads) void q38_kv_append_##name(q38_kv_rows_args a) { kv_append<T>(a); } \
+    extern "C" __global__ __launch_bounds__(kThreads) void q38_kv_gather_##name(q38_kv_rows_args a) {            \
+        kv_gather<T, false>(a);                                                                                  \
     }
 Q38_KV_ROWS_KERNELS(f32, Q38_KV_F32)
 Q38_KV_ROWS_KERNELS(f16, Q38_KV_F16)
@@ -115,6 +398,6 @@ Q38_KV_ROWS_KERNELS(bf16, Q38_KV_BF16)
 Q38_KV_ROWS_KERNELS(q8k, Q38_KV_Q8)
 
 /* 16-bit rows as they are stored, F16 or BF16. */
-extern "C" __global__ __launch_bounds__(256) void q38_kv_gather_16(q38_kv_rows_args a) {
+extern "C" __global__ __launch_bounds__(kThreads) void q38_kv_gather_16(q38_kv_rows_args a) {
     kv_gather<Q38_KV_BF16, true>(a);
 }

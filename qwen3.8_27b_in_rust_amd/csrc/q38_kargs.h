@@ -95,7 +95,10 @@ typedef struct {
  * row_base[b] + i is position pos0[b] + i of sequence seq[b].  grid
  * (page_base[n_seq], 2): workgroup x serves one page of one sequence -- page
  * pos0[b] / 16 + x - page_base[b] of the sequence b that holds x -- and y = 0
- * moves K, y = 1 moves V; 256 threads, a wave per kv head. */
+ * moves K, y = 1 moves V; Q38_KV_ROWS_THREADS threads, a wave per kv head and
+ * four tokens.  page_base past n_seq holds INT_MAX (the sequence of a page is
+ * found eight entries at a time). */
+#define Q38_KV_ROWS_THREADS 1024
 typedef struct {
     void *kpool;
     void *vpool;
@@ -110,7 +113,7 @@ typedef struct {
     int32_t seq[Q38_MAX_BATCH];
     int32_t pos0[Q38_MAX_BATCH];
     int32_t row_base[Q38_MAX_BATCH + 1];
-    int32_t page_base[Q38_MAX_BATCH + 1];
+    int32_t page_base[Q38_MAX_BATCH + 8];
 } q38_kv_rows_args;
 
 /* q/gate split, q and k RMSNorm, RoPE.  grid (n_tokens, 28): y < 24 is a

@@ -24,7 +24,7 @@ static std::vector<unsigned> g_grid;
 static hipError_t check_launch(hipFunction_t, unsigned gx, unsigned gy, unsigned, unsigned block, unsigned, unsigned,
                                unsigned, hipStream_t, void **params, void **) {
     ++g_launches;
-    if (gy != 2 || block != 256) { printf("unexpected grid\n"); exit(1); }
+    if (gy != 2 || block != Q38_KV_ROWS_THREADS) { printf("unexpected grid\n"); exit(1); }
     const char *p = static_cast<const char *>(params[0]);
     g_args.emplace_back(p, p + sizeof(q38_kv_rows_args));
     g_grid.push_back(gx);
@@ -109,7 +109,10 @@ static void walk(const Cache &c, int slot, const std::vector<int32_t> &seq, cons
         REQUIRE(row_off == (size_t)(static_cast<char *>(a.v_rows) - d_v) / (1024 * elem));
         for (unsigned x = 0; x < g_grid[l]; ++x) {
             int b = 0;
-            while (b + 1 < a.n_seq && a.page_base[b + 1] <= (int)x) ++b;
+            for (int i0 = 1; i0 < a.n_seq; i0 += 8)
+                for (int i = 0; i < 8; ++i) b += a.page_base[i0 + i] <= (int)x ? 1 : 0;
+            REQUIRE(((a.n_seq - 2) / 8) * 8 + 8 < Q38_MAX_BATCH + 8);
+            REQUIRE(b < a.n_seq && a.page_base[b] <= (int)x && (int)x < a.page_base[b + 1]);
             const int first = a.pos0[b], n = a.row_base[b + 1] - a.row_base[b];
             const int lp = (first >> 4) + (int)x - a.page_base[b];
             const int p0 = std::max(first, lp * 16), p1 = std::min(first + n, (lp + 1) * 16);
