@@ -123,19 +123,18 @@ constexpr GemvType kGemv[] = {
     {Q38_GGML_IQ1_M, "q38_gemv_q8k_iq1m", "q38_gemm_q8k_iq1m", "q38_gemm_ks_q8k_iq1m", "q38_gemm_ks16_q8k_iq1m", "q38_gemm_ks4_q8k_iq1m", nullptr, 1, 2048 * 8, 0.0, 0.0},
 };
 constexpr int kGemvTypes = (int)(sizeof(kGemv) / sizeof(kGemv[0]));
-/* Row types of a KV cache: the bytes of a page's block (one kv head's 16
- * tokens), and the suffix of the kernels that read and write it.  Index 0 is
+/* Row types of a KV cache: the bytes of a page, and the suffix of the kernels that read and write it.  Index 0 is
  * the f32 cache. */
 struct KvType {
     int ggml_type;
-    size_t block_bytes;
+    size_t page_bytes;
     const char *suffix;
 };
 constexpr KvType kKvTypes[] = {
-    {Q38_GGML_F32, Q38_KV_BLOCK_F32, "f32"},
-    {Q38_GGML_F16, Q38_KV_BLOCK_16, "f16"},
-    {Q38_GGML_BF16, Q38_KV_BLOCK_16, "bf16"},
-    {Q38_GGML_Q8_K, Q38_KV_BLOCK_Q8, "q8k"},
+    {Q38_GGML_F32, Q38_KV_PAGE_F32, "f32"},
+    {Q38_GGML_F16, Q38_KV_PAGE_16, "f16"},
+    {Q38_GGML_BF16, Q38_KV_PAGE_16, "bf16"},
+    {Q38_GGML_Q8_K, Q38_KV_PAGE_Q8, "q8k"},
 };
 constexpr int kKvTypeCount = (int)(sizeof(kKvTypes) / sizeof(kKvTypes[0]));
 /* q38_add_rms_norm's kernels that hold a row in registers: 256 or 1024
@@ -338,7 +337,7 @@ struct q38_kv {
     }
 
     /* a slot's pages; a typed cache's kernels read them as bytes */
-    size_t slot_bytes() const { return (size_t)max_pages * Q38_ATTN_KV_HEADS * kKvTypes[type].block_bytes; }
+    size_t slot_bytes() const { return (size_t)max_pages * kKvTypes[type].page_bytes; }
     float *slot_of_pool(float *pool, int slot) const {
         return reinterpret_cast<float *>(reinterpret_cast<char *>(pool) + (size_t)slot * slot_bytes());
     }
@@ -1172,13 +1171,48 @@ struct decode_plan {
     size_t work_bytes = 0;
 };
 
-int plan_decode(const q38_ctx *ctx, int n_seq, const int32_t *positions, decode_plan *plan) {
+/* Tokens per split over 16- or 8-bit rows (unless q38_set_decode_split fixed
+ * it).  A workgroup there costs as much as streaming some hundreds of tokens
+ * before its first and after its last page, and a CU holds one at a time, so
+ * few rounds of large splits win: the fewest rounds that splits of at most
+ * Q38_MAX_SPLIT_TOKENS allow, and the smallest split that fits them.  Measured
+ * against one workgroup per CU by the total but at most 1024 tokens for batches,
+ * as over f32 rows (us, Q8_K): 3 sequences of 2K-32K 22.7 against 33.6, 24 of
+ * 200-3000 20.8 against 30.0, 16 of 2K-32K 69.8 against 78.1, 64 of 100-20000
+ * 230 against 278.  Where every sequence has kOneSplitTokens at most, one split
+ * each needs no merge launch: one sequence of 17 / 128 / 256 tokens 6.6 / 7.6 /
+ * 8.9 against 9.6 / 9.8 / 10.0 (512: 11.6 against 10.2). */
+constexpr int kOneSplitTokens = 256;
+int typed_split_tokens(const q38_ctx *ctx, int n_seq, const int32_t *positions, long max_tokens) {
+    if (max_tokens <= kOneSplitTokens) return kOneSplitTokens;
+    auto splits = [&](long split) {
+        long n = 0;
+        for (int b = 0; b < n_seq; ++b) n += (positions[b] + split) / split; /* ceil((pos+1)/split) */
+        return n;
+    };
+    const long slots = std::max(ctx->cu_count / Q38_ATTN_KV_HEADS, 1);
+    const long rounds = (splits(Q38_MAX_SPLIT_TOKENS) + slots - 1) / slots;
+    long lo = 1, hi = Q38_MAX_SPLIT_TOKENS / Q38_PAGE_TOKENS; /* pages */
+    while (lo < hi) {
+        const long mid = (lo + hi) / 2;
+        if (splits(mid * Q38_PAGE_TOKENS) <= rounds * slots)
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    return (int)(lo * Q38_PAGE_TOKENS);
+}
+
+int plan_decode(const q38_ctx *ctx, bool typed, int n_seq, const int32_t *positions, decode_plan *plan) {
     long total_tokens = 0, max_tokens = 0;
     for (int b = 0; b < n_seq; ++b) {
         total_tokens += positions[b] + 1;
         max_tokens = std::max<long>(max_tokens, positions[b] + 1);
     }
-    if (choose_split_tokens(ctx, n_seq, total_tokens, max_tokens, &plan->split_tokens)) return -1;
+    if (typed && ctx->split_tokens == 0)
+        plan->split_tokens = typed_split_tokens(ctx, n_seq, positions, max_tokens);
+    else if (choose_split_tokens(ctx, n_seq, total_tokens, max_tokens, &plan->split_tokens))
+        return -1;
     int total = 0;
     bool any_multi = false;
     for (int b = 0; b < n_seq; ++b) {
@@ -1250,6 +1284,7 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
         total += (positions[b] + split_tokens) / split_tokens; /* ceil((pos+1)/split) */
     }
     a.split_base[n_seq] = total;
+    for (int b = n_seq + 1; b < Q38_MAX_BATCH + 8; ++b) a.split_base[b] = INT_MAX;
     a.total_splits = total;
     /* up to 256 splits, each split's first two page ids ride in the launch
      * arguments (from the host mirror of the page table), so the kernel's
@@ -1364,7 +1399,7 @@ int decode_all(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const i
     size_t work_bytes = 0;
     for (int b0 = 0; b0 < n_seq; b0 += Q38_MAX_BATCH) {
         decode_plan plan;
-        if (plan_decode(ctx, std::min(Q38_MAX_BATCH, n_seq - b0), positions + b0, &plan)) return -1;
+        if (plan_decode(ctx, kv->type != 0, std::min(Q38_MAX_BATCH, n_seq - b0), positions + b0, &plan)) return -1;
         work_bytes = std::max(work_bytes, plan.work_bytes);
     }
     void *work = nullptr;
@@ -1386,7 +1421,7 @@ int decode_all(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const i
     for (int b0 = 0; b0 < n_seq; b0 += Q38_MAX_BATCH) {
         const int n = std::min(Q38_MAX_BATCH, n_seq - b0);
         decode_plan plan;
-        if (plan_decode(ctx, n, positions + b0, &plan)) return -1;
+        if (plan_decode(ctx, kv->type != 0, n, positions + b0, &plan)) return -1;
         const size_t kvoff = (size_t)b0 * Q38_ATTN_KV_DIM;
         const size_t qoff = (size_t)b0 * Q38_ATTN_Q_DIM;
         if (decode_chunk(kv, slot, n, seq_ids + b0, positions + b0, d_q + (size_t)b0 * q_rows,
@@ -1498,7 +1533,7 @@ struct q38_decode_graph {
     /* The split-K workspace for `pos`, grown only while no replay runs
      * (the caller's stream has been waited for). */
     int ensure_work(const int32_t *pos, decode_plan *plan) {
-        if (plan_decode(kv->ctx, n_seq, pos, plan)) return -1;
+        if (plan_decode(kv->ctx, kv->type != 0, n_seq, pos, plan)) return -1;
         if (arg_pages && plan->total_splits > Q38_HEAD_PAGE_SPLITS)
             return fail("%d splits: this graph's split kernel takes at most %d", plan->total_splits,
                         Q38_HEAD_PAGE_SPLITS);

@@ -56,21 +56,31 @@ struct Page {
     f32x4 ks, vs; /* 8-bit rows: the scales of tokens 4 (lane / 16) .. + 3 */
 };
 
-Q38_DEV q38_u32x4 ld_stream(const char *p) {
-    return __builtin_nontemporal_load(reinterpret_cast<const q38_u32x4 *>(p));
+/* Loads of a page's block go through a buffer resource that ends with it (8-bit
+ * rows: with its scales), or of no size at all: past the wave's last page they fetch nothing, without a branch
+ * that would make the compiler wait for every load before it. */
+Q38_DEV __amdgpu_buffer_rsrc_t block_rsrc(char *block, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(block, 0, bytes, 0x00027000);
+}
+Q38_DEV q38_u32x4 ld_block(__amdgpu_buffer_rsrc_t r, int at) {
+    constexpr int kStream = 2; /* non-temporal */
+    return __builtin_bit_cast(q38_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, kStream));
 }
 
 template <int T>
-Q38_DEV void load_page(Page<T> &p, const q38_decode_args &a, int page, int j, int lane) {
-    const char *kb = q38_kv_block<T>(a.kpool, page, j), *vb = q38_kv_block<T>(a.vpool, page, j);
+Q38_DEV void load_page(Page<T> &p, const q38_decode_args &a, int page, bool live, int j, int lane) {
+    const int scales = q38_kv_scales_offset(j);
+    const int bytes = !live ? 0 : T == Q38_KV_Q8 ? scales + Q38_PAGE_TOKENS * 4 : q38_kv_block_bytes<T>();
+    const __amdgpu_buffer_rsrc_t k = block_rsrc(q38_kv_block<T>(a.kpool, page, j), bytes);
+    const __amdgpu_buffer_rsrc_t v = block_rsrc(q38_kv_block<T>(a.vpool, page, j), bytes);
 #pragma unroll
-    for (int i = 0; i < Page<T>::kLoads; ++i) p.k[i] = ld_stream(kb + 1024 * i + 16 * lane);
+    for (int i = 0; i < Page<T>::kLoads; ++i) p.k[i] = ld_block(k, 1024 * i + 16 * lane);
     if (T == Q38_KV_Q8) {
-        p.ks = *reinterpret_cast<const f32x4 *>(kb + 4096 + 16 * (lane >> 4));
-        p.vs = *reinterpret_cast<const f32x4 *>(vb + 4096 + 16 * (lane >> 4));
+        p.ks = __builtin_bit_cast(f32x4, ld_block(k, scales + 16 * (lane >> 4)));
+        p.vs = __builtin_bit_cast(f32x4, ld_block(v, scales + 16 * (lane >> 4)));
     }
 #pragma unroll
-    for (int i = 0; i < Page<T>::kLoads; ++i) p.v[i] = ld_stream(vb + 1024 * i + 16 * lane);
+    for (int i = 0; i < Page<T>::kLoads; ++i) p.v[i] = ld_block(v, 1024 * i + 16 * lane);
 }
 
 /* Two biased bytes of u as two halves: 0x6400 | b is 1024 + b, and 1152 less
@@ -125,14 +135,14 @@ Q38_DEV uint32_t pack16(uint16_t lo, uint16_t hi) { return (uint32_t)hi << 16 | 
  * values.  valid: tokens of the page that count (16 but for the sequence's
  * last page). */
 template <int T>
-Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (&q)[8], const q38_u32x4 (*q2)[64], float unscale,
-                       int valid, int lane) {
+Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64], float unscale, int valid, int lane) {
     const int c = lane & 15, g = lane >> 4;
     f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
-    /* bf16's third part is read from LDS at every page (an index that the
-     * compiler cannot see through keeps it from 32 registers of the loop's) */
+    /* the queries are read from LDS at every page: an index that the compiler
+     * cannot see through keeps it from holding them in registers, 32 a part,
+     * which the pages in flight need (8-bit pages leave room) */
     int ql = lane;
-    if (T == Q38_KV_BF16) asm volatile("" : "+v"(ql));
+    if (T != Q38_KV_Q8) asm volatile("" : "+v"(ql));
     if (T == Q38_KV_Q8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -141,15 +151,15 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (&q)[8], con
                                  halves_of<0x04030402u>(u[1])};
             const q38_u32x4 b = {halves_of<0x04010400u>(u[2]), halves_of<0x04030402u>(u[2]), halves_of<0x04010400u>(u[3]),
                                  halves_of<0x04030402u>(u[3])};
-            s0 = mma_k<T>(a, q[2 * i], s0);
-            s1 = mma_k<T>(b, q[2 * i + 1], s1);
+            s0 = mma_k<T>(a, q[0][2 * i][ql], s0);
+            s1 = mma_k<T>(b, q[0][2 * i + 1][ql], s1);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             f32x4 &s = T == Q38_KV_F16 && (i & 1) ? s1 : s0;
-            s = mma_k<T>(p.k[i], q[i], s);
-            if (T == Q38_KV_BF16) s1 = mma_k<T>(p.k[i], q2[i][ql], s1);
+            s = mma_k<T>(p.k[i], q[0][i][ql], s);
+            if (T == Q38_KV_BF16) s1 = mma_k<T>(p.k[i], q[1][i][ql], s1);
         }
     }
     float s[4];
@@ -255,15 +265,98 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (&q)[8], con
     }
 }
 
+/* The new token's rows in LDS as they are stored: the key's elements in order
+ * of dims, the value's so that a lane's (dim 16 n + c for each tile n of one
+ * load) lie in one word. */
+struct NewRows {
+    uint32_t k[Q38_ATTN_HEAD_DIM / 2], v[Q38_ATTN_HEAD_DIM / 2]; /* 16-bit elements, or bytes */
+    float scale[2];
+};
+template <int T>
+Q38_DEV int new_value_index(int d) {
+    return T == Q38_KV_Q8 ? (d >> 6) * 64 + (d & 15) * 4 + ((d >> 4) & 3) : (d >> 5) * 32 + (d & 15) * 2 + ((d >> 4) & 1);
+}
+
+/* They take the place of token t in what the page held. */
+template <int T>
+Q38_DEV void put_new_token(Page<T> &p, const NewRows &row, int t, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    const bool key_lane = c == t, value_lane = g == (t >> 2);
+    constexpr uint32_t kKeep = 0x07060504u; /* a word's own bytes */
+#pragma unroll
+    for (int s = 0; s < Page<T>::kLoads; ++s) {
+        const q38_u32x4 kw = *reinterpret_cast<const q38_u32x4 *>(row.k + (s * 4 + g) * 4);
+        if (key_lane) p.k[s] = kw;
+        const uint32_t vw = row.v[s * 16 + c];
+        if (T == Q38_KV_Q8) {
+            const uint32_t sh = 8 * (t & 3);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t sel = (kKeep & ~(255u << sh)) | (uint32_t)w << sh;
+                p.v[s][w] = __builtin_amdgcn_perm(p.v[s][w], vw, value_lane ? sel : kKeep);
+            }
+        } else {
+            const uint32_t sh = 16 * (t & 1);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t sel = (kKeep & ~(0xFFFFu << sh)) | (w < 2 ? 0x0100u : 0x0302u) << sh;
+                p.v[s][w] = __builtin_amdgcn_perm(p.v[s][w], vw, value_lane && ((t >> 1) & 1) == (w & 1) ? sel : kKeep);
+            }
+        }
+    }
+    if (T == Q38_KV_Q8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (value_lane && (t & 3) == e) p.ks[e] = row.scale[0], p.vs[e] = row.scale[1];
+    }
+}
+
+/* Workgroup barrier for LDS alone: loads of pages stay in flight across it
+ * (__syncthreads() would wait for them). */
+Q38_DEV void lds_barrier() { q38_barrier_vm<63>(); }
+
+/* Dims 4 lane .. + 3 of column c's (and c + 8's) parts to the query operands:
+ * operand i, lane 16 g + c holds the 8 dims that k step i's group g takes. */
+template <int T>
+Q38_DEV void store_query(q38_u32x4 (*q)[8][64], int c, int lane, f32x4 x) {
+    const int d = 4 * lane;
+    const int i = T == Q38_KV_Q8 ? 2 * (d >> 6) + ((d >> 3) & 1) : d >> 5;
+    const int g = T == Q38_KV_Q8 ? (d >> 4) & 3 : (d >> 3) & 3;
+    auto put = [&](int set, int col, const uint16_t (&e)[4]) {
+        q38_u32x2 *at = reinterpret_cast<q38_u32x2 *>(&q[set][i][16 * g + col]) + ((d >> 2) & 1);
+        *at = q38_u32x2{pack16(e[0], e[1]), pack16(e[2], e[3])};
+    };
+    uint16_t a[4], b[4], third[4], none[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (T == Q38_KV_BF16) {
+            const uint32_t hi = __float_as_uint(x[e]) & 0xFFFF0000u;
+            const float r = x[e] - __uint_as_float(hi);
+            const uint32_t mid = __float_as_uint(r) & 0xFFFF0000u;
+            a[e] = (uint16_t)(hi >> 16);
+            b[e] = (uint16_t)(mid >> 16);
+            third[e] = (uint16_t)(__float_as_uint(r - __uint_as_float(mid)) >> 16);
+        } else {
+            const _Float16 hi = (_Float16)x[e];
+            a[e] = __builtin_bit_cast(uint16_t, hi);
+            b[e] = __builtin_bit_cast(uint16_t, (_Float16)(x[e] - (float)hi));
+        }
+    }
+    put(0, c, a);
+    put(0, c + 8, b);
+    if (T == Q38_KV_BF16) {
+        put(1, c, third);
+        put(1, c + 8, none);
+    }
+}
+
 template <int T, bool kPre>
 Q38_DEV void decode_typed(const q38_decode_args &a) {
     constexpr int kQSets = T == Q38_KV_BF16 ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) float q_rows[8][Q38_ATTN_HEAD_DIM];
+    constexpr int kDepth = T == Q38_KV_Q8 ? 2 : 1; /* pages of a wave in registers */
     __shared__ q38_u32x4 q_frag[kQSets][8][64];
     __shared__ float q_unscale[8];
-    /* the new token's rows as they are stored: 16-bit values, or biased bytes */
-    __shared__ __attribute__((aligned(16))) uint16_t new_row[2][Q38_ATTN_HEAD_DIM];
-    __shared__ float new_scale[2];
+    __shared__ __attribute__((aligned(16))) NewRows new_rows;
     __shared__ float rope_cs[kPre ? kWaves : 1][32][2];
     __shared__ float red_o[kWaves][kGroup][Q38_ATTN_HEAD_DIM];
     __shared__ float red_m[kWaves][8];
@@ -272,8 +365,11 @@ Q38_DEV void decode_typed(const q38_decode_args &a) {
 
     const int g_split = blockIdx.x, j = blockIdx.y, tid = threadIdx.x;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    /* the sequence of this split: entries past n_seq are INT_MAX */
     int b = 0;
-    while (b + 1 < a.n_seq && a.split_base[b + 1] <= g_split) ++b;
+    for (int i0 = 1; i0 < a.n_seq; i0 += 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b += a.split_base[i0 + i] <= g_split ? 1 : 0;
     const int seq = a.seq[b], pos = a.pos[b];
     const int split = g_split - a.split_base[b], nsplit = a.split_base[b + 1] - a.split_base[b];
     const int t_begin = split * a.split_tokens, t_end = min(pos + 1, t_begin + a.split_tokens);
@@ -290,16 +386,20 @@ Q38_DEV void decode_typed(const q38_decode_args &a) {
     const int q_stride = kPre ? 2 * Q38_ATTN_HEAD_DIM : Q38_ATTN_HEAD_DIM;
     const bool forms_q = wave < kGroup;
     const bool forms_new = !forms_q && a.k_new != nullptr && has_pos;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f}, xw = x;
-    if (forms_q) {
-        x = q38_ld4(a.q + ((size_t)b * Q38_ATTN_HEADS + j * kGroup + wave) * q_stride + 4 * lane);
-        if (kPre) xw = q38_ld4(a.q_norm + 4 * lane);
-    } else if (forms_new) {
-        x = q38_ld4((wave == kGroup ? a.k_new : a.v_new) + (size_t)b * Q38_ATTN_KV_DIM + j * Q38_ATTN_HEAD_DIM + 4 * lane);
-        if (kPre) xw = q38_ld4(a.k_norm + 4 * lane);
-    }
-    Page<T> cur;
-    if (wave < n_pages) load_page<T>(cur, a, __builtin_amdgcn_readlane(my_pages, 0), j, lane);
+    /* (a wave that forms nothing loads head 0's) */
+    const float *src = a.q + ((size_t)b * Q38_ATTN_HEADS + j * kGroup + (forms_q ? wave : 0)) * q_stride;
+    if (forms_new) src = (wave == kGroup ? a.k_new : a.v_new) + (size_t)b * Q38_ATTN_KV_DIM + j * Q38_ATTN_HEAD_DIM;
+    f32x4 x = q38_ld4(src + 4 * lane), xw = {0.f, 0.f, 0.f, 0.f};
+    if (kPre) xw = q38_ld4((forms_q ? a.q_norm : a.k_norm) + 4 * lane);
+    /* the wave's first pages: no load from here to the first score sits under
+     * a branch, so the rows above are waited for alone and the pages come in
+     * while the queries are formed */
+    Page<T> buf[kDepth];
+    auto fetch = [&](Page<T> &p, int at) {
+        load_page<T>(p, a, __builtin_amdgcn_readlane(my_pages, (at / kWaves) & 63), at < n_pages, j, lane);
+    };
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) fetch(buf[u], wave + kWaves * u);
 
     if (kPre && (forms_q || (forms_new && wave == kGroup))) {
         q38_rope_table(rope_cs[wave], lane, pos, a.theta_scale);
@@ -319,9 +419,9 @@ Q38_DEV void decode_typed(const q38_decode_args &a) {
             x *= __uint_as_float((uint32_t)(127 + 10 - e) << 23);
             if (lane == 0) q_unscale[wave] = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
         }
-        q38_st4(&q_rows[wave][4 * lane], x);
+        store_query<T>(q_frag, wave, lane, x);
     } else {
-        q38_st4(&q_rows[wave][4 * lane], f32x4{0.f, 0.f, 0.f, 0.f}); /* columns 6 and 7 */
+        store_query<T>(q_frag, wave, lane, f32x4{0.f, 0.f, 0.f, 0.f}); /* columns 6 and 7 */
         if (lane == 0) q_unscale[wave] = 1.0f;
         if (forms_new) {
             const int which = wave - kGroup;
@@ -330,58 +430,30 @@ Q38_DEV void decode_typed(const q38_decode_args &a) {
             int qv[4] = {0, 0, 0, 0};
             float scale = 0.0f;
             if (T == Q38_KV_Q8) q38_wave_q8k(x, qv, scale);
+            void *row = which ? new_rows.v : new_rows.k;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int d = 4 * lane + i;
+                const int to = which ? new_value_index<T>(d) : d;
                 const int at = which ? q38_v_index<T>(t, d) : q38_k_index<T>(t, d);
                 if (T == Q38_KV_Q8) {
-                    new_row[which][d] = (uint16_t)(qv[i] + 128);
+                    static_cast<uint8_t *>(row)[to] = (uint8_t)(qv[i] + 128);
                     reinterpret_cast<uint8_t *>(block)[at] = (uint8_t)(qv[i] + 128);
                 } else {
-                    new_row[which][d] = q38_to16<T>(x[i]);
+                    static_cast<uint16_t *>(row)[to] = q38_to16<T>(x[i]);
                     reinterpret_cast<uint16_t *>(block)[at] = q38_to16<T>(x[i]);
                 }
             }
             if (T == Q38_KV_Q8 && lane == 0) {
-                new_scale[which] = scale;
-                q38_kv_scales(block)[t] = scale;
+                new_rows.scale[which] = scale;
+                q38_kv_scales(block, j)[t] = scale;
             }
         }
     }
-    __syncthreads();
+    lds_barrier();
     const int c = lane & 15, g = lane >> 4;
-    {
-        /* operand `wave` of the queries: column c, dims d0 .. d0 + 7 */
-        const int d0 = T == Q38_KV_Q8 ? 64 * (wave >> 1) + 16 * g + 8 * (wave & 1) : 32 * wave + 8 * g;
-        const bool first = c < 8;
-        uint16_t f0[8], f1[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float v = q_rows[c & 7][d0 + e];
-            if (T == Q38_KV_BF16) {
-                const uint32_t hi = __float_as_uint(v) & 0xFFFF0000u;
-                const float r = v - __uint_as_float(hi);
-                const uint32_t mid = __float_as_uint(r) & 0xFFFF0000u;
-                const float lo = r - __uint_as_float(mid);
-                f0[e] = (uint16_t)((first ? hi : mid) >> 16);
-                f1[e] = first ? (uint16_t)(__float_as_uint(lo) >> 16) : 0;
-            } else {
-                const _Float16 hi = (_Float16)v;
-                const _Float16 lo = (_Float16)(v - (float)hi);
-                f0[e] = __builtin_bit_cast(uint16_t, first ? hi : lo);
-            }
-        }
-        q_frag[0][wave][lane] = q38_u32x4{pack16(f0[0], f0[1]), pack16(f0[2], f0[3]), pack16(f0[4], f0[5]), pack16(f0[6], f0[7])};
-        if (kQSets > 1)
-            q_frag[kQSets - 1][wave][lane] =
-                q38_u32x4{pack16(f1[0], f1[1]), pack16(f1[2], f1[3]), pack16(f1[4], f1[5]), pack16(f1[6], f1[7])};
-    }
-    __syncthreads();
 
     if (wave < n_pages) {
-        q38_u32x4 q[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = q_frag[0][i][lane];
         const float unscale = q_unscale[c & 7];
         State st;
         st.ref = -INFINITY;
@@ -389,53 +461,23 @@ Q38_DEV void decode_typed(const q38_decode_args &a) {
         st.cap = __uint_as_float(27u << 23); /* 2^-100 */
 #pragma unroll
         for (int n = 0; n < 16; ++n) st.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int i = wave; i < n_pages; i += kWaves) {
-            Page<T> next;
-            if (i + kWaves < n_pages) load_page<T>(next, a, __builtin_amdgcn_readlane(my_pages, (i + kWaves) / kWaves), j, lane);
-            int valid = Q38_PAGE_TOKENS;
-            if (i == n_pages - 1) {
-                valid = t_end - t_begin - Q38_PAGE_TOKENS * i;
-                if (has_pos && a.k_new != nullptr) {
-                    /* the new token's rows in place of what the page held */
-                    const int t = valid - 1;
-                    const bool key_lane = c == t, value_lane = g == (t >> 2);
-                    if (T == Q38_KV_Q8) {
+        /* the only ways out are the gotos: a page's loads are behind the same
+         * number of younger ones on every path, and are waited for alone */
+        for (int i = wave;; i += kWaves * kDepth) {
 #pragma unroll
-                        for (int s = 0; s < 4; ++s)
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) {
-                                uint32_t kw = 0;
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) kw |= (uint32_t)new_row[0][64 * s + 16 * g + 4 * w + e] << (8 * e);
-                                if (key_lane) cur.k[s][w] = kw;
-                                const uint32_t sh = 8 * (t & 3);
-                                const uint32_t vw = (uint32_t)new_row[1][64 * s + 16 * w + c] << sh;
-                                if (value_lane) cur.v[s][w] = (cur.v[s][w] & ~(255u << sh)) | vw;
-                            }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (value_lane && (t & 3) == e) cur.ks[e] = new_scale[0], cur.vs[e] = new_scale[1];
-                    } else {
-#pragma unroll
-                        for (int s = 0; s < 8; ++s) {
-                            const q38_u32x4 kw = *reinterpret_cast<const q38_u32x4 *>(&new_row[0][32 * s + 8 * g]);
-                            if (key_lane) cur.k[s] = kw;
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint32_t sh = 16 * (t & 1);
-                                const uint32_t vw = (uint32_t)new_row[1][32 * s + 16 * h + c] << sh;
-#pragma unroll
-                                for (int w = 0; w < 2; ++w)
-                                    if (value_lane && ((t >> 1) & 1) == w)
-                                        cur.v[s][2 * h + w] = (cur.v[s][2 * h + w] & ~(0xFFFFu << sh)) | vw;
-                            }
-                        }
-                    }
+            for (int u = 0; u < kDepth; ++u) {
+                const int at = i + kWaves * u;
+                if (at >= n_pages) goto done;
+                int valid = Q38_PAGE_TOKENS;
+                if (at == n_pages - 1) {
+                    valid = t_end - t_begin - Q38_PAGE_TOKENS * at;
+                    if (has_pos && a.k_new != nullptr) put_new_token<T>(buf[u], new_rows, valid - 1, lane);
                 }
+                page_step<T>(st, buf[u], q_frag, unscale, valid, lane);
+                fetch(buf[u], at + kWaves * kDepth);
             }
-            page_step<T>(st, cur, q, q_frag[kQSets - 1], unscale, valid, lane);
-            cur = next;
         }
+    done:
         /* both parts' rows added (lanes l and l ^ 32), the lower half of the wave
          * storing the even tiles and the upper half the odd ones */
         const float l = column_sum(st.l);
@@ -458,16 +500,26 @@ Q38_DEV void decode_typed(const q38_decode_args &a) {
     }
     __syncthreads();
 
-    const int live = min(kWaves, n_pages);
-    for (int i = tid; i < kGroup * Q38_ATTN_HEAD_DIM; i += 64 * kWaves) {
-        const int hh = i >> 8, d = i & 255;
-        float M = -INFINITY;
-        for (int w = 0; w < live; ++w) M = fmaxf(M, red_m[w][hh]);
-        float L = 0.0f, O = 0.0f;
-        for (int w = 0; w < live; ++w) {
-            const float f = red_m[w][hh] == -INFINITY ? 0.0f : q38_exp2(red_m[w][hh] - M);
-            L += red_l[w][hh] * f;
-            O += red_o[w][hh][d] * f;
+    /* a thread per 3 outputs: heads tid / 256, + 2, + 4 of one dim */
+    const int d = tid & 255;
+#pragma unroll
+    for (int k = 0; k < kGroup / 2; ++k) {
+        const int hh = 2 * k + (tid >> 8);
+        float m[kWaves], l[kWaves], o[kWaves];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            m[w] = red_m[w][hh];
+            l[w] = red_l[w][hh];
+            o[w] = red_o[w][hh][d];
+        }
+        float M = -INFINITY, L = 0.0f, O = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, w < n_pages ? m[w] : -INFINITY);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = q38_exp2(m[w] - M);
+            L += w < n_pages ? l[w] * f : 0.0f;
+            O += w < n_pages ? o[w] * f : 0.0f;
         }
         const int h = j * kGroup + hh;
         if (nsplit == 1) {

@@ -152,7 +152,7 @@ Q38_DEV void kv_split(const q38_prefill_args &a) {
         if (T == Q38_KV_F32)
             kx[m] = q38_ld4(row_of(a.kpool, i >> 6) + 4 * (i & 63));
         else
-            kx[m] = q38_k_load4<T>(block_of(a.kpool, i >> 6), token_of(i >> 6), 4 * (i & 63));
+            kx[m] = q38_k_load4<T>(block_of(a.kpool, i >> 6), j, token_of(i >> 6), 4 * (i & 63));
     }
 #pragma unroll
     for (int m = 0; m < kVPer; ++m) {
@@ -162,7 +162,7 @@ Q38_DEV void kv_split(const q38_prefill_args &a) {
             vx[2 * m] = q38_ld4(row_of(a.vpool, r) + 4 * c4);
             vx[2 * m + 1] = q38_ld4(row_of(a.vpool, r + 1) + 4 * c4);
         } else {
-            q38_v_load4<T>(block_of(a.vpool, r), token_of(r), token_of(r + 1), 4 * c4, vx[2 * m], vx[2 * m + 1]);
+            q38_v_load4<T>(block_of(a.vpool, r), j, token_of(r), token_of(r + 1), 4 * c4, vx[2 * m], vx[2 * m + 1]);
         }
     }
 #pragma unroll

@@ -192,7 +192,7 @@ Q38_DEV float q8k_quad(const f32x4 (&x)[4], int lane, uint32_t (&b)[4]) {
 }
 
 template <int T>
-Q38_DEV void store_quad(char *block, Stage &stage, bool key, int quad, int first, int last, int lane, const f32x4 (&x)[4]) {
+Q38_DEV void store_quad(char *block, Stage &stage, bool key, int head, int quad, int first, int last, int lane, const f32x4 (&x)[4]) {
     /* tokens first .. last - 1 of the quad are the batch's */
     if (T == Q38_KV_F32) {
 #pragma unroll
@@ -207,7 +207,7 @@ Q38_DEV void store_quad(char *block, Stage &stage, bool key, int quad, int first
         const float scale = q8k_quad(x, lane, q);
 #pragma unroll
         for (int i = 0; i < 4; ++i) b[i][0] = q[i];
-        if (lane >= first && lane < last) q38_kv_scales(block)[4 * quad + lane] = scale;
+        if (lane >= first && lane < last) q38_kv_scales(block, head)[4 * quad + lane] = scale;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -307,8 +307,8 @@ Q38_DEV void kv_append(const q38_kv_rows_args &a) {
         for (int i = 0; i < 4; ++i) t[i] = 4 * quad + min(max(i, first), last - 1);
         norm_rope_quad(x, w, lane, cs, t);
     }
-    store_quad<T>(q38_kv_block<T>(key ? a.kpool : a.vpool, sp.page, head), stages[T == Q38_KV_F32 ? 0 : wave], key, quad,
-                  first, last, lane, x);
+    store_quad<T>(q38_kv_block<T>(key ? a.kpool : a.vpool, sp.page, head), stages[T == Q38_KV_F32 ? 0 : wave], key, head,
+                  quad, first, last, lane, x);
 }
 
 /* OUT16: rows in the cache's 16 bits, moved as they are (T is BF16 for both). */
@@ -338,7 +338,7 @@ Q38_DEV void kv_gather(const q38_kv_rows_args &a) {
         f32x4 scale = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < kPieces / 64; ++k) piece[k] = in[piece_at(key, quad, lane + 64 * k)];
-        if (T == Q38_KV_Q8) scale = q38_ld4(q38_kv_scales(block) + 4 * quad);
+        if (T == Q38_KV_Q8) scale = q38_ld4(q38_kv_scales(block, head) + 4 * quad);
 #pragma unroll
         for (int k = 0; k < kPieces / 64; ++k) stage[lane + 64 * k] = piece[k];
         stage_fence();

@@ -15,10 +15,12 @@ typedef uint32_t q38_u32x4 __attribute__((ext_vector_type(4)));
 /* The block of (page, kv head) in a slot's pool. */
 template <int T>
 Q38_DEV char *q38_kv_block(void *pool, int page, int head) {
-    return static_cast<char *>(pool) + ((size_t)page * Q38_ATTN_KV_HEADS + head) * q38_kv_block_bytes<T>();
+    return static_cast<char *>(pool) + (size_t)page * q38_kv_page_bytes<T>() + head * q38_kv_block_bytes<T>();
 }
 
-Q38_DEV float *q38_kv_scales(char *block) { return reinterpret_cast<float *>(block + 4096); }
+Q38_DEV float *q38_kv_scales(char *block, int head) {
+    return reinterpret_cast<float *>(block + q38_kv_scales_offset(head));
+}
 
 /* A 16-bit value of the type, rounded to nearest even (F16: past 65504 to
  * infinity), and back. */
@@ -33,23 +35,14 @@ Q38_DEV float q38_from16(uint16_t b) {
     return __uint_as_float((uint32_t)b << 16);
 }
 
-/* One value of a block as f32. */
-template <int T>
-Q38_DEV float q38_kv_value(char *block, int index, int t) {
-    if (T == Q38_KV_F32) return reinterpret_cast<const float *>(block)[index];
-    if (T == Q38_KV_Q8)
-        return (float)((int)reinterpret_cast<const uint8_t *>(block)[index] - 128) * q38_kv_scales(block)[t];
-    return q38_from16<T>(reinterpret_cast<const uint16_t *>(block)[index]);
-}
-
 /* Dims d .. d + 3 (d a multiple of 4) of one token's key. */
 template <int T>
-Q38_DEV f32x4 q38_k_load4(char *block, int t, int d) {
+Q38_DEV f32x4 q38_k_load4(char *block, int head, int t, int d) {
     const int i = q38_k_index<T>(t, d);
     f32x4 x;
     if (T == Q38_KV_Q8) {
         const uint32_t u = *reinterpret_cast<const uint32_t *>(block + i);
-        const float s = q38_kv_scales(block)[t];
+        const float s = q38_kv_scales(block, head)[t];
 #pragma unroll
         for (int c = 0; c < 4; ++c) x[c] = (float)((int)((u >> (8 * c)) & 255u) - 128) * s;
     } else {
@@ -63,9 +56,9 @@ Q38_DEV f32x4 q38_k_load4(char *block, int t, int d) {
 /* Dims d .. d + 3 of the values of tokens t0 and t1, which share a pair of
  * tokens (2n, 2n + 1), maybe the same one twice. */
 template <int T>
-Q38_DEV void q38_v_load4(char *block, int t0, int t1, int d, f32x4 &x0, f32x4 &x1) {
-    const float s0 = T == Q38_KV_Q8 ? q38_kv_scales(block)[t0] : 0.0f;
-    const float s1 = T == Q38_KV_Q8 ? q38_kv_scales(block)[t1] : 0.0f;
+Q38_DEV void q38_v_load4(char *block, int head, int t0, int t1, int d, f32x4 &x0, f32x4 &x1) {
+    const float s0 = T == Q38_KV_Q8 ? q38_kv_scales(block, head)[t0] : 0.0f;
+    const float s1 = T == Q38_KV_Q8 ? q38_kv_scales(block, head)[t1] : 0.0f;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const int i = q38_v_index<T>(t0 & ~1, d + c);

@@ -24,11 +24,11 @@
 /* one page of one layer: [4 kv heads][16 tokens][256] floats, K and V pools apart */
 #define Q38_PAGE_FLOATS (Q38_ATTN_KV_HEADS * Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM)
 
-/* bytes of one kv head's 16 tokens x 256 values in a page, by the cache's type
- * (Q8_K: quants, then the 16 tokens' f32 scales) */
-#define Q38_KV_BLOCK_F32 (Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM * 4)
-#define Q38_KV_BLOCK_16 (Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM * 2)
-#define Q38_KV_BLOCK_Q8 (Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM + Q38_PAGE_TOKENS * 4)
+/* bytes of a page, by the cache's type: per kv head 16 tokens x 256 values (Q8_K:
+ * quants, and after the four heads' the f32 scales [head][token]) */
+#define Q38_KV_PAGE_F32 (Q38_PAGE_FLOATS * 4)
+#define Q38_KV_PAGE_16 (Q38_PAGE_FLOATS * 2)
+#define Q38_KV_PAGE_Q8 (Q38_PAGE_FLOATS + Q38_ATTN_KV_HEADS * Q38_PAGE_TOKENS * 4)
 
 #define Q38_LIN_QK_HEADS 16
 #define Q38_LIN_V_HEADS 48
@@ -69,7 +69,7 @@ typedef struct {
     int32_t total_splits;
     int32_t seq[Q38_MAX_BATCH];
     int32_t pos[Q38_MAX_BATCH]; /* attend over positions 0..pos inclusive */
-    int32_t split_base[Q38_MAX_BATCH + 1];
+    int32_t split_base[Q38_MAX_BATCH + 8]; /* past n_seq: INT_MAX */
     int32_t head_pages[Q38_HEAD_PAGE_SPLITS][2]; /* physical ids of split g's first two pages (the
                                                     second repeats the first where the split has
                                                     one), when total_splits <= 256 */

@@ -15,8 +15,9 @@
  * Q8_K: a token's 256 values of one head are one Q8_K block -- the first
  * value m of largest magnitude sets the scale 1 / (-127 / m), quants are
  * round-to-nearest-even of x * (-127 / m) capped at 127 -- kept as quant +
- * 128 in a byte (the decode kernel makes f16 of it without a sign step),
- * with the 16 tokens' f32 scales after the block's 4096 bytes.
+ * 128 in a byte (the decode kernel makes f16 of it without a sign step).  The
+ * f32 scales, [head][token], follow the page's four blocks, so that every
+ * block starts on a cache line.
  */
 #ifndef Q38_KV_LAYOUT_H
 #define Q38_KV_LAYOUT_H
@@ -30,8 +31,17 @@
 enum { Q38_KV_F32 = 0, Q38_KV_F16 = 1, Q38_KV_BF16 = 2, Q38_KV_Q8 = 3 };
 
 template <int T>
+Q38_LAYOUT_FN constexpr int q38_kv_page_bytes() {
+    return T == Q38_KV_F32 ? Q38_KV_PAGE_F32 : T == Q38_KV_Q8 ? Q38_KV_PAGE_Q8 : Q38_KV_PAGE_16;
+}
+/* Of a block: one kv head's values. */
+template <int T>
 Q38_LAYOUT_FN constexpr int q38_kv_block_bytes() {
-    return T == Q38_KV_F32 ? Q38_KV_BLOCK_F32 : T == Q38_KV_Q8 ? Q38_KV_BLOCK_Q8 : Q38_KV_BLOCK_16;
+    return Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM * (T == Q38_KV_F32 ? 4 : T == Q38_KV_Q8 ? 1 : 2);
+}
+/* Q8_K: a block's scales, in bytes after its first quant. */
+Q38_LAYOUT_FN int q38_kv_scales_offset(int head) {
+    return (Q38_ATTN_KV_HEADS - head) * Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM + head * Q38_PAGE_TOKENS * 4;
 }
 
 /* Element offset of (token, dim) in a block. */

@@ -58,8 +58,10 @@ static void check_layout() {
         }
     REQUIRE(k.size() == 4096 && *k.begin() == 0 && *k.rbegin() == 4095);
     REQUIRE(v.size() == 4096 && *v.begin() == 0 && *v.rbegin() == 4095);
-    REQUIRE(q38_kv_block_bytes<T>() == 4096 * size + (T == Q38_KV_Q8 ? 64 : 0));
-    REQUIRE(q38_kv_block_bytes<T>() % 64 == 0);
+    REQUIRE(q38_kv_block_bytes<T>() == 4096 * size && q38_kv_page_bytes<T>() % 128 == 0);
+    REQUIRE(q38_kv_page_bytes<T>() == 4 * q38_kv_block_bytes<T>() + (T == Q38_KV_Q8 ? 4 * 64 : 0));
+    for (int head = 0; head < 4; ++head) /* past the four blocks, a line apart, inside the page */
+        REQUIRE(head * 4096 + q38_kv_scales_offset(head) == 4 * 4096 + 64 * head);
 }
 
 struct Cache {
