@@ -11,6 +11,7 @@ __graft_entry__.py), or call the library through any FFI directly.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
@@ -50,7 +51,7 @@ class _DecodeCall(ctypes.Structure):
 
 
 _P = c_void_p
-_I32P = POINTER(c_int32)
+_I32P = c_void_p  # const int32_t *: bytes from _i32, or a ctypes array
 _SIGNATURES = {
     "q38_last_error": (c_char_p, []),
     "q38_device_count": (c_int, [POINTER(c_int)]),
@@ -164,11 +165,9 @@ def device_count() -> int:
     return n.value
 
 
-def _i32(seq) -> ctypes.Array:
-    a = (c_int32 * len(seq))()
-    for i, v in enumerate(seq):
-        a[i] = int(v)
-    return a
+def _i32(seq) -> bytes:
+    """Host integers as the int32 array that a call reads (and does not keep)."""
+    return array.array("i", seq).tobytes()
 
 
 class DeviceArray:
@@ -365,17 +364,18 @@ class Context:
 
 
 def _ptr(x):
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     if isinstance(x, DeviceArray):
         return x.ptr
     return int(x)
 
 
-def _same_length(*lists) -> int:
-    if len({len(x) for x in lists}) != 1:
+def _same_length(seq_ids, pos0, n_tokens) -> int:
+    n = len(seq_ids)
+    if len(pos0) != n or len(n_tokens) != n:
         raise Q38Error("sequence ids, positions and counts differ in number")
-    return len(lists[0])
+    return n
 
 
 class KVCache:

@@ -29,6 +29,7 @@ extern "C" hipError_t hipExtModuleLaunchKernel(hipFunction_t f, uint32_t globalW
 #include <climits>
 #include <cmath>
 #include <cstdarg>
+#include <cstddef>
 #include <cstdio>
 #include <cstring>
 #include <memory>
@@ -177,9 +178,12 @@ struct q38_ctx {
     hipFunction_t f_decode_merge = nullptr;
     hipFunction_t f_kv_copy = nullptr;
     hipModule_t mod_rows = nullptr;
-    hipFunction_t f_kv_append[kKvTypeCount] = {};  /* by kKvTypes index */
-    hipFunction_t f_kv_gather[kKvTypeCount] = {};
-    hipFunction_t f_kv_gather_16 = nullptr;        /* 16-bit rows as they are stored */
+    struct RowsKernel {
+        hipFunction_t many = nullptr, few = nullptr; /* up to Q38_MAX_BATCH sequences, Q38_KV_ROWS_FEW */
+    };
+    RowsKernel f_kv_append[kKvTypeCount]; /* by kKvTypes index */
+    RowsKernel f_kv_gather[kKvTypeCount];
+    RowsKernel f_kv_gather_16;            /* 16-bit rows as they are stored */
     hipFunction_t f_kv_split_typed[kKvTypeCount] = {}; /* from index 1 on */
     hipModule_t mod_norm = nullptr;
     hipFunction_t f_norm[2][kNormVectors] = {}; /* [256 or 1024 threads][vectors a thread - 1] */
@@ -487,11 +491,15 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
     const std::string p_rows = dir + "/kv_rows.hsaco", p_typed = dir + "/attn_decode_typed.hsaco";
     Q38_HIP(hipModuleLoad(&ctx->mod_rows, p_rows.c_str()));
     Q38_HIP(hipModuleLoad(&ctx->mod_typed, p_typed.c_str()));
-    Q38_HIP(hipModuleGetFunction(&ctx->f_kv_gather_16, ctx->mod_rows, "q38_kv_gather_16"));
+    auto rows_kernel = [&](q38_ctx::RowsKernel *k, const std::string &name) {
+        const hipError_t e = hipModuleGetFunction(&k->many, ctx->mod_rows, name.c_str());
+        return e != hipSuccess ? e : hipModuleGetFunction(&k->few, ctx->mod_rows, (name + "_few").c_str());
+    };
+    Q38_HIP(rows_kernel(&ctx->f_kv_gather_16, "q38_kv_gather_16"));
     for (int i = 0; i < kKvTypeCount; ++i) {
         const std::string ty = kKvTypes[i].suffix;
-        Q38_HIP(hipModuleGetFunction(&ctx->f_kv_append[i], ctx->mod_rows, ("q38_kv_append_" + ty).c_str()));
-        Q38_HIP(hipModuleGetFunction(&ctx->f_kv_gather[i], ctx->mod_rows, ("q38_kv_gather_" + ty).c_str()));
+        Q38_HIP(rows_kernel(&ctx->f_kv_append[i], "q38_kv_append_" + ty));
+        Q38_HIP(rows_kernel(&ctx->f_kv_gather[i], "q38_kv_gather_" + ty));
         if (i == 0) continue;
         Q38_HIP(hipModuleGetFunction(&ctx->f_kv_split_typed[i], ctx->mod_prefill, ("q38_kv_split_mfma_" + ty).c_str()));
         Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed[i][0], ctx->mod_typed, ("q38_attn_decode_" + ty).c_str()));
@@ -755,8 +763,12 @@ int q38_kernel_timer_start(q38_ctx *ctx, const char *kernel_name, int max_launch
     else {
         for (int i = 0; i < kKvTypeCount; ++i) {
             const std::string ty = kKvTypes[i].suffix;
-            if (name == "q38_kv_append_" + ty) f = ctx->f_kv_append[i];
-            if (name == "q38_kv_gather_" + ty) f = ctx->f_kv_gather[i];
+            for (const auto &k : {std::make_pair("q38_kv_append_" + ty, &ctx->f_kv_append[i]),
+                                  std::make_pair("q38_kv_gather_" + ty, &ctx->f_kv_gather[i]),
+                                  std::make_pair(std::string("q38_kv_gather_16"), &ctx->f_kv_gather_16)}) {
+                if (name == k.first) f = k.second->many;
+                if (name == k.first + "_few") f = k.second->few;
+            }
             if (i > 0 && name == "q38_kv_split_mfma_" + ty) f = ctx->f_kv_split_typed[i];
             if (i > 0 && name == "q38_attn_decode_" + ty) f = ctx->f_decode_typed[i][0];
             if (i > 0 && name == "q38_attn_decode_" + ty + "_pre") f = ctx->f_decode_typed[i][1];
@@ -766,7 +778,6 @@ int q38_kernel_timer_start(q38_ctx *ctx, const char *kernel_name, int max_launch
                 if (name == norm_kernel_name(w, v)) f = ctx->f_norm[w][v];
         if (name == "q38_add_rms_norm_any") f = ctx->f_norm_any;
         if (name == "q38_dequantize_q8k") f = ctx->f_dequantize_q8k;
-        if (name == "q38_kv_gather_16") f = ctx->f_kv_gather_16;
         for (int i = 0; i < kGemvTypes; ++i) {
             if (name == kGemv[i].kernel) f = ctx->f_gemv_q8k[i];
             if (kGemv[i].gemm_kernel != nullptr && name == kGemv[i].gemm_kernel) f = ctx->f_gemm[i];
@@ -1009,7 +1020,7 @@ int validate_rows(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
 
 /* Moves a validated batch whose pages are reserved, in launches of up to
  * Q38_MAX_BATCH sequences; rows of `elem_bytes` a value. */
-int launch_rows(q38_kv *kv, hipFunction_t f, int slot, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
+int launch_rows(q38_kv *kv, const q38_ctx::RowsKernel &f, int slot, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
                 const int32_t *n_tokens, void *d_k, void *d_v, size_t elem_bytes, const float *d_k_norm) {
     size_t row = 0;
     for (int b = 0; b < n_seq;) {
@@ -1036,7 +1047,18 @@ int launch_rows(q38_kv *kv, hipFunction_t f, int slot, int n_seq, const int32_t 
         if (n == 0) break;
         a.n_seq = n;
         for (int i = n + 1; i < Q38_MAX_BATCH + 8; ++i) a.page_base[i] = INT_MAX;
-        if (kv->ctx->launch(f, (unsigned)a.page_base[n], 2, 1, Q38_KV_ROWS_THREADS, &a)) return -1;
+        q38_kv_rows_few_args few;
+        const bool is_few = n <= Q38_KV_ROWS_FEW;
+        if (is_few) {
+            memcpy(&few, &a, offsetof(q38_kv_rows_few_args, seq));
+            memcpy(few.seq, a.seq, sizeof(few.seq));
+            memcpy(few.pos0, a.pos0, sizeof(few.pos0));
+            memcpy(few.row_base, a.row_base, sizeof(few.row_base));
+            memcpy(few.page_base, a.page_base, sizeof(few.page_base));
+        }
+        if (kv->ctx->launch(is_few ? f.few : f.many, (unsigned)a.page_base[n], 2, 1, Q38_KV_ROWS_THREADS,
+                            is_few ? (void *)&few : (void *)&a))
+            return -1;
         row += (size_t)a.row_base[n];
     }
     return 0;
@@ -1920,6 +1942,11 @@ retry:
  * carries on every HIP runtime */
 static_assert(sizeof(q38_prefill_args) <= 4096, "prefill arguments exceed 4 KiB");
 static_assert(sizeof(q38_decode_args) <= 4096, "decode arguments exceed 4 KiB");
+/* a typed launch passes the same block, of which its kernel takes the front */
+static_assert(offsetof(q38_kv_rows_few_args, seq) == offsetof(q38_kv_rows_args, seq), "one head");
+static_assert(offsetof(q38_decode_args, head_pages) == sizeof(q38_decode_typed_args) &&
+                  offsetof(q38_decode_args, split_base) == offsetof(q38_decode_typed_args, split_base),
+              "q38_decode_typed_args is the front of q38_decode_args");
 static_assert(sizeof(q38_prefill_merge_args) <= 4096, "prefill merge arguments exceed 4 KiB");
 
 int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens, const float *d_q,

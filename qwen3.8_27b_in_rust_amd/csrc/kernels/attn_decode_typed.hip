@@ -68,7 +68,7 @@ Q38_DEV q38_u32x4 ld_block(__amdgpu_buffer_rsrc_t r, int at) {
 }
 
 template <int T>
-Q38_DEV void load_page(Page<T> &p, const q38_decode_args &a, int page, bool live, int j, int lane) {
+Q38_DEV void load_page(Page<T> &p, const q38_decode_typed_args &a, int page, bool live, int j, int lane) {
     const int scales = q38_kv_scales_offset(j);
     const int bytes = !live ? 0 : T == Q38_KV_Q8 ? scales + Q38_PAGE_TOKENS * 4 : q38_kv_block_bytes<T>();
     const __amdgpu_buffer_rsrc_t k = block_rsrc(q38_kv_block<T>(a.kpool, page, j), bytes);
@@ -351,7 +351,7 @@ Q38_DEV void store_query(q38_u32x4 (*q)[8][64], int c, int lane, f32x4 x) {
 }
 
 template <int T, bool kPre>
-Q38_DEV void decode_typed(const q38_decode_args &a) {
+Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
     constexpr int kQSets = T == Q38_KV_BF16 ? 2 : 1;
     constexpr int kDepth = T == Q38_KV_Q8 ? 2 : 1; /* pages of a wave in registers */
     __shared__ q38_u32x4 q_frag[kQSets][8][64];
@@ -539,10 +539,10 @@ Q38_DEV void decode_typed(const q38_decode_args &a) {
 }  // namespace
 
 #define Q38_DECODE_KERNELS(name, T)                                                                                  \
-    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name(q38_decode_args a) {            \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name(q38_decode_typed_args a) {            \
         decode_typed<T, false>(a);                                                                                   \
     }                                                                                                                \
-    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name##_pre(q38_decode_args a) {      \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name##_pre(q38_decode_typed_args a) {      \
         decode_typed<T, true>(a);                                                                                    \
     }
 Q38_DECODE_KERNELS(f16, Q38_KV_F16)

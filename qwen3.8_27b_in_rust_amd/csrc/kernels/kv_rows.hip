@@ -13,7 +13,16 @@
  * CU keep the memory busy -- and the quad's part of the page is put together
  * in the wave's own LDS, where the page's element order (q38_kv_layout.h)
  * makes it 16-byte pieces: of one token for K, of all four for V.  The page's
- * rotation angles are formed once per workgroup.
+ * rotation angles are formed once per workgroup (half as many heads in one,
+ * and the angles twice, took 13.4 us where this takes 12.5).
+ *
+ * Measured (us, the kernel alone): 4096 tokens to Q8_K 12.5 (42 MB) and back
+ * 7.8 (5.4 TB/s); 1531 tokens of 12 sequences to bf16 8.4 and back 6.3; 6
+ * tokens to f16 4.3 and back 3.5, of which an empty launch is about half.
+ * Keys are held up by their arithmetic as much as by memory: the angles and,
+ * per token and head, the f64 sum, the rotation and the quantiser are some
+ * 500 instructions a wave and quad (1500 with four reductions one by one,
+ * 19 us).
  */
 #include "q38_kv_types.h"
 #include "q38_rope.h"
@@ -31,7 +40,8 @@ struct PageSpan {
     int page;     /* physical page */
 };
 
-Q38_DEV PageSpan page_span(const q38_kv_rows_args &a, int x) {
+template <typename Args>
+Q38_DEV PageSpan page_span(const Args &a, int x) {
     /* the sequence that holds page x: entries past n_seq are INT_MAX, so eight
      * are compared at a time, without a chain of dependent scalar loads */
     int b = 0;
@@ -273,8 +283,8 @@ Q38_DEV void store_quad(char *block, Stage &stage, bool key, int head, int quad,
     }
 }
 
-template <int T>
-Q38_DEV void kv_append(const q38_kv_rows_args &a) {
+template <int T, typename Args>
+Q38_DEV void kv_append(const Args &a) {
     __shared__ __attribute__((aligned(16))) float cs[Q38_PAGE_TOKENS][32][2];
     __shared__ Stage stages[T == Q38_KV_F32 ? 1 : kThreads / 64];
     const PageSpan sp = page_span(a, blockIdx.x);
@@ -312,8 +322,8 @@ Q38_DEV void kv_append(const q38_kv_rows_args &a) {
 }
 
 /* OUT16: rows in the cache's 16 bits, moved as they are (T is BF16 for both). */
-template <int T, bool OUT16>
-Q38_DEV void kv_gather(const q38_kv_rows_args &a) {
+template <int T, bool OUT16, typename Args>
+Q38_DEV void kv_gather(const Args &a) {
     __shared__ Stage stages[T == Q38_KV_F32 ? 1 : kThreads / 64];
     const PageSpan sp = page_span(a, blockIdx.x);
     const bool key = blockIdx.y == 0;
@@ -387,17 +397,16 @@ Q38_DEV void kv_gather(const q38_kv_rows_args &a) {
 
 }  // namespace
 
-#define Q38_KV_ROWS_KERNELS(name, T)                                                                             \
-    extern "C" __global__ __launch_bounds__(kThreads) void q38_kv_append_##name(q38_kv_rows_args a) { kv_append<T>(a); } \
-    extern "C" __global__ __launch_bounds__(kThreads) void q38_kv_gather_##name(q38_kv_rows_args a) {            \
-        kv_gather<T, false>(a);                                                                                  \
-    }
-Q38_KV_ROWS_KERNELS(f32, Q38_KV_F32)
-Q38_KV_ROWS_KERNELS(f16, Q38_KV_F16)
-Q38_KV_ROWS_KERNELS(bf16, Q38_KV_BF16)
-Q38_KV_ROWS_KERNELS(q8k, Q38_KV_Q8)
-
+#define Q38_KV_ROWS_KERNEL(name, call)                                                                          \
+    extern "C" __global__ __launch_bounds__(kThreads) void name(q38_kv_rows_args a) { call(a); }                \
+    extern "C" __global__ __launch_bounds__(kThreads) void name##_few(q38_kv_rows_few_args a) { call(a); }
+Q38_KV_ROWS_KERNEL(q38_kv_append_f32, kv_append<Q38_KV_F32>)
+Q38_KV_ROWS_KERNEL(q38_kv_append_f16, kv_append<Q38_KV_F16>)
+Q38_KV_ROWS_KERNEL(q38_kv_append_bf16, kv_append<Q38_KV_BF16>)
+Q38_KV_ROWS_KERNEL(q38_kv_append_q8k, kv_append<Q38_KV_Q8>)
+Q38_KV_ROWS_KERNEL(q38_kv_gather_f32, (kv_gather<Q38_KV_F32, false>))
+Q38_KV_ROWS_KERNEL(q38_kv_gather_f16, (kv_gather<Q38_KV_F16, false>))
+Q38_KV_ROWS_KERNEL(q38_kv_gather_bf16, (kv_gather<Q38_KV_BF16, false>))
+Q38_KV_ROWS_KERNEL(q38_kv_gather_q8k, (kv_gather<Q38_KV_Q8, false>))
 /* 16-bit rows as they are stored, F16 or BF16. */
-extern "C" __global__ __launch_bounds__(kThreads) void q38_kv_gather_16(q38_kv_rows_args a) {
-    kv_gather<Q38_KV_BF16, true>(a);
-}
+Q38_KV_ROWS_KERNEL(q38_kv_gather_16, (kv_gather<Q38_KV_BF16, true>))

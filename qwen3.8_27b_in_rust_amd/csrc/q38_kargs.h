@@ -45,7 +45,33 @@
 #define Q38_DECODE_TYPED_WAVES 8 /* waves of a decode workgroup over 16- or 8-bit rows */
 #define Q38_HEAD_PAGE_SPLITS 256 /* splits whose first page ids a decode launch can carry */
 
-/* Split-K paged decode: grid (total_splits, 4 kv heads). */
+/* Split-K paged decode: grid (total_splits, 4 kv heads).  Over 16- or 8-bit rows
+ * the pools are bytes (q38_kv_layout.h) and the launch carries no page ids. */
+typedef struct {
+    float *kpool;              /* this layer's K pages: [max_pages][4][16][256] */
+    float *vpool;              /* this layer's V pages */
+    const int32_t *page_table; /* [max_seqs][pt_stride] physical page ids */
+    const float *q;            /* [n_seq][24][256], post-norm, post-RoPE (fused pre step:
+                                  raw [n_seq][24][512] q|gate rows) */
+    const float *k_new;        /* [n_seq][1024] appended at pos[b] first, or NULL (fused pre
+                                  step: the raw key, normed and rotated before the append) */
+    const float *v_new;        /* [n_seq][1024] or NULL */
+    const float *gate;         /* [n_seq][24][256] output gate logits, or NULL */
+    float *out;                /* [n_seq][24][256] */
+    float *part_o;             /* [total_splits][24][256] unnormalised partial outputs */
+    float *part_ml;            /* [total_splits][24][2]  (running max in log2 units, sum) */
+    const float *q_norm;       /* fused pre step: [256] q RMSNorm weight, else unused */
+    const float *k_norm;       /* fused pre step: [256] k RMSNorm weight */
+    float theta_scale;         /* fused pre step: RoPE 1e7^(-2/64) in f32 */
+    int32_t gate_head_stride;  /* floats between heads' gates: 256, or 512 in q|gate rows */
+    int32_t pt_stride;
+    int32_t n_seq;
+    int32_t split_tokens; /* multiple of Q38_PAGE_TOKENS */
+    int32_t total_splits;
+    int32_t seq[Q38_MAX_BATCH];
+    int32_t pos[Q38_MAX_BATCH]; /* attend over positions 0..pos inclusive */
+    int32_t split_base[Q38_MAX_BATCH + 8]; /* past n_seq: INT_MAX */
+} q38_decode_typed_args;
 typedef struct {
     float *kpool;              /* this layer's K pages: [max_pages][4][16][256] */
     float *vpool;              /* this layer's V pages */
@@ -99,22 +125,28 @@ typedef struct {
  * four tokens.  page_base past n_seq holds INT_MAX (the sequence of a page is
  * found eight entries at a time). */
 #define Q38_KV_ROWS_THREADS 1024
-typedef struct {
-    void *kpool;
-    void *vpool;
-    const int32_t *page_table;
-    void *k_rows; /* [rows][1024]: f32, or (gathering only) the cache's 16-bit type */
-    void *v_rows;
-    const float *k_norm; /* append of raw keys: [256] RMSNorm weight; NULL: rows stored as they are */
-    float theta_scale;   /* append of raw keys: RoPE 1e7^(-2/64) in f32 */
-    int32_t pt_stride;
-    int32_t n_seq;
-    int32_t pad_;
-    int32_t seq[Q38_MAX_BATCH];
-    int32_t pos0[Q38_MAX_BATCH];
-    int32_t row_base[Q38_MAX_BATCH + 1];
-    int32_t page_base[Q38_MAX_BATCH + 8];
-} q38_kv_rows_args;
+#define Q38_KV_ROWS_FEW 8
+#define Q38_KV_ROWS_ARGS(N)  \
+    struct {  \
+        void *kpool; \
+        void *vpool; \
+        const int32_t *page_table; \
+        void *k_rows; /* [rows][1024]: f32, or (gathering only) the cache's 16-bit type */ \
+        void *v_rows; \
+        const float *k_norm; /* append of raw keys: [256] RMSNorm weight; NULL: rows stored as they are */ \
+        float theta_scale;   /* append of raw keys: RoPE 1e7^(-2/64) in f32 */ \
+        int32_t pt_stride; \
+        int32_t n_seq; \
+        int32_t pad_; \
+        int32_t seq[N]; \
+        int32_t pos0[N]; \
+        int32_t row_base[N + 1]; \
+        int32_t page_base[N + 8]; \
+    }
+typedef Q38_KV_ROWS_ARGS(Q38_MAX_BATCH) q38_kv_rows_args;
+/* up to Q38_KV_ROWS_FEW sequences: the launch carries 300 bytes of arguments
+ * instead of 1200, 0.8 us less on the host */
+typedef Q38_KV_ROWS_ARGS(Q38_KV_ROWS_FEW) q38_kv_rows_few_args;
 
 /* q/gate split, q and k RMSNorm, RoPE.  grid (n_tokens, 28): y < 24 is a
  * query head, y >= 24 a kv head. */

@@ -11,6 +11,8 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
+#include <cstring>
+#include <cstddef>
 #include <map>
 #include <set>
 #include <string>
@@ -21,12 +23,27 @@
 static int g_launches = 0;
 static std::vector<std::vector<char>> g_args;
 static std::vector<unsigned> g_grid;
-static hipError_t check_launch(hipFunction_t, unsigned gx, unsigned gy, unsigned, unsigned block, unsigned, unsigned,
+/* the functions that a launch names: one handle for each argument block */
+static hipFunction_t const kMany = (hipFunction_t)0x1000, kFew = (hipFunction_t)0x2000;
+static hipError_t check_launch(hipFunction_t f, unsigned gx, unsigned gy, unsigned, unsigned block, unsigned, unsigned,
                                unsigned, hipStream_t, void **params, void **) {
     ++g_launches;
     if (gy != 2 || block != Q38_KV_ROWS_THREADS) { printf("unexpected grid\n"); exit(1); }
-    const char *p = static_cast<const char *>(params[0]);
-    g_args.emplace_back(p, p + sizeof(q38_kv_rows_args));
+    q38_kv_rows_args a;
+    if (f == kFew) {
+        const q38_kv_rows_few_args &w = *static_cast<const q38_kv_rows_few_args *>(params[0]);
+        memset(&a, 0xAB, sizeof(a)); /* what the kernel does not get */
+        memcpy(&a, &w, offsetof(q38_kv_rows_few_args, seq));
+        memcpy(a.seq, w.seq, sizeof(w.seq));
+        memcpy(a.pos0, w.pos0, sizeof(w.pos0));
+        memcpy(a.row_base, w.row_base, sizeof(w.row_base));
+        memcpy(a.page_base, w.page_base, sizeof(w.page_base));
+        if (a.n_seq > Q38_KV_ROWS_FEW) { printf("too many sequences for the small block\n"); exit(1); }
+    } else {
+        a = *static_cast<const q38_kv_rows_args *>(params[0]);
+    }
+    const char *p = reinterpret_cast<const char *>(&a);
+    g_args.emplace_back(p, p + sizeof(a));
     g_grid.push_back(gx);
     return hipSuccess;
 }
@@ -69,6 +86,11 @@ struct Cache {
     q38_kv kv;
     std::vector<int32_t> staging;
     Cache(int type, int slots, int pages, int seqs, int tokens) {
+        for (int i = 0; i < kKvTypeCount; ++i)
+            for (q38_ctx::RowsKernel *k : {&ctx.f_kv_append[i], &ctx.f_kv_gather[i], &ctx.f_kv_gather_16}) {
+                k->many = kMany;
+                k->few = kFew;
+            }
         kv.ctx = &ctx;
         kv.type = type;
         kv.n_slots = slots;
@@ -152,7 +174,7 @@ int main() {
             /* distinct sequences in a random order, 1 .. 150 of them, pieces of 0 .. 70 tokens */
             std::vector<int32_t> seq(ids.begin(), ids.end()), pos, cnt;
             for (size_t i = seq.size() - 1; i > 0; --i) std::swap(seq[i], seq[rand() % (i + 1)]);
-            seq.resize(1 + rand() % seq.size());
+            seq.resize(1 + rand() % (it % 3 == 0 ? 12 : seq.size()));
             for (size_t i = 0; i < seq.size(); ++i) pos.push_back(rand() % 300), cnt.push_back(rand() % 4 ? rand() % 71 : 0);
             g_args.clear(), g_grid.clear();
             REQUIRE(q38_kv_append(&c.kv, 7, (int)seq.size(), seq.data(), pos.data(), cnt.data(), w, k, v) == 0);
