@@ -159,7 +159,9 @@ int q38_kv_read(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, float *d
  * position, then stored, as the value row is, in the cache's type; the result
  * equals q38_attn_pre's k rows stored with q38_kv_write, bit for bit.
  * Sequence ids must be distinct; pages are reserved as needed.  At most 2^25
- * rows a call. */
+ * rows a call.  Like q38_full_core it is for stream capture only where its
+ * pages are reserved beforehand (a new page's id is uploaded), and its
+ * positions are then the captured ones. */
 int q38_kv_append(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
                   const int32_t *n_tokens, const float *d_k_norm, const float *d_key, const float *d_value);
 
@@ -384,7 +386,7 @@ int q38_dequantize_q8_k(q38_ctx *ctx, int n_tokens, int width, const void *d_q8k
  * d_sum receives h, d_y receives y, d_q8k the Q8_K rows of y (as
  * q38_quantize_q8_k of y, bit for bit, for finite y); each may be NULL, not
  * all three.  d_q8k needs a width that is a multiple of 256 and 16-byte
- * alignment; any width >= 1 does without.  d_sum or d_y may be d_x or
+ * alignment; any width from 1 to 2^24 does without.  d_sum or d_y may be d_x or
  * d_residual itself (the residual stream updated in place), and no buffer
  * else may overlap an output.  It allocates nothing and may be captured. */
 int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, const float *d_residual,

@@ -1653,7 +1653,7 @@ int q38_decode_graph_begin(q38_kv *kv, int n_seq, const int32_t *seq_ids, const 
     g->n_seq = n_seq;
     memcpy(g->seq_ids, seq_ids, sizeof(int32_t) * n_seq);
     memcpy(g->positions, positions, sizeof(int32_t) * n_seq);
-    g->arg_pages = n_seq == 1 && kv->ctx->split_tokens == 0 ? 1 : 0;
+    g->arg_pages = kv->type == 0 && n_seq == 1 && kv->ctx->split_tokens == 0 ? 1 : 0;
     Q38_HIP(hipGraphCreate(&g->graph, 0));
     *out = g.release();
     return 0;
@@ -2570,6 +2570,7 @@ int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, co
     if (ctx == nullptr) return fail("ctx is NULL");
     if (n_tokens < 0) return fail("negative n_tokens");
     if (width < 1) return fail("width %d is not positive", width);
+    if (width > 1 << 24) return fail("width %d above 2^24", width);
     if (d_q8k != nullptr && width % Q38_Q8K_BLOCK != 0)
         return fail("Q8_K rows need a width that is a multiple of 256, not %d", width);
     if (n_tokens == 0) return 0;

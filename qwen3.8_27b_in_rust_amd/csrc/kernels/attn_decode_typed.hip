@@ -24,8 +24,10 @@
  *    8-bit rows: the value's scale goes into its weight, over a power of two
  *    at or above every scale seen so far, which keeps f16 clear of overflow.
  *  - softmax in base 2 against a reference per head that is raised (and O and
- *    the sum rescaled) only when a score passes it by 2^8: weights stay below
- *    2^15, which f16 holds, and most pages rescale nothing.
+ *    the sum rescaled) only when a score passes the one that set it by 2^8, so
+ *    most pages rescale nothing.  In f16 the weights are taken 2^7 times as
+ *    large, up to 2^15, which leaves their small parts more of its range; the
+ *    partials leave without that factor.
  * A row's position past the sequence's end counts nothing whatever it holds:
  * its scores are -inf and its values, which a weight of 0 would not keep NaN
  * out of, are cleared.
@@ -44,9 +46,11 @@ namespace {
 
 constexpr int kWaves = Q38_DECODE_TYPED_WAVES;
 constexpr int kGroup = Q38_ATTN_GROUP;
-/* A head's reference lies kRefBelow under the score that set it, and is
- * raised once a score passes it by kRefSlack: weights are at most 2^15. */
-constexpr float kRefBelow = 7.0f, kRefSlack = 15.0f;
+/* A head's reference lies kRefBelow under the score that set it, and is raised
+ * once a score passes that one by kRefSlack. */
+template <int T>
+constexpr float kRefBelow = T == Q38_KV_BF16 ? 0.0f : 7.0f;
+constexpr float kRefSlack = 8.0f;
 
 /* One page of one kv head as a wave holds it. */
 template <int T>
@@ -178,9 +182,9 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         }
     }
     const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    if (__any(mx > st.ref + kRefSlack)) {
+    if (__any(mx > st.ref + (kRefBelow<T> + kRefSlack))) {
         /* the page's maximum per head; heads that it does not raise keep theirs */
-        const float top = column_max(mx) - kRefBelow;
+        const float top = column_max(mx) - kRefBelow<T>;
         const float ref = fmaxf(st.ref, top);
         const float f = st.ref == -INFINITY ? 0.0f : q38_exp2(st.ref - ref);
         st.ref = ref;
@@ -480,11 +484,13 @@ Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
     done:
         /* both parts' rows added (lanes l and l ^ 32), the lower half of the wave
          * storing the even tiles and the upper half the odd ones */
+        constexpr float kUnit = T == Q38_KV_BF16 ? 1.0f : 0x1p-7f; /* 2^-kRefBelow */
         const float l = column_sum(st.l);
         if (lane < 8) {
-            red_m[wave][lane] = st.ref;
-            red_l[wave][lane] = l;
+            red_m[wave][lane] = st.ref + kRefBelow<T>;
+            red_l[wave][lane] = l * kUnit;
         }
+        const float out_unit = T == Q38_KV_Q8 ? st.cap * kUnit : kUnit;
         const bool upper = lane >= 32;
 #pragma unroll
         for (int n = 0; n < 16; n += 2) {
@@ -492,7 +498,7 @@ Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
             for (int i = 0; i < 4; ++i) {
                 const q38_halves e = q38_both_halves(st.o[n][i]), o = q38_both_halves(st.o[n + 1][i]);
                 float v = upper ? o.a + o.b : e.a + e.b;
-                if (T == Q38_KV_Q8) v *= st.cap;
+                v *= out_unit;
                 const int head = 4 * (g & 1) + i;
                 if (head < kGroup) red_o[wave][head][16 * (n + (upper ? 1 : 0)) + c] = v;
             }

@@ -196,7 +196,9 @@ Q38_DEV float q8k_quad(const f32x4 (&x)[4], int lane, uint32_t (&b)[4]) {
         uint32_t q[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) q[c] = (uint32_t)(min(q38_nearest_int(inv * x[i][c]), 127) + 128);
-        b[i] = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
+        /* the low bytes (a block whose inverse scale overflows has quants past them, and a scale of 0) */
+        b[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[3], q[2], 0x0C0C0400u),
+                                     __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0400u), 0x05040100u);
     }
     return scale;
 }

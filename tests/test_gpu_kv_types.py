@@ -94,12 +94,17 @@ def test_rows_of_every_size(pkg, ctx, ref, ty):
     if ty == "f16":
         x[9, :4] = [65504.0, 65519.0, 65520.0, -1e6]
         x[10] *= 1e-7                        # subnormal halves
+    if ty == "q8_k":
+        x[11, :512] *= 1e-38                 # no finite inverse scale
     v = x[::-1].copy()
     with Cache(pkg, ctx, ty, [32]) as c:
         c.kv.write(3, c.seqs[0], 0, 32, ctx.array(x), ctx.array(v))
         k, got_v = c.read(c.seqs[0], 0, 32)
-        assert np.array_equal(_bits(k), _bits(stored(x, c.ty)))
-        assert np.array_equal(_bits(got_v), _bits(stored(v, c.ty)))
+        zero = np.abs(x) < 3e-37 if ty == "q8_k" else np.zeros(x.shape, bool)  # zeros of either sign there
+        assert np.array_equal(np.where(zero, 0, _bits(k)), np.where(zero, 0, _bits(stored(x, c.ty))))
+        zero = zero[::-1]
+        assert np.array_equal(np.where(zero, 0, _bits(got_v)), np.where(zero, 0, _bits(stored(v, c.ty))))
+        assert not k[np.abs(x) < 3e-37].any() or ty != "q8_k"
         if ty == "q8_k":
             q, _, s = ref.q8k_split(ref.quantize_q8_k(x), 32, 1024)
             want = (q.reshape(32, 4, 256) * s[:, :, None]).astype(np.float32).reshape(32, 1024)
@@ -220,6 +225,30 @@ def _check(got, want, bound, normal=False):
     assert not normal or off_by(got, want) <= NORMAL_TOL
 
 
+def test_nan_in_one_head_stays_there(pkg, ctx):
+    """A query head of NaN, and a cached key of NaN or infinity in one kv head, leave the other heads as they are."""
+    P = 300
+    rng = np.random.default_rng(19)
+    K, V = _rows(rng, P), _rows(rng, P)
+    Q = rng.standard_normal((24, 256)).astype(np.float32)
+    for ty in sorted(TYPES):
+        with Cache(pkg, ctx, ty, [P]) as c:
+            for split in (None, 4096):
+                clean = _decode(ctx, c, K, V, Q, None, P, split=split).reshape(24, 256)
+                q = Q.copy()
+                q[8, 3] = np.nan
+                got = _decode(ctx, c, K, V, q, None, P, split=split).reshape(24, 256)
+                other = np.arange(24) != 8
+                assert np.isnan(got[8]).all() and np.array_equal(_bits(got[other]), _bits(clean[other]))
+                k = K.copy()
+                k[100, 256 * 2 + 7] = np.nan
+                got = _decode(ctx, c, k, V, Q, None, P, split=split).reshape(24, 256)
+                other = np.arange(24) // 6 != 2
+                assert np.array_equal(_bits(got[other]), _bits(clean[other]))
+                if ty != "q8_k":  # (a quantised row's NaN is a zero)
+                    assert np.isnan(got[~other]).all()
+
+
 def _decode(ctx, c, K, V, Q, G, P, split=None, appends=True, layer=3):
     """The last token appended by the call or beforehand; returns the output."""
     s = c.seqs[0]
@@ -273,7 +302,7 @@ def test_decode_splits(pkg, ctx, ty, split):
 
 
 @typed
-@pytest.mark.parametrize("case", ["rising", "falling", "peaked", "large", "tiny", "flat", "huge_q", "mixed_heads"])
+@pytest.mark.parametrize("case", ["rising", "falling", "peaked", "large", "tiny", "flat", "huge_q", "huge_v", "mixed_heads"])
 def test_decode_score_ranges(pkg, ctx, ty, case):
     """Running maxima that rise at every page or never, one weight that takes
     all, scores of hundreds, values that vanish, queries near the ends of the
@@ -302,6 +331,9 @@ def test_decode_score_ranges(pkg, ctx, ty, case):
         Q *= 1e18
         K *= 1e-18 if ty != "f16" else 1.0
         Q *= 1.0 if ty != "f16" else 1e-18
+    elif case == "huge_v":
+        V *= 1e32 if ty != "f16" else 1e4
+        Q *= 4
     elif case == "mixed_heads":
         Q *= (10.0 ** rng.uniform(-6, 1, (24, 1))).astype(np.float32)
     with Cache(pkg, ctx, ty, [P]) as c:

@@ -28,6 +28,8 @@ def stored(x: np.ndarray, ty: int) -> np.ndarray:
         # whole numbers: a quant of zero has no sign of its own
         q = np.nan_to_num(np.minimum(np.rint(inverse * b), np.float32(127.0))).astype(np.int32).astype(np.float32)
         scale = np.float32(1.0) / inverse
+        # a size under 127 / 3.4e38 has no finite inverse scale: its scale is 0, whatever the quants
+        q = np.where(np.isinf(inverse), np.float32(0.0), q)
     return np.where(m == 0, np.float32(0.0), q * scale).astype(np.float32).reshape(x.shape)
 
 
