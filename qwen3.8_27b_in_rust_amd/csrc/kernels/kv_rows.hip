@@ -16,9 +16,9 @@
  * rotation angles are formed once per workgroup (half as many heads in one,
  * and the angles twice, took 13.4 us where this takes 12.5).
  *
- * Measured (us, the kernel alone): 4096 tokens to Q8_K 12.5 (42 MB) and back
- * 7.8 (5.4 TB/s); 1531 tokens of 12 sequences to bf16 8.4 and back 6.3; 6
- * tokens to f16 4.3 and back 3.5, of which an empty launch is about half.
+ * Measured (us, the kernel alone): 4096 tokens to Q8_K 11.1 (42 MB) and back
+ * 7.8 (5.4 TB/s); 1531 tokens of 12 sequences to bf16 8.5 and back 6.2; 6
+ * tokens to f16 3.9 and back 3.3, of which an empty launch is about half.
  * Keys are held up by their arithmetic as much as by memory: the angles and,
  * per token and head, the f64 sum, the rotation and the quantiser are some
  * 500 instructions a wave and quad (1500 with four reductions one by one,
@@ -83,6 +83,21 @@ Q38_DEV int piece_at(bool key, int quad, int p) {
     return key ? (p >> 2) * 16 + 4 * quad + (p & 3) : (p >> 4) * 64 + quad * 16 + (p & 15);
 }
 
+/* A lane's value moved within its row of 16 (every lane of the row is active and
+ * has a source, so no value of the destination's own is kept: the move folds
+ * into the operation that reads it). */
+template <int CTRL>
+Q38_DEV float row_move(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL>
+Q38_DEV double row_move_f64(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
 /* Four tokens' wave-wide sums or maxima at once: each step halves the values a
  * lane still carries, so that lane l ends with token l % 4's, in 7 operations
  * where four separate reductions take 24 -- and what follows (a division, a
@@ -99,8 +114,8 @@ Q38_DEV V quad_reduce(const V (&s)[4], int lane, DPP1 xor1, DPP2 xor2, DPP4 ror4
 }
 Q38_DEV double quad_sum_f64(const double (&s)[4], int lane) {
     return quad_reduce(
-        s, lane, [](double x) { return q38_dpp_f64<0xB1>(x); }, [](double x) { return q38_dpp_f64<0x4E>(x); },
-        [](double x) { return q38_dpp_f64<0x124>(x); }, [](double x) { return q38_dpp_f64<0x128>(x); },
+        s, lane, [](double x) { return row_move_f64<0xB1>(x); }, [](double x) { return row_move_f64<0x4E>(x); },
+        [](double x) { return row_move_f64<0x124>(x); }, [](double x) { return row_move_f64<0x128>(x); },
         [](double x, double y) { return x + y; },
         [](double x) {
             uint64_t b = __builtin_bit_cast(uint64_t, x);
@@ -116,8 +131,8 @@ Q38_DEV double quad_sum_f64(const double (&s)[4], int lane) {
 }
 Q38_DEV float quad_max(const float (&s)[4], int lane) {
     return quad_reduce(
-        s, lane, [](float x) { return q38_dpp<0xB1>(x); }, [](float x) { return q38_dpp<0x4E>(x); },
-        [](float x) { return q38_dpp<0x124>(x); }, [](float x) { return q38_dpp<0x128>(x); },
+        s, lane, [](float x) { return row_move<0xB1>(x); }, [](float x) { return row_move<0x4E>(x); },
+        [](float x) { return row_move<0x124>(x); }, [](float x) { return row_move<0x128>(x); },
         [](float x, float y) { return fmaxf(x, y); },
         [](float x) {
             auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -128,7 +143,7 @@ Q38_DEV float quad_max(const float (&s)[4], int lane) {
 }
 /* Token i's value of one that lane l holds for token l % 4. */
 Q38_DEV float quad_value(float x, int i) {
-    return i == 0 ? q38_dpp<0x00>(x) : i == 1 ? q38_dpp<0x55>(x) : i == 2 ? q38_dpp<0xAA>(x) : q38_dpp<0xFF>(x);
+    return i == 0 ? row_move<0x00>(x) : i == 1 ? row_move<0x55>(x) : i == 2 ? row_move<0xAA>(x) : row_move<0xFF>(x);
 }
 
 /* RMSNorm and rotation of the quad's keys (q38_norm_rope4_cs, four at once).
@@ -148,7 +163,7 @@ Q38_DEV void norm_rope_quad(f32x4 (&x)[4], f32x4 w, int lane, const float (*cs)[
         /* lanes 0-7 hold dims 0 .. 31, lanes 8-15 their partners 32 .. 63 */
         f32x4 partner;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) partner[c] = q38_dpp<0x128>(x[i][c]);
+        for (int c = 0; c < 4; ++c) partner[c] = row_move<0x128>(x[i][c]);
         if (lane < 16) {
             const f32x4 *p = reinterpret_cast<const f32x4 *>(&cs[t[i]][4 * (lane & 7)][0]);
             const f32x4 p0 = p[0], p1 = p[1];
@@ -193,12 +208,15 @@ Q38_DEV float q8k_quad(const f32x4 (&x)[4], int lane, uint32_t (&b)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float inv = quad_value(inverse, i);
+        /* q38_nearest_int's sum holds the rounded quant in its low bits, and no
+         * product rounds past 127 (|x| <= |m|), so its low byte is the quant;
+         * plus 128 is the top bit turned.  (A block whose inverse scale
+         * overflows gets 0, and has a scale of 0.) */
         uint32_t q[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) q[c] = (uint32_t)(min(q38_nearest_int(inv * x[i][c]), 127) + 128);
-        /* the low bytes (a block whose inverse scale overflows has quants past them, and a scale of 0) */
-        b[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[3], q[2], 0x0C0C0400u),
-                                     __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0400u), 0x05040100u);
+        for (int c = 0; c < 4; ++c) q[c] = __float_as_uint(inv * x[i][c] + 12582912.0f);
+        b[i] = 0x80808080u ^ __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[3], q[2], 0x0C0C0400u),
+                                                   __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0400u), 0x05040100u);
     }
     return scale;
 }
