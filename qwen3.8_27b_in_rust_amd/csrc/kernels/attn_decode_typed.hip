@@ -137,9 +137,10 @@ Q38_DEV uint32_t pack16(uint16_t lo, uint16_t hi) { return (uint32_t)hi << 16 | 
 
 /* Scores of a page's tokens, the softmax update, the weighted sum of its
  * values.  valid: tokens of the page that count (16 but for the sequence's
- * last page). */
+ * last page); first: nothing is summed yet. */
 template <int T>
-Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64], float unscale, int valid, int lane) {
+Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64], float unscale, int valid, bool first,
+                       int lane) {
     const int c = lane & 15, g = lane >> 4;
     f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
     /* the queries are read from LDS at every page: an index that the compiler
@@ -189,13 +190,15 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         const float f = st.ref == -INFINITY ? 0.0f : q38_exp2(st.ref - ref);
         st.ref = ref;
         st.l *= f;
-        float fr[4];
+        if (!first) {
+            float fr[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * g + i, 64);
+            for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * g + i, 64);
 #pragma unroll
-        for (int n = 0; n < 16; ++n)
+            for (int n = 0; n < 16; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) st.o[n][i] *= fr[i];
+                for (int i = 0; i < 4; ++i) st.o[n][i] *= fr[i];
+        }
     }
     float vinv = 1.0f;
     if (T == Q38_KV_Q8) {
@@ -208,8 +211,10 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
             const float cap = __uint_as_float(min(e, 254u) << 23);
             const float f = st.cap / cap;
             st.cap = cap;
+            if (!first) {
 #pragma unroll
-            for (int n = 0; n < 16; ++n) st.o[n] *= f;
+                for (int n = 0; n < 16; ++n) st.o[n] *= f;
+            }
         }
         vinv = 1.0f / st.cap;
     }
@@ -225,7 +230,7 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
     /* the weights' parts: rows 0-5 the first (and, in a product of its own,
      * the third), rows 8-13 the second */
     q38_u32x2 a0, a1;
-    const bool first = c < 8;
+    const bool upper = c >= 8;
     if (T == Q38_KV_BF16) {
         uint32_t x[4], y[4];
 #pragma unroll
@@ -234,8 +239,8 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
             const float r = w[i] - __uint_as_float(hi);
             const uint32_t mid = __float_as_uint(r) & 0xFFFF0000u;
             const float lo = r - __uint_as_float(mid);
-            x[i] = first ? hi : mid;
-            y[i] = first ? __float_as_uint(lo) : 0u;
+            x[i] = upper ? mid : hi;
+            y[i] = upper ? 0u : __float_as_uint(lo);
         }
         a0 = q38_u32x2{__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
         a1 = q38_u32x2{__builtin_amdgcn_perm(y[1], y[0], 0x07060302u), __builtin_amdgcn_perm(y[3], y[2], 0x07060302u)};
@@ -245,7 +250,7 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         for (int i = 0; i < 4; ++i) {
             const _Float16 hi = (_Float16)w[i];
             const _Float16 lo = (_Float16)(w[i] - (float)hi);
-            x[i] = __builtin_bit_cast(uint16_t, first ? hi : lo);
+            x[i] = __builtin_bit_cast(uint16_t, upper ? lo : hi);
         }
         a0 = q38_u32x2{pack16(x[0], x[1]), pack16(x[2], x[3])};
     }
@@ -361,10 +366,10 @@ Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
     __shared__ q38_u32x4 q_frag[kQSets][8][64];
     __shared__ float q_unscale[8];
     __shared__ __attribute__((aligned(16))) NewRows new_rows;
-    __shared__ float rope_cs[kPre ? kWaves : 1][32][2];
-    __shared__ float red_o[kWaves][kGroup][Q38_ATTN_HEAD_DIM];
-    __shared__ float red_m[kWaves][8];
-    __shared__ float red_l[kWaves][8];
+    __shared__ __attribute__((aligned(16))) float rope_cs[kPre ? kWaves : 1][32][2];
+    __shared__ __attribute__((aligned(16))) float red_o[kWaves][kGroup][Q38_ATTN_HEAD_DIM];
+    __shared__ __attribute__((aligned(16))) float red_m[8][kWaves], red_l[8][kWaves]; /* [column][wave] */
+    __shared__ __attribute__((aligned(16))) float red_unit[kWaves]; /* of red_o */
     static_assert(kWaves == 8 && kGroup == 6, "a wave per query head, one for the key and one for the value");
 
     const int g_split = blockIdx.x, j = blockIdx.y, tid = threadIdx.x;
@@ -406,12 +411,12 @@ Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
     for (int u = 0; u < kDepth; ++u) fetch(buf[u], wave + kWaves * u);
 
     if (kPre && (forms_q || (forms_new && wave == kGroup))) {
-        q38_rope_table(rope_cs[wave], lane, pos, a.theta_scale);
+        q38_rope_table_half(rope_cs[wave], lane & 31, pos, a.theta_scale);
         /* the lanes read each other's entries below: LDS serves a wave in
          * order, the fence keeps the compiler to it */
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        q38_norm_rope4_cs(x, xw, lane, rope_cs[wave]);
+        q38_norm_rope_row(x, xw, lane, rope_cs[wave]);
     }
     if (forms_q) {
         x *= Q38_SCORE_LOG2;
@@ -477,67 +482,77 @@ Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
                     valid = t_end - t_begin - Q38_PAGE_TOKENS * at;
                     if (has_pos && a.k_new != nullptr) put_new_token<T>(buf[u], new_rows, valid - 1, lane);
                 }
-                page_step<T>(st, buf[u], q_frag, unscale, valid, lane);
+                page_step<T>(st, buf[u], q_frag, unscale, valid, at == wave, lane);
                 fetch(buf[u], at + kWaves * kDepth);
             }
         }
     done:
-        /* both parts' rows added (lanes l and l ^ 32), the lower half of the wave
-         * storing the even tiles and the upper half the odd ones */
+        /* Both parts' rows added (lanes l and l ^ 32): exchanging tile n's upper
+         * half for tile n + 1's lower one puts both tiles' pairs side by side, the
+         * even tile's sums in the lower half of the wave, the odd one's in the
+         * upper. */
         constexpr float kUnit = T == Q38_KV_BF16 ? 1.0f : 0x1p-7f; /* 2^-kRefBelow */
         const float l = column_sum(st.l);
         if (lane < 8) {
-            red_m[wave][lane] = st.ref + kRefBelow<T>;
-            red_l[wave][lane] = l * kUnit;
+            red_m[lane][wave] = st.ref + kRefBelow<T>;
+            red_l[lane][wave] = l * kUnit;
         }
-        const float out_unit = T == Q38_KV_Q8 ? st.cap * kUnit : kUnit;
-        const bool upper = lane >= 32;
+        if (lane == 0) red_unit[wave] = T == Q38_KV_Q8 ? st.cap * kUnit : kUnit;
+        float *out = &red_o[wave][4 * (g & 1)][16 * (g >> 1) + c];
 #pragma unroll
         for (int n = 0; n < 16; n += 2) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const q38_halves e = q38_both_halves(st.o[n][i]), o = q38_both_halves(st.o[n + 1][i]);
-                float v = upper ? o.a + o.b : e.a + e.b;
-                v *= out_unit;
-                const int head = 4 * (g & 1) + i;
-                if (head < kGroup) red_o[wave][head][16 * (n + (upper ? 1 : 0)) + c] = v;
+                auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(st.o[n][i]), __float_as_uint(st.o[n + 1][i]), false, false);
+                if (i < 2 || (g & 1) == 0) /* heads 4 (g & 1) + i < 6 */
+                    out[i * Q38_ATTN_HEAD_DIM + 16 * n] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
             }
         }
     }
     __syncthreads();
 
-    /* a thread per 3 outputs: heads tid / 256, + 2, + 4 of one dim */
-    const int d = tid & 255;
-#pragma unroll
-    for (int k = 0; k < kGroup / 2; ++k) {
-        const int hh = 2 * k + (tid >> 8);
-        float m[kWaves], l[kWaves], o[kWaves];
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            m[w] = red_m[w][hh];
-            l[w] = red_l[w][hh];
-            o[w] = red_o[w][hh][d];
-        }
-        float M = -INFINITY, L = 0.0f, O = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, w < n_pages ? m[w] : -INFINITY);
+    /* a wave per head joins the waves' parts, lane l dims 4l .. 4l + 3 */
+    if (wave >= kGroup) return;
+    float M = -INFINITY, L = 0.0f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    const int h = j * kGroup + wave;
+    const size_t at = (size_t)h * Q38_ATTN_HEAD_DIM + 4 * lane;
+    if (n_pages == 1) {
+        M = red_m[wave][0];
+        L = red_l[wave][0];
+        O = q38_ld4(&red_o[0][wave][4 * lane]) * red_unit[0];
+    } else {
+        float m[kWaves], f[kWaves];
+        f32x4 o[kWaves];
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float f = q38_exp2(m[w] - M);
-            L += w < n_pages ? l[w] * f : 0.0f;
-            O += w < n_pages ? o[w] * f : 0.0f;
+            m[w] = w < n_pages ? red_m[wave][w] : -INFINITY;
+            o[w] = q38_ld4(&red_o[w][wave][4 * lane]);
+            M = fmaxf(M, m[w]);
         }
-        const int h = j * kGroup + hh;
-        if (nsplit == 1) {
-            float r = O / L;
-            if (a.gate != nullptr) r *= q38_sigmoid(a.gate[((size_t)b * Q38_ATTN_HEADS + h) * a.gate_head_stride + d]);
-            a.out[(size_t)b * Q38_ATTN_Q_DIM + h * Q38_ATTN_HEAD_DIM + d] = r;
-        } else {
-            a.part_o[((size_t)g_split * Q38_ATTN_HEADS + h) * Q38_ATTN_HEAD_DIM + d] = O;
-            if (d == 0) {
-                a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 0] = M;
-                a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 1] = L;
-            }
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            f[w] = q38_exp2(m[w] - M);
+            /* a wave without pages has left nothing there */
+            L += w < n_pages ? red_l[wave][w] * f[w] : 0.0f;
+            const float fu = f[w] * red_unit[w];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[e] = w < n_pages ? __builtin_fmaf(fu, o[w][e], O[e]) : O[e];
+        }
+    }
+    if (nsplit == 1) {
+        f32x4 r = O / L;
+        if (a.gate != nullptr) {
+            const f32x4 gate = q38_ld4(a.gate + ((size_t)b * Q38_ATTN_HEADS + h) * a.gate_head_stride + 4 * lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] *= q38_sigmoid(gate[e]);
+        }
+        q38_st4(a.out + (size_t)b * Q38_ATTN_Q_DIM + at, r);
+    } else {
+        q38_st4(a.part_o + (size_t)g_split * Q38_ATTN_Q_DIM + at, O);
+        if (lane == 0) {
+            a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 0] = M;
+            a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 1] = L;
         }
     }
 }

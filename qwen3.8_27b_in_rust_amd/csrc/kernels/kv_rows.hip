@@ -83,21 +83,6 @@ Q38_DEV int piece_at(bool key, int quad, int p) {
     return key ? (p >> 2) * 16 + 4 * quad + (p & 3) : (p >> 4) * 64 + quad * 16 + (p & 15);
 }
 
-/* A lane's value moved within its row of 16 (every lane of the row is active and
- * has a source, so no value of the destination's own is kept: the move folds
- * into the operation that reads it). */
-template <int CTRL>
-Q38_DEV float row_move(float x) {
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
-}
-template <int CTRL>
-Q38_DEV double row_move_f64(double x) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, x);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xF, 0xF, true);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-
 /* Four tokens' wave-wide sums or maxima at once: each step halves the values a
  * lane still carries, so that lane l ends with token l % 4's, in 7 operations
  * where four separate reductions take 24 -- and what follows (a division, a
@@ -114,25 +99,15 @@ Q38_DEV V quad_reduce(const V (&s)[4], int lane, DPP1 xor1, DPP2 xor2, DPP4 ror4
 }
 Q38_DEV double quad_sum_f64(const double (&s)[4], int lane) {
     return quad_reduce(
-        s, lane, [](double x) { return row_move_f64<0xB1>(x); }, [](double x) { return row_move_f64<0x4E>(x); },
-        [](double x) { return row_move_f64<0x124>(x); }, [](double x) { return row_move_f64<0x128>(x); },
+        s, lane, [](double x) { return q38_row_move_f64<0xB1>(x); }, [](double x) { return q38_row_move_f64<0x4E>(x); },
+        [](double x) { return q38_row_move_f64<0x124>(x); }, [](double x) { return q38_row_move_f64<0x128>(x); },
         [](double x, double y) { return x + y; },
-        [](double x) {
-            uint64_t b = __builtin_bit_cast(uint64_t, x);
-            auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
-            auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
-            x = __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
-            b = __builtin_bit_cast(uint64_t, x);
-            auto lo2 = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
-            auto hi2 = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
-            return __builtin_bit_cast(double, (uint64_t)hi2[0] << 32 | lo2[0]) +
-                   __builtin_bit_cast(double, (uint64_t)hi2[1] << 32 | lo2[1]);
-        });
+        [](double x) { return q38_rows_sum_f64(x); });
 }
 Q38_DEV float quad_max(const float (&s)[4], int lane) {
     return quad_reduce(
-        s, lane, [](float x) { return row_move<0xB1>(x); }, [](float x) { return row_move<0x4E>(x); },
-        [](float x) { return row_move<0x124>(x); }, [](float x) { return row_move<0x128>(x); },
+        s, lane, [](float x) { return q38_row_move<0xB1>(x); }, [](float x) { return q38_row_move<0x4E>(x); },
+        [](float x) { return q38_row_move<0x124>(x); }, [](float x) { return q38_row_move<0x128>(x); },
         [](float x, float y) { return fmaxf(x, y); },
         [](float x) {
             auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -143,7 +118,7 @@ Q38_DEV float quad_max(const float (&s)[4], int lane) {
 }
 /* Token i's value of one that lane l holds for token l % 4. */
 Q38_DEV float quad_value(float x, int i) {
-    return i == 0 ? row_move<0x00>(x) : i == 1 ? row_move<0x55>(x) : i == 2 ? row_move<0xAA>(x) : row_move<0xFF>(x);
+    return i == 0 ? q38_row_move<0x00>(x) : i == 1 ? q38_row_move<0x55>(x) : i == 2 ? q38_row_move<0xAA>(x) : q38_row_move<0xFF>(x);
 }
 
 /* RMSNorm and rotation of the quad's keys (q38_norm_rope4_cs, four at once).
@@ -160,20 +135,7 @@ Q38_DEV void norm_rope_quad(f32x4 (&x)[4], f32x4 w, int lane, const float (*cs)[
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         x[i] = x[i] * quad_value(scale, i) * w;
-        /* lanes 0-7 hold dims 0 .. 31, lanes 8-15 their partners 32 .. 63 */
-        f32x4 partner;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) partner[c] = row_move<0x128>(x[i][c]);
-        if (lane < 16) {
-            const f32x4 *p = reinterpret_cast<const f32x4 *>(&cs[t[i]][4 * (lane & 7)][0]);
-            const f32x4 p0 = p[0], p1 = p[1];
-            const float cosine[4] = {p0[0], p0[2], p1[0], p1[2]}, sine[4] = {p0[1], p0[3], p1[1], p1[3]};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float own = x[i][c] * cosine[c], other = partner[c] * sine[c];
-                x[i][c] = lane < 8 ? own - other : other + own;
-            }
-        }
+        q38_rope_row(x[i], lane, cs[t[i]]);
     }
 }
 
@@ -327,7 +289,7 @@ Q38_DEV void kv_append(const Args &a) {
     if (turns) {
         /* the page's angles: a half-wave per token */
         const int t = tid >> 5;
-        if (t >= sp.t0 && t < sp.t1) q38_rope_table(cs[t], lane & 31, sp.pos0 + t - sp.t0, a.theta_scale);
+        if (t >= sp.t0 && t < sp.t1) q38_rope_table_half(cs[t], lane & 31, sp.pos0 + t - sp.t0, a.theta_scale);
         __syncthreads();
     }
     if (!live) return;

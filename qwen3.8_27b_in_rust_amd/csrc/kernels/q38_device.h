@@ -143,6 +143,33 @@ Q38_DEV double q38_wave_sum_f64(double x) {
            __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
 }
 
+/* The sum of the four rows' values (each row of 16 lanes holding its own). */
+Q38_DEV double q38_rows_sum_f64(double x) {
+    uint64_t b = __builtin_bit_cast(uint64_t, x);
+    auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+    auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+    x = __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+    b = __builtin_bit_cast(uint64_t, x);
+    lo = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+    hi = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+    return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+}
+
+/* A lane's value moved within its row of 16 (every lane of the row is active and
+ * has a source, so no value of the destination's own is kept: the move folds
+ * into the operation that reads it). */
+template <int CTRL>
+Q38_DEV float q38_row_move(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL>
+Q38_DEV double q38_row_move_f64(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
 /* s_waitcnt immediate (gfx9 encoding: vmcnt bits 3:0 and 15:14, expcnt 6:4,
  * lgkmcnt 11:8) that waits until at most `vm` vector memory operations and
  * `lgkm` LDS/scalar operations of this wave are outstanding. */

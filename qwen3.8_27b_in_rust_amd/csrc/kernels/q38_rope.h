@@ -84,3 +84,50 @@ Q38_DEV void q38_norm_rope4_cs(f32x4 &x, f32x4 w, int lane, const float (*cs)[2]
     for (int c = 0; c < 4; ++c) x[c] = x[c] * scale * w[c];
     q38_rope_lanes_cs(x, lane, cs);
 }
+
+/* q38_rope_table for a half-wave whose lane li is the wave's lane li or li + 32:
+ * which lanes keep a step's angle is a constant mask rather than a comparison. */
+Q38_DEV void q38_rope_table_half(float (*cs)[2], int li, int position, float theta_scale) {
+    float theta = (float)position, mine = theta;
+#pragma unroll
+    for (int i = 1; i < 32; ++i) {
+        theta *= theta_scale;
+        mine = __builtin_amdgcn_inverse_ballot_w64(1ull << i | 1ull << (i + 32)) ? theta : mine;
+    }
+    float sine, cosine;
+    sincosf(mine, &sine, &cosine);
+    cs[li][0] = cosine;
+    cs[li][1] = sine;
+}
+
+/* q38_rope_lanes_cs with the partner lane (l ^ 8) reached inside its row of 16. */
+Q38_DEV void q38_rope_row(f32x4 &x, int lane, const float (*cs)[2]) {
+    f32x4 partner;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) partner[c] = q38_row_move<0x128>(x[c]);
+    if (lane < 16) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(&cs[4 * (lane & 7)][0]);
+        const f32x4 p0 = p[0], p1 = p[1];
+        const float cosine[4] = {p0[0], p0[2], p1[0], p1[2]}, sine[4] = {p0[1], p0[3], p1[1], p1[3]};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            /* lanes 0-7 hold dims 0 .. 31, lanes 8-15 their partners 32 .. 63 */
+            const float own = x[c] * cosine[c], other = partner[c] * sine[c];
+            x[c] = lane < 8 ? own - other : other + own;
+        }
+    }
+}
+
+/* q38_norm_rope4_cs by row moves.  Every f32 square is exact in f64, so the
+ * fused sums are the plain ones. */
+Q38_DEV void q38_norm_rope_row(f32x4 &x, f32x4 w, int lane, const float (*cs)[2]) {
+    double ss = (double)x.x * (double)x.x;
+#pragma unroll
+    for (int c = 1; c < 4; ++c) ss = __builtin_fma((double)x[c], (double)x[c], ss);
+    ss += q38_row_move_f64<0xB1>(ss);
+    ss += q38_row_move_f64<0x4E>(ss);
+    ss += q38_row_move_f64<0x141>(ss);
+    ss += q38_row_move_f64<0x140>(ss);
+    x = x * q38_rms_scale_of(q38_rows_sum_f64(ss)) * w;
+    q38_rope_row(x, lane, cs);
+}
