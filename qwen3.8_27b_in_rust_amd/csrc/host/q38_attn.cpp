@@ -1199,11 +1199,12 @@ struct decode_plan {
  * few rounds of large splits win: the fewest rounds that splits of at most
  * Q38_MAX_SPLIT_TOKENS allow, and the smallest split that fits them.  Measured
  * against one workgroup per CU by the total but at most 1024 tokens for batches,
- * as over f32 rows (us, Q8_K): 3 sequences of 2K-32K 22.7 against 33.6, 24 of
- * 200-3000 20.8 against 30.0, 16 of 2K-32K 69.8 against 78.1, 64 of 100-20000
- * 230 against 278.  Where every sequence has kOneSplitTokens at most, one split
- * each needs no merge launch: one sequence of 17 / 128 / 256 tokens 6.6 / 7.6 /
- * 8.9 against 9.6 / 9.8 / 10.0 (512: 11.6 against 10.2). */
+ * as over f32 rows (us, f16 and Q8_K): 3 sequences of 2K-32K 33.1 against 44.9
+ * and 21.0 against 30.0, 24 of 200-3000 25.9 / 34.7 and 19.2 / 27.0, 16 of 2K-32K
+ * 120 / 125 and 68 / 74, 64 of 100-20000 417 / 458 and 226 / 266.  Where every
+ * sequence has kOneSplitTokens at most, one split each needs no merge launch: one
+ * Q8_K sequence of 17 / 128 / 256 tokens 5.1 / 5.7 / 7.2 against 7.7 / 7.8 / 7.9
+ * (512: 12.4 against 8.1). */
 constexpr int kOneSplitTokens = 256;
 int typed_split_tokens(const q38_ctx *ctx, int n_seq, const int32_t *positions, long max_tokens) {
     if (max_tokens <= kOneSplitTokens) return kOneSplitTokens;

@@ -31,6 +31,14 @@
  * A row's position past the sequence's end counts nothing whatever it holds:
  * its scores are -inf and its values, which a weight of 0 would not keep NaN
  * out of, are cleared.
+ *
+ * Measured (us of a whole pass with its merge; one sequence; forming q in the
+ * kernel adds about 1): bf16 rows 17 tokens 5.6, 1021 8.8, 4096 10.7, 32K 26.9 (5.0
+ * TB/s), 128K 85.2 (6.3 TB/s, what pages read once in any order reach); Q8_K 5.8,
+ * 9.2, 10.2, 18.2 and 47.2 (5.8 TB/s).  Long 16-bit contexts are bound by memory,
+ * Q8_K ones by memory and the some 300 vector instructions a page and head that
+ * turn bytes into operands; short ones by the two launches and the chain
+ * arguments - page id - page - scores - join, 3-4 us of them.
  */
 #include "q38_kv_types.h"
 #include "q38_rope.h"
@@ -61,8 +69,10 @@ struct Page {
 };
 
 /* Loads of a page's block go through a buffer resource that ends with it (8-bit
- * rows: with its scales), or of no size at all: past the wave's last page they fetch nothing, without a branch
- * that would make the compiler wait for every load before it. */
+ * rows: with its scales), or of no size at all: past the wave's last page they
+ * fetch nothing, without a branch that would make the compiler wait for every
+ * load before it.  They are non-temporal, each page being read once: 128K tokens
+ * of bf16 84 us against 100 without, Q8_K 47.5 against 54.6. */
 Q38_DEV __amdgpu_buffer_rsrc_t block_rsrc(char *block, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(block, 0, bytes, 0x00027000);
 }
@@ -362,7 +372,10 @@ Q38_DEV void store_query(q38_u32x4 (*q)[8][64], int c, int lane, f32x4 x) {
 template <int T, bool kPre>
 Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
     constexpr int kQSets = T == Q38_KV_BF16 ? 2 : 1;
-    constexpr int kDepth = T == Q38_KV_Q8 ? 2 : 1; /* pages of a wave in registers */
+    /* pages of a wave in registers: two 16-bit ones leave too few for the rest
+     * (128K tokens 95 us against 85), 8-bit ones are half as large (1 / 2 / 3
+     * pages: 49.9 / 47.5 / 48.8 us) */
+    constexpr int kDepth = T == Q38_KV_Q8 ? 2 : 1;
     __shared__ q38_u32x4 q_frag[kQSets][8][64];
     __shared__ float q_unscale[8];
     __shared__ __attribute__((aligned(16))) NewRows new_rows;
@@ -385,11 +398,13 @@ Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
     const int n_pages = (t_end - t_begin + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS;
     const bool has_pos = t_end == pos + 1;
 
-    /* this wave's page ids, the i-th in lane i: pages wave, wave + 8, ... (64
-     * of them cover the largest split) */
+    /* this wave's first page id through the scalar cache: as a vector load it
+     * comes back to the workgroup's later waves behind the page loads of the
+     * earlier ones (forming q and reading 1021 tokens 9.6 us with it against
+     * 9.75, Q8_K 10.0 against 10.1) */
     static_assert(Q38_MAX_SPLIT_TOKENS <= 64 * kWaves * Q38_PAGE_TOKENS, "a lane per page id");
     const int32_t *pt = a.page_table + (size_t)seq * a.pt_stride + (t_begin >> 4);
-    const int my_pages = pt[min(wave + kWaves * lane, n_pages - 1)];
+    const int first_page = pt[min(wave, n_pages - 1)];
 
     /* the rows that this wave forms: query head `wave`, or the new key or value */
     const int q_stride = kPre ? 2 * Q38_ATTN_HEAD_DIM : Q38_ATTN_HEAD_DIM;
@@ -404,11 +419,15 @@ Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
      * a branch, so the rows above are waited for alone and the pages come in
      * while the queries are formed */
     Page<T> buf[kDepth];
+    load_page<T>(buf[0], a, first_page, wave < n_pages, j, lane);
+    /* all of its page ids, the i-th in lane i: pages wave, wave + 8, ... (64 of
+     * them cover the largest split) */
+    const int my_pages = pt[min(wave + kWaves * lane, n_pages - 1)];
     auto fetch = [&](Page<T> &p, int at) {
         load_page<T>(p, a, __builtin_amdgcn_readlane(my_pages, (at / kWaves) & 63), at < n_pages, j, lane);
     };
 #pragma unroll
-    for (int u = 0; u < kDepth; ++u) fetch(buf[u], wave + kWaves * u);
+    for (int u = 1; u < kDepth; ++u) fetch(buf[u], wave + kWaves * u);
 
     if (kPre && (forms_q || (forms_new && wave == kGroup))) {
         q38_rope_table_half(rope_cs[wave], lane & 31, pos, a.theta_scale);
