@@ -388,7 +388,9 @@ int q38_dequantize_q8_k(q38_ctx *ctx, int n_tokens, int width, const void *d_q8k
  * all three.  d_q8k needs a width that is a multiple of 256 and 16-byte
  * alignment; any width from 1 to 2^24 does without.  d_sum or d_y may be d_x or
  * d_residual itself (the residual stream updated in place), and no buffer
- * else may overlap an output.  It allocates nothing and may be captured. */
+ * else may overlap an output.  At most 2^24 - 1 rows a call; 2^22 - 1 of rows
+ * above 5120 values or that are not whole 16-byte vectors.  It allocates nothing
+ * and may be captured. */
 int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, const float *d_residual,
                      const float *d_weight, float *d_sum, float *d_y, void *d_q8k);
 

@@ -167,7 +167,7 @@ def device_count() -> int:
 
 def _i32(seq) -> bytes:
     """Host integers as the int32 array that a call reads (and does not keep)."""
-    return array.array("i", seq).tobytes()
+    return array.array("i", map(int, seq)).tobytes()
 
 
 class DeviceArray:

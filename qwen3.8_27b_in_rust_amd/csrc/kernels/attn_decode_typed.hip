@@ -442,8 +442,9 @@ Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
         if (T != Q38_KV_BF16) {
             float big = q38_max16(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
             big = column_max(big);
-            /* exponent of the largest, kept where 2^(10 - e) and its inverse are normal */
-            const int e = min(max((int)(__float_as_uint(big) >> 23) - 126, -100), 100);
+            /* exponent of the largest (129 at most, of infinity or NaN), kept where
+             * 2^(10 - e) and its inverse are normal */
+            const int e = max((int)(__float_as_uint(big) >> 23) - 126, -116);
             x *= __uint_as_float((uint32_t)(127 + 10 - e) << 23);
             if (lane == 0) q_unscale[wave] = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
         }

@@ -157,6 +157,27 @@ def test_many_rows(ctx):
     assert np.array_equal(other.download(), q8.download())
 
 
+@pytest.mark.parametrize("width,rows", [(4, (1 << 24) - 1), (1, (1 << 22) - 1)])
+def test_most_rows_of_a_call(pkg, ctx, width, rows):
+    """The most rows that one launch holds, in registers and value by value; one more is refused."""
+    rng = np.random.default_rng(12)
+    x = rng.standard_normal((rows, width), np.float32)
+    w = (1 + 0.2 * rng.standard_normal(width)).astype(np.float32)
+    d_x, d_w, d_y = ctx.array(x), ctx.array(w), ctx.empty((rows + 1, width))
+    d_y.upload(np.full((rows + 1, width), -7.0, np.float32))
+    ctx.add_rms_norm(rows, width, d_x, d_w, y=d_y)
+    got = d_y.download()
+    assert np.all(got[rows] == -7.0)
+    for at in (slice(0, 5000), slice(rows // 2, rows // 2 + 5000), slice(rows - 5000, rows)):
+        assert np.array_equal(got[at], _formula(x[at], None, w)[1])
+    assert not np.any(got[:rows] == -7.0)
+    d_more = ctx.empty((rows + 1, width))
+    with pytest.raises(pkg.Q38Error, match="too large"):
+        ctx.add_rms_norm(rows + 1, width, d_more, d_w, y=d_y)
+    for d in (d_x, d_w, d_y, d_more):
+        d.free()
+
+
 def test_captured_and_replayed(pkg, ctx):
     """Captured from the context's stream and replayed: every replay equals the
     eager call, with eager work between the replays."""

@@ -302,6 +302,36 @@ def test_decode_splits(pkg, ctx, ty, split):
 
 
 @typed
+@pytest.mark.parametrize("size", [2.0 ** 90, 2.0 ** 104, 2.0 ** 112])
+def test_decode_queries_near_the_end_of_f32(pkg, ctx, ty, size):
+    """Scores so large that each head's best token takes all: the output is
+    that token's value.  Scores lie at most some 2^7 from the query's size, far
+    from 2^128, and each is off by 264 u S at most (typed_rows.attend), S = sum
+    |q k| / 16: a head whose first two are further apart than twice that has
+    every other weight underflow.  Its value then passes through a sum over
+    one weight's two or three parts, the joins' products and a division: 2^-21
+    of it at most."""
+    P = 300
+    rng = np.random.default_rng(int(np.log2(size)))
+    K, V = _rows(rng, P), _rows(rng, P)
+    Q = (size * rng.standard_normal((24, 256))).astype(np.float32)
+    with Cache(pkg, ctx, ty, [P]) as c:
+        k, v = (stored(x, c.ty).reshape(P, 4, 256).astype(np.float64) for x in (K, V))
+        for split in (None, 4096):
+            got = _decode(ctx, c, K, V, Q, None, P, split=split).reshape(24, 256)
+            checked = 0
+            for h in range(24):
+                s = k[:, h // 6] @ Q[h].astype(np.float64) / 16
+                first, second = np.sort(s)[::-1][:2]
+                if first - second < 4 * 264 * 2.0 ** -24 * (np.abs(k[:, h // 6]) @ np.abs(Q[h].astype(np.float64)) / 16).max():
+                    continue
+                want = v[s.argmax(), h // 6]
+                assert np.all(np.abs(got[h] - want) <= 2.0 ** -21 * np.abs(want)), h
+                checked += 1
+            assert checked >= 20
+
+
+@typed
 @pytest.mark.parametrize("case", ["rising", "falling", "peaked", "large", "tiny", "flat", "huge_q", "huge_v", "mixed_heads"])
 def test_decode_score_ranges(pkg, ctx, ty, case):
     """Running maxima that rise at every page or never, one weight that takes
