@@ -36,7 +36,7 @@
  * kernel adds about 1): bf16 rows 17 tokens 5.6, 1021 8.8, 4096 10.7, 32K 26.9 (5.0
  * TB/s), 128K 85.2 (6.3 TB/s, what pages read once in any order reach); Q8_K 5.8,
  * 9.2, 10.2, 18.2 and 47.2 (5.8 TB/s).  Long 16-bit contexts are bound by memory,
- * Q8_K ones by memory and the some 300 vector instructions a page and head that
+ * Q8_K ones by memory and the 273 vector instructions a page and head that mostly
  * turn bytes into operands; short ones by the two launches and the chain
  * arguments - page id - page - scores - join, 3-4 us of them.
  */
