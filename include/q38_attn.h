@@ -159,9 +159,8 @@ int q38_kv_read(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, float *d
  * position, then stored, as the value row is, in the cache's type; the result
  * equals q38_attn_pre's k rows stored with q38_kv_write, bit for bit.
  * Sequence ids must be distinct; pages are reserved as needed.  At most 2^25
- * rows a call.  Like q38_full_core it is for stream capture only where its
- * pages are reserved beforehand (a new page's id is uploaded), and its
- * positions are then the captured ones. */
+ * rows a call.  It cannot be captured (fails with -1): it keeps the page table
+ * and the prefill images in step on the host. */
 int q38_kv_append(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
                   const int32_t *n_tokens, const float *d_k_norm, const float *d_key, const float *d_value);
 

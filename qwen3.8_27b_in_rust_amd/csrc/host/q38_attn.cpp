@@ -1118,6 +1118,10 @@ int q38_kv_append(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
     if (!d_k_norm || !d_key || !d_value) return fail("NULL argument");
     if (((uintptr_t)d_k_norm | (uintptr_t)d_key | (uintptr_t)d_value) % 16 != 0)
         return fail("d_k_norm, d_key and d_value must be 16-byte aligned");
+    /* a replay would change rows without this call's part on the host: pages, and prefill images that end there */
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    Q38_HIP(hipStreamIsCapturing(kv->ctx->stream, &capture));
+    if (capture != hipStreamCaptureStatusNone) return fail("an append cannot be captured");
     for (int b = 0; b < n_seq; ++b) {
         if (n_tokens[b] == 0) continue;
         if (kv->reserve(seq_ids[b], pos0[b] + n_tokens[b])) return -1;

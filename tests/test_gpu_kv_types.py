@@ -2,6 +2,9 @@
 and every call that reads them, against plain 64-bit arithmetic on the values
 that the stored rows stand for (tests/typed_rows.py has the references and the
 derivation of the bounds)."""
+import ctypes
+import os
+
 import numpy as np
 import pytest
 from parity import decode_split
@@ -604,6 +607,29 @@ def test_refused_calls_change_nothing(pkg, ctx):
         assert state() == before
         for s in c.seqs:
             assert np.array_equal(c.read(s, 0, 40)[0], stored(K, c.ty))
+
+
+def test_append_is_not_captured(pkg, ctx):
+    """Refused while the context's stream captures (a replay would leave stale
+    prefill images), with the capture and the cache as they were."""
+    hip = ctypes.CDLL(os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "lib", "libamdhip64.so"))
+    rng = np.random.default_rng(17)
+    stream, graph = ctypes.c_void_p(ctx.stream()), ctypes.c_void_p()
+    with Cache(pkg, ctx, "f16", [40]) as c:
+        w, k = ctx.array(np.ones(256, np.float32)), ctx.array(_rows(rng, 40))
+        c.kv.write(3, c.seqs[0], 0, 40, k, k)
+        before = c.read(c.seqs[0], 0, 40)
+        ctx.sync()
+        assert hip.hipStreamBeginCapture(stream, 2) == 0
+        try:
+            with pytest.raises(pkg.Q38Error, match="captured"):
+                c.kv.append(3, c.seqs, [0], [4], w, k, k)
+        finally:
+            assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+        hip.hipGraphDestroy(graph)
+        assert all(np.array_equal(a, b) for a, b in zip(before, c.read(c.seqs[0], 0, 40)))
+        c.kv.append(3, c.seqs, [0], [4], w, k, k)
+        assert not np.array_equal(before[0], c.read(c.seqs[0], 0, 40)[0])
 
 
 @typed
