@@ -14,6 +14,7 @@ from __future__ import annotations
 import array
 import ctypes
 import os
+import struct
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 import numpy as np
@@ -167,7 +168,10 @@ def device_count() -> int:
 
 def _i32(seq) -> bytes:
     """Host integers as the int32 array that a call reads (and does not keep)."""
-    return array.array("i", map(int, seq)).tobytes()
+    try:
+        return struct.pack("%di" % len(seq), *seq)
+    except struct.error:  # values that convert to int
+        return array.array("i", map(int, seq)).tobytes()
 
 
 class DeviceArray:

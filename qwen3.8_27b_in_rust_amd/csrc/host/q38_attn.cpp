@@ -191,6 +191,8 @@ struct q38_ctx {
     hipFunction_t f_dequantize_q8k = nullptr;
     hipModule_t mod_typed = nullptr;
     hipFunction_t f_decode_typed[kKvTypeCount][2] = {}; /* from index 1 on; [1]: the pre step fused */
+    hipFunction_t f_decode_typed_one[kKvTypeCount][2] = {};
+    hipFunction_t f_decode_merge_one = nullptr;
     hipFunction_t f_attn_pre = nullptr;
     hipFunction_t f_gdn_decode = nullptr;
     hipFunction_t f_gdn_pre = nullptr;
@@ -468,6 +470,7 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
     Q38_HIP(hipModuleGetFunction(&ctx->f_decode_split_pre_many, ctx->mod_decode,
                                  "q38_attn_decode_split_pre_many"));
     Q38_HIP(hipModuleGetFunction(&ctx->f_decode_merge, ctx->mod_decode, "q38_attn_decode_merge"));
+    Q38_HIP(hipModuleGetFunction(&ctx->f_decode_merge_one, ctx->mod_decode, "q38_attn_decode_merge_one"));
     Q38_HIP(hipModuleGetFunction(&ctx->f_kv_copy, ctx->mod_decode, "q38_kv_copy"));
     Q38_HIP(hipModuleGetFunction(&ctx->f_attn_pre, ctx->mod_decode, "q38_attn_pre"));
     Q38_HIP(hipModuleGetFunction(&ctx->f_gdn_decode, ctx->mod_gdn, "q38_gdn_decode"));
@@ -502,8 +505,11 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
         Q38_HIP(rows_kernel(&ctx->f_kv_gather[i], "q38_kv_gather_" + ty));
         if (i == 0) continue;
         Q38_HIP(hipModuleGetFunction(&ctx->f_kv_split_typed[i], ctx->mod_prefill, ("q38_kv_split_mfma_" + ty).c_str()));
-        Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed[i][0], ctx->mod_typed, ("q38_attn_decode_" + ty).c_str()));
-        Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed[i][1], ctx->mod_typed, ("q38_attn_decode_" + ty + "_pre").c_str()));
+        for (int pre = 0; pre < 2; ++pre) {
+            const std::string name = "q38_attn_decode_" + ty + (pre ? "_pre" : "");
+            Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed[i][pre], ctx->mod_typed, name.c_str()));
+            Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed_one[i][pre], ctx->mod_typed, (name + "_one").c_str()));
+        }
     }
     const std::string p_proj = dir + "/proj.hsaco";
     Q38_HIP(hipModuleLoad(&ctx->mod_proj, p_proj.c_str()));
@@ -722,6 +728,7 @@ int q38_kernel_timer_start(q38_ctx *ctx, const char *kernel_name, int max_launch
     else if (name == "q38_attn_decode_split_one") f = ctx->f_decode_split_one;
     else if (name == "q38_attn_decode_split_pre_one") f = ctx->f_decode_split_pre_one;
     else if (name == "q38_attn_decode_merge") f = ctx->f_decode_merge;
+    else if (name == "q38_attn_decode_merge_one") f = ctx->f_decode_merge_one;
     else if (name == "q38_kv_copy") f = ctx->f_kv_copy;
     else if (name == "q38_attn_pre") f = ctx->f_attn_pre;
     else if (name == "q38_gdn_decode") f = ctx->f_gdn_decode;
@@ -770,8 +777,11 @@ int q38_kernel_timer_start(q38_ctx *ctx, const char *kernel_name, int max_launch
                 if (name == k.first + "_few") f = k.second->few;
             }
             if (i > 0 && name == "q38_kv_split_mfma_" + ty) f = ctx->f_kv_split_typed[i];
-            if (i > 0 && name == "q38_attn_decode_" + ty) f = ctx->f_decode_typed[i][0];
-            if (i > 0 && name == "q38_attn_decode_" + ty + "_pre") f = ctx->f_decode_typed[i][1];
+            for (int pre = 0; i > 0 && pre < 2; ++pre) {
+                const std::string decode = "q38_attn_decode_" + ty + (pre ? "_pre" : "");
+                if (name == decode) f = ctx->f_decode_typed[i][pre];
+                if (name == decode + "_one") f = ctx->f_decode_typed_one[i][pre];
+            }
         }
         for (int v = 0; v < kNormVectors; ++v)
             for (int w = 0; w < 2; ++w)
@@ -1207,8 +1217,8 @@ struct decode_plan {
  * and 21.0 against 30.0, 24 of 200-3000 25.9 / 34.7 and 19.2 / 27.0, 16 of 2K-32K
  * 120 / 125 and 68 / 74, 64 of 100-20000 417 / 458 and 226 / 266.  Where every
  * sequence has kOneSplitTokens at most, one split each needs no merge launch: one
- * Q8_K sequence of 17 / 128 / 256 tokens 5.1 / 5.7 / 7.2 against 7.7 / 7.8 / 7.9
- * (512: 12.4 against 8.1). */
+ * Q8_K sequence of 17 / 128 / 256 tokens 5.1 / 5.9 / 7.2 against 7.7 / 7.8 / 8.0
+ * (512: 10.0 against 8.2). */
 constexpr int kOneSplitTokens = 256;
 int typed_split_tokens(const q38_ctx *ctx, int n_seq, const int32_t *positions, long max_tokens) {
     if (max_tokens <= kOneSplitTokens) return kOneSplitTokens;
@@ -1264,10 +1274,17 @@ struct decode_pre {
 struct decode_launch {
     q38_decode_args a;
     q38_merge_args m;
-    hipFunction_t f = nullptr;
+    /* one sequence of a typed cache: the arguments that its kernels take instead */
+    bool one = false;
+    q38_decode_typed_one_args a_one;
+    q38_merge_one_args m_one;
+    hipFunction_t f = nullptr, f_merge = nullptr;
     unsigned grid_x = 0;
     unsigned block = 0;
     bool merge = false;
+
+    void *split_args() { return one ? static_cast<void *>(&a_one) : &a; }
+    void *merge_args() { return one ? static_cast<void *>(&m_one) : &m; }
 };
 
 /* Arguments of one decode launch for n_seq <= Q38_MAX_BATCH sequences whose
@@ -1344,11 +1361,19 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
                                  : arg_pages ? ctx->f_decode_split_pre : ctx->f_decode_split_pre_many)
                           : (one ? ctx->f_decode_split_one : arg_pages ? ctx->f_decode_split : ctx->f_decode_split_many);
     L->block = (unsigned)ctx->decode_block;
+    L->one = kv->type != 0 && n_seq == 1;
+    L->f_merge = L->one ? ctx->f_decode_merge_one : ctx->f_decode_merge;
     if (kv->type != 0) {
-        L->f = ctx->f_decode_typed[kv->type][pre != nullptr ? 1 : 0];
+        L->f = (L->one ? ctx->f_decode_typed_one : ctx->f_decode_typed)[kv->type][pre != nullptr ? 1 : 0];
         L->block = 64 * Q38_DECODE_TYPED_WAVES;
     }
     L->grid_x = (unsigned)total;
+    if (L->one) {
+        memcpy(&L->a_one, &a, offsetof(q38_decode_typed_one_args, seq));
+        L->a_one.seq = seq_ids[0];
+        L->a_one.pos = positions[0];
+        L->m_one = {a.part_o, a.part_ml, a.gate, d_out, total, a.gate_head_stride};
+    }
     q38_merge_args &m = L->m;
     memset(&m, 0, sizeof(m));
     m.part_o = a.part_o;
@@ -1371,8 +1396,8 @@ int decode_chunk(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
     if (build_decode(kv, slot, n_seq, seq_ids, positions, d_q, d_k_new, d_v_new, d_gate, d_out, plan,
                      plan.work_bytes > 0 ? work : nullptr, pre, -1, &L))
         return -1;
-    if (ctx->launch(L.f, L.grid_x, Q38_ATTN_KV_HEADS, 1, L.block, &L.a)) return -1;
-    if (L.merge && ctx->launch(ctx->f_decode_merge, n_seq, Q38_ATTN_HEADS, 4, 256, &L.m)) return -1;
+    if (ctx->launch(L.f, L.grid_x, Q38_ATTN_KV_HEADS, 1, L.block, L.split_args())) return -1;
+    if (L.merge && ctx->launch(L.f_merge, n_seq, Q38_ATTN_HEADS, 4, 256, L.merge_args())) return -1;
     return 0;
 }
 
@@ -1612,13 +1637,13 @@ struct q38_decode_graph {
     void node_params(Call &k, bool merge, hipKernelNodeParams *p, void **arg) {
         *p = hipKernelNodeParams{};
         if (!merge) {
-            *arg = &k.L.a;
+            *arg = k.L.split_args();
             p->func = reinterpret_cast<void *>(k.L.f);
             p->gridDim = dim3(k.L.grid_x, Q38_ATTN_KV_HEADS, 1);
             p->blockDim = dim3(k.L.block, 1, 1);
         } else {
-            *arg = &k.L.m;
-            p->func = reinterpret_cast<void *>(kv->ctx->f_decode_merge);
+            *arg = k.L.merge_args();
+            p->func = reinterpret_cast<void *>(k.L.f_merge);
             p->gridDim = dim3(n_seq, Q38_ATTN_HEADS, 4);
             p->blockDim = dim3(256, 1, 1);
         }
@@ -1952,6 +1977,7 @@ static_assert(offsetof(q38_kv_rows_few_args, seq) == offsetof(q38_kv_rows_args, 
 static_assert(offsetof(q38_decode_args, head_pages) == sizeof(q38_decode_typed_args) &&
                   offsetof(q38_decode_args, split_base) == offsetof(q38_decode_typed_args, split_base),
               "q38_decode_typed_args is the front of q38_decode_args");
+static_assert(offsetof(q38_decode_typed_one_args, seq) == offsetof(q38_decode_args, seq), "one head");
 static_assert(sizeof(q38_prefill_merge_args) <= 4096, "prefill merge arguments exceed 4 KiB");
 
 int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens, const float *d_q,

@@ -407,6 +407,8 @@ extern "C" __global__ __launch_bounds__(64 * Q38_DECODE_WAVES, Q38_DECODE_MIN_WG
     decode_split<true, false>(a);
 }
 
+namespace {
+
 /* Combine the splits of each (sequence, head): rescale every partial to the
  * common max, sum, normalise, gate.  grid (n_seq, 24, 4): z picks 64 of the
  * 256 dims, so 96 workgroups share a sequence's merge.  Thread (sl, dl)
@@ -414,17 +416,14 @@ extern "C" __global__ __launch_bounds__(64 * Q38_DECODE_WAVES, Q38_DECODE_MIN_WG
  * sum and output in registers); up to 8 splits' (m, l, o) are loaded at
  * once, so a merge of up to 128 splits costs one memory round trip.  The 16
  * per-thread results of each dim quad then meet in LDS. */
-extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_merge(q38_merge_args a) {
+template <typename Args>
+Q38_DEV void merge_splits(const Args &a, int b, int base, int n) {
     constexpr int kBatch = 8;
     __shared__ f32x4 red_o[16][16];
     __shared__ float red_m[16][16];
     __shared__ float red_l[16][16];
-    const int b = blockIdx.x;
     const int h = blockIdx.y;
     const int dq = blockIdx.z;
-    const int base = a.split_base[b];
-    const int n = a.split_base[b + 1] - base;
-    if (n <= 1) return;
     const int tid = threadIdx.x;
     const int dl = tid & 15;
     const int sl = tid >> 4;
@@ -495,6 +494,17 @@ extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_merge(q38_merg
         }
         q38_st4(a.out + off, r);
     }
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_merge(q38_merge_args a) {
+    const int b = blockIdx.x, base = a.split_base[b], n = a.split_base[b + 1] - base;
+    if (n > 1) merge_splits(a, b, base, n);
+}
+
+extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_merge_one(q38_merge_one_args a) {
+    if (a.n_splits > 1) merge_splits(a, 0, 0, a.n_splits);
 }
 
 /* Rows <-> pages.  grid (n_tokens, 2), 256 threads x float4 = one 1024-float row. */

@@ -33,9 +33,9 @@
  * out of, are cleared.
  *
  * Measured (us of a whole pass with its merge; one sequence; forming q in the
- * kernel adds about 1): bf16 rows 17 tokens 5.6, 1021 8.8, 4096 10.7, 32K 26.9 (5.0
- * TB/s), 128K 85.2 (6.3 TB/s, what pages read once in any order reach); Q8_K 5.8,
- * 9.2, 10.2, 18.2 and 47.2 (5.8 TB/s).  Long 16-bit contexts are bound by memory,
+ * kernel adds about 1): bf16 rows 17 tokens 5.2, 1021 8.6, 4096 10.4, 32K 26.5 (5.1
+ * TB/s), 128K 85.2 (6.3 TB/s, what pages read once in any order reach); Q8_K 5.5,
+ * 8.9, 10.0, 17.7 and 46.9 (5.8 TB/s).  Long 16-bit contexts are bound by memory,
  * Q8_K ones by memory and the 273 vector instructions a page and head that mostly
  * turn bytes into operands; short ones by the two launches and the chain
  * arguments - page id - page - scores - join, 3-4 us of them.
@@ -81,8 +81,8 @@ Q38_DEV q38_u32x4 ld_block(__amdgpu_buffer_rsrc_t r, int at) {
     return __builtin_bit_cast(q38_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, kStream));
 }
 
-template <int T>
-Q38_DEV void load_page(Page<T> &p, const q38_decode_typed_args &a, int page, bool live, int j, int lane) {
+template <int T, typename Args>
+Q38_DEV void load_page(Page<T> &p, const Args &a, int page, bool live, int j, int lane) {
     const int scales = q38_kv_scales_offset(j);
     const int bytes = !live ? 0 : T == Q38_KV_Q8 ? scales + Q38_PAGE_TOKENS * 4 : q38_kv_block_bytes<T>();
     const __amdgpu_buffer_rsrc_t k = block_rsrc(q38_kv_block<T>(a.kpool, page, j), bytes);
@@ -369,8 +369,22 @@ Q38_DEV void store_query(q38_u32x4 (*q)[8][64], int c, int lane, f32x4 x) {
     }
 }
 
-template <int T, bool kPre>
-Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
+/* The sequence of a split: b in the batch, its first split and their number. */
+struct Where {
+    int b, seq, pos, base, n;
+};
+Q38_DEV Where find(const q38_decode_typed_one_args &a, int) { return {0, a.seq, a.pos, 0, a.total_splits}; }
+Q38_DEV Where find(const q38_decode_typed_args &a, int g) {
+    /* entries past n_seq are INT_MAX */
+    int b = 0;
+    for (int i0 = 1; i0 < a.n_seq; i0 += 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b += a.split_base[i0 + i] <= g ? 1 : 0;
+    return {b, a.seq[b], a.pos[b], a.split_base[b], a.split_base[b + 1] - a.split_base[b]};
+}
+
+template <int T, bool kPre, typename Args>
+Q38_DEV void decode_typed(const Args &a) {
     constexpr int kQSets = T == Q38_KV_BF16 ? 2 : 1;
     /* pages of a wave in registers: two 16-bit ones leave too few for the rest
      * (128K tokens 95 us against 85), 8-bit ones are half as large (1 / 2 / 3
@@ -387,20 +401,15 @@ Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
 
     const int g_split = blockIdx.x, j = blockIdx.y, tid = threadIdx.x;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    /* the sequence of this split: entries past n_seq are INT_MAX */
-    int b = 0;
-    for (int i0 = 1; i0 < a.n_seq; i0 += 8)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) b += a.split_base[i0 + i] <= g_split ? 1 : 0;
-    const int seq = a.seq[b], pos = a.pos[b];
-    const int split = g_split - a.split_base[b], nsplit = a.split_base[b + 1] - a.split_base[b];
+    const Where at_seq = find(a, g_split);
+    const int b = at_seq.b, seq = at_seq.seq, pos = at_seq.pos, split = g_split - at_seq.base, nsplit = at_seq.n;
     const int t_begin = split * a.split_tokens, t_end = min(pos + 1, t_begin + a.split_tokens);
     const int n_pages = (t_end - t_begin + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS;
     const bool has_pos = t_end == pos + 1;
 
     /* this wave's first page id through the scalar cache: as a vector load it
      * comes back to the workgroup's later waves behind the page loads of the
-     * earlier ones (forming q and reading 1021 tokens 9.6 us with it against
+     * earlier ones (forming q and reading 1021 tokens took 9.6 us with it against
      * 9.75, Q8_K 10.0 against 10.1) */
     static_assert(Q38_MAX_SPLIT_TOKENS <= 64 * kWaves * Q38_PAGE_TOKENS, "a lane per page id");
     const int32_t *pt = a.page_table + (size_t)seq * a.pt_stride + (t_begin >> 4);
@@ -579,13 +588,17 @@ Q38_DEV void decode_typed(const q38_decode_typed_args &a) {
 
 }  // namespace
 
-#define Q38_DECODE_KERNELS(name, T)                                                                                  \
-    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name(q38_decode_typed_args a) {            \
-        decode_typed<T, false>(a);                                                                                   \
-    }                                                                                                                \
-    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name##_pre(q38_decode_typed_args a) {      \
-        decode_typed<T, true>(a);                                                                                    \
+/* name: a batch; name_one: one sequence; with pre, the pre step of full_core in the kernel. */
+#define Q38_DECODE_KERNEL(name, T, PRE)                                                                             \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name(q38_decode_typed_args a) {     \
+        decode_typed<T, PRE>(a);                                                                                    \
+    }                                                                                                               \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name##_one(q38_decode_typed_one_args a) { \
+        decode_typed<T, PRE>(a);                                                                                    \
     }
-Q38_DECODE_KERNELS(f16, Q38_KV_F16)
-Q38_DECODE_KERNELS(bf16, Q38_KV_BF16)
-Q38_DECODE_KERNELS(q8k, Q38_KV_Q8)
+Q38_DECODE_KERNEL(f16, Q38_KV_F16, false)
+Q38_DECODE_KERNEL(f16_pre, Q38_KV_F16, true)
+Q38_DECODE_KERNEL(bf16, Q38_KV_BF16, false)
+Q38_DECODE_KERNEL(bf16_pre, Q38_KV_BF16, true)
+Q38_DECODE_KERNEL(q8k, Q38_KV_Q8, false)
+Q38_DECODE_KERNEL(q8k_pre, Q38_KV_Q8, true)

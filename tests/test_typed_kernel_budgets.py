@@ -41,7 +41,7 @@ def decode(tmp_path_factory):
 
 def test_decode(decode):
     got = _budgets(decode)
-    assert sorted(got) == sorted(f"q38_attn_decode_{t}{p}" for t in TYPES for p in ("", "_pre"))
+    assert sorted(got) == sorted(f"q38_attn_decode_{t}{p}" for t in TYPES for p in ("", "_pre", "_one", "_pre_one"))
     for name, (vgpr, scratch) in got.items():
         assert scratch == 0 and vgpr <= 256, (name, vgpr, scratch)
 
