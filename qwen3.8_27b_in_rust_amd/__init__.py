@@ -166,11 +166,15 @@ def device_count() -> int:
     return n.value
 
 
+# packers of up to a launch's sequences
+_PACK = [struct.Struct("%di" % n).pack for n in range(65)]
+
+
 def _i32(seq) -> bytes:
     """Host integers as the int32 array that a call reads (and does not keep)."""
     try:
-        return struct.pack("%di" % len(seq), *seq)
-    except struct.error:  # values that convert to int
+        return _PACK[len(seq)](*seq)
+    except (IndexError, struct.error):  # more of them, or values that convert to int
         return array.array("i", map(int, seq)).tobytes()
 
 

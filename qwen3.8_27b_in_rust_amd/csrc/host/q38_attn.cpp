@@ -1036,14 +1036,10 @@ int launch_rows(q38_kv *kv, const q38_ctx::RowsKernel &f, int slot, int n_seq, c
     for (int b = 0; b < n_seq;) {
         q38_kv_rows_args a;
         memset(&a, 0, sizeof(a));
-        a.kpool = kv->kslot(slot);
-        a.vpool = kv->vslot(slot);
-        a.page_table = kv->d_page_table;
-        a.k_rows = static_cast<char *>(d_k) + row * Q38_ATTN_KV_DIM * elem_bytes;
-        a.v_rows = static_cast<char *>(d_v) + row * Q38_ATTN_KV_DIM * elem_bytes;
-        a.k_norm = d_k_norm;
-        a.theta_scale = kv->ctx->rope_theta_scale;
-        a.pt_stride = kv->pt_stride;
+        a.head = {kv->kslot(slot), kv->vslot(slot), kv->d_page_table,
+                  static_cast<char *>(d_k) + row * Q38_ATTN_KV_DIM * elem_bytes,
+                  static_cast<char *>(d_v) + row * Q38_ATTN_KV_DIM * elem_bytes, d_k_norm, kv->ctx->rope_theta_scale,
+                  kv->pt_stride};
         int n = 0;
         for (; b < n_seq && n < Q38_MAX_BATCH; ++b) {
             if (n_tokens[b] == 0) continue;
@@ -1057,14 +1053,15 @@ int launch_rows(q38_kv *kv, const q38_ctx::RowsKernel &f, int slot, int n_seq, c
         if (n == 0) break;
         a.n_seq = n;
         for (int i = n + 1; i < Q38_MAX_BATCH + 8; ++i) a.page_base[i] = INT_MAX;
-        q38_kv_rows_few_args few;
+        q38_kv_rows_few_args few = {};
         const bool is_few = n <= Q38_KV_ROWS_FEW;
         if (is_few) {
-            memcpy(&few, &a, offsetof(q38_kv_rows_few_args, seq));
-            memcpy(few.seq, a.seq, sizeof(few.seq));
-            memcpy(few.pos0, a.pos0, sizeof(few.pos0));
-            memcpy(few.row_base, a.row_base, sizeof(few.row_base));
-            memcpy(few.page_base, a.page_base, sizeof(few.page_base));
+            few.head = a.head;
+            for (int i = 0; i < n; ++i) {
+                few.seq[i] = a.seq[i];
+                few.pos0[i] = a.pos0[i];
+                few.n_tokens[i] = a.row_base[i + 1] - a.row_base[i];
+            }
         }
         if (kv->ctx->launch(is_few ? f.few : f.many, (unsigned)a.page_base[n], 2, 1, Q38_KV_ROWS_THREADS,
                             is_few ? (void *)&few : (void *)&a))
@@ -1973,7 +1970,6 @@ retry:
 static_assert(sizeof(q38_prefill_args) <= 4096, "prefill arguments exceed 4 KiB");
 static_assert(sizeof(q38_decode_args) <= 4096, "decode arguments exceed 4 KiB");
 /* a typed launch passes the same block, of which its kernel takes the front */
-static_assert(offsetof(q38_kv_rows_few_args, seq) == offsetof(q38_kv_rows_args, seq), "one head");
 static_assert(offsetof(q38_decode_args, head_pages) == sizeof(q38_decode_typed_args) &&
                   offsetof(q38_decode_args, split_base) == offsetof(q38_decode_typed_args, split_base),
               "q38_decode_typed_args is the front of q38_decode_args");

@@ -40,20 +40,35 @@ struct PageSpan {
     int page;     /* physical page */
 };
 
-template <typename Args>
-Q38_DEV PageSpan page_span(const Args &a, int x) {
+Q38_DEV PageSpan page_span(const q38_kv_rows_head &a, int seq, int first, int n, int row, int page_base, int x) {
+    const int lp = (first >> 4) + x - page_base;
+    const int p0 = max(first, lp * Q38_PAGE_TOKENS);
+    const int p1 = min(first + n, (lp + 1) * Q38_PAGE_TOKENS);
+    return {p0 & 15, (p0 & 15) + p1 - p0, row + p0 - first, p0, a.page_table[(size_t)seq * a.pt_stride + lp]};
+}
+Q38_DEV PageSpan page_span(const q38_kv_rows_args &a, int x) {
     /* the sequence that holds page x: entries past n_seq are INT_MAX, so eight
      * are compared at a time, without a chain of dependent scalar loads */
     int b = 0;
     for (int i0 = 1; i0 < a.n_seq; i0 += 8)
 #pragma unroll
         for (int i = 0; i < 8; ++i) b += a.page_base[i0 + i] <= x ? 1 : 0;
-    const int first = a.pos0[b], n = a.row_base[b + 1] - a.row_base[b];
-    const int lp = (first >> 4) + x - a.page_base[b];
-    const int p0 = max(first, lp * Q38_PAGE_TOKENS);
-    const int p1 = min(first + n, (lp + 1) * Q38_PAGE_TOKENS);
-    return {p0 & 15, (p0 & 15) + p1 - p0, a.row_base[b] + p0 - first, p0,
-            a.page_table[(size_t)a.seq[b] * a.pt_stride + lp]};
+    return page_span(a.head, a.seq[b], a.pos0[b], a.row_base[b + 1] - a.row_base[b], a.row_base[b], a.page_base[b], x);
+}
+Q38_DEV PageSpan page_span(const q38_kv_rows_few_args &a, int x) {
+    int seq = a.seq[0], first = a.pos0[0], n = a.n_tokens[0], row = 0, page_base = 0;
+    int pages = ((first + n - 1) >> 4) - (first >> 4) + 1;
+#pragma unroll
+    for (int i = 1; i < Q38_KV_ROWS_FEW; ++i) {
+        const bool on = x >= page_base + pages; /* past the sequence before: never past the last */
+        page_base += on ? pages : 0;
+        row += on ? n : 0;
+        seq = on ? a.seq[i] : seq;
+        first = on ? a.pos0[i] : first;
+        n = on ? a.n_tokens[i] : n;
+        pages = ((first + n - 1) >> 4) - (first >> 4) + 1;
+    }
+    return page_span(a.head, seq, first, n, row, page_base, x);
 }
 
 /* LDS of one wave: a quad's elements in page order, 16-bit (2 KiB) or 8-bit. */
@@ -273,10 +288,10 @@ Q38_DEV void kv_append(const Args &a) {
     const bool key = blockIdx.y == 0;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int head = wave & 3, quad = wave >> 2;
-    const bool turns = key && a.k_norm != nullptr;
+    const bool turns = key && a.head.k_norm != nullptr;
     const int first = max(sp.t0 - 4 * quad, 0), last = min(sp.t1 - 4 * quad, 4);
     const bool live = first < last;
-    const float *rows = static_cast<const float *>(key ? a.k_rows : a.v_rows) +
+    const float *rows = static_cast<const float *>(key ? a.head.k_rows : a.head.v_rows) +
                         (size_t)sp.row0 * Q38_ATTN_KV_DIM + head * Q38_ATTN_HEAD_DIM + 4 * lane;
     f32x4 x[4], w = {0.f, 0.f, 0.f, 0.f};
     if (live) {
@@ -284,12 +299,12 @@ Q38_DEV void kv_append(const Args &a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             x[i] = q38_ld4_stream(rows + (size_t)(4 * quad + min(max(i, first), last - 1) - sp.t0) * Q38_ATTN_KV_DIM);
-        if (turns) w = q38_ld4(a.k_norm + 4 * lane);
+        if (turns) w = q38_ld4(a.head.k_norm + 4 * lane);
     }
     if (turns) {
         /* the page's angles: a half-wave per token */
         const int t = tid >> 5;
-        if (t >= sp.t0 && t < sp.t1) q38_rope_table_half(cs[t], lane & 31, sp.pos0 + t - sp.t0, a.theta_scale);
+        if (t >= sp.t0 && t < sp.t1) q38_rope_table_half(cs[t], lane & 31, sp.pos0 + t - sp.t0, a.head.theta_scale);
         __syncthreads();
     }
     if (!live) return;
@@ -299,7 +314,7 @@ Q38_DEV void kv_append(const Args &a) {
         for (int i = 0; i < 4; ++i) t[i] = 4 * quad + min(max(i, first), last - 1);
         norm_rope_quad(x, w, lane, cs, t);
     }
-    store_quad<T>(q38_kv_block<T>(key ? a.kpool : a.vpool, sp.page, head), stages[T == Q38_KV_F32 ? 0 : wave], key, head,
+    store_quad<T>(q38_kv_block<T>(key ? a.head.kpool : a.head.vpool, sp.page, head), stages[T == Q38_KV_F32 ? 0 : wave], key, head,
                   quad, first, last, lane, x);
 }
 
@@ -313,9 +328,9 @@ Q38_DEV void kv_gather(const Args &a) {
     const int head = wave & 3, quad = wave >> 2;
     const int first = max(sp.t0 - 4 * quad, 0), last = min(sp.t1 - 4 * quad, 4);
     if (first >= last) return;
-    char *block = q38_kv_block<T>(key ? a.kpool : a.vpool, sp.page, head);
+    char *block = q38_kv_block<T>(key ? a.head.kpool : a.head.vpool, sp.page, head);
     const size_t row = (size_t)(sp.row0 + 4 * quad - sp.t0) * Q38_ATTN_KV_DIM + head * Q38_ATTN_HEAD_DIM + 4 * lane;
-    void *rows = key ? a.k_rows : a.v_rows;
+    void *rows = key ? a.head.k_rows : a.head.v_rows;
     f32x4 x[4];
     q38_u32x2 raw[4];
     if (T == Q38_KV_F32) {

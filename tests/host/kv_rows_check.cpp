@@ -33,12 +33,20 @@ static hipError_t check_launch(hipFunction_t f, unsigned gx, unsigned gy, unsign
     if (f == kFew) {
         const q38_kv_rows_few_args &w = *static_cast<const q38_kv_rows_few_args *>(params[0]);
         memset(&a, 0xAB, sizeof(a)); /* what the kernel does not get */
-        memcpy(&a, &w, offsetof(q38_kv_rows_few_args, seq));
-        memcpy(a.seq, w.seq, sizeof(w.seq));
-        memcpy(a.pos0, w.pos0, sizeof(w.pos0));
-        memcpy(a.row_base, w.row_base, sizeof(w.row_base));
-        memcpy(a.page_base, w.page_base, sizeof(w.page_base));
-        if (a.n_seq > Q38_KV_ROWS_FEW) { printf("too many sequences for the small block\n"); exit(1); }
+        a.head = w.head;
+        /* the bases as the kernel finds them from the counts, 0 past the last sequence */
+        a.n_seq = 0;
+        a.row_base[0] = a.page_base[0] = 0;
+        for (int i = 0; i < Q38_KV_ROWS_FEW; ++i) {
+            a.seq[i] = w.seq[i];
+            a.pos0[i] = w.pos0[i];
+            const int pages = ((w.pos0[i] + w.n_tokens[i] - 1) >> 4) - (w.pos0[i] >> 4) + 1;
+            if ((pages > 0) != (w.n_tokens[i] > 0) || (pages > 0 && a.n_seq != i)) { printf("counts with a gap\n"); exit(1); }
+            a.n_seq += pages > 0;
+            a.row_base[i + 1] = a.row_base[i] + w.n_tokens[i];
+            a.page_base[i + 1] = a.page_base[i] + pages;
+        }
+        for (int i = a.n_seq + 1; i < Q38_MAX_BATCH + 8; ++i) a.page_base[i] = INT_MAX;
     } else {
         a = *static_cast<const q38_kv_rows_args *>(params[0]);
     }
@@ -49,6 +57,11 @@ static hipError_t check_launch(hipFunction_t f, unsigned gx, unsigned gy, unsign
 }
 static hipError_t check_copy(void *, const void *, size_t, hipMemcpyKind, hipStream_t) { return hipSuccess; }
 static hipError_t check_sync(hipStream_t) { return hipSuccess; }
+static hipError_t check_capturing(hipStream_t, hipStreamCaptureStatus *status) {
+    *status = hipStreamCaptureStatusNone;
+    return hipSuccess;
+}
+#define hipStreamIsCapturing check_capturing
 #define hipModuleLaunchKernel check_launch
 #define hipMemcpyAsync check_copy
 #define hipStreamSynchronize check_sync
@@ -127,10 +140,10 @@ static void walk(const Cache &c, int slot, const std::vector<int32_t> &seq, cons
     for (size_t l = 0; l < g_args.size(); ++l) {
         q38_kv_rows_args a;
         memcpy(&a, g_args[l].data(), sizeof(a));
-        REQUIRE(a.kpool == c.kv.kslot(slot) && a.vpool == c.kv.vslot(slot));
+        REQUIRE(a.head.kpool == c.kv.kslot(slot) && a.head.vpool == c.kv.vslot(slot));
         REQUIRE(a.n_seq >= 1 && a.n_seq <= Q38_MAX_BATCH && (unsigned)a.page_base[a.n_seq] == g_grid[l]);
-        const size_t row_off = (static_cast<char *>(a.k_rows) - d_k) / (1024 * elem);
-        REQUIRE(row_off == (size_t)(static_cast<char *>(a.v_rows) - d_v) / (1024 * elem));
+        const size_t row_off = (static_cast<char *>(a.head.k_rows) - d_k) / (1024 * elem);
+        REQUIRE(row_off == (size_t)(static_cast<char *>(a.head.v_rows) - d_v) / (1024 * elem));
         for (unsigned x = 0; x < g_grid[l]; ++x) {
             int b = 0;
             for (int i0 = 1; i0 < a.n_seq; i0 += 8)
