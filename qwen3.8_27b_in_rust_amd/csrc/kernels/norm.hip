@@ -60,30 +60,48 @@ Q38_DEV void store_q8k(const Q8kRow &r, int b, int lane, f32x4 y) {
  * dims 4 (i + NT v) .. + 3, so a wave's v-th vectors are 256 consecutive dims,
  * a Q8_K block.  Every load is issued at once and every value read once, so
  * the kernel runs at the memory's rate: 4096 rows of 5120 with all outputs
- * (17.14 bytes a value) 67 us, 5.4 TB/s; 1024 rows of 10240 6.7 TB/s; one row
- * 3.9 us a launch among others, where an empty one takes about as long.  A first
- * version that read its row twice and value by value took 187 us. */
+ * (17.14 bytes a value) 67 us, 5.4 TB/s; 512 rows of 12288 to 20480 6.5 to 6.7
+ * TB/s; one row 3.9 us a launch among others, where an empty one takes about as
+ * long.  A first version that read its row twice and value by value took 187 us. */
 template <int NT, int V>
 Q38_DEV void norm_row(const q38_norm_args &a) {
     __shared__ double part[NT / 64];
     const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, width = a.width;
     const size_t row = (size_t)t * width;
     const bool adds = a.residual != nullptr;
+    /* 1024 threads of long rows: the weights come after the rows' registers are
+     * added up, kAhead of them and one more a step, so that 64 registers do and
+     * a CU holds two rows (509 rows of 17408 22.8 us against 26.6, one row 6.7
+     * against 6.9; at 256 threads the same costs 70.0 against 67.9) */
+    constexpr bool kLate = NT == 1024 && V > 3;
+    constexpr int kAhead = 3;
     f32x4 h[V], r[V], w[V];
     /* threads past the row load its last vector and leave it out: no load
-     * sits under a branch, so all of them are in flight together */
+     * sits under a branch, so all of them are in flight together.  Nothing
+     * reads these rows again, and loads that say so (non-temporal) keep them
+     * from pushing the outputs out of the caches: 509 rows of 17408 from HBM
+     * 28.7 us against 35.1, 256 rows 15.1 against 18.9; from the last level's
+     * cache, as right after a small copy, they are slower (27.5 against 22.8,
+     * 1024 rows of 5120 18.3 against 14.3), and with the residual's row
+     * there and x's in HBM the two are even (after its producer 14.2 and 14.5 at
+     * 256 rows of 5120, 87.1 and 87.5 at 4096) */
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int d = min(4 * (tid + NT * v), width - 4);
-        h[v] = q38_ld4(a.x + row + d);
-        w[v] = q38_ld4(a.weight + d);
+        h[v] = q38_ld4_stream(a.x + row + d);
+        if (!kLate) w[v] = q38_ld4(a.weight + d);
     }
     if (adds) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) r[v] = q38_ld4(a.residual + row + min(4 * (tid + NT * v), width - 4));
+        for (int v = 0; v < V; ++v) r[v] = q38_ld4_stream(a.residual + row + min(4 * (tid + NT * v), width - 4));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] += r[v];
+    }
+    if (kLate) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int v = 0; v < kAhead; ++v) w[v] = q38_ld4(a.weight + min(4 * (tid + NT * v), width - 4));
     }
     double ss = 0.0;
 #pragma unroll
@@ -96,6 +114,7 @@ Q38_DEV void norm_row(const q38_norm_args &a) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int d = 4 * (tid + NT * v);
+        if (kLate && v + kAhead < V) w[v + kAhead] = q38_ld4(a.weight + min(4 * (tid + NT * (v + kAhead)), width - 4));
         if (d - 4 * lane >= width) break; /* past the row for the whole wave */
         const f32x4 y = h[v] * scale * w[v];
         if (d < width) {
@@ -113,7 +132,7 @@ Q38_DEV void norm_row(const q38_norm_args &a) {
 }  // namespace
 
 #define Q38_NORM_KERNEL(NT, V)                                                                              \
-    extern "C" __global__ __launch_bounds__(NT) void q38_add_rms_norm_##NT##_##V(q38_norm_args a) { norm_row<NT, V>(a); }
+    extern "C" __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 1) /* (waves a SIMD) */ void q38_add_rms_norm_##NT##_##V(q38_norm_args a) { norm_row<NT, V>(a); }
 Q38_NORM_KERNEL(256, 1)
 Q38_NORM_KERNEL(256, 2)
 Q38_NORM_KERNEL(256, 3)

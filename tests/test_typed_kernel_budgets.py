@@ -67,4 +67,4 @@ def test_norm(tmp_path_factory):
     got = _budgets(_assembly(tmp_path_factory, "norm"))
     assert len(got) == 12
     for name, (vgpr, scratch) in got.items():
-        assert scratch == 0 and vgpr <= (64 if name.endswith(("_1", "_2", "_3")) else 84), (name, vgpr, scratch)
+        assert scratch == 0 and vgpr <= (64 if "_1024_" in name or name.endswith(("_1", "_2", "_3")) else 84), (name, vgpr, scratch)
