@@ -16,9 +16,10 @@
  * rotation angles are formed once per workgroup (half as many heads in one,
  * and the angles twice, took 13.4 us where this takes 12.5).
  *
- * Measured (us, the kernel alone): 4096 tokens to Q8_K 11.1 (42 MB) and back
- * 7.8 (5.4 TB/s); 1531 tokens of 12 sequences to bf16 8.5 and back 6.2; 6
- * tokens to f16 3.9 and back 3.3, of which an empty launch is about half.
+ * Measured (us, calls of one kind in turn over buffers that no cache holds):
+ * 4096 tokens to Q8_K 9.9 (42 MB) and back 8.3 (5.1 TB/s); 1531 tokens of 12
+ * sequences to bf16 7.7 and back 6.3; 6 tokens to f16 3.9 and back 3.9, which
+ * is what the launches of so small calls take on the host.
  * Keys are held up by their arithmetic as much as by memory: the angles and,
  * per token and head, the f64 sum, the rotation and the quantiser are some
  * 500 instructions a wave and quad (1500 with four reductions one by one,
@@ -318,7 +319,13 @@ Q38_DEV void kv_append(const Args &a) {
                   quad, first, last, lane, x);
 }
 
-/* OUT16: rows in the cache's 16 bits, moved as they are (T is BF16 for both). */
+/* OUT16: rows in the cache's 16 bits, moved as they are (T is BF16 for both).
+ * The rows leave for a reader elsewhere, by non-temporal stores: 4096 tokens of
+ * Q8_K 8.3 us against 11.3, 1531 of BF16 6.3 against 8.7, as they are stored 6.1
+ * against 7.2 (a kernel that reads 4096 of them at once takes 1.2 us longer for
+ * it).  The append's pages stay in the caches for the call that reads them next:
+ * stored past them they cost 9.0 us instead of 9.9, and the gather after it 2
+ * more. */
 template <int T, bool OUT16, typename Args>
 Q38_DEV void kv_gather(const Args &a) {
     __shared__ Stage stages[T == Q38_KV_F32 ? 1 : kThreads / 64];
@@ -386,9 +393,10 @@ Q38_DEV void kv_gather(const Args &a) {
     for (int i = 0; i < 4; ++i) {
         if (i < first || i >= last) continue;
         if (OUT16)
-            *reinterpret_cast<q38_u32x2 *>(static_cast<uint16_t *>(rows) + row + (size_t)i * Q38_ATTN_KV_DIM) = raw[i];
+            __builtin_nontemporal_store(raw[i], reinterpret_cast<q38_u32x2 *>(static_cast<uint16_t *>(rows) + row +
+                                                                              (size_t)i * Q38_ATTN_KV_DIM));
         else
-            q38_st4(static_cast<float *>(rows) + row + (size_t)i * Q38_ATTN_KV_DIM, x[i]);
+            q38_st4_stream(static_cast<float *>(rows) + row + (size_t)i * Q38_ATTN_KV_DIM, x[i]);
     }
 }
 
