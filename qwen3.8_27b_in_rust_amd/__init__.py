@@ -11,7 +11,6 @@ __graft_entry__.py), or call the library through any FFI directly.
 """
 from __future__ import annotations
 
-import array
 import ctypes
 import os
 import struct
@@ -175,7 +174,7 @@ def _i32(seq) -> bytes:
     try:
         return _PACK[len(seq)](*seq)
     except (IndexError, struct.error):  # more of them, or values that convert to int
-        return array.array("i", map(int, seq)).tobytes()
+        return bytes((c_int32 * len(seq))(*map(int, seq)))
 
 
 class DeviceArray:

@@ -210,8 +210,27 @@ def test_far_positions(pkg, ctx, ty):
         step = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8, "q8_k": 0.5 / 127}[ty] * 1.01
         size = np.abs(want).max() if ty == "q8_k" else np.abs(want)
         assert np.all(np.abs(k.download() - want) <= step * size + 1e-5)
-        kv.read(3, s, pos, 30, k, v)
-        assert not k.download().any()
+        # one token's attention over all of them: the positions before are zero
+        # rows, whose weight is exp(0) each
+        q = (8 * rng.standard_normal((24, 256))).astype(np.float32)
+        d_o = ctx.empty((24, 256))
+        kv.attn_decode(7, [s], [pos + 29], ctx.array(q), d_o)
+        got, k, v = d_o.download(), k.download().astype(np.float64), v.download().astype(np.float64)
+        for h in range(24):
+            kk, vv = (x[:, 256 * (h // 6):256 * (h // 6) + 256] for x in (k, v))
+            sc = kk @ q[h] / 16
+            top = max(sc.max(), 0.0)
+            p = np.exp(sc - top) / (np.exp(sc - top).sum() + pos * np.exp(-top))
+            want = p @ vv
+            # typed_rows.attend's bound; a sum's longest chain is no n terms: a
+            # lane adds 4 weights a page, 128 at most of a split's 4096 / 8 tokens,
+            # the joins of lanes, waves and splits add fewer than 100
+            big = (np.abs(kk) @ np.abs(q[h])).max() / 16
+            e = 2 * (264 * big + 4 + np.abs(sc).max()) * 2.0 ** -24 + 256 * 2.0 ** -24 + 2.0 ** -21
+            bound = 1.01 * e * (p @ np.abs(vv)) + 30 * 2.0 ** -31 * np.abs(vv).max()
+            assert np.all(np.abs(got[h] - want) <= bound), h
+        kv.read(3, s, pos, 30, k_rest := ctx.empty((30, 1024)), ctx.empty((30, 1024)))
+        assert not k_rest.download().any()
     finally:
         kv.close()
 
