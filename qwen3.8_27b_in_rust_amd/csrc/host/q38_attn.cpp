@@ -273,6 +273,11 @@ struct q38_ctx {
     int launch(hipFunction_t f, unsigned gx, unsigned gy, unsigned gz, unsigned block, void *args,
                unsigned lds_bytes = 0) {
         void *params[] = {args};
+        return launch_params(f, gx, gy, gz, block, params, lds_bytes);
+    }
+
+    int launch_params(hipFunction_t f, unsigned gx, unsigned gy, unsigned gz, unsigned block, void **params,
+                      unsigned lds_bytes = 0) {
         /* the stamped form takes the grid in threads, a 32-bit count */
         if ((uint64_t)gx * block > 0xFFFFFFFFull) return fail("grid of %u workgroups too large", gx);
         const bool timing = f == timed && timer_used + 2 <= (int)timer_events.size();
@@ -1273,15 +1278,33 @@ struct decode_launch {
     q38_merge_args m;
     /* one sequence of a typed cache: the arguments that its kernels take instead */
     bool one = false;
-    q38_decode_typed_one_args a_one;
+    q38_decode_one_args a_one;
     q38_merge_one_args m_one;
     hipFunction_t f = nullptr, f_merge = nullptr;
     unsigned grid_x = 0;
     unsigned block = 0;
     bool merge = false;
 
-    void *split_args() { return one ? static_cast<void *>(&a_one) : &a; }
-    void *merge_args() { return one ? static_cast<void *>(&m_one) : &m; }
+    /* where the kernels' arguments are, kMaxParams of them at most */
+    static constexpr int kMaxParams = 10;
+    void split_params(void **p) {
+        if (!one) {
+            p[0] = &a;
+            return;
+        }
+        q38_decode_one_args &o = a_one;
+        void *const each[kMaxParams] = {&o.page_row, &o.q, &o.kpool, &o.vpool, &o.q_norm, &o.pos, &o.split_tokens,
+                                        &o.total_splits, &o.gate_head_stride, &o.rest};
+        std::copy(each, each + kMaxParams, p);
+    }
+    void merge_params(void **p) {
+        if (!one) {
+            p[0] = &m;
+            return;
+        }
+        void *const each[] = {&m_one.part_o, &m_one.part_ml, &m_one.gate, &m_one.out, &m_one.n_splits, &m_one.gate_head_stride};
+        std::copy(each, each + 6, p);
+    }
 };
 
 /* Arguments of one decode launch for n_seq <= Q38_MAX_BATCH sequences whose
@@ -1366,9 +1389,9 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
     }
     L->grid_x = (unsigned)total;
     if (L->one) {
-        memcpy(&L->a_one, &a, offsetof(q38_decode_typed_one_args, seq));
-        L->a_one.seq = seq_ids[0];
-        L->a_one.pos = positions[0];
+        L->a_one = {a.page_table + (size_t)seq_ids[0] * a.pt_stride, a.q, a.kpool, a.vpool, a.q_norm, positions[0],
+                    split_tokens, total, a.gate_head_stride,
+                    {a.k_new, a.v_new, a.gate, a.out, a.part_o, a.part_ml, a.k_norm, a.theta_scale, 0}};
         L->m_one = {a.part_o, a.part_ml, a.gate, d_out, total, a.gate_head_stride};
     }
     q38_merge_args &m = L->m;
@@ -1393,8 +1416,12 @@ int decode_chunk(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
     if (build_decode(kv, slot, n_seq, seq_ids, positions, d_q, d_k_new, d_v_new, d_gate, d_out, plan,
                      plan.work_bytes > 0 ? work : nullptr, pre, -1, &L))
         return -1;
-    if (ctx->launch(L.f, L.grid_x, Q38_ATTN_KV_HEADS, 1, L.block, L.split_args())) return -1;
-    if (L.merge && ctx->launch(L.f_merge, n_seq, Q38_ATTN_HEADS, 4, 256, L.merge_args())) return -1;
+    void *params[decode_launch::kMaxParams];
+    L.split_params(params);
+    if (ctx->launch_params(L.f, L.grid_x, Q38_ATTN_KV_HEADS, 1, L.block, params)) return -1;
+    if (!L.merge) return 0;
+    L.merge_params(params);
+    if (ctx->launch_params(L.f_merge, n_seq, Q38_ATTN_HEADS, 4, 256, params)) return -1;
     return 0;
 }
 
@@ -1631,20 +1658,20 @@ struct q38_decode_graph {
                             arg_pages, &k.L);
     }
 
-    void node_params(Call &k, bool merge, hipKernelNodeParams *p, void **arg) {
+    void node_params(Call &k, bool merge, hipKernelNodeParams *p, void **params) {
         *p = hipKernelNodeParams{};
         if (!merge) {
-            *arg = k.L.split_args();
+            k.L.split_params(params);
             p->func = reinterpret_cast<void *>(k.L.f);
             p->gridDim = dim3(k.L.grid_x, Q38_ATTN_KV_HEADS, 1);
             p->blockDim = dim3(k.L.block, 1, 1);
         } else {
-            *arg = k.L.merge_args();
+            k.L.merge_params(params);
             p->func = reinterpret_cast<void *>(k.L.f_merge);
             p->gridDim = dim3(n_seq, Q38_ATTN_HEADS, 4);
             p->blockDim = dim3(256, 1, 1);
         }
-        p->kernelParams = arg;
+        p->kernelParams = params;
         p->sharedMemBytes = 0;
         p->extra = nullptr;
     }
@@ -1715,19 +1742,19 @@ int q38_decode_graph_add_decode(q38_decode_graph *g, const q38_decode_call *call
     for (q38_decode_graph::Call &o : g->calls) {
         if (g->build(o, g->positions, plan)) return -1;
         hipKernelNodeParams p;
-        void *arg = nullptr;
-        g->node_params(o, false, &p, &arg);
+        void *arg[decode_launch::kMaxParams];
+        g->node_params(o, false, &p, arg);
         Q38_HIP(hipGraphKernelNodeSetParams(o.split_node, &p));
-        g->node_params(o, true, &p, &arg);
+        g->node_params(o, true, &p, arg);
         Q38_HIP(hipGraphKernelNodeSetParams(o.merge_node, &p));
     }
     g->calls.push_back(k);
     q38_decode_graph::Call &kk = g->calls.back();
     hipKernelNodeParams p;
-    void *arg = nullptr;
-    g->node_params(kk, false, &p, &arg);
+    void *arg[decode_launch::kMaxParams];
+    g->node_params(kk, false, &p, arg);
     if (g->add_kernel(&kk.split_node, p)) return -1;
-    g->node_params(kk, true, &p, &arg);
+    g->node_params(kk, true, &p, arg);
     return g->add_kernel(&kk.merge_node, p);
 }
 
@@ -1819,10 +1846,10 @@ int q38_decode_graph_set_positions(q38_decode_graph *g, const int32_t *positions
     if (g->prepare(positions)) return -1;
     for (q38_decode_graph::Call &k : g->calls) {
         hipKernelNodeParams p;
-        void *arg = nullptr;
-        g->node_params(k, false, &p, &arg);
+        void *arg[decode_launch::kMaxParams];
+        g->node_params(k, false, &p, arg);
         Q38_HIP(hipGraphExecKernelNodeSetParams(g->exec, k.split_node, &p));
-        g->node_params(k, true, &p, &arg);
+        g->node_params(k, true, &p, arg);
         Q38_HIP(hipGraphExecKernelNodeSetParams(g->exec, k.merge_node, &p));
     }
     return 0;
@@ -1973,7 +2000,6 @@ static_assert(sizeof(q38_decode_args) <= 4096, "decode arguments exceed 4 KiB");
 static_assert(offsetof(q38_decode_args, head_pages) == sizeof(q38_decode_typed_args) &&
                   offsetof(q38_decode_args, split_base) == offsetof(q38_decode_typed_args, split_base),
               "q38_decode_typed_args is the front of q38_decode_args");
-static_assert(offsetof(q38_decode_typed_one_args, seq) == offsetof(q38_decode_args, seq), "one head");
 static_assert(sizeof(q38_prefill_merge_args) <= 4096, "prefill merge arguments exceed 4 KiB");
 
 int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens, const float *d_q,
@@ -2589,7 +2615,8 @@ int q38_dequantize_q8_k(q38_ctx *ctx, int n_tokens, int width, const void *d_q8k
     const size_t groups = ((size_t)n_tokens * width + 1023) / 1024;
     if (groups > 0xFFFFFFFFull / 256) return fail("%d rows of %d: too many for one call", n_tokens, width);
     q38_dequantize_args a = {d_q8k, d_x, width, n_tokens};
-    return ctx->launch(ctx->f_dequantize_q8k, (unsigned)groups, 1, 1, 256, &a);
+    void *params[] = {&a.q8k, &a.out, &a.width, &a.n_tokens};
+    return ctx->launch_params(ctx->f_dequantize_q8k, (unsigned)groups, 1, 1, 256, params);
 }
 
 int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, const float *d_residual,
@@ -2624,11 +2651,12 @@ int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, co
         overlaps(d_q8k, q_bytes, d_weight, (size_t)width * sizeof(float)))
         return fail("d_q8k overlaps an input");
     q38_norm_args a = {d_x, d_residual, d_weight, d_sum, d_y, d_q8k, width, n_tokens};
+    void *params[] = {&a.x, &a.residual, &a.weight, &a.sum, &a.y, &a.q8k, &a.width, &a.n_tokens};
     /* rows of whole 16-byte vectors stay in registers where they fit */
     const bool vectors = width % 4 == 0 && ((uintptr_t)d_x | (uintptr_t)d_residual | (uintptr_t)d_weight |
                                             (uintptr_t)d_sum | (uintptr_t)d_y) % 16 == 0;
     if (!vectors || width > 1024 * 4 * kNormVectors)
-        return ctx->launch(ctx->f_norm_any, (unsigned)n_tokens, 1, 1, 1024, &a);
+        return ctx->launch_params(ctx->f_norm_any, (unsigned)n_tokens, 1, 1, 1024, params);
     /* up to two rows per CU the chip has waves to spare, and 1024 threads a row
      * shorten the row's own chain; past that 256 keep more rows in flight and
      * waste fewer lanes on short ones (rows of 5120, us: 1 row 3.9 against 4.2,
@@ -2636,7 +2664,8 @@ int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, co
      * 17.3 against 11.7) */
     const int wide = width > 256 * 4 * kNormVectors || n_tokens <= 2 * ctx->cu_count;
     const int per = (wide ? 1024 : 256) * 4;
-    return ctx->launch(ctx->f_norm[wide][(width + per - 1) / per - 1], (unsigned)n_tokens, 1, 1, wide ? 1024 : 256, &a);
+    return ctx->launch_params(ctx->f_norm[wide][(width + per - 1) / per - 1], (unsigned)n_tokens, 1, 1,
+                              wide ? 1024 : 256, params);
 }
 
 int q38_gemv_q8_k(q38_ctx *ctx, int ggml_type, int rows, int width, const void *d_weights, const void *d_q8k,

@@ -503,8 +503,9 @@ extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_merge(q38_merg
     if (n > 1) merge_splits(a, b, base, n);
 }
 
-extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_merge_one(q38_merge_one_args a) {
-    if (a.n_splits > 1) merge_splits(a, 0, 0, a.n_splits);
+extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_merge_one(Q38_MERGE_ONE_PARAMS) {
+    const q38_merge_one_args a = {part_o, part_ml, gate, out, n_splits, gate_head_stride};
+    if (n_splits > 1) merge_splits(a, 0, 0, n_splits);
 }
 
 /* Rows <-> pages.  grid (n_tokens, 2), 256 threads x float4 = one 1024-float row. */

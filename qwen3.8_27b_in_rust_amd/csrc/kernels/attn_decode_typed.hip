@@ -33,9 +33,9 @@
  * out of, are cleared.
  *
  * Measured (us of a whole pass with its merge; one sequence; forming q in the
- * kernel adds about 1): bf16 rows 17 tokens 5.2, 1021 8.6, 4096 10.4, 32K 26.5 (5.1
- * TB/s), 128K 85.2 (6.3 TB/s, what pages read once in any order reach); Q8_K 5.5,
- * 8.9, 10.0, 17.7 and 46.9 (5.8 TB/s).  Long 16-bit contexts are bound by memory,
+ * kernel adds under 1): bf16 rows 17 tokens 5.1, 1021 8.3, 4096 10.0, 32K 26.3 (5.1
+ * TB/s), 128K 84.1 (6.4 TB/s, what pages read once in any order reach); Q8_K 5.3,
+ * 8.6, 9.6, 17.2 and 46.7 (5.8 TB/s).  Long 16-bit contexts are bound by memory,
  * Q8_K ones by memory and the 273 vector instructions a page and head that mostly
  * turn bytes into operands; short ones by the two launches and the chain
  * arguments - page id - page - scores - join, 3-4 us of them.
@@ -373,7 +373,18 @@ Q38_DEV void store_query(q38_u32x4 (*q)[8][64], int c, int lane, f32x4 x) {
 struct Where {
     int b, seq, pos, base, n;
 };
-Q38_DEV Where find(const q38_decode_typed_one_args &a, int) { return {0, a.seq, a.pos, 0, a.total_splits}; }
+/* One sequence's arguments under the names of a batch's. */
+struct OneArgs {
+    float *kpool, *vpool;
+    const int32_t *page_table;
+    const float *q, *k_new, *v_new, *gate;
+    float *out, *part_o, *part_ml;
+    const float *q_norm, *k_norm;
+    float theta_scale;
+    int32_t gate_head_stride, pos, split_tokens, total_splits;
+    static constexpr int32_t pt_stride = 0;
+};
+Q38_DEV Where find(const OneArgs &a, int) { return {0, 0, a.pos, 0, a.total_splits}; }
 Q38_DEV Where find(const q38_decode_typed_args &a, int g) {
     /* entries past n_seq are INT_MAX */
     int b = 0;
@@ -418,12 +429,20 @@ Q38_DEV void decode_typed(const Args &a) {
     /* the rows that this wave forms: query head `wave`, or the new key or value */
     const int q_stride = kPre ? 2 * Q38_ATTN_HEAD_DIM : Q38_ATTN_HEAD_DIM;
     const bool forms_q = wave < kGroup;
-    const bool forms_new = !forms_q && a.k_new != nullptr && has_pos;
+    bool forms_new = false;
     /* (a wave that forms nothing loads head 0's) */
     const float *src = a.q + ((size_t)b * Q38_ATTN_HEADS + j * kGroup + (forms_q ? wave : 0)) * q_stride;
-    if (forms_new) src = (wave == kGroup ? a.k_new : a.v_new) + (size_t)b * Q38_ATTN_KV_DIM + j * Q38_ATTN_HEAD_DIM;
+    const float *weight = a.q_norm;
+    if (!forms_q) {
+        /* (kept a branch: the other waves wait for none of these arguments) */
+        asm volatile("");
+        forms_new = a.k_new != nullptr && has_pos;
+        if (forms_new) src = (wave == kGroup ? a.k_new : a.v_new) + (size_t)b * Q38_ATTN_KV_DIM + j * Q38_ATTN_HEAD_DIM;
+        weight = a.k_norm;
+    }
     f32x4 x = q38_ld4(src + 4 * lane), xw = {0.f, 0.f, 0.f, 0.f};
-    if (kPre) xw = q38_ld4((forms_q ? a.q_norm : a.k_norm) + 4 * lane);
+    if (kPre) xw = q38_ld4(weight + 4 * lane);
+    __builtin_amdgcn_sched_barrier(0); /* on their way before the page id is waited for */
     /* the wave's first pages: no load from here to the first score sits under
      * a branch, so the rows above are waited for alone and the pages come in
      * while the queries are formed */
@@ -438,13 +457,17 @@ Q38_DEV void decode_typed(const Args &a) {
 #pragma unroll
     for (int u = 1; u < kDepth; ++u) fetch(buf[u], wave + kWaves * u);
 
-    if (kPre && (forms_q || (forms_new && wave == kGroup))) {
+    if (kPre) {
+        /* (every wave, so that the weights' load above stays before the pages':
+         * under a branch it would sink into it) */
         q38_rope_table_half(rope_cs[wave], lane & 31, pos, a.theta_scale);
         /* the lanes read each other's entries below: LDS serves a wave in
          * order, the fence keeps the compiler to it */
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        q38_norm_rope_row(x, xw, lane, rope_cs[wave]);
+        f32x4 y = x;
+        q38_norm_rope_row(y, xw, lane, rope_cs[wave]);
+        if (wave <= kGroup) x = y; /* the value goes as it is */
     }
     if (forms_q) {
         x *= Q38_SCORE_LOG2;
@@ -593,8 +616,10 @@ Q38_DEV void decode_typed(const Args &a) {
     extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name(q38_decode_typed_args a) {     \
         decode_typed<T, PRE>(a);                                                                                    \
     }                                                                                                               \
-    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name##_one(q38_decode_typed_one_args a) { \
-        decode_typed<T, PRE>(a);                                                                                    \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name##_one(Q38_DECODE_ONE_PARAMS) { \
+        decode_typed<T, PRE>(OneArgs{kpool, vpool, page_row, q, rest.k_new, rest.v_new, rest.gate, rest.out,        \
+                                     rest.part_o, rest.part_ml, q_norm, rest.k_norm, rest.theta_scale,              \
+                                     gate_head_stride, pos, split_tokens, total_splits});                           \
     }
 Q38_DECODE_KERNEL(f16, Q38_KV_F16, false)
 Q38_DECODE_KERNEL(f16_pre, Q38_KV_F16, true)

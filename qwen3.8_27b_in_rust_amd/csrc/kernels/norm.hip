@@ -129,24 +129,9 @@ Q38_DEV void norm_row(const q38_norm_args &a) {
     }
 }
 
-}  // namespace
-
-#define Q38_NORM_KERNEL(NT, V)                                                                              \
-    extern "C" __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 1) /* (waves a SIMD) */ void q38_add_rms_norm_##NT##_##V(q38_norm_args a) { norm_row<NT, V>(a); }
-Q38_NORM_KERNEL(256, 1)
-Q38_NORM_KERNEL(256, 2)
-Q38_NORM_KERNEL(256, 3)
-Q38_NORM_KERNEL(256, 4)
-Q38_NORM_KERNEL(256, 5)
-Q38_NORM_KERNEL(1024, 1)
-Q38_NORM_KERNEL(1024, 2)
-Q38_NORM_KERNEL(1024, 3)
-Q38_NORM_KERNEL(1024, 4)
-Q38_NORM_KERNEL(1024, 5)
-
 /* Rows that are not whole aligned vectors, or too long for registers: the row
  * is read again after its sum (from the cache), value by value. */
-extern "C" __global__ __launch_bounds__(1024) void q38_add_rms_norm_any(q38_norm_args a) {
+Q38_DEV void norm_row_any(const q38_norm_args &a) {
     __shared__ double part[16];
     const int t = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, width = a.width;
     const size_t row = (size_t)t * width;
@@ -177,17 +162,38 @@ extern "C" __global__ __launch_bounds__(1024) void q38_add_rms_norm_any(q38_norm
     }
 }
 
+}  // namespace
+
+#define Q38_NORM_KERNEL(NT, V)                                                                              \
+    extern "C" __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 1) /* (waves a SIMD) */                    \
+    void q38_add_rms_norm_##NT##_##V(Q38_NORM_PARAMS) {                                                     \
+        norm_row<NT, V>({x, residual, weight, sum, y, q8k, width, n_tokens});                               \
+    }
+Q38_NORM_KERNEL(256, 1)
+Q38_NORM_KERNEL(256, 2)
+Q38_NORM_KERNEL(256, 3)
+Q38_NORM_KERNEL(256, 4)
+Q38_NORM_KERNEL(256, 5)
+Q38_NORM_KERNEL(1024, 1)
+Q38_NORM_KERNEL(1024, 2)
+Q38_NORM_KERNEL(1024, 3)
+Q38_NORM_KERNEL(1024, 4)
+Q38_NORM_KERNEL(1024, 5)
+extern "C" __global__ __launch_bounds__(1024) void q38_add_rms_norm_any(Q38_NORM_PARAMS) {
+    norm_row_any({x, residual, weight, sum, y, q8k, width, n_tokens});
+}
+
 /* The values that Q8_K rows stand for: grid (ceil(n_tokens * width / 1024)),
  * 256 threads, 4 values each. */
-extern "C" __global__ __launch_bounds__(256) void q38_dequantize_q8k(q38_dequantize_args a) {
-    const size_t n = (size_t)a.n_tokens * a.width;
+extern "C" __global__ __launch_bounds__(256) void q38_dequantize_q8k(Q38_DEQUANTIZE_PARAMS) {
+    const size_t n = (size_t)n_tokens * width;
     const size_t i = 4 * ((size_t)blockIdx.x * 256 + threadIdx.x);
     if (i >= n) return;
-    const char *base = static_cast<const char *>(a.q8k);
+    const char *base = static_cast<const char *>(q8k);
     const uint32_t u = *reinterpret_cast<const uint32_t *>(base + i);
     const float s = reinterpret_cast<const float *>(base + n + n / 8)[i >> 8];
     f32x4 v;
 #pragma unroll
     for (int c = 0; c < 4; ++c) v[c] = (float)(int8_t)(u >> (8 * c)) * s;
-    q38_st4(a.out + i, v);
+    q38_st4(out + i, v);
 }

@@ -72,34 +72,35 @@ typedef struct {
     int32_t pos[Q38_MAX_BATCH]; /* attend over positions 0..pos inclusive */
     int32_t split_base[Q38_MAX_BATCH + 8]; /* past n_seq: INT_MAX */
 } q38_decode_typed_args;
-/* One sequence's: the same up to total_splits, which are all its own.  A launch
- * carries 128 bytes of arguments instead of 920 and the kernel looks for no
- * sequence: with the merge's likewise, a call of 1021 tokens takes 5.8 us on the
- * host instead of 6.8 and 9.3 in all instead of 9.6. */
+/* One sequence's, as its kernels take them: what a wave needs before its first
+ * loads as plain arguments, of which the first 14 words are in its registers
+ * when it starts, then the rest as a block.  Forming q and reading 1021 tokens of
+ * bf16 takes 9.0 us with it, 9.25 with all of them in a block, 9.6 with a
+ * batch's 920 bytes; 32K tokens 26.9, 27.8 and 28.1. */
 typedef struct {
-    float *kpool;              /* this layer's K pages: [max_pages][4][16][256] */
-    float *vpool;              /* this layer's V pages */
-    const int32_t *page_table; /* [max_seqs][pt_stride] physical page ids */
-    const float *q;            /* [n_seq][24][256], post-norm, post-RoPE (fused pre step:
-                                  raw [n_seq][24][512] q|gate rows) */
-    const float *k_new;        /* [n_seq][1024] appended at pos[b] first, or NULL (fused pre
-                                  step: the raw key, normed and rotated before the append) */
-    const float *v_new;        /* [n_seq][1024] or NULL */
-    const float *gate;         /* [n_seq][24][256] output gate logits, or NULL */
-    float *out;                /* [n_seq][24][256] */
-    float *part_o;             /* [total_splits][24][256] unnormalised partial outputs */
-    float *part_ml;            /* [total_splits][24][2]  (running max in log2 units, sum) */
-    const float *q_norm;       /* fused pre step: [256] q RMSNorm weight, else unused */
-    const float *k_norm;       /* fused pre step: [256] k RMSNorm weight */
-    float theta_scale;         /* fused pre step: RoPE 1e7^(-2/64) in f32 */
-    int32_t gate_head_stride;  /* floats between heads' gates: 256, or 512 in q|gate rows */
-    int32_t pt_stride;
-    int32_t n_seq;
-    int32_t split_tokens; /* multiple of Q38_PAGE_TOKENS */
-    int32_t total_splits;
-    int32_t seq;
+    const float *k_new, *v_new;
+    const float *gate;
+    float *out;
+    float *part_o, *part_ml;
+    const float *k_norm;
+    float theta_scale;
+    int32_t pad_;
+} q38_decode_one_rest;
+#define Q38_DECODE_ONE_PARAMS                                                                                  \
+    const int32_t *page_row, const float *q, float *kpool, float *vpool, const float *q_norm, int32_t pos,     \
+        int32_t split_tokens, int32_t total_splits, int32_t gate_head_stride, q38_decode_one_rest rest
+typedef struct {
+    const int32_t *page_row; /* the sequence's page table */
+    const float *q;
+    float *kpool;
+    float *vpool;
+    const float *q_norm;
     int32_t pos;
-} q38_decode_typed_one_args;
+    int32_t split_tokens;
+    int32_t total_splits;
+    int32_t gate_head_stride;
+    q38_decode_one_rest rest;
+} q38_decode_one_args; /* the same as the host keeps them */
 typedef struct {
     float *kpool;              /* this layer's K pages: [max_pages][4][16][256] */
     float *vpool;              /* this layer's V pages */
@@ -434,6 +435,11 @@ typedef struct {
     int32_t width;
     int32_t n_tokens;
 } q38_norm_args;
+/* The kernels take them one by one: plain arguments are in a wave's registers
+ * when it starts. */
+#define Q38_NORM_PARAMS                                                                               \
+    const float *x, const float *residual, const float *weight, float *sum, float *y, void *q8k,      \
+        int32_t width, int32_t n_tokens
 
 /* Q8_K rows as f32: grid (ceil(T * W / 1024)), 256 threads. */
 typedef struct {
@@ -442,6 +448,7 @@ typedef struct {
     int32_t width;
     int32_t n_tokens;
 } q38_dequantize_args;
+#define Q38_DEQUANTIZE_PARAMS const void *q8k, float *out, int32_t width, int32_t n_tokens
 
 /* K-quant x Q8_K GEMV / GEMM over up to Q38_GEMV_MAX_MATS matrices of one
  * type and width that read the same activations: G = wg_begin[n_mats] row
@@ -537,7 +544,8 @@ typedef struct {
     int32_t gate_head_stride; /* floats between heads' gates: 256, or 512 in q|gate rows */
     int32_t split_base[Q38_MAX_BATCH + 1];
 } q38_merge_args;
-/* Of one sequence's splits.  grid (1, 24, 4). */
+/* Of one sequence's splits, grid (1, 24, 4): plain arguments, in registers when
+ * a wave starts. */
 typedef struct {
     const float *part_o;
     const float *part_ml;
@@ -546,5 +554,7 @@ typedef struct {
     int32_t n_splits;
     int32_t gate_head_stride;
 } q38_merge_one_args;
+#define Q38_MERGE_ONE_PARAMS                                                                             \
+    const float *part_o, const float *part_ml, const float *gate, float *out, int32_t n_splits, int32_t gate_head_stride
 
 #endif
