@@ -180,6 +180,7 @@ struct q38_ctx {
     hipModule_t mod_rows = nullptr;
     struct RowsKernel {
         hipFunction_t many = nullptr, few = nullptr; /* up to Q38_MAX_BATCH sequences, Q38_KV_ROWS_FEW */
+        bool gathers = false;
     };
     RowsKernel f_kv_append[kKvTypeCount]; /* by kKvTypes index */
     RowsKernel f_kv_gather[kKvTypeCount];
@@ -499,15 +500,16 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
     const std::string p_rows = dir + "/kv_rows.hsaco", p_typed = dir + "/attn_decode_typed.hsaco";
     Q38_HIP(hipModuleLoad(&ctx->mod_rows, p_rows.c_str()));
     Q38_HIP(hipModuleLoad(&ctx->mod_typed, p_typed.c_str()));
-    auto rows_kernel = [&](q38_ctx::RowsKernel *k, const std::string &name) {
+    auto rows_kernel = [&](q38_ctx::RowsKernel *k, const std::string &name, bool gathers) {
+        k->gathers = gathers;
         const hipError_t e = hipModuleGetFunction(&k->many, ctx->mod_rows, name.c_str());
         return e != hipSuccess ? e : hipModuleGetFunction(&k->few, ctx->mod_rows, (name + "_few").c_str());
     };
-    Q38_HIP(rows_kernel(&ctx->f_kv_gather_16, "q38_kv_gather_16"));
+    Q38_HIP(rows_kernel(&ctx->f_kv_gather_16, "q38_kv_gather_16", true));
     for (int i = 0; i < kKvTypeCount; ++i) {
         const std::string ty = kKvTypes[i].suffix;
-        Q38_HIP(rows_kernel(&ctx->f_kv_append[i], "q38_kv_append_" + ty));
-        Q38_HIP(rows_kernel(&ctx->f_kv_gather[i], "q38_kv_gather_" + ty));
+        Q38_HIP(rows_kernel(&ctx->f_kv_append[i], "q38_kv_append_" + ty, false));
+        Q38_HIP(rows_kernel(&ctx->f_kv_gather[i], "q38_kv_gather_" + ty, true));
         if (i == 0) continue;
         Q38_HIP(hipModuleGetFunction(&ctx->f_kv_split_typed[i], ctx->mod_prefill, ("q38_kv_split_mfma_" + ty).c_str()));
         for (int pre = 0; pre < 2; ++pre) {
@@ -1059,17 +1061,25 @@ int launch_rows(q38_kv *kv, const q38_ctx::RowsKernel &f, int slot, int n_seq, c
         a.n_seq = n;
         for (int i = n + 1; i < Q38_MAX_BATCH + 8; ++i) a.page_base[i] = INT_MAX;
         q38_kv_rows_few_args few = {};
-        const bool is_few = n <= Q38_KV_ROWS_FEW;
-        if (is_few) {
-            few.head = a.head;
-            for (int i = 0; i < n; ++i) {
-                few.seq[i] = a.seq[i];
-                few.pos0[i] = a.pos0[i];
-                few.n_tokens[i] = a.row_base[i + 1] - a.row_base[i];
-            }
+        bool is_few = n <= Q38_KV_ROWS_FEW;
+        for (int i = 0; is_few && i < n; ++i) {
+            const long table = (long)a.seq[i] * kv->pt_stride;
+            is_few = table <= INT_MAX;
+            few.table[i] = (int32_t)table;
+            few.pos0[i] = a.pos0[i];
+            few.n_tokens[i] = a.row_base[i + 1] - a.row_base[i];
         }
-        if (kv->ctx->launch(is_few ? f.few : f.many, (unsigned)a.page_base[n], 2, 1, Q38_KV_ROWS_THREADS,
-                            is_few ? (void *)&few : (void *)&a))
+        few.head = a.head;
+        q38_kv_gather_few_rest rest = {a.head.k_rows, a.head.v_rows, a.head.kpool, a.head.vpool};
+        void *params[3 * Q38_KV_ROWS_FEW + 2] = {is_few ? (void *)&few : (void *)&a};
+        if (is_few && f.gathers) {
+            void **p = params;
+            *p++ = &few.head.page_table;
+            for (int32_t *v : {few.pos0, few.n_tokens, few.table})
+                for (int i = 0; i < Q38_KV_ROWS_FEW; ++i) *p++ = &v[i];
+            *p++ = &rest;
+        }
+        if (kv->ctx->launch_params(is_few ? f.few : f.many, (unsigned)a.page_base[n], 2, 1, Q38_KV_ROWS_THREADS, params))
             return -1;
         row += (size_t)a.row_base[n];
     }

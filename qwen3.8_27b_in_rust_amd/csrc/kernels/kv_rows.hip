@@ -17,8 +17,8 @@
  * and the angles twice, took 13.4 us where this takes 12.5).
  *
  * Measured (us, calls of one kind in turn over buffers that no cache holds):
- * 4096 tokens to Q8_K 9.9 (42 MB) and back 8.3 (5.1 TB/s); 1531 tokens of 12
- * sequences to bf16 7.7 and back 6.3; 6 tokens to f16 3.9 and back 3.9, which
+ * 4096 tokens to Q8_K 9.9 (42 MB) and back 7.4 (5.7 TB/s); 1531 tokens of 12
+ * sequences to bf16 7.7 and back 6.2; 6 tokens to f16 3.9 and back 3.9, which
  * is what the launches of so small calls take on the host.
  * Keys are held up by their arithmetic as much as by memory: the angles and,
  * per token and head, the f64 sum, the rotation and the quantiser are some
@@ -41,11 +41,13 @@ struct PageSpan {
     int page;     /* physical page */
 };
 
-Q38_DEV PageSpan page_span(const q38_kv_rows_head &a, int seq, int first, int n, int row, int page_base, int x) {
+/* Page x of a batch: of the sequence whose rows from `first` on are n, whose
+ * first row is `row`, first page page_base and page table starts at `table`. */
+Q38_DEV PageSpan page_span(const int32_t *page_table, size_t table, int first, int n, int row, int page_base, int x) {
     const int lp = (first >> 4) + x - page_base;
     const int p0 = max(first, lp * Q38_PAGE_TOKENS);
     const int p1 = min(first + n, (lp + 1) * Q38_PAGE_TOKENS);
-    return {p0 & 15, (p0 & 15) + p1 - p0, row + p0 - first, p0, a.page_table[(size_t)seq * a.pt_stride + lp]};
+    return {p0 & 15, (p0 & 15) + p1 - p0, row + p0 - first, p0, page_table[table + lp]};
 }
 Q38_DEV PageSpan page_span(const q38_kv_rows_args &a, int x) {
     /* the sequence that holds page x: entries past n_seq are INT_MAX, so eight
@@ -54,22 +56,24 @@ Q38_DEV PageSpan page_span(const q38_kv_rows_args &a, int x) {
     for (int i0 = 1; i0 < a.n_seq; i0 += 8)
 #pragma unroll
         for (int i = 0; i < 8; ++i) b += a.page_base[i0 + i] <= x ? 1 : 0;
-    return page_span(a.head, a.seq[b], a.pos0[b], a.row_base[b + 1] - a.row_base[b], a.row_base[b], a.page_base[b], x);
+    return page_span(a.head.page_table, (size_t)a.seq[b] * a.head.pt_stride, a.pos0[b], a.row_base[b + 1] - a.row_base[b],
+                     a.row_base[b], a.page_base[b], x);
 }
 Q38_DEV PageSpan page_span(const q38_kv_rows_few_args &a, int x) {
-    int seq = a.seq[0], first = a.pos0[0], n = a.n_tokens[0], row = 0, page_base = 0;
+    int table = a.table[0], first = a.pos0[0], n = a.n_tokens[0], row = 0, page_base = 0;
     int pages = ((first + n - 1) >> 4) - (first >> 4) + 1;
+    if (a.n_tokens[1] == 0) return page_span(a.head.page_table, (size_t)table, first, n, 0, 0, x);
 #pragma unroll
     for (int i = 1; i < Q38_KV_ROWS_FEW; ++i) {
         const bool on = x >= page_base + pages; /* past the sequence before: never past the last */
         page_base += on ? pages : 0;
         row += on ? n : 0;
-        seq = on ? a.seq[i] : seq;
+        table = on ? a.table[i] : table;
         first = on ? a.pos0[i] : first;
         n = on ? a.n_tokens[i] : n;
         pages = ((first + n - 1) >> 4) - (first >> 4) + 1;
     }
-    return page_span(a.head, seq, first, n, row, page_base, x);
+    return page_span(a.head.page_table, (size_t)table, first, n, row, page_base, x);
 }
 
 /* LDS of one wave: a quad's elements in page order, 16-bit (2 KiB) or 8-bit. */
@@ -402,16 +406,23 @@ Q38_DEV void kv_gather(const Args &a) {
 
 }  // namespace
 
-#define Q38_KV_ROWS_KERNEL(name, call)                                                                          \
-    extern "C" __global__ __launch_bounds__(kThreads) void name(q38_kv_rows_args a) { call(a); }                \
-    extern "C" __global__ __launch_bounds__(kThreads) void name##_few(q38_kv_rows_few_args a) { call(a); }
-Q38_KV_ROWS_KERNEL(q38_kv_append_f32, kv_append<Q38_KV_F32>)
-Q38_KV_ROWS_KERNEL(q38_kv_append_f16, kv_append<Q38_KV_F16>)
-Q38_KV_ROWS_KERNEL(q38_kv_append_bf16, kv_append<Q38_KV_BF16>)
-Q38_KV_ROWS_KERNEL(q38_kv_append_q8k, kv_append<Q38_KV_Q8>)
-Q38_KV_ROWS_KERNEL(q38_kv_gather_f32, (kv_gather<Q38_KV_F32, false>))
-Q38_KV_ROWS_KERNEL(q38_kv_gather_f16, (kv_gather<Q38_KV_F16, false>))
-Q38_KV_ROWS_KERNEL(q38_kv_gather_bf16, (kv_gather<Q38_KV_BF16, false>))
-Q38_KV_ROWS_KERNEL(q38_kv_gather_q8k, (kv_gather<Q38_KV_Q8, false>))
+#define Q38_KV_APPEND_KERNEL(name, T)                                                                            \
+    extern "C" __global__ __launch_bounds__(kThreads) void name(q38_kv_rows_args a) { kv_append<T>(a); }         \
+    extern "C" __global__ __launch_bounds__(kThreads) void name##_few(q38_kv_rows_few_args a) { kv_append<T>(a); }
+#define Q38_KV_GATHER_KERNEL(name, T, OUT16)                                                                     \
+    extern "C" __global__ __launch_bounds__(kThreads) void name(q38_kv_rows_args a) { kv_gather<T, OUT16>(a); }  \
+    extern "C" __global__ __launch_bounds__(kThreads) void name##_few(Q38_KV_GATHER_FEW_PARAMS) {                \
+        kv_gather<T, OUT16>(                                                                                     \
+            q38_kv_rows_few_args{{rest.kpool, rest.vpool, page_table, rest.k_rows, rest.v_rows, nullptr, 0.f, 0}, \
+                                 {t0, t1, t2, t3}, {p0, p1, p2, p3}, {n0, n1, n2, n3}});                         \
+    }
+Q38_KV_APPEND_KERNEL(q38_kv_append_f32, Q38_KV_F32)
+Q38_KV_APPEND_KERNEL(q38_kv_append_f16, Q38_KV_F16)
+Q38_KV_APPEND_KERNEL(q38_kv_append_bf16, Q38_KV_BF16)
+Q38_KV_APPEND_KERNEL(q38_kv_append_q8k, Q38_KV_Q8)
+Q38_KV_GATHER_KERNEL(q38_kv_gather_f32, Q38_KV_F32, false)
+Q38_KV_GATHER_KERNEL(q38_kv_gather_f16, Q38_KV_F16, false)
+Q38_KV_GATHER_KERNEL(q38_kv_gather_bf16, Q38_KV_BF16, false)
+Q38_KV_GATHER_KERNEL(q38_kv_gather_q8k, Q38_KV_Q8, false)
 /* 16-bit rows as they are stored, F16 or BF16. */
-Q38_KV_ROWS_KERNEL(q38_kv_gather_16, (kv_gather<Q38_KV_BF16, true>))
+Q38_KV_GATHER_KERNEL(q38_kv_gather_16, Q38_KV_BF16, true)

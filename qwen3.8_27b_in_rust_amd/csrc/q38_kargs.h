@@ -179,10 +179,22 @@ typedef struct {
 #define Q38_KV_ROWS_FEW 4
 typedef struct {
     q38_kv_rows_head head;
-    int32_t seq[Q38_KV_ROWS_FEW];
+    int32_t table[Q38_KV_ROWS_FEW]; /* seq * pt_stride */
     int32_t pos0[Q38_KV_ROWS_FEW];
     int32_t n_tokens[Q38_KV_ROWS_FEW];
 } q38_kv_rows_few_args;
+/* A gather takes what finds its page as plain arguments, which are in a wave's
+ * registers when it starts: 4096 tokens of Q8_K 7.5 us against 8.3.  (An append,
+ * whose rows come first and page id last, gains nothing by it.) */
+typedef struct {
+    void *k_rows;
+    void *v_rows;
+    void *kpool;
+    void *vpool;
+} q38_kv_gather_few_rest;
+#define Q38_KV_GATHER_FEW_PARAMS                                                                               \
+    const int32_t *page_table, int32_t p0, int32_t p1, int32_t p2, int32_t p3, int32_t n0, int32_t n1,         \
+        int32_t n2, int32_t n3, int32_t t0, int32_t t1, int32_t t2, int32_t t3, q38_kv_gather_few_rest rest
 
 /* q/gate split, q and k RMSNorm, RoPE.  grid (n_tokens, 28): y < 24 is a
  * query head, y >= 24 a kv head. */

@@ -24,21 +24,38 @@ static int g_launches = 0;
 static std::vector<std::vector<char>> g_args;
 static std::vector<unsigned> g_grid;
 /* the functions that a launch names: one handle for each argument block */
-static hipFunction_t const kMany = (hipFunction_t)0x1000, kFew = (hipFunction_t)0x2000;
+static hipFunction_t const kMany = (hipFunction_t)0x1000, kFew = (hipFunction_t)0x2000, kFewGather = (hipFunction_t)0x3000;
+static int g_pt_stride; /* of the cache at hand */
 static hipError_t check_launch(hipFunction_t f, unsigned gx, unsigned gy, unsigned, unsigned block, unsigned, unsigned,
                                unsigned, hipStream_t, void **params, void **) {
     ++g_launches;
     if (gy != 2 || block != Q38_KV_ROWS_THREADS) { printf("unexpected grid\n"); exit(1); }
     q38_kv_rows_args a;
-    if (f == kFew) {
-        const q38_kv_rows_few_args &w = *static_cast<const q38_kv_rows_few_args *>(params[0]);
+    if (f == kFew || f == kFewGather) {
+        /* the arguments one by one, in the kernels' order */
+        q38_kv_rows_few_args w;
+        void **p = params;
+        auto take = [&](auto &x) { memcpy(&x, *p++, sizeof(x)); };
+        auto each = [&](int32_t (&v)[Q38_KV_ROWS_FEW]) {
+            for (int32_t &x : v) take(x);
+        };
+        memset(&w, 0xAB, sizeof(w));
+        if (f == kFewGather) {
+            q38_kv_gather_few_rest rest;
+            take(w.head.page_table), each(w.pos0), each(w.n_tokens), each(w.table), take(rest);
+            w.head.k_rows = rest.k_rows, w.head.v_rows = rest.v_rows;
+            w.head.kpool = rest.kpool, w.head.vpool = rest.vpool;
+        } else {
+            take(w);
+        }
         memset(&a, 0xAB, sizeof(a)); /* what the kernel does not get */
         a.head = w.head;
         /* the bases as the kernel finds them from the counts, 0 past the last sequence */
         a.n_seq = 0;
         a.row_base[0] = a.page_base[0] = 0;
         for (int i = 0; i < Q38_KV_ROWS_FEW; ++i) {
-            a.seq[i] = w.seq[i];
+            if (w.table[i] % g_pt_stride != 0) { printf("a table that is no sequence's\n"); exit(1); }
+            a.seq[i] = w.table[i] / g_pt_stride;
             a.pos0[i] = w.pos0[i];
             const int pages = ((w.pos0[i] + w.n_tokens[i] - 1) >> 4) - (w.pos0[i] >> 4) + 1;
             if ((pages > 0) != (w.n_tokens[i] > 0) || (pages > 0 && a.n_seq != i)) { printf("counts with a gap\n"); exit(1); }
@@ -102,14 +119,15 @@ struct Cache {
         for (int i = 0; i < kKvTypeCount; ++i)
             for (q38_ctx::RowsKernel *k : {&ctx.f_kv_append[i], &ctx.f_kv_gather[i], &ctx.f_kv_gather_16}) {
                 k->many = kMany;
-                k->few = kFew;
+                k->gathers = k != &ctx.f_kv_append[i];
+                k->few = k->gathers ? kFewGather : kFew;
             }
         kv.ctx = &ctx;
         kv.type = type;
         kv.n_slots = slots;
         kv.max_pages = pages;
         kv.max_seqs = seqs;
-        kv.pt_stride = (tokens + 15) / 16;
+        kv.pt_stride = g_pt_stride = (tokens + 15) / 16;
         kv.kpool = reinterpret_cast<float *>(0x100000000000ull);
         kv.vpool = reinterpret_cast<float *>(0x200000000000ull);
         kv.d_page_table = reinterpret_cast<int32_t *>(0x300000000000ull);
