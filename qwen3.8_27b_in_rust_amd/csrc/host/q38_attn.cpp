@@ -1079,7 +1079,7 @@ int launch_rows(q38_kv *kv, const q38_ctx::RowsKernel &f, int slot, int n_seq, c
                 for (int i = 0; i < Q38_KV_ROWS_FEW; ++i) *p++ = &v[i];
             *p++ = &rest;
         }
-        if (kv->ctx->launch_params(is_few ? f.few : f.many, (unsigned)a.page_base[n], 2, 1, Q38_KV_ROWS_THREADS, params))
+        if (kv->ctx->launch_params(is_few ? f.few : f.many, (unsigned)a.page_base[n] * Q38_KV_ROWS_PARTS, 2, 1, Q38_KV_ROWS_THREADS, params))
             return -1;
         row += (size_t)a.row_base[n];
     }

@@ -7,18 +7,22 @@
  * values that the rows stand for as f32, or 16-bit rows as they are stored.
  *
  * Both move bytes: 4 KB of f32 a row and half or a quarter of that in the
- * page.  A workgroup of 16 waves serves one page of one sequence; a wave has
+ * page.  A workgroup of 8 waves serves half a page of one sequence; a wave has
  * four tokens (a quad) of one kv head, lane l the dims 4l .. 4l + 3 of each.
- * All its loads go out at once -- 16 waves a workgroup and two workgroups a
- * CU keep the memory busy -- and the quad's part of the page is put together
- * in the wave's own LDS, where the page's element order (q38_kv_layout.h)
- * makes it 16-byte pieces: of one token for K, of all four for V.  The page's
- * rotation angles are formed once per workgroup (half as many heads in one,
- * and the angles twice, took 13.4 us where this takes 12.5).
+ * All its loads go out at once -- four workgroups a CU keep the memory busy --
+ * and the quad's part of the page is put together in the wave's own LDS, where
+ * the page's element order (q38_kv_layout.h) makes it 16-byte pieces: of one
+ * token for K, of all four for V.  The rotation angles are formed once per token,
+ * by a workgroup whose waves share them (half as many heads in one, and the
+ * angles twice, took 13.4 us where this took 12.5).  A workgroup for a whole page
+ * leaves the keys' arithmetic to half as many CUs where there are few pages,
+ * one for a quarter costs its start too often: 1531 tokens of 12 sequences to
+ * bf16 7.7 us, 6.7 by halves, 7.0 by quarters, and back 6.3, 6.0, 6.4; 4096 to
+ * Q8_K 9.9, 9.2, 9.3 and back 7.6, 7.5, 8.0; to bf16 9.4, 10.1, 11.2.
  *
  * Measured (us, calls of one kind in turn over buffers that no cache holds):
- * 4096 tokens to Q8_K 9.9 (42 MB) and back 7.4 (5.7 TB/s); 1531 tokens of 12
- * sequences to bf16 7.7 and back 6.2; 6 tokens to f16 3.9 and back 3.9, which
+ * 4096 tokens to Q8_K 9.2 (42 MB) and back 7.5 (5.6 TB/s); 1531 tokens of 12
+ * sequences to bf16 6.7 and back 6.0; 6 tokens to f16 3.8 and back 3.8, which
  * is what the launches of so small calls take on the host.
  * Keys are held up by their arithmetic as much as by memory: the angles and,
  * per token and head, the f64 sum, the rotation and the quantiser are some
@@ -30,9 +34,9 @@
 
 namespace {
 
-constexpr int kQuads = Q38_PAGE_TOKENS / 4;
+constexpr int kQuads = Q38_KV_ROWS_QUADS, kParts = Q38_KV_ROWS_PARTS;
 constexpr int kThreads = 64 * Q38_ATTN_KV_HEADS * kQuads;
-static_assert(kThreads == Q38_KV_ROWS_THREADS, "a wave per head and quad");
+static_assert(kThreads == Q38_KV_ROWS_THREADS && 4 * kQuads * kParts == Q38_PAGE_TOKENS, "a wave per head and quad");
 
 struct PageSpan {
     int t0, t1;   /* tokens of the page, [t0, t1) */
@@ -287,12 +291,13 @@ Q38_DEV void store_quad(char *block, Stage &stage, bool key, int head, int quad,
 
 template <int T, typename Args>
 Q38_DEV void kv_append(const Args &a) {
-    __shared__ __attribute__((aligned(16))) float cs[Q38_PAGE_TOKENS][32][2];
+    __shared__ __attribute__((aligned(16))) float cs[4 * kQuads][32][2];
     __shared__ Stage stages[T == Q38_KV_F32 ? 1 : kThreads / 64];
-    const PageSpan sp = page_span(a, blockIdx.x);
+    const PageSpan sp = page_span(a, blockIdx.x / kParts);
+    const int quad0 = blockIdx.x % kParts * kQuads;
     const bool key = blockIdx.y == 0;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int head = wave & 3, quad = wave >> 2;
+    const int head = wave & 3, quad = quad0 + (wave >> 2);
     const bool turns = key && a.head.k_norm != nullptr;
     const int first = max(sp.t0 - 4 * quad, 0), last = min(sp.t1 - 4 * quad, 4);
     const bool live = first < last;
@@ -308,15 +313,16 @@ Q38_DEV void kv_append(const Args &a) {
     }
     if (turns) {
         /* the page's angles: a half-wave per token */
-        const int t = tid >> 5;
-        if (t >= sp.t0 && t < sp.t1) q38_rope_table_half(cs[t], lane & 31, sp.pos0 + t - sp.t0, a.head.theta_scale);
+        const int t = 4 * quad0 + (tid >> 5);
+        if (tid < 128 * kQuads && t >= sp.t0 && t < sp.t1)
+            q38_rope_table_half(cs[tid >> 5], lane & 31, sp.pos0 + t - sp.t0, a.head.theta_scale);
         __syncthreads();
     }
     if (!live) return;
     if (turns) {
         int t[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = 4 * quad + min(max(i, first), last - 1);
+        for (int i = 0; i < 4; ++i) t[i] = 4 * (wave >> 2) + min(max(i, first), last - 1);
         norm_rope_quad(x, w, lane, cs, t);
     }
     store_quad<T>(q38_kv_block<T>(key ? a.head.kpool : a.head.vpool, sp.page, head), stages[T == Q38_KV_F32 ? 0 : wave], key, head,
@@ -333,10 +339,11 @@ Q38_DEV void kv_append(const Args &a) {
 template <int T, bool OUT16, typename Args>
 Q38_DEV void kv_gather(const Args &a) {
     __shared__ Stage stages[T == Q38_KV_F32 ? 1 : kThreads / 64];
-    const PageSpan sp = page_span(a, blockIdx.x);
+    const PageSpan sp = page_span(a, blockIdx.x / kParts);
+    const int quad0 = blockIdx.x % kParts * kQuads;
     const bool key = blockIdx.y == 0;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int head = wave & 3, quad = wave >> 2;
+    const int head = wave & 3, quad = quad0 + (wave >> 2);
     const int first = max(sp.t0 - 4 * quad, 0), last = min(sp.t1 - 4 * quad, 4);
     if (first >= last) return;
     char *block = q38_kv_block<T>(key ? a.head.kpool : a.head.vpool, sp.page, head);

@@ -148,12 +148,15 @@ typedef struct {
 
 /* Rows of a ragged batch to or from the pages of a cache of any type: row
  * row_base[b] + i is position pos0[b] + i of sequence seq[b].  grid
- * (page_base[n_seq], 2): workgroup x serves one page of one sequence -- page
- * pos0[b] / 16 + x - page_base[b] of the sequence b that holds x -- and y = 0
- * moves K, y = 1 moves V; Q38_KV_ROWS_THREADS threads, a wave per kv head and
- * four tokens.  page_base past n_seq holds INT_MAX (the sequence of a page is
- * found eight entries at a time). */
-#define Q38_KV_ROWS_THREADS 1024
+ * (page_base[n_seq] * Q38_KV_ROWS_PARTS, 2): workgroup x serves part of page x /
+ * Q38_KV_ROWS_PARTS of the batch, which is page pos0[b] / 16 + that -
+ * page_base[b] of the sequence b that holds it, and y = 0 moves K, y = 1 moves V;
+ * Q38_KV_ROWS_THREADS threads, a wave per kv head and four tokens.  page_base
+ * past n_seq holds INT_MAX (the sequence of a page is found eight entries at a
+ * time). */
+#define Q38_KV_ROWS_QUADS 2 /* of a page's four, a workgroup */
+#define Q38_KV_ROWS_PARTS (4 / Q38_KV_ROWS_QUADS)
+#define Q38_KV_ROWS_THREADS (256 * Q38_KV_ROWS_QUADS)
 typedef struct {
     void *kpool;
     void *vpool;

@@ -69,7 +69,8 @@ static hipError_t check_launch(hipFunction_t f, unsigned gx, unsigned gy, unsign
     }
     const char *p = reinterpret_cast<const char *>(&a);
     g_args.emplace_back(p, p + sizeof(a));
-    g_grid.push_back(gx);
+    if (gx % Q38_KV_ROWS_PARTS != 0) { printf("a page in part\n"); exit(1); }
+    g_grid.push_back(gx / Q38_KV_ROWS_PARTS); /* pages */
     return hipSuccess;
 }
 static hipError_t check_copy(void *, const void *, size_t, hipMemcpyKind, hipStream_t) { return hipSuccess; }
