@@ -1071,14 +1071,9 @@ int launch_rows(q38_kv *kv, const q38_ctx::RowsKernel &f, int slot, int n_seq, c
         }
         few.head = a.head;
         q38_kv_gather_few_rest rest = {a.head.k_rows, a.head.v_rows, a.head.kpool, a.head.vpool};
-        void *params[3 * Q38_KV_ROWS_FEW + 2] = {is_few ? (void *)&few : (void *)&a};
-        if (is_few && f.gathers) {
-            void **p = params;
-            *p++ = &few.head.page_table;
-            for (int32_t *v : {few.pos0, few.n_tokens, few.table})
-                for (int i = 0; i < Q38_KV_ROWS_FEW; ++i) *p++ = &v[i];
-            *p++ = &rest;
-        }
+        void *gathered[] = {few.table, few.pos0, few.n_tokens, &few.head.page_table, &rest};
+        void *block[] = {is_few ? (void *)&few : (void *)&a};
+        void **params = is_few && f.gathers ? gathered : block;
         if (kv->ctx->launch_params(is_few ? f.few : f.many, (unsigned)a.page_base[n] * Q38_KV_ROWS_PARTS, 2, 1, Q38_KV_ROWS_THREADS, params))
             return -1;
         row += (size_t)a.row_base[n];
@@ -1295,25 +1290,26 @@ struct decode_launch {
     unsigned block = 0;
     bool merge = false;
 
-    /* where the kernels' arguments are, kMaxParams of them at most */
-    static constexpr int kMaxParams = 10;
+    /* where the kernels' arguments are (a vector's at its first), kMaxParams of them at most */
+    static constexpr int kMaxParams = 4;
     void split_params(void **p) {
         if (!one) {
             p[0] = &a;
             return;
         }
         q38_decode_one_args &o = a_one;
-        void *const each[kMaxParams] = {&o.page_row, &o.q, &o.kpool, &o.vpool, &o.q_norm, &o.pos, &o.split_tokens,
-                                        &o.total_splits, &o.gate_head_stride, &o.rest};
-        std::copy(each, each + kMaxParams, p);
+        p[0] = &o.page_row;
+        p[1] = &o.pos;
+        p[2] = &o.q_norm;
+        p[3] = &o.rest;
     }
     void merge_params(void **p) {
         if (!one) {
             p[0] = &m;
             return;
         }
-        void *const each[] = {&m_one.part_o, &m_one.part_ml, &m_one.gate, &m_one.out, &m_one.n_splits, &m_one.gate_head_stride};
-        std::copy(each, each + 6, p);
+        p[0] = &m_one.part_o;
+        p[1] = &m_one.n_splits;
     }
 };
 
@@ -1399,8 +1395,8 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
     }
     L->grid_x = (unsigned)total;
     if (L->one) {
-        L->a_one = {a.page_table + (size_t)seq_ids[0] * a.pt_stride, a.q, a.kpool, a.vpool, a.q_norm, positions[0],
-                    split_tokens, total, a.gate_head_stride,
+        L->a_one = {a.page_table + (size_t)seq_ids[0] * a.pt_stride, a.q, a.kpool, a.vpool, positions[0], split_tokens,
+                    total, a.gate_head_stride, a.q_norm,
                     {a.k_new, a.v_new, a.gate, a.out, a.part_o, a.part_ml, a.k_norm, a.theta_scale, 0}};
         L->m_one = {a.part_o, a.part_ml, a.gate, d_out, total, a.gate_head_stride};
     }
@@ -2010,6 +2006,15 @@ static_assert(sizeof(q38_decode_args) <= 4096, "decode arguments exceed 4 KiB");
 static_assert(offsetof(q38_decode_args, head_pages) == sizeof(q38_decode_typed_args) &&
                   offsetof(q38_decode_args, split_base) == offsetof(q38_decode_typed_args, split_base),
               "q38_decode_typed_args is the front of q38_decode_args");
+/* vectors of arguments lie side by side */
+static_assert(offsetof(q38_decode_one_args, vpool) == 24 && offsetof(q38_decode_one_args, pos) == 32 &&
+                  offsetof(q38_decode_one_args, gate_head_stride) == 44 && offsetof(q38_decode_one_args, q_norm) == 48 &&
+                  offsetof(q38_merge_one_args, out) == 24 && offsetof(q38_merge_one_args, n_splits) == 32,
+              "four pointers, four numbers");
+static_assert(offsetof(q38_norm_args, sum) == 24 && offsetof(q38_norm_args, y) == 32 && offsetof(q38_norm_args, q8k) == 40 &&
+                  offsetof(q38_norm_args, width) == 48 && offsetof(q38_norm_args, n_tokens) == 52 &&
+                  offsetof(q38_dequantize_args, n_tokens) == offsetof(q38_dequantize_args, width) + 4,
+              "four pointers, two, two numbers");
 static_assert(sizeof(q38_prefill_merge_args) <= 4096, "prefill merge arguments exceed 4 KiB");
 
 int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens, const float *d_q,
@@ -2625,7 +2630,7 @@ int q38_dequantize_q8_k(q38_ctx *ctx, int n_tokens, int width, const void *d_q8k
     const size_t groups = ((size_t)n_tokens * width + 1023) / 1024;
     if (groups > 0xFFFFFFFFull / 256) return fail("%d rows of %d: too many for one call", n_tokens, width);
     q38_dequantize_args a = {d_q8k, d_x, width, n_tokens};
-    void *params[] = {&a.q8k, &a.out, &a.width, &a.n_tokens};
+    void *params[] = {&a.q8k, &a.out, &a.width};
     return ctx->launch_params(ctx->f_dequantize_q8k, (unsigned)groups, 1, 1, 256, params);
 }
 
@@ -2661,7 +2666,7 @@ int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, co
         overlaps(d_q8k, q_bytes, d_weight, (size_t)width * sizeof(float)))
         return fail("d_q8k overlaps an input");
     q38_norm_args a = {d_x, d_residual, d_weight, d_sum, d_y, d_q8k, width, n_tokens};
-    void *params[] = {&a.x, &a.residual, &a.weight, &a.sum, &a.y, &a.q8k, &a.width, &a.n_tokens};
+    void *params[] = {&a.x, &a.y, &a.width}; /* each a vector's first */
     /* rows of whole 16-byte vectors stay in registers where they fit */
     const bool vectors = width % 4 == 0 && ((uintptr_t)d_x | (uintptr_t)d_residual | (uintptr_t)d_weight |
                                             (uintptr_t)d_sum | (uintptr_t)d_y) % 16 == 0;

@@ -504,8 +504,9 @@ extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_merge(q38_merg
 }
 
 extern "C" __global__ __launch_bounds__(256) void q38_attn_decode_merge_one(Q38_MERGE_ONE_PARAMS) {
-    const q38_merge_one_args a = {part_o, part_ml, gate, out, n_splits, gate_head_stride};
-    if (n_splits > 1) merge_splits(a, 0, 0, n_splits);
+    const q38_merge_one_args a = {q38_global<const float>(p[0]), q38_global<const float>(p[1]),
+                                  q38_global<const float>(p[2]), q38_global<float>(p[3]), n[0], n[1]};
+    if (a.n_splits > 1) merge_splits(a, 0, 0, a.n_splits);
 }
 
 /* Rows <-> pages.  grid (n_tokens, 2), 256 threads x float4 = one 1024-float row. */

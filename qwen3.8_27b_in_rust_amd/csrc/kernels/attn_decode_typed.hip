@@ -617,9 +617,10 @@ Q38_DEV void decode_typed(const Args &a) {
         decode_typed<T, PRE>(a);                                                                                    \
     }                                                                                                               \
     extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_attn_decode_##name##_one(Q38_DECODE_ONE_PARAMS) { \
-        decode_typed<T, PRE>(OneArgs{kpool, vpool, page_row, q, rest.k_new, rest.v_new, rest.gate, rest.out,        \
-                                     rest.part_o, rest.part_ml, q_norm, rest.k_norm, rest.theta_scale,              \
-                                     gate_head_stride, pos, split_tokens, total_splits});                           \
+        decode_typed<T, PRE>(OneArgs{                                                                               \
+            q38_global<float>(rows[2]), q38_global<float>(rows[3]), q38_global<const int32_t>(rows[0]),             \
+            q38_global<const float>(rows[1]), rest.k_new, rest.v_new, rest.gate, rest.out, rest.part_o,             \
+            rest.part_ml, q_norm, rest.k_norm, rest.theta_scale, span[3], span[0], span[1], span[2]});              \
     }
 Q38_DECODE_KERNEL(f16, Q38_KV_F16, false)
 Q38_DECODE_KERNEL(f16_pre, Q38_KV_F16, true)

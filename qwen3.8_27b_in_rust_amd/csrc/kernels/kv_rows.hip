@@ -421,7 +421,9 @@ Q38_DEV void kv_gather(const Args &a) {
     extern "C" __global__ __launch_bounds__(kThreads) void name##_few(Q38_KV_GATHER_FEW_PARAMS) {                \
         kv_gather<T, OUT16>(                                                                                     \
             q38_kv_rows_few_args{{rest.kpool, rest.vpool, page_table, rest.k_rows, rest.v_rows, nullptr, 0.f, 0}, \
-                                 {t0, t1, t2, t3}, {p0, p1, p2, p3}, {n0, n1, n2, n3}});                         \
+                                 {table[0], table[1], table[2], table[3]},                                  \
+                                 {pos0[0], pos0[1], pos0[2], pos0[3]},                                           \
+                                 {n_tokens[0], n_tokens[1], n_tokens[2], n_tokens[3]}});                         \
     }
 Q38_KV_APPEND_KERNEL(q38_kv_append_f32, Q38_KV_F32)
 Q38_KV_APPEND_KERNEL(q38_kv_append_f16, Q38_KV_F16)

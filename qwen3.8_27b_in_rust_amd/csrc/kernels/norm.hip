@@ -167,7 +167,7 @@ Q38_DEV void norm_row_any(const q38_norm_args &a) {
 #define Q38_NORM_KERNEL(NT, V)                                                                              \
     extern "C" __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 1) /* (waves a SIMD) */                    \
     void q38_add_rms_norm_##NT##_##V(Q38_NORM_PARAMS) {                                                     \
-        norm_row<NT, V>({x, residual, weight, sum, y, q8k, width, n_tokens});                               \
+        norm_row<NT, V>(Q38_NORM_ARGS);                               \
     }
 Q38_NORM_KERNEL(256, 1)
 Q38_NORM_KERNEL(256, 2)
@@ -180,18 +180,18 @@ Q38_NORM_KERNEL(1024, 3)
 Q38_NORM_KERNEL(1024, 4)
 Q38_NORM_KERNEL(1024, 5)
 extern "C" __global__ __launch_bounds__(1024) void q38_add_rms_norm_any(Q38_NORM_PARAMS) {
-    norm_row_any({x, residual, weight, sum, y, q8k, width, n_tokens});
+    norm_row_any(Q38_NORM_ARGS);
 }
 
 /* The values that Q8_K rows stand for: grid (ceil(n_tokens * width / 1024)),
  * 256 threads, 4 values each. */
 extern "C" __global__ __launch_bounds__(256) void q38_dequantize_q8k(Q38_DEQUANTIZE_PARAMS) {
-    const size_t n = (size_t)n_tokens * width;
+    const size_t total = (size_t)n[0] * n[1];
     const size_t i = 4 * ((size_t)blockIdx.x * 256 + threadIdx.x);
-    if (i >= n) return;
+    if (i >= total) return;
     const char *base = static_cast<const char *>(q8k);
     const uint32_t u = *reinterpret_cast<const uint32_t *>(base + i);
-    const float s = reinterpret_cast<const float *>(base + n + n / 8)[i >> 8];
+    const float s = reinterpret_cast<const float *>(base + total + total / 8)[i >> 8];
     f32x4 v;
 #pragma unroll
     for (int c = 0; c < 4; ++c) v[c] = (float)(int8_t)(u >> (8 * c)) * s;

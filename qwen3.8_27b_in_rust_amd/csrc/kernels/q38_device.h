@@ -62,6 +62,16 @@ Q38_DEV q38_halves q38_both_halves(float x) {
 }
 
 Q38_DEV f32x4 q38_ld4(const float *p) { return *reinterpret_cast<const f32x4 *>(p); }
+/* Kernel arguments passed as vectors, and an address out of one. */
+typedef unsigned long long q38_u64x4 __attribute__((ext_vector_type(4)));
+typedef unsigned long long q38_u64x2 __attribute__((ext_vector_type(2)));
+typedef int q38_i32x4 __attribute__((ext_vector_type(4)));
+typedef int q38_i32x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+Q38_DEV T *q38_global(unsigned long long address) {
+    return (T *)reinterpret_cast<__attribute__((address_space(1))) T *>(address);
+}
+
 Q38_DEV void q38_st4(float *p, f32x4 v) { *reinterpret_cast<f32x4 *>(p) = v; }
 
 /* Streaming loads that are read once: keep them out of the way of reused

@@ -72,11 +72,12 @@ typedef struct {
     int32_t pos[Q38_MAX_BATCH]; /* attend over positions 0..pos inclusive */
     int32_t split_base[Q38_MAX_BATCH + 8]; /* past n_seq: INT_MAX */
 } q38_decode_typed_args;
-/* One sequence's, as its kernels take them: what a wave needs before its first
- * loads as plain arguments, of which the first 14 words are in its registers
- * when it starts, then the rest as a block.  Forming q and reading 1021 tokens of
- * bf16 takes 9.0 us with it, 9.25 with all of them in a block, 9.6 with a
- * batch's 920 bytes; 32K tokens 26.9, 27.8 and 28.1. */
+/* One sequence's.  Its kernels take what a wave needs before its first loads as
+ * plain arguments, which are in its registers when it starts (14 words at most),
+ * several to a vector since each argument costs a launch 0.04 us on the host; the
+ * rest as a block.  Forming q and reading 1021 tokens of bf16 takes 9.0 us with
+ * it, 9.25 with all of them in a block, 9.6 with a batch's 920 bytes; 32K tokens
+ * 26.9, 27.8 and 28.1. */
 typedef struct {
     const float *k_new, *v_new;
     const float *gate;
@@ -86,21 +87,21 @@ typedef struct {
     float theta_scale;
     int32_t pad_;
 } q38_decode_one_rest;
-#define Q38_DECODE_ONE_PARAMS                                                                                  \
-    const int32_t *page_row, const float *q, float *kpool, float *vpool, const float *q_norm, int32_t pos,     \
-        int32_t split_tokens, int32_t total_splits, int32_t gate_head_stride, q38_decode_one_rest rest
 typedef struct {
+    /* one vector */
     const int32_t *page_row; /* the sequence's page table */
     const float *q;
     float *kpool;
     float *vpool;
-    const float *q_norm;
+    /* one vector */
     int32_t pos;
     int32_t split_tokens;
     int32_t total_splits;
     int32_t gate_head_stride;
+    const float *q_norm;
     q38_decode_one_rest rest;
-} q38_decode_one_args; /* the same as the host keeps them */
+} q38_decode_one_args;
+#define Q38_DECODE_ONE_PARAMS q38_u64x4 rows, q38_i32x4 span, const float *q_norm, q38_decode_one_rest rest
 typedef struct {
     float *kpool;              /* this layer's K pages: [max_pages][4][16][256] */
     float *vpool;              /* this layer's V pages */
@@ -195,9 +196,8 @@ typedef struct {
     void *kpool;
     void *vpool;
 } q38_kv_gather_few_rest;
-#define Q38_KV_GATHER_FEW_PARAMS                                                                               \
-    const int32_t *page_table, int32_t p0, int32_t p1, int32_t p2, int32_t p3, int32_t n0, int32_t n1,         \
-        int32_t n2, int32_t n3, int32_t t0, int32_t t1, int32_t t2, int32_t t3, q38_kv_gather_few_rest rest
+#define Q38_KV_GATHER_FEW_PARAMS                                                                    \
+    q38_i32x4 table, q38_i32x4 pos0, q38_i32x4 n_tokens, const int32_t *page_table, q38_kv_gather_few_rest rest
 
 /* q/gate split, q and k RMSNorm, RoPE.  grid (n_tokens, 28): y < 24 is a
  * query head, y >= 24 a kv head. */
@@ -450,11 +450,15 @@ typedef struct {
     int32_t width;
     int32_t n_tokens;
 } q38_norm_args;
-/* The kernels take them one by one: plain arguments are in a wave's registers
- * when it starts. */
-#define Q38_NORM_PARAMS                                                                               \
-    const float *x, const float *residual, const float *weight, float *sum, float *y, void *q8k,      \
-        int32_t width, int32_t n_tokens
+/* The kernels take them as plain vectors, in registers when a wave starts: one
+ * row's norm 3.4 us against 3.5 where the GPU is what bounds (as a block; one by
+ * one the eight arguments cost a launch 0.3 us on the host, three 0.1). */
+#define Q38_NORM_PARAMS q38_u64x4 in, q38_u64x2 out, q38_i32x2 n
+#define Q38_NORM_ARGS                                                                                     \
+    {                                                                                                     \
+        q38_global<const float>(in[0]), q38_global<const float>(in[1]), q38_global<const float>(in[2]),   \
+            q38_global<float>(in[3]), q38_global<float>(out[0]), q38_global<void>(out[1]), n[0], n[1]     \
+    }
 
 /* Q8_K rows as f32: grid (ceil(T * W / 1024)), 256 threads. */
 typedef struct {
@@ -463,7 +467,7 @@ typedef struct {
     int32_t width;
     int32_t n_tokens;
 } q38_dequantize_args;
-#define Q38_DEQUANTIZE_PARAMS const void *q8k, float *out, int32_t width, int32_t n_tokens
+#define Q38_DEQUANTIZE_PARAMS const void *q8k, float *out, q38_i32x2 n
 
 /* K-quant x Q8_K GEMV / GEMM over up to Q38_GEMV_MAX_MATS matrices of one
  * type and width that read the same activations: G = wg_begin[n_mats] row
@@ -559,8 +563,8 @@ typedef struct {
     int32_t gate_head_stride; /* floats between heads' gates: 256, or 512 in q|gate rows */
     int32_t split_base[Q38_MAX_BATCH + 1];
 } q38_merge_args;
-/* Of one sequence's splits, grid (1, 24, 4): plain arguments, in registers when
- * a wave starts. */
+/* Of one sequence's splits, grid (1, 24, 4): two vectors, in registers when a
+ * wave starts. */
 typedef struct {
     const float *part_o;
     const float *part_ml;
@@ -569,7 +573,6 @@ typedef struct {
     int32_t n_splits;
     int32_t gate_head_stride;
 } q38_merge_one_args;
-#define Q38_MERGE_ONE_PARAMS                                                                             \
-    const float *part_o, const float *part_ml, const float *gate, float *out, int32_t n_splits, int32_t gate_head_stride
+#define Q38_MERGE_ONE_PARAMS q38_u64x4 p, q38_i32x2 n
 
 #endif

@@ -32,17 +32,14 @@ static hipError_t check_launch(hipFunction_t f, unsigned gx, unsigned gy, unsign
     if (gy != 2 || block != Q38_KV_ROWS_THREADS) { printf("unexpected grid\n"); exit(1); }
     q38_kv_rows_args a;
     if (f == kFew || f == kFewGather) {
-        /* the arguments one by one, in the kernels' order */
+        /* the arguments in the kernels' order */
         q38_kv_rows_few_args w;
         void **p = params;
         auto take = [&](auto &x) { memcpy(&x, *p++, sizeof(x)); };
-        auto each = [&](int32_t (&v)[Q38_KV_ROWS_FEW]) {
-            for (int32_t &x : v) take(x);
-        };
         memset(&w, 0xAB, sizeof(w));
         if (f == kFewGather) {
             q38_kv_gather_few_rest rest;
-            take(w.head.page_table), each(w.pos0), each(w.n_tokens), each(w.table), take(rest);
+            take(w.table), take(w.pos0), take(w.n_tokens), take(w.head.page_table), take(rest);
             w.head.k_rows = rest.k_rows, w.head.v_rows = rest.v_rows;
             w.head.kpool = rest.kpool, w.head.vpool = rest.vpool;
         } else {
