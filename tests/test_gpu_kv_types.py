@@ -628,6 +628,51 @@ def test_refused_calls_change_nothing(pkg, ctx):
             assert np.array_equal(c.read(s, 0, 40)[0], stored(K, c.ty))
 
 
+@typed
+def test_two_contexts_at_once(pkg, ctx, ty):
+    """Calls of two contexts in turn, neither waited for: each has its stream
+    and workspace, and gives what it gives alone."""
+    rng = np.random.default_rng(23)
+    other = pkg.Context(0)
+    try:
+        lengths, sides = [1500, 900, 40], []
+        for c in (ctx, other):
+            cache = Cache(pkg, c, ty, lengths, seed=len(sides))
+            key, val = _rows(rng, sum(lengths)), _rows(rng, sum(lengths))
+            w = c.array((1 + 0.2 * rng.standard_normal(256)).astype(np.float32))
+            qg, k, v = (c.array(rng.standard_normal((3, n)).astype(np.float32)) for n in (12288, 1024, 1024))
+            sides.append((c, cache, c.array(key), c.array(val), w, qg, k, v, [c.empty((3, 6144)) for _ in range(6)]))
+
+        def step(i, side):
+            c, cache, key, val, w, qg, k, v, out = side
+            if i == 0:
+                cache.kv.append(3, cache.seqs, [0, 0, 0], lengths, w, key, val)
+            cache.kv.full_core(3, cache.seqs, [n + i for n in lengths], w, w, qg, k, v, out[i])
+            c.add_rms_norm(3, 6144, out[i], qg, residual=qg, y=out[i])
+
+        for side in sides:  # alone
+            for i in range(6):
+                step(i, side)
+            side[0].sync()
+        alone = [[o.download() for o in side[-1]] for side in sides]
+        for side in sides:
+            for s in side[1].seqs:
+                side[1].kv.seq_truncate(s, 0)
+            for o in side[-1]:
+                o.zero()
+            side[0].sync()
+        for i in range(6):  # and in turn
+            for side in sides:
+                step(i, side)
+        for side, want in zip(sides, alone):
+            for o, x in zip(side[-1], want):
+                assert np.isfinite(x).all() and np.array_equal(_bits(o.download()), _bits(x))
+        for side in sides:
+            side[1].kv.close()
+    finally:
+        other.close()
+
+
 def test_append_is_not_captured(pkg, ctx):
     """Refused while the context's stream captures (a replay would leave stale
     prefill images), with the capture and the cache as they were."""
