@@ -20,7 +20,10 @@
  *  - O = P V, 16 rows x 16 dims.  The lanes that hold a score are those that
  *    supply its weight as an operand (C's column l % 16, rows 4 (l / 16) + i
  *    are A's row l % 16, k 4 (l / 16) + i), so the weights never leave their
- *    registers; they are split like the queries, into rows 0-5 and 8-13.
+ *    registers; they are split like the queries, into rows 0-5 and 8-13, an f16
+ *    lower part taken 2^11 times as large: f16's fixed step below 2^-14 then is
+ *    2^-36 of a weight's unit (2^-43 of the largest weight), not 2^-24, and a
+ *    small weight on a large value keeps its bits.
  *    8-bit rows: the value's scale goes into its weight, over a power of two
  *    at or above every scale seen so far, which keeps f16 clear of overflow.
  *  - softmax in base 2 against a reference per head that is raised (and O and
@@ -59,6 +62,10 @@ constexpr int kGroup = Q38_ATTN_GROUP;
 template <int T>
 constexpr float kRefBelow = T == Q38_KV_BF16 ? 0.0f : 7.0f;
 constexpr float kRefSlack = 8.0f;
+/* f16 weights: what their lower part is larger by (the upper one's rounding
+ * leaves 2^-11 of the weight at most, 2^4). */
+template <int T>
+constexpr float kLowUnit = T == Q38_KV_BF16 ? 1.0f : 0x1p11f;
 
 /* One page of one kv head as a wave holds it. */
 template <int T>
@@ -259,7 +266,7 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const _Float16 hi = (_Float16)w[i];
-            const _Float16 lo = (_Float16)(w[i] - (float)hi);
+            const _Float16 lo = (_Float16)((w[i] - (float)hi) * kLowUnit<T>);
             x[i] = __builtin_bit_cast(uint16_t, upper ? lo : hi);
         }
         a0 = q38_u32x2{pack16(x[0], x[1]), pack16(x[2], x[3])};
@@ -557,7 +564,7 @@ Q38_DEV void decode_typed(const Args &a) {
             for (int i = 0; i < 4; ++i) {
                 auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(st.o[n][i]), __float_as_uint(st.o[n + 1][i]), false, false);
                 if (i < 2 || (g & 1) == 0) /* heads 4 (g & 1) + i < 6 */
-                    out[i * Q38_ATTN_HEAD_DIM + 16 * n] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+                    out[i * Q38_ATTN_HEAD_DIM + 16 * n] = __builtin_fmaf(__uint_as_float(r[1]), 1.0f / kLowUnit<T>, __uint_as_float(r[0]));
             }
         }
     }
