@@ -25,7 +25,8 @@
  *    2^-36 of a weight's unit (2^-43 of the largest weight), not 2^-24, and a
  *    small weight on a large value keeps its bits.
  *    8-bit rows: the value's scale goes into its weight, over a power of two
- *    at or above every scale seen so far, which keeps f16 clear of overflow.
+ *    per head that follows the largest product of the two, so that a row of
+ *    large values without weight takes nothing from the others.
  *  - softmax in base 2 against a reference per head that is raised (and O and
  *    the sum rescaled) only when a score passes the one that set it by 2^8, so
  *    most pages rescale nothing.  In f16 the weights are taken 2^7 times as
@@ -66,6 +67,13 @@ constexpr float kRefSlack = 8.0f;
  * leaves 2^-11 of the weight at most, 2^4). */
 template <int T>
 constexpr float kLowUnit = T == Q38_KV_BF16 ? 1.0f : 0x1p11f;
+/* 8-bit rows, weight times scale: the largest one of a page that raises a
+ * head's power of two becomes 2^6 .. 2^8 units of it, and up to 2^15 raise
+ * nothing.  The powers' ends keep them, their inverses and a weight (2^15 at
+ * most) over them normal, and the largest scale (2^121) times such a weight
+ * within f16. */
+constexpr float kWeightedMax = 0x1p15f;
+constexpr int kWeightedBits = 8, kUnitMin = -112, kUnitMax = 121;
 
 /* One page of one kv head as a wave holds it. */
 template <int T>
@@ -133,7 +141,8 @@ Q38_DEV float column_sum(float x) {
 struct State {
     float ref; /* column l % 16's reference, in log2 units */
     float l;   /* the sum of this lane's weights */
-    float cap; /* 8-bit rows: a power of two at or above every value scale so far */
+    int unit;   /* 8-bit rows: o is in units of 2^unit, in which a scaled weight fits f16 */
+    float inv;  /* 2^-unit */
     f32x4 o[16]; /* o[n][i]: row 4 (l / 16) + i, dim 16 n + l % 16 */
 };
 
@@ -200,49 +209,63 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         }
     }
     const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    if (__any(mx > st.ref + (kRefBelow<T> + kRefSlack))) {
+    float f = 1.0f; /* o's */
+    bool raised = __any(mx > st.ref + (kRefBelow<T> + kRefSlack));
+    if (raised) {
         /* the page's maximum per head; heads that it does not raise keep theirs */
         const float top = column_max(mx) - kRefBelow<T>;
         const float ref = fmaxf(st.ref, top);
-        const float f = st.ref == -INFINITY ? 0.0f : q38_exp2(st.ref - ref);
-        st.ref = ref;
+        f = st.ref == -INFINITY ? 0.0f : q38_exp2(st.ref - ref);
         st.l *= f;
-        if (!first) {
-            float fr[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * g + i, 64);
-#pragma unroll
-            for (int n = 0; n < 16; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) st.o[n][i] *= fr[i];
+        if (T == Q38_KV_Q8) {
+            /* what o holds shrinks with the weights: its unit follows by whole
+             * powers, the next above, and o is left up to twice as large */
+            const float by = st.ref == -INFINITY ? 512.0f : fminf(ref - st.ref, 512.0f);
+            const int unit = max(st.unit - (int)ceilf(by), kUnitMin);
+            f = q38_exp2((float)(st.unit - unit) - by);
+            st.unit = unit;
+            st.inv = __builtin_amdgcn_ldexpf(1.0f, -unit);
         }
-    }
-    float vinv = 1.0f;
-    if (T == Q38_KV_Q8) {
-        /* scales are signed (the largest value is quant -127) */
-        const float big = fmaxf(fmaxf(fabsf(vs[0]), fabsf(vs[1])), fmaxf(fabsf(vs[2]), fabsf(vs[3])));
-        if (__any(big > st.cap)) {
-            const float top = column_max(big);
-            /* the next power of two, not below 2^-100 */
-            const uint32_t e = max((__float_as_uint(top) >> 23) + 1u, 27u);
-            const float cap = __uint_as_float(min(e, 254u) << 23);
-            const float f = st.cap / cap;
-            st.cap = cap;
-            if (!first) {
-#pragma unroll
-                for (int n = 0; n < 16; ++n) st.o[n] *= f;
-            }
-        }
-        vinv = 1.0f / st.cap;
+        st.ref = ref;
     }
     float w[4], sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         w[i] = q38_exp2(s[i] - st.ref);
         sum += w[i];
-        if (T == Q38_KV_Q8) w[i] *= vs[i] * vinv;
     }
     st.l += sum;
+    if (T == Q38_KV_Q8) {
+        /* scales are signed (the largest value is quant -127) */
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = w[i] * st.inv * vs[i];
+        if (__any(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))) > kWeightedMax)) {
+            int need = kUnitMin;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (x[i] != 0.0f)
+                    need = max(need, __builtin_amdgcn_frexp_expf(w[i]) + __builtin_amdgcn_frexp_expf(vs[i]) - kWeightedBits);
+            const int unit = min(max(st.unit, (int)column_max((float)need)), kUnitMax);
+            f = __builtin_amdgcn_ldexpf(f, st.unit - unit);
+            raised = true;
+            st.unit = unit;
+            st.inv = __builtin_amdgcn_ldexpf(1.0f, -unit);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = w[i] * st.inv * vs[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = x[i];
+    }
+    if (raised && !first) {
+        float fr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * g + i, 64);
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st.o[n][i] *= fr[i];
+    }
 
     /* the weights' parts: rows 0-5 the first (and, in a product of its own,
      * the third), rows 8-13 the second */
@@ -414,7 +437,7 @@ Q38_DEV void decode_typed(const Args &a) {
     __shared__ __attribute__((aligned(16))) float rope_cs[kPre ? kWaves : 1][32][2];
     __shared__ __attribute__((aligned(16))) float red_o[kWaves][kGroup][Q38_ATTN_HEAD_DIM];
     __shared__ __attribute__((aligned(16))) float red_m[8][kWaves], red_l[8][kWaves]; /* [column][wave] */
-    __shared__ __attribute__((aligned(16))) float red_unit[kWaves]; /* of red_o */
+    __shared__ __attribute__((aligned(16))) float red_unit[8][kWaves]; /* of red_o */
     static_assert(kWaves == 8 && kGroup == 6, "a wave per query head, one for the key and one for the value");
 
     const int g_split = blockIdx.x, j = blockIdx.y, tid = threadIdx.x;
@@ -526,7 +549,8 @@ Q38_DEV void decode_typed(const Args &a) {
         State st;
         st.ref = -INFINITY;
         st.l = 0.0f;
-        st.cap = __uint_as_float(27u << 23); /* 2^-100 */
+        st.unit = kUnitMin;
+        st.inv = __builtin_amdgcn_ldexpf(1.0f, -kUnitMin);
 #pragma unroll
         for (int n = 0; n < 16; ++n) st.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
         /* the only ways out are the gotos: a page's loads are behind the same
@@ -555,8 +579,8 @@ Q38_DEV void decode_typed(const Args &a) {
         if (lane < 8) {
             red_m[lane][wave] = st.ref + kRefBelow<T>;
             red_l[lane][wave] = l * kUnit;
+            red_unit[lane][wave] = T == Q38_KV_Q8 ? __builtin_amdgcn_ldexpf(kUnit, st.unit) : kUnit;
         }
-        if (lane == 0) red_unit[wave] = T == Q38_KV_Q8 ? st.cap * kUnit : kUnit;
         float *out = &red_o[wave][4 * (g & 1)][16 * (g >> 1) + c];
 #pragma unroll
         for (int n = 0; n < 16; n += 2) {
@@ -579,7 +603,7 @@ Q38_DEV void decode_typed(const Args &a) {
     if (n_pages == 1) {
         M = red_m[wave][0];
         L = red_l[wave][0];
-        O = q38_ld4(&red_o[0][wave][4 * lane]) * red_unit[0];
+        O = q38_ld4(&red_o[0][wave][4 * lane]) * red_unit[wave][0];
     } else {
         float m[kWaves], f[kWaves];
         f32x4 o[kWaves];
@@ -594,7 +618,7 @@ Q38_DEV void decode_typed(const Args &a) {
             f[w] = q38_exp2(m[w] - M);
             /* a wave without pages has left nothing there */
             L += w < n_pages ? red_l[wave][w] * f[w] : 0.0f;
-            const float fu = f[w] * red_unit[w];
+            const float fu = f[w] * red_unit[wave][w];
 #pragma unroll
             for (int e = 0; e < 4; ++e) O[e] = w < n_pages ? __builtin_fmaf(fu, o[w][e], O[e]) : O[e];
         }

@@ -1,10 +1,10 @@
-"""One token's attention over 16-bit rows whose values differ by many
+"""One token's attention over 16- and 8-bit rows whose values differ by many
 orders (tests/typed_ranges.py has the inputs and the limits)."""
 import numpy as np
 import pytest
 from parity import decode_split
 from typed_ranges import CASES, IDENT, IDS, attend_by_weight, case, check, heads_of
-from typed_rows import stored
+from typed_rows import attend, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,25 @@ def test_a_batch_of_them(pkg, ctx, ty):
     finally:
         kv.close()
 
+
+def test_values_near_the_ends_of_f32(pkg, ctx):
+    """8-bit rows of 1e-34 and of 1e37 values, alone and mixed."""
+    P = 300
+    for seed, sizes in enumerate(([1e-34], [1e37], [1e-34, 1e37], [1e37, 1e-30, 1.0])):
+        rng = np.random.default_rng(seed)
+        Q = rng.standard_normal((24, 256)).astype(np.float32)
+        K, V = rng.standard_normal((P, 1024)).astype(np.float32), rng.uniform(-1, 1, (P, 1024)).astype(np.float32)
+        V *= np.resize(np.array(sizes, np.float32), P)[:, None]
+        kv, ids = _cache(pkg, ctx, "q8_k", [(K, V)])
+        out = ctx.empty((24, 256))
+        try:
+            for split in (4096, None):
+                with decode_split(ctx, split):
+                    kv.attn_decode(3, ids, [P - 1], ctx.array(Q), out)
+                k, v = stored(K, IDENT["q8_k"]), stored(V, IDENT["q8_k"])
+                want, bound = attend_by_weight(Q, k, v, IDENT["q8_k"])
+                off = np.abs(out.download().astype(np.float64) - want)
+                assert np.all(off <= bound), (sizes, float((off / bound).max()))
+                assert np.all(off <= attend(Q, k, v)[1])
+        finally:
+            kv.close()

@@ -26,6 +26,16 @@ def _whole(w, vv):
     return w
 
 
+def _by_largest_scale(w, vv):
+    """Two f16 parts of weight times scale over the largest scale's power of two."""
+    scale = np.abs(vv).max(1) / np.float32(127.0)
+    unit = np.exp2(np.ceil(np.log2(scale.max()))).astype(np.float32)
+    x = w * np.float32(2.0 ** 7) * (scale / unit)
+    hi = x.astype(np.float16).astype(np.float32)
+    lo = (x - hi).astype(np.float16).astype(np.float32)
+    return np.where(scale > 0, (hi + lo) / np.float32(2.0 ** 7) * (unit / np.where(scale > 0, scale, 1)), 0).astype(np.float32)
+
+
 def _plain_f16_parts(w, vv):
     x = w * np.float32(2.0 ** 7)
     hi = x.astype(np.float16).astype(np.float32)
@@ -40,7 +50,10 @@ def test_plain_arithmetic_holds(ty, name, args):
     check(got, want, bound, tol, heads_of(name))
 
 
-@pytest.mark.parametrize("ty,name,args,lose", [("f16", "little_weight", (16, 26, 2.0 ** -12), _plain_f16_parts)])
+@pytest.mark.parametrize("ty,name,args,lose", [
+    ("q8_k", "no_weight", (1e5, 200), _by_largest_scale), ("q8_k", "no_weight", (1e8, 37), _by_largest_scale),
+    ("q8_k", "little_weight", (10, 40, 1.0), _by_largest_scale), ("q8_k", "one_heads_row", (1e8, 399), _by_largest_scale),
+    ("q8_k", "slope", (60, 1.0, True), _by_largest_scale), ("f16", "little_weight", (16, 26, 2.0 ** -12), _plain_f16_parts)])
 def test_lost_parts_are_noticed(ty, name, args, lose):
     Q, _, _, k, v, tol = case(ty, name, args)
     want, bound = attend_by_weight(Q, k, v, IDENT[ty])

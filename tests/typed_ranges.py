@@ -8,7 +8,7 @@ is measured by what is added, not by the largest value in the cache.
 from __future__ import annotations
 
 import numpy as np
-from typed_rows import BF16, F16, NORMAL_TOL, off_by, stored
+from typed_rows import BF16, F16, NORMAL_TOL, Q8_K, off_by, stored
 
 U = 2.0 ** -24
 
@@ -21,7 +21,9 @@ def attend_by_weight(q, k, v, ty):
     2^11 times as large, a weight is off by half of f16's smallest step over 2^11 --
     2^-36 of its unit -- where its parts are no longer normal: for F16 rows the
     largest weight of a chain is 2^7 units at least, so 2^-43 of the largest
-    weight times the value.  Twice that for the joins."""
+    weight times the value; for Q8_K rows the largest weight times scale of a
+    chain is 2^6 units at least, so 2^-42 of that times a quant, 127 at most:
+    2^-42 of the largest weighted value.  Twice that for the joins."""
     n = k.shape[0]
     out, bound = np.empty((24, 256)), np.empty((24, 256))
     q, k, v = q.reshape(24, 256).astype(np.float64), k.astype(np.float64), v.astype(np.float64)
@@ -35,7 +37,8 @@ def attend_by_weight(q, k, v, ty):
         out[h] = p @ vv
         top = float(((264 * size + np.abs(s)) * p).sum())  # the denominator's, by weight
         e = (264 * size + np.abs(s) + top + 8 + n + 16) * U + 2.0 ** -21
-        least = {BF16: 2.0 ** -125 * np.abs(vv).max(), F16: 2.0 ** -42 * p.max() * np.abs(vv).max()}[ty]
+        least = {BF16: 2.0 ** -125 * np.abs(vv).max(), F16: 2.0 ** -42 * p.max() * np.abs(vv).max(),
+                 Q8_K: 2.0 ** -41 * (p * np.abs(vv).max(1)).max()}[ty]
         bound[h] = (e * p) @ np.abs(vv) * 1.01 + n * least + 1e-44
     return out, bound
 
@@ -100,18 +103,18 @@ def slope(seed, binades, base, rising, P=700):
 
 
 # (type, name, arguments after the seed)
-CASES = [(ty, "no_weight", (r, at)) for ty in ("bf16",) for r, at in
+CASES = [(ty, "no_weight", (r, at)) for ty in ("q8_k", "bf16") for r, at in
          ((1e3, 399), (1e4, 7), (1e5, 200), (1e6, 0), (1e8, 37), (1e10, 350), (1e20, 100))]
 CASES += [("f16", "no_weight", (1e4, 0)), ("f16", "no_weight", (1e4, 250))]
-CASES += [(ty, "little_weight", (16, 26, 2.0 ** -12)) for ty in ("f16", "bf16")]
-CASES += [(ty, "little_weight", a) for ty in ("bf16",) for a in ((10, 40, 1.0), (30, 100, 1.0))]
-CASES += [("f16", "one_heads_row", (1e4, 50))] + [(ty, "one_heads_row", (r, at)) for ty in ("bf16",)
+CASES += [(ty, "little_weight", (16, 26, 2.0 ** -12)) for ty in ("f16", "bf16", "q8_k")]
+CASES += [(ty, "little_weight", a) for ty in ("bf16", "q8_k") for a in ((10, 40, 1.0), (30, 100, 1.0))]
+CASES += [("f16", "one_heads_row", (1e4, 50))] + [(ty, "one_heads_row", (r, at)) for ty in ("bf16", "q8_k")
                                                   for r, at in ((1e8, 0), (1e8, 399), (1e25, 160), (1e-8, 30))]
 CASES += [("f16", "slope", (24, 2.0 ** 10, up)) for up in (True, False)]
-CASES += [(ty, "slope", (b, base, up)) for ty in ("bf16",) for up in (True, False)
+CASES += [(ty, "slope", (b, base, up)) for ty in ("bf16", "q8_k") for up in (True, False)
           for b, base in ((60, 1.0), (110, 1.0), (110, 2.0 ** 100))]
 IDS = ["-".join([ty, name] + [str(a) for a in args]) for ty, name, args in CASES]
-IDENT = {"f16": F16, "bf16": BF16}
+IDENT = {"f16": F16, "bf16": BF16, "q8_k": Q8_K}
 
 
 def case(ty, name, args):
