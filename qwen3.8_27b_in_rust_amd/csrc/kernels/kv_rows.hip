@@ -112,19 +112,21 @@ Q38_DEV int piece_at(bool key, int quad, int p) {
  * where four separate reductions take 24 -- and what follows (a division, a
  * root) is done once for all four. */
 template <typename V, typename DPP1, typename DPP2, typename DPP4, typename DPP8, typename Join, typename Halves>
-Q38_DEV V quad_reduce(const V (&s)[4], int lane, DPP1 xor1, DPP2 xor2, DPP4 ror4, DPP8 ror8, Join join, Halves across) {
+Q38_DEV V quad_reduce(const V (&s)[4], int lane, DPP1 xor1, DPP2 xor2, DPP4 by4, DPP8 ror8, Join join, Halves across) {
     const bool b0 = lane & 1, b1 = lane & 2;
     const V a = join(b0 ? s[1] : s[0], xor1(b0 ? s[0] : s[1]));
     const V c = join(b0 ? s[3] : s[2], xor1(b0 ? s[2] : s[3]));
     V r = join(b1 ? c : a, xor2(b1 ? a : c));
-    r = join(r, ror4(r));
+    r = join(r, by4(r));
     r = join(r, ror8(r));
     return across(r);
 }
+/* The sums are taken in q38_wave_sum_f64's order: a key's mean, and so its row, is
+ * the same whichever kernel forms it. */
 Q38_DEV double quad_sum_f64(const double (&s)[4], int lane) {
     return quad_reduce(
         s, lane, [](double x) { return q38_row_move_f64<0xB1>(x); }, [](double x) { return q38_row_move_f64<0x4E>(x); },
-        [](double x) { return q38_row_move_f64<0x124>(x); }, [](double x) { return q38_row_move_f64<0x128>(x); },
+        [](double x) { return q38_row_xor4_f64(x); }, [](double x) { return q38_row_move_f64<0x128>(x); },
         [](double x, double y) { return x + y; },
         [](double x) { return q38_rows_sum_f64(x); });
 }
@@ -146,7 +148,7 @@ Q38_DEV float quad_value(float x, int i) {
 }
 
 /* RMSNorm and rotation of the quad's keys (q38_norm_rope4_cs, four at once).
- * Every f32 square is exact in f64, so the fused sum is the plain one. */
+ * Every f32 square is exact in f64, so a fused addition rounds as the plain one. */
 Q38_DEV void norm_rope_quad(f32x4 (&x)[4], f32x4 w, int lane, const float (*cs)[32][2], const int (&t)[4]) {
     double ss[4];
 #pragma unroll

@@ -180,6 +180,17 @@ Q38_DEV double q38_row_move_f64(double x) {
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
+/* Lane l ^ 4's value within the row: the next four lanes' for the first and third
+ * four, the previous ones' for the others (two rotations, each into its own). */
+Q38_DEV double q38_row_xor4_f64(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    auto move = [](int v) {
+        const int next = __builtin_amdgcn_update_dpp(v, v, 0x12C, 0xF, 0x5, false);
+        return (uint32_t)__builtin_amdgcn_update_dpp(next, v, 0x124, 0xF, 0xA, false);
+    };
+    return __builtin_bit_cast(double, (uint64_t)move((int)(uint32_t)(b >> 32)) << 32 | move((int)(uint32_t)b));
+}
+
 /* s_waitcnt immediate (gfx9 encoding: vmcnt bits 3:0 and 15:14, expcnt 6:4,
  * lgkmcnt 11:8) that waits until at most `vm` vector memory operations and
  * `lgkm` LDS/scalar operations of this wave are outstanding. */

@@ -74,8 +74,11 @@ Q38_DEV void q38_norm_rope8(f32x4 &x0, f32x4 &x1, f32x4 w0, f32x4 w1, int li, co
 
 /* RMSNorm with weight w (rms_scale / rmsnorm_inplace, ops.rs:476-498: f64 sum
  * of squares, eps 1e-6), then the RoPE of q38_rope_lanes_cs, of a head held 4
- * dims per lane by a whole wave.  Every f32 square is exact in f64, so the f64
- * sum rounds to the same f32 mean in any order. */
+ * dims per lane by a whole wave.  Every f32 square is exact in f64, its sums are
+ * not: two orders of them give the same f32 mean unless it lies within some
+ * 2^-50 of halfway between two.  The forms of a whole wave (this, q38_norm_rope_row, the
+ * append's) add in one order and agree bit for bit; a half-wave's
+ * (q38_norm_rope8) adds in another. */
 Q38_DEV void q38_norm_rope4_cs(f32x4 &x, f32x4 w, int lane, const float (*cs)[2]) {
     double ss = (double)x.x * (double)x.x + (double)x.y * (double)x.y + (double)x.z * (double)x.z +
                 (double)x.w * (double)x.w;
@@ -118,8 +121,8 @@ Q38_DEV void q38_rope_row(f32x4 &x, int lane, const float (*cs)[2]) {
     }
 }
 
-/* q38_norm_rope4_cs by row moves.  Every f32 square is exact in f64, so the
- * fused sums are the plain ones. */
+/* q38_norm_rope4_cs by row moves, its sums in the same order.  Every f32 square
+ * is exact in f64, so a fused addition rounds as the plain one. */
 Q38_DEV void q38_norm_rope_row(f32x4 &x, f32x4 w, int lane, const float (*cs)[2]) {
     double ss = (double)x.x * (double)x.x;
 #pragma unroll
