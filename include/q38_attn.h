@@ -99,7 +99,12 @@ int q38_kv_create(q38_ctx *ctx, int n_slots, int max_pages, int max_seqs, int ma
  * format per kv head (256 values share a scale), with the quants and scale of
  * q38_quantize_q8_k for finite values -- and every call below reads the values
  * that the stored rows stand for: a token appended by q38_attn_decode or
- * q38_full_core attends to its own row as it is stored.  A page takes 64 KiB
+ * q38_full_core attends to its own row as it is stored.  A stored infinity or
+ * NaN spoils what it meets, in calls over its position (in a prefill, for every
+ * token of the call): a key's, the six query heads of its kv head; a value's,
+ * its dim of those heads' outputs (Q8_K, whose block shares a scale: every dim).
+ * What is left there is not specified -- infinite, NaN, or as if the row were not there.
+ * Other heads, dims and sequences stay as they are.  A page takes 64 KiB
  * per slot for K and V together in 16 bits and 32.5 KiB in Q8_K, against
  * 128 KiB in F32.  No counterpart in the reference (its cache is f32). */
 int q38_kv_create_typed(q38_ctx *ctx, int ggml_type, int n_slots, int max_pages, int max_seqs,

@@ -32,6 +32,8 @@
  *    most pages rescale nothing.  In f16 the weights are taken 2^7 times as
  *    large, up to 2^15, which leaves their small parts more of its range; the
  *    partials leave without that factor.
+ * An infinity in a row that counts meets a lower part that may be 0 or of the
+ * other sign: NaN, in the heads of a key, in the dim of a value (16-bit rows).
  * A row's position past the sequence's end counts nothing whatever it holds:
  * its scores are -inf and its values, which a weight of 0 would not keep NaN
  * out of, are cleared.
