@@ -379,7 +379,7 @@ int q38_q8k_bytes(int n_tokens, int width, size_t *bytes);
 int q38_quantize_q8_k(q38_ctx *ctx, int n_tokens, int width, const float *d_x, void *d_q8k);
 
 /* The f32 values that a device Q8_K buffer stands for (quant times its block's
- * scale): d_x [n_tokens][width], both pointers 16-byte aligned. */
+ * scale): d_x [n_tokens][width], both pointers 16-byte aligned, the buffers apart. */
 int q38_dequantize_q8_k(q38_ctx *ctx, int n_tokens, int width, const void *d_q8k, float *d_x);
 
 /* The residual's addition and the layer norm before a layer's projections

@@ -1035,6 +1035,11 @@ int validate_rows(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
     return 0;
 }
 
+/* Whether np bytes at p and nq bytes at q share one. */
+bool overlaps(const void *p, size_t np, const void *q, size_t nq) {
+    return p != nullptr && q != nullptr && (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
+}
+
 /* Moves a validated batch whose pages are reserved, in launches of up to
  * Q38_MAX_BATCH sequences; rows of `elem_bytes` a value. */
 int launch_rows(q38_kv *kv, const q38_ctx::RowsKernel &f, int slot, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
@@ -2627,6 +2632,8 @@ int q38_dequantize_q8_k(q38_ctx *ctx, int n_tokens, int width, const void *d_q8k
     if (n_tokens == 0) return 0;
     if (!d_q8k || !d_x) return fail("NULL argument");
     if (((uintptr_t)d_q8k | (uintptr_t)d_x) % 16 != 0) return fail("d_q8k and d_x must be 16-byte aligned");
+    if (overlaps(d_q8k, Q38_Q8K_BYTES(n_tokens, width), d_x, (size_t)n_tokens * width * sizeof(float)))
+        return fail("d_x overlaps d_q8k");
     const size_t groups = ((size_t)n_tokens * width + 1023) / 1024;
     if (groups > 0xFFFFFFFFull / 256) return fail("%d rows of %d: too many for one call", n_tokens, width);
     q38_dequantize_args a = {d_q8k, d_x, width, n_tokens};
@@ -2651,9 +2658,6 @@ int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, co
     /* an output may be one of the inputs' rows themselves: a row is read whole
      * before any of it is written; overlapping in part it is not */
     const size_t bytes = (size_t)n_tokens * width * sizeof(float);
-    auto overlaps = [](const void *p, size_t np, const void *q, size_t nq) {
-        return p != nullptr && q != nullptr && (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
-    };
     const size_t q_bytes = d_q8k != nullptr ? Q38_Q8K_BYTES(n_tokens, width) : 0;
     for (float *o : {d_sum, d_y}) {
         for (const float *in : {d_x, d_residual})
