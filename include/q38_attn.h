@@ -171,7 +171,7 @@ int q38_kv_append(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
 
 /* The stored rows of a ragged batch back (q38_kv_read for many sequences, e.g.
  * to hand a prompt's cache to another context): rows packed in order in d_k
- * and d_v (16-byte aligned), as f32 (ggml_type 0), or, for an F16 or BF16
+ * and d_v (16-byte aligned, apart), as f32 (ggml_type 0), or, for an F16 or BF16
  * cache and that ggml_type, in 16 bits as they are stored. */
 int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
                   const int32_t *n_tokens, int ggml_type, void *d_k, void *d_v);

@@ -1167,6 +1167,8 @@ int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
     if (n_rows == 0) return 0;
     if (!d_k || !d_v) return fail("NULL argument");
     if (((uintptr_t)d_k | (uintptr_t)d_v) % 16 != 0) return fail("d_k and d_v must be 16-byte aligned");
+    const size_t bytes = (size_t)n_rows * Q38_ATTN_KV_DIM * (as_stored ? 2 : sizeof(float));
+    if (overlaps(d_k, bytes, d_v, bytes)) return fail("d_k overlaps d_v");
     return launch_rows(kv, as_stored ? kv->ctx->f_kv_gather_16 : kv->ctx->f_kv_gather[kv->type], slot, n_seq, seq_ids,
                        pos0, n_tokens, d_k, d_v, as_stored ? 2 : sizeof(float), nullptr);
 }

@@ -21,6 +21,24 @@ int main() {
     REQUIRE(q38_dequantize_q8_k(&ctx, 0, 512, base, reinterpret_cast<float *>(base)) == 0);
     REQUIRE(g_launches == launches);
     REQUIRE(Q38_Q8K_BYTES(3, 512) == 1752);
+
+    /* 40 rows of two sequences: 4096 bytes a row, 2048 as stored */
+    for (int type : {0, 2}) {
+        Cache c(type, 1, 64, 4, 512);
+        int32_t s[2], p[2] = {3, 0}, n[2] = {33, 7};
+        for (int i = 0; i < 2; ++i) {
+            REQUIRE(q38_seq_create(&c.kv, &s[i]) == 0);
+            REQUIRE(q38_seq_reserve(&c.kv, s[i], 64) == 0);
+        }
+        const int own = kKvTypes[type].ggml_type;
+        const long bytes = 40l * 1024 * (type == 0 ? 4 : 2);
+        const int before = g_launches;
+        for (long at : {0l, 16l, bytes - 16, -16l, 16 - bytes})
+            refused(q38_kv_gather(&c.kv, 3, 2, s, p, n, own, base, base + at), "overlaps");
+        REQUIRE(g_launches == before);
+        for (long at : {bytes, -bytes}) REQUIRE(q38_kv_gather(&c.kv, 3, 2, s, p, n, own, base, base + at) == 0);
+        REQUIRE(g_launches == before + 2);
+    }
     printf("row buffers ok\n");
     return 0;
 }
