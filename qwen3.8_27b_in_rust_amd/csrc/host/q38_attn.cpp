@@ -1229,7 +1229,11 @@ struct decode_plan {
  * against one workgroup per CU by the total but at most 1024 tokens for batches,
  * as over f32 rows (us, f16 and Q8_K): 3 sequences of 2K-32K 33.1 against 44.9
  * and 21.0 against 30.0, 24 of 200-3000 25.9 / 34.7 and 19.2 / 27.0, 16 of 2K-32K
- * 120 / 125 and 68 / 74, 64 of 100-20000 417 / 458 and 226 / 266.  Where every
+ * 120 / 125 and 68 / 74, 64 of 100-20000 417 / 458 and 226 / 266.  It counts rounds
+ * as if splits were alike, so a long sequence among many short ones is cut too
+ * coarsely: 63 of 50 tokens and one of 4000 take 71.7 and 44.5 where splits of 256
+ * take 21.3 and 21.6, 62 of 50 and one of 8000 79.8 and 49.9 against 21.9 and 21.3
+ * (q38_set_decode_split serves such a batch).  Where every
  * sequence has kOneSplitTokens at most, one split each needs no merge launch: one
  * Q8_K sequence of 17 / 128 / 256 tokens 5.1 / 5.9 / 7.2 against 7.7 / 7.8 / 8.0
  * (512: 10.0 against 8.2). */
@@ -2009,6 +2013,7 @@ retry:
  * carries on every HIP runtime */
 static_assert(sizeof(q38_prefill_args) <= 4096, "prefill arguments exceed 4 KiB");
 static_assert(sizeof(q38_decode_args) <= 4096, "decode arguments exceed 4 KiB");
+static_assert(sizeof(q38_kv_rows_few_args) == 104 && sizeof(q38_kv_rows_args) == 1120, "the sizes that their comment compares");
 /* a typed launch passes the same block, of which its kernel takes the front */
 static_assert(offsetof(q38_decode_args, head_pages) == sizeof(q38_decode_typed_args) &&
                   offsetof(q38_decode_args, split_base) == offsetof(q38_decode_typed_args, split_base),
@@ -2680,9 +2685,9 @@ int q38_add_rms_norm(q38_ctx *ctx, int n_tokens, int width, const float *d_x, co
         return ctx->launch_params(ctx->f_norm_any, (unsigned)n_tokens, 1, 1, 1024, params);
     /* up to two rows per CU the chip has waves to spare, and 1024 threads a row
      * shorten the row's own chain; past that 256 keep more rows in flight and
-     * waste fewer lanes on short ones (rows of 5120, us: 1 row 3.9 against 4.2,
-     * 256 rows 5.3 against 6.1, 1024 rows 15.1 against 14.3; 4096 rows of 1024
-     * 17.3 against 11.7) */
+     * waste fewer lanes on short ones (all outputs, rows that no cache holds, us:
+     * 1024 threads against 256 for 1 row of 5120 3.8 and 4.0, 256 rows 6.8 and 7.5,
+     * 512 rows 9.8 and 10.3, 1024 rows 19.5 and 18.2; 4096 rows of 1024 22.7 and 14.9) */
     const int wide = width > 256 * 4 * kNormVectors || n_tokens <= 2 * ctx->cu_count;
     const int per = (wide ? 1024 : 256) * 4;
     return ctx->launch_params(ctx->f_norm[wide][(width + per - 1) / per - 1], (unsigned)n_tokens, 1, 1,

@@ -21,9 +21,10 @@
  * Q8_K 9.9, 9.2, 9.3 and back 7.6, 7.5, 8.0; to bf16 9.4, 10.1, 11.2.
  *
  * Measured (us, calls of one kind in turn over buffers that no cache holds):
- * 4096 tokens to Q8_K 9.2 (42 MB) and back 7.5 (5.6 TB/s); 1531 tokens of 12
- * sequences to bf16 6.7 and back 6.0; 6 tokens to f16 3.8 and back 3.8, which
- * is what the launches of so small calls take on the host.
+ * 4096 tokens to Q8_K 9.2 (42 MB) and back 7.4 (5.7 TB/s); 1531 tokens of 12
+ * sequences to bf16 6.8 and back 5.2; 6 tokens to f16 4.1 and back 3.8, which
+ * is what the launches of so small calls take on the host.  (Traced in turn with
+ * each other, 4096 tokens take the kernels 10.1 and 6.7.)
  * Keys are held up by their arithmetic as much as by memory: the angles and,
  * per token and head, the f64 sum, the rotation and the quantiser are some
  * 500 instructions a wave and quad (1500 with four reductions one by one,

@@ -60,9 +60,9 @@ Q38_DEV void store_q8k(const Q8kRow &r, int b, int lane, f32x4 y) {
  * dims 4 (i + NT v) .. + 3, so a wave's v-th vectors are 256 consecutive dims,
  * a Q8_K block.  Every load is issued at once and every value read once, so
  * the kernel runs at the memory's rate: 4096 rows of 5120 with all outputs
- * (17.14 bytes a value) 67 us, 5.4 TB/s; 512 rows of 12288 to 20480 6.5 to 6.7
- * TB/s; one row 3.9 us a launch among others, where an empty one takes about as
- * long.  A first version that read its row twice and value by value took 187 us. */
+ * (17.14 bytes a value) 67 us, 5.4 TB/s, 512 rows of 12288 to 20480 5.3 to 5.6
+ * TB/s, rows and outputs that no cache holds; one row 3.5 us a call among others (the
+ * kernel 3.3), where an empty launch takes about as long.  A first version that read its row twice and value by value took 187 us. */
 template <int NT, int V>
 Q38_DEV void norm_row(const q38_norm_args &a) {
     __shared__ double part[NT / 64];

@@ -177,7 +177,7 @@ typedef struct {
     int32_t page_base[Q38_MAX_BATCH + 8];
 } q38_kv_rows_args;
 /* Up to Q38_KV_ROWS_FEW sequences, from whose counts (0 past the last) the
- * kernel finds the bases: 112 bytes of arguments instead of 1128.  An append
+ * kernel finds the bases: 104 bytes of arguments instead of 1120.  An append
  * of 6 tokens takes 3.4 us on the host (3.9 with 232 bytes, which hold the bases
  * of eight sequences). */
 #define Q38_KV_ROWS_FEW 4
@@ -451,7 +451,7 @@ typedef struct {
     int32_t n_tokens;
 } q38_norm_args;
 /* The kernels take them as plain vectors, in registers when a wave starts: one
- * row's norm 3.4 us against 3.5 where the GPU is what bounds (as a block; one by
+ * row's norm 3.5 us a call against 3.6 where the GPU is what bounds (as a block; one by
  * one the eight arguments cost a launch 0.3 us on the host, three 0.1). */
 #define Q38_NORM_PARAMS q38_u64x4 in, q38_u64x2 out, q38_i32x2 n
 #define Q38_NORM_ARGS                                                                                     \
