@@ -14,16 +14,16 @@
  *    stands (an 8-bit quant as a whole number in f16, its row's scale applied
  *    to the score).  A query is split into parts whose sum it is -- f16 hi and
  *    lo (22 bits, after a power of two per head brings the largest to 2^9..10,
- *    clear of f16's ends), or bf16 hi, mid and lo (24 bits) -- and the 6 heads
+ *    clear of f16's ends; lo taken 2^11 times as large, so that f16's fixed step
+ *    below 2^-14 is 2^-45 of the largest or less and a small one on a large key keeps its
+ *    bits), or bf16 hi, mid and lo (24 bits) -- and the 6 heads
  *    fill columns 0-5 with one part and 8-13 with another, so two parts cost
  *    one product; a rotation of the 16 lanes by 8 adds them up.
  *  - O = P V, 16 rows x 16 dims.  The lanes that hold a score are those that
  *    supply its weight as an operand (C's column l % 16, rows 4 (l / 16) + i
  *    are A's row l % 16, k 4 (l / 16) + i), so the weights never leave their
- *    registers; they are split like the queries, into rows 0-5 and 8-13, an f16
- *    lower part taken 2^11 times as large: f16's fixed step below 2^-14 then is
- *    2^-36 of a weight's unit (2^-43 of the largest weight), not 2^-24, and a
- *    small weight on a large value keeps its bits.
+ *    registers; they are split like the queries, into rows 0-5 and 8-13, and held
+ *    to 2^-36 of their unit (2^-43 of the largest weight) or to 22 bits.
  *    8-bit rows: the value's scale goes into its weight, over a power of two
  *    per head that follows the largest product of the two, so that a row of
  *    large values without weight takes nothing from the others.
@@ -67,8 +67,8 @@ constexpr int kGroup = Q38_ATTN_GROUP;
 template <int T>
 constexpr float kRefBelow = T == Q38_KV_BF16 ? 0.0f : 7.0f;
 constexpr float kRefSlack = 8.0f;
-/* f16 weights: what their lower part is larger by (the upper one's rounding
- * leaves 2^-11 of the weight at most, 2^4). */
+/* f16 weights and queries: what their lower part is larger by (the upper one's
+ * rounding leaves 2^-11 of them at most, 2^4 and 2^-1). */
 template <int T>
 constexpr float kLowUnit = T == Q38_KV_BF16 ? 1.0f : 0x1p11f;
 /* 8-bit rows, weight times scale: the largest one of a page that raises a
@@ -202,11 +202,9 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float x = s0[i] + s1[i];
-        s[i] = x + row_ror8(x);
-        if (T == Q38_KV_Q8)
-            s[i] *= ks[i] * unscale;
-        else if (T == Q38_KV_F16)
-            s[i] *= unscale;
+        const float y = T == Q38_KV_BF16 ? x : x * unscale;
+        s[i] = y + row_ror8(y);
+        if (T == Q38_KV_Q8) s[i] *= ks[i];
         if (valid < 16 && 4 * g + i >= valid) {
             s[i] = -INFINITY;
             vs[i] = 0.0f;
@@ -392,7 +390,7 @@ Q38_DEV void store_query(q38_u32x4 (*q)[8][64], int c, int lane, f32x4 x) {
         } else {
             const _Float16 hi = (_Float16)x[e];
             a[e] = __builtin_bit_cast(uint16_t, hi);
-            b[e] = __builtin_bit_cast(uint16_t, (_Float16)(x[e] - (float)hi));
+            b[e] = __builtin_bit_cast(uint16_t, (_Float16)((x[e] - (float)hi) * kLowUnit<T>));
         }
     }
     put(0, c, a);
@@ -549,7 +547,7 @@ Q38_DEV void decode_typed(const Args &a) {
     const int c = lane & 15, g = lane >> 4;
 
     if (wave < n_pages) {
-        const float unscale = q_unscale[c & 7];
+        const float unscale = q_unscale[c & 7] * (c < 8 ? 1.0f : 1.0f / kLowUnit<T>); /* the column's */
         State st;
         st.ref = -INFINITY;
         st.l = 0.0f;
