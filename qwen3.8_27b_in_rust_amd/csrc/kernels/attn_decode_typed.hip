@@ -211,7 +211,16 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         }
     }
     const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    float f = 1.0f; /* o's */
+    auto scale_heads = [&](float f) { /* o by each head's factor */
+        float fr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * g + i, 64);
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st.o[n][i] *= fr[i];
+    };
+    float f = 1.0f;
     bool raised = __any(mx > st.ref + (kRefBelow<T> + kRefSlack));
     if (raised) {
         /* the page's maximum per head; heads that it does not raise keep theirs */
@@ -229,6 +238,7 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
             st.inv = __builtin_amdgcn_ldexpf(1.0f, -unit);
         }
         st.ref = ref;
+        if (T != Q38_KV_Q8 && !first) scale_heads(f);
     }
     float w[4], sum = 0.0f;
 #pragma unroll
@@ -238,35 +248,27 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
     }
     st.l += sum;
     if (T == Q38_KV_Q8) {
-        /* scales are signed (the largest value is quant -127) */
+        /* scales are signed (the largest value is quant -127).  A product past f32's
+         * end raises the unit by 2^120, which leaves it 2^8 at least, and is looked
+         * at once more; the second raise always does. */
         float x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = w[i] * st.inv * vs[i];
-        if (__any(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))) > kWeightedMax)) {
-            int need = kUnitMin;
+        for (int turn = 0;; ++turn) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (x[i] != 0.0f)
-                    need = max(need, __builtin_amdgcn_frexp_expf(w[i]) + __builtin_amdgcn_frexp_expf(vs[i]) - kWeightedBits);
-            const int unit = min(max(st.unit, (int)column_max((float)need)), kUnitMax);
+            for (int i = 0; i < 4; ++i) x[i] = w[i] * st.inv * vs[i];
+            const float big = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+            if (turn == 2 || !__any(big > kWeightedMax)) break;
+            const int top = __builtin_amdgcn_frexp_expf(fminf(column_max(big), 0x1.fffffep127f));
+            const int unit = min(st.unit + max(top - kWeightedBits, 0), kUnitMax);
             f = __builtin_amdgcn_ldexpf(f, st.unit - unit);
             raised = true;
             st.unit = unit;
             st.inv = __builtin_amdgcn_ldexpf(1.0f, -unit);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = w[i] * st.inv * vs[i];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = x[i];
-    }
-    if (raised && !first) {
-        float fr[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * g + i, 64);
-#pragma unroll
-        for (int n = 0; n < 16; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) st.o[n][i] *= fr[i];
+        /* once for both raises: two of these take registers that pages need */
+        if (raised && !first) scale_heads(f);
     }
 
     /* the weights' parts: rows 0-5 the first (and, in a product of its own,
