@@ -40,11 +40,11 @@
  *
  * Measured (us of a whole pass with its merge; one sequence, 600 MB of caches in
  * turn, so that nothing is in the last level's cache; forming q in the
- * kernel adds under 1): bf16 rows 17 tokens 5.1, 1021 8.3, 4096 10.4, 32K 26.5 (5.1
- * TB/s), 128K 86.3 (6.2 TB/s, what pages read once in any order reach); Q8_K 5.3,
- * 8.5, 9.9, 17.5 and 46.6 (5.9 TB/s).  One cache again and again: 8.0, 8.7, 25.7, 83.9
- * and 8.2, 9.0, 16.4, 46.9.  Long 16-bit contexts are bound by memory,
- * Q8_K ones by memory and the 267 vector instructions a page and head that mostly
+ * kernel adds under 1): bf16 rows 17 tokens 4.8, 1021 8.3, 4096 10.5, 32K 26.1 (5.1
+ * TB/s), 128K 85.9 (6.2 TB/s, what pages read once in any order reach); Q8_K 5.3,
+ * 8.5, 10.0, 17.6 and 47.1 (5.8 TB/s).  One cache again and again, 1021 to 128K: 8.0,
+ * 8.7, 25.7, 83.9 and 8.2, 9.0, 16.4, 46.9.  Long 16-bit contexts are bound by memory,
+ * Q8_K ones by memory and the 266 vector instructions a page and head that mostly
  * turn bytes into operands; short ones by the two launches and the chain
  * arguments - page id - page - scores - join, 3-4 us of them.
  */
