@@ -93,19 +93,23 @@ int q38_set_decode_split(q38_ctx *ctx, int tokens);
 int q38_kv_create(q38_ctx *ctx, int n_slots, int max_pages, int max_seqs, int max_tokens_per_seq,
                   q38_kv **out);
 /* The same cache with rows of another type: F32 (ggml type 0, q38_kv_create's),
- * F16 (1), BF16 (30) or Q8_K (15); other types fail with -1.  Every row is
+ * F16 (1), BF16 (30), Q8_K (15) or MXFP4 (39); other types fail with -1.  Every row is
  * rounded to the type once, when it is stored -- F16 and BF16 to nearest even
  * (F16: magnitudes from 65520 on become infinity), Q8_K one block of the
  * format per kv head (256 values share a scale), with the quants and scale of
- * q38_quantize_q8_k for finite values -- and every call below reads the values
+ * q38_quantize_q8_k for finite values; MXFP4 in blocks of 32 values that share
+ * a power of two, the smallest of which the largest value has at most 7 (within
+ * 2^-125 .. 2^125), each value the nearest of 0, 0.5, 1, 1.5, 2, 3, 4 and 6 of
+ * them with its sign, halfway to the one of the even code, 6 above -- and every call below reads the values
  * that the stored rows stand for: a token appended by q38_attn_decode or
  * q38_full_core attends to its own row as it is stored.  A stored infinity or
  * NaN spoils what it meets, in calls over its position (in a prefill, for every
  * token of the call): a key's, the six query heads of its kv head; a value's,
- * its dim of those heads' outputs (Q8_K, whose block shares a scale: every dim).
+ * its dim of those heads' outputs (Q8_K, whose block shares a scale: every dim;
+ * MXFP4: the block's 32).
  * What is left there is not specified -- infinite, NaN, or as if the row were not there.
  * Other heads, dims and sequences stay as they are.  A page takes 64 KiB
- * per slot for K and V together in 16 bits and 32.5 KiB in Q8_K, against
+ * per slot for K and V together in 16 bits, 32.5 KiB in Q8_K and 17 KiB in MXFP4, against
  * 128 KiB in F32.  No counterpart in the reference (its cache is f32). */
 int q38_kv_create_typed(q38_ctx *ctx, int ggml_type, int n_slots, int max_pages, int max_seqs,
                         int max_tokens_per_seq, q38_kv **out);

@@ -32,7 +32,7 @@ LIN_QK_DIM, LIN_V_DIM, LIN_QKV_DIM = 2048, 6144, 10240
 LIN_STATE_FLOATS = LIN_V_HEADS * LIN_HEAD_DIM * LIN_HEAD_DIM
 PAGE_TOKENS = 16
 # ggml type ids of a KV cache's rows
-GGML_F32, GGML_F16, GGML_Q8_K, GGML_BF16 = 0, 1, 15, 30
+GGML_F32, GGML_F16, GGML_Q8_K, GGML_BF16, GGML_MXFP4 = 0, 1, 15, 30, 39
 NOALLOC_SCRATCH_BYTES = 16 << 20  # Q38_NOALLOC_SCRATCH_BYTES of include/q38_attn.h
 
 
@@ -386,7 +386,7 @@ def _same_length(seq_ids, pos0, n_tokens) -> int:
 
 
 class KVCache:
-    """Paged device KV cache (q38_kv_*) of F32, F16, BF16 or Q8_K rows."""
+    """Paged device KV cache (q38_kv_*) of F32, F16, BF16, Q8_K or MXFP4 rows."""
 
     def __init__(self, ctx: Context, n_slots: int, max_pages: int, max_seqs: int, max_tokens_per_seq: int,
                  ggml_type: int = GGML_F32):

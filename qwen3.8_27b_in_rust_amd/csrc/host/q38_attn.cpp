@@ -124,18 +124,20 @@ constexpr GemvType kGemv[] = {
     {Q38_GGML_IQ1_M, "q38_gemv_q8k_iq1m", "q38_gemm_q8k_iq1m", "q38_gemm_ks_q8k_iq1m", "q38_gemm_ks16_q8k_iq1m", "q38_gemm_ks4_q8k_iq1m", nullptr, 1, 2048 * 8, 0.0, 0.0},
 };
 constexpr int kGemvTypes = (int)(sizeof(kGemv) / sizeof(kGemv[0]));
-/* Row types of a KV cache: the bytes of a page, and the suffix of the kernels that read and write it.  Index 0 is
- * the f32 cache. */
+/* Row types of a KV cache: the bytes of a page, the suffix of the kernels that read and write it, and whether they
+ * have code objects of their own.  Index 0 is the f32 cache. */
 struct KvType {
     int ggml_type;
     size_t page_bytes;
     const char *suffix;
+    bool own_objects;
 };
 constexpr KvType kKvTypes[] = {
-    {Q38_GGML_F32, Q38_KV_PAGE_F32, "f32"},
-    {Q38_GGML_F16, Q38_KV_PAGE_16, "f16"},
-    {Q38_GGML_BF16, Q38_KV_PAGE_16, "bf16"},
-    {Q38_GGML_Q8_K, Q38_KV_PAGE_Q8, "q8k"},
+    {Q38_GGML_F32, Q38_KV_PAGE_F32, "f32", false},
+    {Q38_GGML_F16, Q38_KV_PAGE_16, "f16", false},
+    {Q38_GGML_BF16, Q38_KV_PAGE_16, "bf16", false},
+    {Q38_GGML_Q8_K, Q38_KV_PAGE_Q8, "q8k", false},
+    {Q38_GGML_MXFP4, Q38_KV_PAGE_MX4, "mxfp4", true},
 };
 constexpr int kKvTypeCount = (int)(sizeof(kKvTypes) / sizeof(kKvTypes[0]));
 /* q38_add_rms_norm's kernels that hold a row in registers: 256 or 1024
@@ -191,6 +193,7 @@ struct q38_ctx {
     hipFunction_t f_norm_any = nullptr;
     hipFunction_t f_dequantize_q8k = nullptr;
     hipModule_t mod_typed = nullptr;
+    hipModule_t mod_rows_own[kKvTypeCount] = {}, mod_decode_own[kKvTypeCount] = {}; /* types with own_objects */
     hipFunction_t f_decode_typed[kKvTypeCount][2] = {}; /* from index 1 on; [1]: the pre step fused */
     hipFunction_t f_decode_typed_one[kKvTypeCount][2] = {};
     hipFunction_t f_decode_merge_one = nullptr;
@@ -500,22 +503,29 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
     const std::string p_rows = dir + "/kv_rows.hsaco", p_typed = dir + "/attn_decode_typed.hsaco";
     Q38_HIP(hipModuleLoad(&ctx->mod_rows, p_rows.c_str()));
     Q38_HIP(hipModuleLoad(&ctx->mod_typed, p_typed.c_str()));
-    auto rows_kernel = [&](q38_ctx::RowsKernel *k, const std::string &name, bool gathers) {
+    auto rows_kernel = [&](hipModule_t module, q38_ctx::RowsKernel *k, const std::string &name, bool gathers) {
         k->gathers = gathers;
-        const hipError_t e = hipModuleGetFunction(&k->many, ctx->mod_rows, name.c_str());
-        return e != hipSuccess ? e : hipModuleGetFunction(&k->few, ctx->mod_rows, (name + "_few").c_str());
+        const hipError_t e = hipModuleGetFunction(&k->many, module, name.c_str());
+        return e != hipSuccess ? e : hipModuleGetFunction(&k->few, module, (name + "_few").c_str());
     };
-    Q38_HIP(rows_kernel(&ctx->f_kv_gather_16, "q38_kv_gather_16", true));
+    Q38_HIP(rows_kernel(ctx->mod_rows, &ctx->f_kv_gather_16, "q38_kv_gather_16", true));
     for (int i = 0; i < kKvTypeCount; ++i) {
         const std::string ty = kKvTypes[i].suffix;
-        Q38_HIP(rows_kernel(&ctx->f_kv_append[i], "q38_kv_append_" + ty, false));
-        Q38_HIP(rows_kernel(&ctx->f_kv_gather[i], "q38_kv_gather_" + ty, true));
+        hipModule_t rows = ctx->mod_rows, decode = ctx->mod_typed;
+        if (kKvTypes[i].own_objects) {
+            Q38_HIP(hipModuleLoad(&ctx->mod_rows_own[i], (dir + "/kv_rows_" + ty + ".hsaco").c_str()));
+            Q38_HIP(hipModuleLoad(&ctx->mod_decode_own[i], (dir + "/attn_decode_" + ty + ".hsaco").c_str()));
+            rows = ctx->mod_rows_own[i];
+            decode = ctx->mod_decode_own[i];
+        }
+        Q38_HIP(rows_kernel(rows, &ctx->f_kv_append[i], "q38_kv_append_" + ty, false));
+        Q38_HIP(rows_kernel(rows, &ctx->f_kv_gather[i], "q38_kv_gather_" + ty, true));
         if (i == 0) continue;
         Q38_HIP(hipModuleGetFunction(&ctx->f_kv_split_typed[i], ctx->mod_prefill, ("q38_kv_split_mfma_" + ty).c_str()));
         for (int pre = 0; pre < 2; ++pre) {
             const std::string name = "q38_attn_decode_" + ty + (pre ? "_pre" : "");
-            Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed[i][pre], ctx->mod_typed, name.c_str()));
-            Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed_one[i][pre], ctx->mod_typed, (name + "_one").c_str()));
+            Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed[i][pre], decode, name.c_str()));
+            Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed_one[i][pre], decode, (name + "_one").c_str()));
         }
     }
     const std::string p_proj = dir + "/proj.hsaco";
@@ -586,6 +596,10 @@ int q38_ctx_destroy(q38_ctx *ctx) {
     if (ctx->mod_norm) (void)hipModuleUnload(ctx->mod_norm);
     if (ctx->mod_rows) (void)hipModuleUnload(ctx->mod_rows);
     if (ctx->mod_typed) (void)hipModuleUnload(ctx->mod_typed);
+    for (int i = 0; i < kKvTypeCount; ++i) {
+        if (ctx->mod_rows_own[i]) (void)hipModuleUnload(ctx->mod_rows_own[i]);
+        if (ctx->mod_decode_own[i]) (void)hipModuleUnload(ctx->mod_decode_own[i]);
+    }
     if (ctx->mod_gdn) (void)hipModuleUnload(ctx->mod_gdn);
     if (ctx->mod_prefill) (void)hipModuleUnload(ctx->mod_prefill);
     if (ctx->mod_gdn_chunk) (void)hipModuleUnload(ctx->mod_gdn_chunk);
@@ -845,7 +859,7 @@ int q38_kv_create_typed(q38_ctx *ctx, int ggml_type, int n_slots, int max_pages,
     int type = -1;
     for (int i = 0; i < kKvTypeCount; ++i)
         if (kKvTypes[i].ggml_type == ggml_type) type = i;
-    if (type < 0) return fail("a KV cache holds F32 (0), F16 (1), BF16 (30) or Q8_K (15) rows, not type %d", ggml_type);
+    if (type < 0) return fail("a KV cache holds F32 (0), F16 (1), BF16 (30), Q8_K (15) or MXFP4 (39) rows, not type %d", ggml_type);
     if (n_slots < 1 || n_slots > 17) return fail("n_slots %d outside 1..17", n_slots);
     if (max_pages < 1 || max_seqs < 1 || max_tokens_per_seq < 1)
         return fail("max_pages, max_seqs and max_tokens_per_seq must be positive");

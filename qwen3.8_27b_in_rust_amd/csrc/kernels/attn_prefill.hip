@@ -201,6 +201,7 @@ extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma(q38_prefill_
 extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma_f16(q38_prefill_args a) { kv_split<Q38_KV_F16>(a); }
 extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma_bf16(q38_prefill_args a) { kv_split<Q38_KV_BF16>(a); }
 extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma_q8k(q38_prefill_args a) { kv_split<Q38_KV_Q8>(a); }
+extern "C" __global__ __launch_bounds__(256) void q38_kv_split_mfma_mxfp4(q38_prefill_args a) { kv_split<Q38_KV_MX4>(a); }
 
 extern "C" __global__ __launch_bounds__(kThreads, 1) void q38_attn_prefill_mfma(q38_prefill_args a) {
     __shared__ __attribute__((aligned(16))) Tile tiles[2];

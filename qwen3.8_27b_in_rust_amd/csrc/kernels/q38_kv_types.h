@@ -1,6 +1,6 @@
 /*
  * The rows of a typed KV cache: conversions between f32 and the 16-bit (F16,
- * BF16) and 8-bit (Q8_K) elements of its pages.
+ * BF16), 8-bit (Q8_K) and 4-bit (MXFP4) elements of its pages.
  */
 #pragma once
 #include "q38_device.h"
@@ -22,6 +22,34 @@ Q38_DEV float *q38_kv_scales(char *block, int head) {
     return reinterpret_cast<float *>(block + q38_kv_scales_offset(head));
 }
 
+/* MXFP4.  The conversions take the scale as the power of two that a scale byte E
+ * stands for (E = 255, which an infinity or NaN leaves: an infinity, and every
+ * value of the block NaN). */
+Q38_DEV uint8_t *q38_mx4_scales(char *block, int head) {
+    return reinterpret_cast<uint8_t *>(block + q38_mx4_scales_offset(head));
+}
+typedef float q38_f32x2 __attribute__((ext_vector_type(2)));
+Q38_DEV float q38_mx4_power(uint32_t e) { return __uint_as_float(e << 23); }
+/* The scale byte of a block whose largest size has these bits: 2^(E - 127) is the
+ * smallest power of two of which that is at most 7, the largest that rounds to a
+ * code without being cut (6); from 2^-125, so that its values, from 2^-126 on, are
+ * normal, to 2^125, so that they are finite.  Against the power below the largest
+ * value's own alone, which cuts up to a quarter of it, the error of normal
+ * values is 0.112 of their size, not 0.115. */
+Q38_DEV uint32_t q38_mx4_exponent(uint32_t largest) {
+    const uint32_t e = (largest + 0x1FFFFFu) >> 23;
+    return largest >= 0x7F800000u ? 255u : min(max(e, 4u), 254u) - 2u;
+}
+/* Codes of two values in byte SEL of a word, nearest, halfway to the even code; and back. */
+template <int SEL>
+Q38_DEV uint32_t q38_mx4_pack(uint32_t word, float a, float b, float scale) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, a, b, scale, SEL);
+}
+template <int SEL>
+Q38_DEV q38_f32x2 q38_mx4_pair(uint32_t word, float scale) {
+    return __builtin_bit_cast(q38_f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, scale, SEL));
+}
+
 /* A 16-bit value of the type, rounded to nearest even (F16: past 65504 to
  * infinity), and back. */
 template <int T>
@@ -40,7 +68,12 @@ template <int T>
 Q38_DEV f32x4 q38_k_load4(char *block, int head, int t, int d) {
     const int i = q38_k_index<T>(t, d);
     f32x4 x;
-    if (T == Q38_KV_Q8) {
+    if constexpr (T == Q38_KV_MX4) {
+        const uint32_t u = *reinterpret_cast<const uint16_t *>(block + (i >> 1));
+        const float s = q38_mx4_power(q38_mx4_scales(block, head)[q38_mx4_k_scale(t, d)]);
+        const q38_f32x2 a = q38_mx4_pair<0>(u, s), b = q38_mx4_pair<1>(u, s);
+        x = f32x4{a[0], a[1], b[0], b[1]};
+    } else if (T == Q38_KV_Q8) {
         const uint32_t u = *reinterpret_cast<const uint32_t *>(block + i);
         const float s = q38_kv_scales(block, head)[t];
 #pragma unroll
@@ -57,6 +90,20 @@ Q38_DEV f32x4 q38_k_load4(char *block, int head, int t, int d) {
  * tokens (2n, 2n + 1), maybe the same one twice. */
 template <int T>
 Q38_DEV void q38_v_load4(char *block, int head, int t0, int t1, int d, f32x4 &x0, f32x4 &x1) {
+    if constexpr (T == Q38_KV_MX4) {
+        /* a pair's bytes lie side by side, both hold dim d and its partner 16 away */
+        const uint8_t *scales = q38_mx4_scales(block, head);
+        const float p0 = q38_mx4_power(scales[q38_mx4_v_scale(t0, d)]), p1 = q38_mx4_power(scales[q38_mx4_v_scale(t1, d)]);
+        const int half = (d >> 4) & 1;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const uint32_t u = *reinterpret_cast<const uint16_t *>(block + (q38_v_index<T>(t0 & ~1, d + c) >> 1));
+            const q38_f32x2 a = q38_mx4_pair<0>(u >> (8 * (t0 & 1)), p0), b = q38_mx4_pair<0>(u >> (8 * (t1 & 1)), p1);
+            x0[c] = half ? a[1] : a[0];
+            x1[c] = half ? b[1] : b[0];
+        }
+        return;
+    }
     const float s0 = T == Q38_KV_Q8 ? q38_kv_scales(block, head)[t0] : 0.0f;
     const float s1 = T == Q38_KV_Q8 ? q38_kv_scales(block, head)[t1] : 0.0f;
 #pragma unroll

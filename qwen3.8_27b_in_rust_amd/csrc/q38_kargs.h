@@ -25,10 +25,12 @@
 #define Q38_PAGE_FLOATS (Q38_ATTN_KV_HEADS * Q38_PAGE_TOKENS * Q38_ATTN_HEAD_DIM)
 
 /* bytes of a page, by the cache's type: per kv head 16 tokens x 256 values (Q8_K:
- * quants, and after the four heads' the f32 scales [head][token]) */
+ * quants, and after the four heads' the f32 scales [head][token]; MXFP4: codes, and
+ * after the four heads' the scale bytes [head][token and 32 dims]) */
 #define Q38_KV_PAGE_F32 (Q38_PAGE_FLOATS * 4)
 #define Q38_KV_PAGE_16 (Q38_PAGE_FLOATS * 2)
 #define Q38_KV_PAGE_Q8 (Q38_PAGE_FLOATS + Q38_ATTN_KV_HEADS * Q38_PAGE_TOKENS * 4)
+#define Q38_KV_PAGE_MX4 (Q38_PAGE_FLOATS / 2 + Q38_PAGE_FLOATS / 32)
 
 #define Q38_LIN_QK_HEADS 16
 #define Q38_LIN_V_HEADS 48
@@ -425,6 +427,7 @@ typedef struct {
 #define Q38_GGML_IQ2_S 22
 #define Q38_GGML_IQ1_M 29
 #define Q38_GGML_BF16 30
+#define Q38_GGML_MXFP4 39
 #define Q38_GEMV_TOKENS 8 /* most tokens one GEMV workgroup serves per pass over its weights */
 #define Q38_GEMV_MAX_BLOCKS 192 /* 256-wide blocks per row (width 49152): one token's blocks fit LDS */
 #define Q38_GEMV_UNITS_MAX 1024 /* (row, block) units per GEMV workgroup: four steps of 256 */
