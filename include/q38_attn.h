@@ -180,6 +180,67 @@ int q38_kv_append(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
 int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
                   const int32_t *n_tokens, int ggml_type, void *d_k, void *d_v);
 
+/* ------------------------------- sums of attention weights, and eviction
+ *
+ * For contexts longer than their cache: a cache of F16, BF16, Q8_K or MXFP4 rows
+ * that tracks weights keeps, for each cached token, layer and kv head, the sum of
+ * the softmax weights that the kv head's 6 query heads have given it (f32), and the
+ * token's own position, its place in all that the sequence has read.  An eviction
+ * takes the tokens with the smallest sums out, for each layer and kv head its
+ * own.  No counterpart in the reference (its cache holds the whole context).
+ *
+ * A cache position is then no longer the token's own: after evictions of e tokens
+ * (q38_seq_evicted) the row stored at position p is the sequence's token p + e.
+ * q38_full_core, q38_full_core_noalloc and the graphs turn q and k at p + e by
+ * themselves; q38_attn_pre takes p + e as its pos0, before q38_attn_decode,
+ * q38_kv_write and q38_attn_prefill, which take cache positions as ever;
+ * q38_kv_append refuses a sequence that has evicted tokens.  Rows that stay keep
+ * the turn that they were stored with.  Positions below the last eviction's n_keep are
+ * in no order: q38_seq_truncate goes back to n_keep or to 0, not between.
+ * q38_seq_reset, a truncate to 0 and q38_seq_set_pages begin anew, with none
+ * evicted. */
+
+/* From now on the cache tracks weights (enable 0: no longer; -1 while a sequence has
+ * evicted tokens).  Sums begin at 0.  16 bytes a token and layer each for sums and
+ * positions.  Every call of q38_attn_decode, q38_full_core, q38_full_core_noalloc and the
+ * graphs on a tracking cache adds its weights to the positions that it reads,
+ * and takes a sequence once a call; a stored row, whichever call stores it,
+ * starts at 0 (in a decode call that appends it, at the weight it gives itself).
+ * Such a call needs 24 f32 scores a token in its workspace.  A graph is recorded with tracking
+ * on or off, and its positions are set anew after an eviction. */
+int q38_kv_track_weights(q38_kv *kv, int enable);
+/* Tokens of the sequence that evictions have taken out so far. */
+int q38_seq_evicted(q38_kv *kv, int seq, int *n_tokens);
+
+/* Sums and own positions of a ragged batch of reserved positions, packed in
+ * order in rows [rows][4 kv heads] as q38_kv_gather's, to hand a sequence on
+ * with them or to look at them.  put: d_weights NULL sets zeros, d_tokens NULL
+ * what a row stored there has, position + evicted tokens; a sequence once a
+ * call.  get: either may be NULL, not both. */
+int q38_kv_weights_put(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
+                       const int32_t *n_tokens, const float *d_weights, const int32_t *d_tokens);
+int q38_kv_weights_get(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
+                       const int32_t *n_tokens, float *d_weights, int32_t *d_tokens);
+
+/* A prompt's part in the sums (q38_attn_prefill adds nothing to them): the weights
+ * that the queries d_q [n_tokens][24][256] (post-norm, post-RoPE, 16-byte
+ * aligned) of positions base_pos .. base_pos + n_tokens - 1, whose rows are in
+ * the cache, give causally to all positions up to their own.  All of a prompt's
+ * queries, or its last ones, as the caller wants them to count. */
+int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens, const float *d_q);
+
+/* Of the n_tokens[b] tokens that sequence seq_ids[b] holds (positions 0 ..
+ * n_tokens[b] - 1, written in every layer), n_keep[b] stay, in each layer and kv
+ * head: those among its last n_recent[b] <= n_keep[b] by their own positions, then
+ * those with the largest sums, of equal ones the lower positions (a NaN is below every
+ * number).  They end at positions 0 .. n_keep[b] - 1: a token that stays below n_keep[b]
+ * keeps its place, and the places of the evicted ones there take those from further on,
+ * in order.  Sums and own positions move with them.  Pages past n_keep[b] are
+ * released.  Sequence ids must be distinct.  Layers of which nothing was stored may be
+ * among the cache's slots.  It cannot be captured. */
+int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n_tokens, const int32_t *n_keep,
+                 const int32_t *n_recent);
+
 /* --------------------------------------------------------- full attention */
 
 /*

@@ -79,6 +79,12 @@ _SIGNATURES = {
     "q38_kv_create_typed": (c_int, [_P, c_int, c_int, c_int, c_int, c_int, POINTER(c_void_p)]),
     "q38_kv_append": (c_int, [_P, c_int, c_int, _I32P, _I32P, _I32P, _P, _P, _P]),
     "q38_kv_gather": (c_int, [_P, c_int, c_int, _I32P, _I32P, _I32P, c_int, _P, _P]),
+    "q38_kv_track_weights": (c_int, [_P, c_int]),
+    "q38_seq_evicted": (c_int, [_P, c_int, POINTER(c_int)]),
+    "q38_kv_weights_put": (c_int, [_P, c_int, c_int, _I32P, _I32P, _I32P, _P, _P]),
+    "q38_kv_weights_get": (c_int, [_P, c_int, c_int, _I32P, _I32P, _I32P, _P, _P]),
+    "q38_attn_observe": (c_int, [_P, c_int, c_int, c_int, c_int, _P]),
+    "q38_kv_evict": (c_int, [_P, c_int, _I32P, _I32P, _I32P, _I32P]),
     "q38_kv_destroy": (c_int, [_P]),
     "q38_kv_free_pages": (c_int, [_P, POINTER(c_int)]),
     "q38_kv_set_prefill_cache": (c_int, [_P, c_int]),
@@ -453,6 +459,36 @@ class KVCache:
         n = _same_length(seq_ids, pos0, n_tokens)
         _check(lib().q38_kv_gather(self.handle, layer, n, _i32(seq_ids), _i32(pos0), _i32(n_tokens), ggml_type,
                                    _ptr(d_k), _ptr(d_v)), "q38_kv_gather")
+
+    def track_weights(self, enable: bool) -> None:
+        """Keep the sums of the attention weights that cached tokens are given."""
+        _check(lib().q38_kv_track_weights(self.handle, int(bool(enable))), "q38_kv_track_weights")
+
+    def seq_evicted(self, seq) -> int:
+        n = c_int()
+        _check(lib().q38_seq_evicted(self.handle, seq, ctypes.byref(n)), "q38_seq_evicted")
+        return n.value
+
+    def weights_put(self, layer, seq_ids, pos0, n_tokens, weights=None, tokens=None):
+        """Sums (None: zeros) and own positions (None: the rows' places) of a ragged batch, rows of 4 kv heads."""
+        n = _same_length(seq_ids, pos0, n_tokens)
+        _check(lib().q38_kv_weights_put(self.handle, layer, n, _i32(seq_ids), _i32(pos0), _i32(n_tokens), _ptr(weights),
+                                        _ptr(tokens)), "q38_kv_weights_put")
+
+    def weights_get(self, layer, seq_ids, pos0, n_tokens, weights=None, tokens=None):
+        n = _same_length(seq_ids, pos0, n_tokens)
+        _check(lib().q38_kv_weights_get(self.handle, layer, n, _i32(seq_ids), _i32(pos0), _i32(n_tokens), _ptr(weights),
+                                        _ptr(tokens)), "q38_kv_weights_get")
+
+    def attn_observe(self, layer, seq, base_pos, n_tokens, q):
+        """Add the weights that a prompt's queries give to the sums."""
+        _check(lib().q38_attn_observe(self.handle, layer, seq, base_pos, n_tokens, _ptr(q)), "q38_attn_observe")
+
+    def evict(self, seq_ids, n_tokens, n_keep, n_recent):
+        """Keep n_keep of each sequence's n_tokens: the n_recent last ones, then those with the largest sums."""
+        n = _same_length(seq_ids, n_tokens, n_keep)
+        _same_length(seq_ids, n_tokens, n_recent)
+        _check(lib().q38_kv_evict(self.handle, n, _i32(seq_ids), _i32(n_tokens), _i32(n_keep), _i32(n_recent)), "q38_kv_evict")
 
     def attn_decode(self, layer, seq_ids, positions, q, out, k_new=None, v_new=None, gate=None):
         n = len(seq_ids)

@@ -193,6 +193,13 @@ struct q38_ctx {
     hipFunction_t f_norm_any = nullptr;
     hipFunction_t f_dequantize_q8k = nullptr;
     hipModule_t mod_typed = nullptr;
+    hipModule_t mod_weigh = nullptr, mod_weights = nullptr, mod_observe = nullptr;
+    hipFunction_t f_weigh[kKvTypeCount][2] = {}; /* from index 1 on; [1]: the pre step fused */
+    hipFunction_t f_weigh_merge = nullptr;
+    hipFunction_t f_weights_copy = nullptr;
+    hipFunction_t f_evict_select = nullptr;
+    hipFunction_t f_evict_move[kKvTypeCount] = {};
+    hipFunction_t f_observe_stats[kKvTypeCount] = {}, f_observe_sums[kKvTypeCount] = {};
     hipModule_t mod_rows_own[kKvTypeCount] = {}, mod_decode_own[kKvTypeCount] = {}; /* types with own_objects */
     hipFunction_t f_decode_typed[kKvTypeCount][2] = {}; /* from index 1 on; [1]: the pre step fused */
     hipFunction_t f_decode_typed_one[kKvTypeCount][2] = {};
@@ -326,6 +333,22 @@ struct q38_kv {
     };
     std::vector<Images> images; /* [max_seqs][n_slots] */
     bool image_cache = true;
+    /* A tracking cache's sums of attention weights and own positions, [n_slots][max_pages][4][16] as the pages
+     * lie, and what each sequence has lost: */
+    bool tracks = false;
+    float *weights = nullptr;
+    int32_t *tokens = nullptr;
+    struct Evicted {
+        int32_t tokens = 0; /* so far: a position's row is that much further on */
+        int32_t kept = 0;   /* by the last eviction: positions before are in no order */
+    };
+    std::vector<Evicted> evicted;
+
+    size_t slot_sums() const { return (size_t)max_pages * Q38_WEIGHTS_PAGE; }
+    int32_t evicted_of(int seq) const { return tracks ? evicted[seq].tokens : 0; }
+    void forget_evicted(int seq) {
+        if (tracks) evicted[seq] = Evicted();
+    }
 
     Images &img(int seq, int slot) { return images[(size_t)seq * n_slots + slot]; }
 
@@ -509,6 +532,12 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
         return e != hipSuccess ? e : hipModuleGetFunction(&k->few, module, (name + "_few").c_str());
     };
     Q38_HIP(rows_kernel(ctx->mod_rows, &ctx->f_kv_gather_16, "q38_kv_gather_16", true));
+    Q38_HIP(hipModuleLoad(&ctx->mod_weigh, (dir + "/attn_weigh.hsaco").c_str()));
+    Q38_HIP(hipModuleLoad(&ctx->mod_weights, (dir + "/kv_weights.hsaco").c_str()));
+    Q38_HIP(hipModuleLoad(&ctx->mod_observe, (dir + "/attn_observe.hsaco").c_str()));
+    Q38_HIP(hipModuleGetFunction(&ctx->f_weigh_merge, ctx->mod_weigh, "q38_attn_weigh_merge"));
+    Q38_HIP(hipModuleGetFunction(&ctx->f_weights_copy, ctx->mod_weights, "q38_kv_weights_copy"));
+    Q38_HIP(hipModuleGetFunction(&ctx->f_evict_select, ctx->mod_weights, "q38_kv_evict_select"));
     for (int i = 0; i < kKvTypeCount; ++i) {
         const std::string ty = kKvTypes[i].suffix;
         hipModule_t rows = ctx->mod_rows, decode = ctx->mod_typed;
@@ -526,7 +555,11 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
             const std::string name = "q38_attn_decode_" + ty + (pre ? "_pre" : "");
             Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed[i][pre], decode, name.c_str()));
             Q38_HIP(hipModuleGetFunction(&ctx->f_decode_typed_one[i][pre], decode, (name + "_one").c_str()));
+            Q38_HIP(hipModuleGetFunction(&ctx->f_weigh[i][pre], ctx->mod_weigh, ("q38_attn_weigh_" + ty + (pre ? "_pre" : "")).c_str()));
         }
+        Q38_HIP(hipModuleGetFunction(&ctx->f_evict_move[i], ctx->mod_weights, ("q38_kv_evict_move_" + ty).c_str()));
+        Q38_HIP(hipModuleGetFunction(&ctx->f_observe_stats[i], ctx->mod_observe, ("q38_observe_stats_" + ty).c_str()));
+        Q38_HIP(hipModuleGetFunction(&ctx->f_observe_sums[i], ctx->mod_observe, ("q38_observe_sums_" + ty).c_str()));
     }
     const std::string p_proj = dir + "/proj.hsaco";
     Q38_HIP(hipModuleLoad(&ctx->mod_proj, p_proj.c_str()));
@@ -596,6 +629,9 @@ int q38_ctx_destroy(q38_ctx *ctx) {
     if (ctx->mod_norm) (void)hipModuleUnload(ctx->mod_norm);
     if (ctx->mod_rows) (void)hipModuleUnload(ctx->mod_rows);
     if (ctx->mod_typed) (void)hipModuleUnload(ctx->mod_typed);
+    if (ctx->mod_weigh) (void)hipModuleUnload(ctx->mod_weigh);
+    if (ctx->mod_weights) (void)hipModuleUnload(ctx->mod_weights);
+    if (ctx->mod_observe) (void)hipModuleUnload(ctx->mod_observe);
     for (int i = 0; i < kKvTypeCount; ++i) {
         if (ctx->mod_rows_own[i]) (void)hipModuleUnload(ctx->mod_rows_own[i]);
         if (ctx->mod_decode_own[i]) (void)hipModuleUnload(ctx->mod_decode_own[i]);
@@ -907,6 +943,8 @@ int q38_kv_destroy(q38_kv *kv) {
     (void)hipFree(kv->kpool);
     (void)hipFree(kv->vpool);
     (void)hipFree(kv->d_page_table);
+    (void)hipFree(kv->weights);
+    (void)hipFree(kv->tokens);
     (void)hipHostFree(kv->staging);
     delete kv;
     return 0;
@@ -933,6 +971,7 @@ int q38_seq_create(q38_kv *kv, int *seq) {
         if (!kv->seq_live[s]) {
             kv->seq_live[s] = 1;
             kv->seq_pages[s] = 0;
+            kv->forget_evicted(s);
             *seq = s;
             return 0;
         }
@@ -953,6 +992,7 @@ int q38_seq_reset(q38_kv *kv, int seq) {
     if (kv == nullptr) return fail("kv is NULL");
     if (kv->check_seq(seq)) return -1;
     kv->release_from(seq, 0);
+    kv->forget_evicted(seq);
     return 0;
 }
 
@@ -960,6 +1000,11 @@ int q38_seq_truncate(q38_kv *kv, int seq, int n_tokens) {
     if (kv == nullptr) return fail("kv is NULL");
     if (kv->check_seq(seq)) return -1;
     if (n_tokens < 0) return fail("negative token count");
+    if (kv->tracks && n_tokens < kv->evicted[seq].kept) {
+        if (n_tokens > 0)
+            return fail("sequence %d: positions before %d have been in no order since the last eviction", seq, kv->evicted[seq].kept);
+        kv->forget_evicted(seq);
+    }
     kv->release_from(seq, (n_tokens + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS);
     return 0;
 }
@@ -987,6 +1032,7 @@ int q38_seq_set_pages(q38_kv *kv, int seq, int n_pages, const int32_t *page_ids)
         avail[p] = 0;
     }
     kv->release_from(seq, 0);
+    kv->forget_evicted(seq);
     std::vector<int32_t> rest;
     rest.reserve(kv->free_pages.size());
     for (int32_t p : kv->free_pages)
@@ -1100,6 +1146,41 @@ int launch_rows(q38_kv *kv, const q38_ctx::RowsKernel &f, int slot, int n_seq, c
     return 0;
 }
 
+/* Sums and own positions of a validated batch to the pages (weights NULL: zeros, tokens NULL: the rows' positions
+ * in what the sequence has read) or from them. */
+int launch_weights(q38_kv *kv, int slot, bool to_pages, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
+                   const int32_t *n_tokens, float *d_weights, int32_t *d_tokens) {
+    size_t row = 0;
+    for (int b = 0; b < n_seq;) {
+        q38_kv_weights_args a;
+        memset(&a, 0, sizeof(a));
+        a.weights = kv->weights + (size_t)slot * kv->slot_sums();
+        a.tokens = kv->tokens + (size_t)slot * kv->slot_sums();
+        a.page_table = kv->d_page_table;
+        a.weight_rows = d_weights != nullptr ? d_weights + row * Q38_ATTN_KV_HEADS : nullptr;
+        a.token_rows = d_tokens != nullptr ? d_tokens + row * Q38_ATTN_KV_HEADS : nullptr;
+        a.pt_stride = kv->pt_stride;
+        a.to_pages = to_pages ? 1 : 0;
+        int n = 0;
+        for (; b < n_seq && n < Q38_MAX_BATCH; ++b) {
+            if (n_tokens[b] == 0) continue;
+            a.seq[n] = seq_ids[b];
+            a.pos0[n] = pos0[b];
+            a.evicted[n] = kv->evicted_of(seq_ids[b]);
+            a.row_base[n + 1] = a.row_base[n] + n_tokens[b];
+            const int first = pos0[b] / Q38_PAGE_TOKENS, last = (pos0[b] + n_tokens[b] - 1) / Q38_PAGE_TOKENS;
+            a.page_base[n + 1] = a.page_base[n] + last - first + 1;
+            ++n;
+        }
+        if (n == 0) break;
+        a.n_seq = n;
+        for (int i = n + 1; i < Q38_MAX_BATCH + 8; ++i) a.page_base[i] = INT_MAX;
+        if (kv->ctx->launch(kv->ctx->f_weights_copy, ((unsigned)a.page_base[n] + 3) / 4, 1, 1, 256, &a)) return -1;
+        row += (size_t)a.row_base[n];
+    }
+    return 0;
+}
+
 }  // namespace
 
 static int kv_copy(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, float *d_k, float *d_v,
@@ -1117,9 +1198,12 @@ static int kv_copy(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, float
     } else if (pos0 + n_tokens > kv->seq_pages[seq] * Q38_PAGE_TOKENS) {
         return fail("positions %d..%d are not reserved", pos0, pos0 + n_tokens - 1);
     }
-    if (kv->type != 0)
-        return launch_rows(kv, to_pages ? kv->ctx->f_kv_append[kv->type] : kv->ctx->f_kv_gather[kv->type], slot, 1, &seq,
-                           &pos0, &n_tokens, d_k, d_v, sizeof(float), nullptr);
+    if (kv->type != 0) {
+        if (launch_rows(kv, to_pages ? kv->ctx->f_kv_append[kv->type] : kv->ctx->f_kv_gather[kv->type], slot, 1, &seq,
+                        &pos0, &n_tokens, d_k, d_v, sizeof(float), nullptr))
+            return -1;
+        return to_pages && kv->tracks ? launch_weights(kv, slot, true, 1, &seq, &pos0, &n_tokens, nullptr, nullptr) : 0;
+    }
     q38_kv_copy_args a;
     memset(&a, 0, sizeof(a));
     a.kpool = kv->kslot(slot);
@@ -1151,6 +1235,10 @@ int q38_kv_append(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
     long n_rows = 0;
     if (validate_rows(kv, layer, n_seq, seq_ids, pos0, n_tokens, true, &slot, &n_rows)) return -1;
     if (n_rows == 0) return 0;
+    /* the kernel turns a key by its place in the cache */
+    for (int b = 0; b < n_seq; ++b)
+        if (n_tokens[b] > 0 && kv->evicted_of(seq_ids[b]) > 0)
+            return fail("sequence %d has evicted tokens: q38_attn_pre at the tokens' own positions, then q38_kv_write", seq_ids[b]);
     if (!d_k_norm || !d_key || !d_value) return fail("NULL argument");
     if (((uintptr_t)d_k_norm | (uintptr_t)d_key | (uintptr_t)d_value) % 16 != 0)
         return fail("d_k_norm, d_key and d_value must be 16-byte aligned");
@@ -1163,8 +1251,10 @@ int q38_kv_append(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
         if (kv->reserve(seq_ids[b], pos0[b] + n_tokens[b])) return -1;
         kv->images_from(seq_ids[b], slot, pos0[b]);
     }
-    return launch_rows(kv, kv->ctx->f_kv_append[kv->type], slot, n_seq, seq_ids, pos0, n_tokens,
-                       const_cast<float *>(d_key), const_cast<float *>(d_value), sizeof(float), d_k_norm);
+    if (launch_rows(kv, kv->ctx->f_kv_append[kv->type], slot, n_seq, seq_ids, pos0, n_tokens,
+                    const_cast<float *>(d_key), const_cast<float *>(d_value), sizeof(float), d_k_norm))
+        return -1;
+    return kv->tracks ? launch_weights(kv, slot, true, n_seq, seq_ids, pos0, n_tokens, nullptr, nullptr) : 0;
 }
 
 int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
@@ -1185,6 +1275,193 @@ int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
     if (overlaps(d_k, bytes, d_v, bytes)) return fail("d_k overlaps d_v");
     return launch_rows(kv, as_stored ? kv->ctx->f_kv_gather_16 : kv->ctx->f_kv_gather[kv->type], slot, n_seq, seq_ids,
                        pos0, n_tokens, d_k, d_v, as_stored ? 2 : sizeof(float), nullptr);
+}
+
+/* ------------------------------------------- sums of attention weights, eviction */
+
+static int check_tracks(const q38_kv *kv) {
+    if (kv == nullptr) return fail("kv is NULL");
+    if (!kv->tracks) return fail("the cache does not track weights (q38_kv_track_weights)");
+    return 0;
+}
+
+static int check_not_capturing(const q38_kv *kv, const char *what) {
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    Q38_HIP(hipStreamIsCapturing(kv->ctx->stream, &capture));
+    return capture != hipStreamCaptureStatusNone ? fail("%s cannot be captured", what) : 0;
+}
+
+int q38_kv_track_weights(q38_kv *kv, int enable) {
+    if (kv == nullptr) return fail("kv is NULL");
+    if ((enable != 0) == kv->tracks) return 0;
+    if (check_not_capturing(kv, "a change of tracking")) return -1;
+    if (!enable) {
+        for (int s = 0; s < kv->max_seqs; ++s)
+            if (kv->seq_live[s] && kv->evicted[s].tokens > 0) return fail("sequence %d has evicted tokens", s);
+        Q38_HIP(hipStreamSynchronize(kv->ctx->stream));
+        (void)hipFree(kv->weights);
+        (void)hipFree(kv->tokens);
+        kv->weights = nullptr;
+        kv->tokens = nullptr;
+        kv->tracks = false;
+        return 0;
+    }
+    if (kv->type == 0) return fail("a cache of F32 rows tracks no weights: F16, BF16, Q8_K or MXFP4 rows do");
+    const size_t bytes = kv->slot_sums() * kv->n_slots * sizeof(float);
+    if (hipMalloc(&kv->weights, bytes) != hipSuccess || hipMalloc(&kv->tokens, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        (void)hipFree(kv->weights);
+        kv->weights = nullptr;
+        return fail("cannot allocate %zu bytes for the sums of weights", 2 * bytes);
+    }
+    Q38_HIP(hipMemsetAsync(kv->weights, 0, bytes, kv->ctx->stream));
+    Q38_HIP(hipMemsetAsync(kv->tokens, 0, bytes, kv->ctx->stream));
+    kv->evicted.assign(kv->max_seqs, q38_kv::Evicted());
+    kv->tracks = true;
+    /* tokens that are there already */
+    for (int s = 0; s < kv->max_seqs; ++s) {
+        const int32_t zero = 0, held = kv->seq_live[s] ? kv->seq_pages[s] * Q38_PAGE_TOKENS : 0;
+        for (int slot = 0; slot < kv->n_slots && held > 0; ++slot)
+            if (launch_weights(kv, slot, true, 1, &s, &zero, &held, nullptr, nullptr)) return -1;
+    }
+    return 0;
+}
+
+int q38_seq_evicted(q38_kv *kv, int seq, int *n_tokens) {
+    if (kv == nullptr || n_tokens == nullptr) return fail("NULL argument");
+    if (kv->check_seq(seq)) return -1;
+    *n_tokens = kv->evicted_of(seq);
+    return 0;
+}
+
+int q38_kv_weights_put(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0, const int32_t *n_tokens,
+                       const float *d_weights, const int32_t *d_tokens) {
+    if (check_tracks(kv)) return -1;
+    int slot = 0;
+    long n_rows = 0;
+    if (validate_rows(kv, layer, n_seq, seq_ids, pos0, n_tokens, false, &slot, &n_rows)) return -1;
+    /* rows of one place twice would race */
+    std::vector<char> seen(kv->max_seqs, 0);
+    for (int b = 0; b < n_seq; ++b) {
+        if (seen[seq_ids[b]]) return fail("sequence %d appears twice", seq_ids[b]);
+        seen[seq_ids[b]] = 1;
+    }
+    return launch_weights(kv, slot, true, n_seq, seq_ids, pos0, n_tokens, const_cast<float *>(d_weights),
+                          const_cast<int32_t *>(d_tokens));
+}
+
+int q38_kv_weights_get(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0, const int32_t *n_tokens,
+                       float *d_weights, int32_t *d_tokens) {
+    if (check_tracks(kv)) return -1;
+    int slot = 0;
+    long n_rows = 0;
+    if (validate_rows(kv, layer, n_seq, seq_ids, pos0, n_tokens, false, &slot, &n_rows)) return -1;
+    if (n_rows == 0) return 0;
+    if (d_weights == nullptr && d_tokens == nullptr) return fail("no output");
+    const size_t bytes = (size_t)n_rows * Q38_ATTN_KV_HEADS * 4;
+    if (overlaps(d_weights, bytes, d_tokens, bytes)) return fail("d_weights overlaps d_tokens");
+    return launch_weights(kv, slot, false, n_seq, seq_ids, pos0, n_tokens, d_weights, d_tokens);
+}
+
+int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens, const float *d_q) {
+    if (check_tracks(kv)) return -1;
+    if (kv->check_seq(seq)) return -1;
+    int slot = 0;
+    if (kv->slot_of(layer, &slot)) return -1;
+    if (n_tokens < 0 || base_pos < 0) return fail("negative count or position");
+    if (n_tokens == 0) return 0;
+    if (d_q == nullptr) return fail("NULL argument");
+    if ((uintptr_t)d_q % 16 != 0) return fail("d_q must be 16-byte aligned");
+    const long end = (long)base_pos + n_tokens;
+    if (end > (long)kv->seq_pages[seq] * Q38_PAGE_TOKENS) return fail("positions %d..%ld are not reserved", base_pos, end - 1);
+    q38_ctx *ctx = kv->ctx;
+    q38_observe_args a;
+    memset(&a, 0, sizeof(a));
+    a.n_groups = (n_tokens + Q38_OBSERVE_QUERIES - 1) / Q38_OBSERVE_QUERIES;
+    if (a.n_groups > 65535) return fail("%d tokens: at most %d a call", n_tokens, 65535 * Q38_OBSERVE_QUERIES);
+    /* a workgroup a CU, each of its waves with whole sets of pages */
+    const int pages = (int)((end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS), step = Q38_DECODE_TYPED_WAVES * Q38_OBSERVE_PAGES;
+    const int slots = std::max(ctx->cu_count / Q38_ATTN_KV_HEADS, 1);
+    a.split_pages = ((pages + slots - 1) / slots + step - 1) / step * step;
+    a.n_splits = (pages + a.split_pages - 1) / a.split_pages;
+    const size_t stats = (size_t)a.n_groups * Q38_ATTN_KV_HEADS * a.n_splits * Q38_OBSERVE_COLS * 2 * sizeof(float);
+    if (ctx->ensure_work(stats)) return -1;
+    a.kpool = reinterpret_cast<const char *>(kv->kslot(slot));
+    a.weights = kv->weights + (size_t)slot * kv->slot_sums();
+    a.page_row = kv->d_page_table + (size_t)seq * kv->pt_stride;
+    a.q = d_q;
+    a.part_ml = static_cast<float *>(ctx->work);
+    a.base_pos = base_pos;
+    a.n_tokens = n_tokens;
+    const unsigned block = 64 * Q38_DECODE_TYPED_WAVES;
+    if (ctx->launch(ctx->f_observe_stats[kv->type], a.n_splits, Q38_ATTN_KV_HEADS, a.n_groups, block, &a)) return -1;
+    return ctx->launch(ctx->f_observe_sums[kv->type], a.n_splits, Q38_ATTN_KV_HEADS, 1, block, &a);
+}
+
+int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n_tokens, const int32_t *n_keep,
+                 const int32_t *n_recent) {
+    if (check_tracks(kv)) return -1;
+    if (n_seq < 0) return fail("negative n_seq");
+    if (n_seq == 0) return 0;
+    if (!seq_ids || !n_tokens || !n_keep || !n_recent) return fail("NULL argument");
+    std::vector<char> seen(kv->max_seqs, 0);
+    long max_moves = 0;
+    for (int b = 0; b < n_seq; ++b) {
+        const int s = seq_ids[b];
+        if (kv->check_seq(s)) return -1;
+        if (seen[s]) return fail("sequence %d appears twice", s);
+        seen[s] = 1;
+        if (n_tokens[b] < 0 || n_keep[b] < 0 || n_recent[b] < 0) return fail("negative count");
+        if (n_tokens[b] > kv->seq_pages[s] * Q38_PAGE_TOKENS)
+            return fail("sequence %d: %d tokens are not reserved", s, n_tokens[b]);
+        if (n_tokens[b] < kv->evicted[s].kept)
+            return fail("sequence %d holds %d tokens since its last eviction, not %d", s, kv->evicted[s].kept, n_tokens[b]);
+        if (n_keep[b] > n_tokens[b]) return fail("sequence %d: %d tokens to keep of %d", s, n_keep[b], n_tokens[b]);
+        if (n_recent[b] > n_keep[b]) return fail("sequence %d: %d recent tokens to keep among %d", s, n_recent[b], n_keep[b]);
+        if ((long)kv->evicted[s].tokens + n_tokens[b] > (1L << 30)) return fail("sequence %d has read more than 2^30 tokens", s);
+        max_moves = std::max<long>(max_moves, std::min(n_keep[b], n_tokens[b] - n_keep[b]));
+    }
+    if (check_not_capturing(kv, "an eviction")) return -1;
+    q38_ctx *ctx = kv->ctx;
+    const int lists = Q38_ATTN_KV_HEADS * kv->n_slots, batch = std::min(n_seq, Q38_MAX_BATCH);
+    const size_t counts = ((size_t)batch * lists * sizeof(int32_t) + 15) / 16 * 16;
+    if (max_moves > 0 && ctx->ensure_work(counts + (size_t)batch * lists * 2 * max_moves * sizeof(int32_t))) return -1;
+    for (int b0 = 0; b0 < n_seq && max_moves > 0; b0 += Q38_MAX_BATCH) {
+        const int n = std::min(Q38_MAX_BATCH, n_seq - b0);
+        q38_evict_args a;
+        memset(&a, 0, sizeof(a));
+        a.kpool = reinterpret_cast<char *>(kv->kpool);
+        a.vpool = reinterpret_cast<char *>(kv->vpool);
+        a.weights = kv->weights;
+        a.tokens = kv->tokens;
+        a.page_table = kv->d_page_table;
+        a.counts = static_cast<int32_t *>(ctx->work);
+        a.moves = reinterpret_cast<int32_t *>(static_cast<char *>(ctx->work) + counts);
+        a.slot_bytes = (int64_t)kv->slot_bytes();
+        a.slot_weights = (int64_t)kv->slot_sums();
+        a.pt_stride = kv->pt_stride;
+        a.max_moves = (int32_t)max_moves;
+        for (int i = 0; i < n; ++i) {
+            const int b = b0 + i;
+            a.seq[i] = seq_ids[b];
+            a.n_tokens[i] = n_tokens[b];
+            a.n_keep[i] = n_keep[b];
+            a.first_recent[i] = kv->evicted[seq_ids[b]].tokens + n_tokens[b] - n_recent[b];
+        }
+        if (ctx->launch(ctx->f_evict_select, lists, n, 1, 1024, &a)) return -1;
+        if (ctx->launch(ctx->f_evict_move[kv->type], (unsigned)((max_moves + Q38_EVICT_ROWS - 1) / Q38_EVICT_ROWS), lists, n, 256, &a))
+            return -1;
+    }
+    for (int b = 0; b < n_seq; ++b) {
+        const int s = seq_ids[b];
+        if (n_keep[b] < n_tokens[b]) {
+            kv->images_from(s, -1, 0);
+            kv->evicted[s].tokens += n_tokens[b] - n_keep[b];
+            kv->evicted[s].kept = n_keep[b];
+        }
+        kv->release_from(s, (n_keep[b] + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS);
+    }
+    return 0;
 }
 
 /* ------------------------------------------------------------ attention decode */
@@ -1233,6 +1510,7 @@ struct decode_plan {
     int split_tokens = 0;
     int total_splits = 0;
     size_t work_bytes = 0;
+    size_t part_bytes = 0; /* of work_bytes: the rest is a tracking cache's scores */
 };
 
 /* Tokens per split over 16- or 8-bit rows (unless q38_set_decode_split fixed
@@ -1272,7 +1550,9 @@ int typed_split_tokens(const q38_ctx *ctx, int n_seq, const int32_t *positions, 
     return (int)(lo * Q38_PAGE_TOKENS);
 }
 
-int plan_decode(const q38_ctx *ctx, bool typed, int n_seq, const int32_t *positions, decode_plan *plan) {
+int plan_decode(const q38_kv *kv, int n_seq, const int32_t *positions, decode_plan *plan) {
+    const q38_ctx *ctx = kv->ctx;
+    const bool typed = kv->type != 0;
     long total_tokens = 0, max_tokens = 0;
     for (int b = 0; b < n_seq; ++b) {
         total_tokens += positions[b] + 1;
@@ -1290,7 +1570,10 @@ int plan_decode(const q38_ctx *ctx, bool typed, int n_seq, const int32_t *positi
         total += ns;
     }
     plan->total_splits = total;
-    plan->work_bytes = any_multi ? (size_t)total * Q38_ATTN_HEADS * (Q38_ATTN_HEAD_DIM + 2) * sizeof(float) : 0;
+    plan->part_bytes = any_multi || kv->tracks ? (size_t)total * Q38_ATTN_HEADS * (Q38_ATTN_HEAD_DIM + 2) * sizeof(float) : 0;
+    const size_t pages = (size_t)total * (plan->split_tokens / Q38_PAGE_TOKENS);
+    plan->work_bytes =
+        plan->part_bytes + (kv->tracks ? pages * Q38_ATTN_KV_HEADS * Q38_SCORES_PAGE * sizeof(float) : 0);
     return 0;
 }
 
@@ -1310,16 +1593,22 @@ struct decode_launch {
     bool one = false;
     q38_decode_one_args a_one;
     q38_merge_one_args m_one;
+    /* a tracking cache: what its kernels take beside `a` and `m` */
+    bool weighs = false;
+    q38_weigh_args w;
+    q38_weigh_merge_args mw;
     hipFunction_t f = nullptr, f_merge = nullptr;
     unsigned grid_x = 0;
     unsigned block = 0;
     bool merge = false;
+    dim3 merge_grid;
 
     /* where the kernels' arguments are (a vector's at its first), kMaxParams of them at most */
     static constexpr int kMaxParams = 4;
     void split_params(void **p) {
         if (!one) {
             p[0] = &a;
+            p[1] = &w;
             return;
         }
         q38_decode_one_args &o = a_one;
@@ -1331,6 +1620,7 @@ struct decode_launch {
     void merge_params(void **p) {
         if (!one) {
             p[0] = &m;
+            p[1] = &mw;
             return;
         }
         p[0] = &m_one.part_o;
@@ -1412,9 +1702,32 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
                                  : arg_pages ? ctx->f_decode_split_pre : ctx->f_decode_split_pre_many)
                           : (one ? ctx->f_decode_split_one : arg_pages ? ctx->f_decode_split : ctx->f_decode_split_many);
     L->block = (unsigned)ctx->decode_block;
-    L->one = kv->type != 0 && n_seq == 1;
+    L->one = kv->type != 0 && n_seq == 1 && !kv->tracks;
     L->f_merge = L->one ? ctx->f_decode_merge_one : ctx->f_decode_merge;
-    if (kv->type != 0) {
+    L->merge_grid = dim3(n_seq, Q38_ATTN_HEADS, 4);
+    L->weighs = kv->tracks;
+    if (L->weighs) {
+        float *scores = reinterpret_cast<float *>(static_cast<char *>(work) + plan.part_bytes);
+        L->f = ctx->f_weigh[kv->type][pre != nullptr ? 1 : 0];
+        L->block = 64 * Q38_DECODE_TYPED_WAVES;
+        L->f_merge = ctx->f_weigh_merge;
+        L->merge_grid = dim3(n_seq * Q38_ATTN_HEADS * 4 + total * Q38_ATTN_KV_HEADS, 1, 1);
+        memset(&L->w, 0, sizeof(L->w));
+        memset(&L->mw, 0, sizeof(L->mw));
+        L->w.scores = scores;
+        L->mw.scores = scores;
+        L->mw.page_table = a.page_table;
+        L->mw.weights = kv->weights + (size_t)slot * kv->slot_sums();
+        L->mw.tokens = kv->tokens + (size_t)slot * kv->slot_sums();
+        L->mw.pt_stride = kv->pt_stride;
+        L->mw.split_tokens = split_tokens;
+        L->mw.appended = d_k_new != nullptr ? 1 : 0;
+        for (int b = 0; b < n_seq; ++b) {
+            L->mw.seq[b] = seq_ids[b];
+            L->mw.pos[b] = positions[b];
+            L->mw.evicted[b] = L->w.evicted[b] = kv->evicted_of(seq_ids[b]);
+        }
+    } else if (kv->type != 0) {
         L->f = (L->one ? ctx->f_decode_typed_one : ctx->f_decode_typed)[kv->type][pre != nullptr ? 1 : 0];
         L->block = 64 * Q38_DECODE_TYPED_WAVES;
     }
@@ -1452,7 +1765,7 @@ int decode_chunk(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
     if (ctx->launch_params(L.f, L.grid_x, Q38_ATTN_KV_HEADS, 1, L.block, params)) return -1;
     if (!L.merge) return 0;
     L.merge_params(params);
-    if (ctx->launch_params(L.f_merge, n_seq, Q38_ATTN_HEADS, 4, 256, params)) return -1;
+    if (ctx->launch_params(L.f_merge, L.merge_grid.x, L.merge_grid.y, L.merge_grid.z, 256, params)) return -1;
     return 0;
 }
 
@@ -1477,7 +1790,7 @@ int validate_decode(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, co
             return fail("position %d is past the context limit %d", positions[b],
                         kv->pt_stride * Q38_PAGE_TOKENS);
         for (int c = 0; c < b; ++c)
-            if (seq_ids[c] == s && appends) return fail("sequence %d appears twice", s);
+            if (seq_ids[c] == s && (appends || kv->tracks)) return fail("sequence %d appears twice", s);
         const int need = positions[b] / Q38_PAGE_TOKENS + 1;
         if (appends) {
             pages_needed += std::max(0, need - kv->seq_pages[s]);
@@ -1506,7 +1819,7 @@ int decode_all(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const i
     size_t work_bytes = 0;
     for (int b0 = 0; b0 < n_seq; b0 += Q38_MAX_BATCH) {
         decode_plan plan;
-        if (plan_decode(ctx, kv->type != 0, std::min(Q38_MAX_BATCH, n_seq - b0), positions + b0, &plan)) return -1;
+        if (plan_decode(kv, std::min(Q38_MAX_BATCH, n_seq - b0), positions + b0, &plan)) return -1;
         work_bytes = std::max(work_bytes, plan.work_bytes);
     }
     void *work = nullptr;
@@ -1528,7 +1841,7 @@ int decode_all(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const i
     for (int b0 = 0; b0 < n_seq; b0 += Q38_MAX_BATCH) {
         const int n = std::min(Q38_MAX_BATCH, n_seq - b0);
         decode_plan plan;
-        if (plan_decode(ctx, kv->type != 0, n, positions + b0, &plan)) return -1;
+        if (plan_decode(kv, n, positions + b0, &plan)) return -1;
         const size_t kvoff = (size_t)b0 * Q38_ATTN_KV_DIM;
         const size_t qoff = (size_t)b0 * Q38_ATTN_Q_DIM;
         if (decode_chunk(kv, slot, n, seq_ids + b0, positions + b0, d_q + (size_t)b0 * q_rows,
@@ -1630,6 +1943,8 @@ struct q38_decode_graph {
     hipGraphExec_t exec = nullptr;
     hipGraphNode_t last = nullptr; /* the node the next step depends on */
     int steps = 0;
+    bool tracks = false; /* recorded over a tracking cache */
+    int32_t evicted[Q38_MAX_BATCH] = {0}; /* each sequence's evicted tokens when the positions were set */
 
     ~q38_decode_graph() {
         if (exec != nullptr) (void)hipGraphExecDestroy(exec);
@@ -1640,11 +1955,12 @@ struct q38_decode_graph {
     /* The split-K workspace for `pos`, grown only while no replay runs
      * (the caller's stream has been waited for). */
     int ensure_work(const int32_t *pos, decode_plan *plan) {
-        if (plan_decode(kv->ctx, kv->type != 0, n_seq, pos, plan)) return -1;
+        if (tracks != kv->tracks) return fail("the cache's tracking of weights has changed since the graph was begun");
+        if (plan_decode(kv, n_seq, pos, plan)) return -1;
         if (arg_pages && plan->total_splits > Q38_HEAD_PAGE_SPLITS)
             return fail("%d splits: this graph's split kernel takes at most %d", plan->total_splits,
                         Q38_HEAD_PAGE_SPLITS);
-        const size_t need = (size_t)plan->total_splits * Q38_ATTN_HEADS * (Q38_ATTN_HEAD_DIM + 2) * sizeof(float);
+        const size_t need = std::max(plan->work_bytes, (size_t)plan->total_splits * Q38_ATTN_HEADS * (Q38_ATTN_HEAD_DIM + 2) * sizeof(float));
         if (need > work_bytes) {
             if (work != nullptr) {
                 Q38_HIP(hipStreamSynchronize(kv->ctx->stream));
@@ -1680,7 +1996,12 @@ struct q38_decode_graph {
         for (Call &k : calls)
             if (build(k, pos, plan)) return -1;
         memcpy(positions, pos, sizeof(int32_t) * n_seq);
+        note_evicted();
         return 0;
+    }
+
+    void note_evicted() {
+        for (int b = 0; b < n_seq; ++b) evicted[b] = kv->evicted_of(seq_ids[b]);
     }
 
     int build(Call &k, const int32_t *pos, const decode_plan &plan) {
@@ -1699,7 +2020,7 @@ struct q38_decode_graph {
         } else {
             k.L.merge_params(params);
             p->func = reinterpret_cast<void *>(k.L.f_merge);
-            p->gridDim = dim3(n_seq, Q38_ATTN_HEADS, 4);
+            p->gridDim = k.L.merge_grid;
             p->blockDim = dim3(256, 1, 1);
         }
         p->kernelParams = params;
@@ -1738,6 +2059,8 @@ int q38_decode_graph_begin(q38_kv *kv, int n_seq, const int32_t *seq_ids, const 
     g->n_seq = n_seq;
     memcpy(g->seq_ids, seq_ids, sizeof(int32_t) * n_seq);
     memcpy(g->positions, positions, sizeof(int32_t) * n_seq);
+    g->tracks = kv->tracks;
+    g->note_evicted();
     g->arg_pages = kv->type == 0 && n_seq == 1 && kv->ctx->split_tokens == 0 ? 1 : 0;
     Q38_HIP(hipGraphCreate(&g->graph, 0));
     *out = g.release();
@@ -1889,6 +2212,10 @@ int q38_decode_graph_set_positions(q38_decode_graph *g, const int32_t *positions
 int q38_decode_graph_launch(q38_decode_graph *g) {
     if (g == nullptr) return fail("graph is NULL");
     if (g->exec == nullptr) return fail("the graph is not instantiated (q38_decode_graph_end)");
+    if (g->tracks != g->kv->tracks) return fail("the cache's tracking of weights has changed since the graph was begun");
+    for (int b = 0; b < g->n_seq; ++b)
+        if (g->evicted[b] != g->kv->evicted_of(g->seq_ids[b]))
+            return fail("sequence %d has evicted tokens since the graph's positions were set", g->seq_ids[b]);
     Q38_HIP(hipGraphLaunch(g->exec, g->kv->ctx->stream));
     return 0;
 }

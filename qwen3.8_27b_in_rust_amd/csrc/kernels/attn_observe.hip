@@ -1,0 +1,308 @@
+/*
+ * The attention weights that a run of a prompt's queries gives to the cached
+ * tokens, added to the sums of a tracking cache.
+ *
+ * Query u (position base_pos + u) sees positions up to its own: token t of a kv
+ * head takes W[t] += sum_u sum_h exp2(s_uht - M_uh) / L_uh over the group's heads
+ * h.  M and L need every position first, so the scores are formed twice, on the
+ * matrix unit both times: to keep 24 scores a query and token instead would write
+ * and read more bytes than the keys have from 12 queries on.  The first launch
+ * leaves each column's (a query's head) maximum and sum over a split of the
+ * positions; the second joins the splits' and adds.
+ *
+ * S^T = K Q^T as in the decode (q38_decode_typed.h: a cached value is an operand
+ * as it stands, a query is split into parts whose sum it is), but with 16 real
+ * columns a product.  A workgroup keeps the parts of 16 queries' 96 columns in
+ * LDS; a wave holds kPages pages of keys as operands and reads each part once for
+ * all of them.  Groups of queries come one after the other in a workgroup of the
+ * second launch, so that every sum has one owner and a fixed order.
+ */
+#include "q38_decode_typed.h"
+
+namespace {
+
+constexpr int kTiles = Q38_OBSERVE_COLS / 16;
+constexpr int kPages = Q38_OBSERVE_PAGES;
+template <int T>
+constexpr int kParts = kInBf16<T> ? 3 : 2;
+static_assert(kTiles * 16 == Q38_OBSERVE_COLS, "whole tiles");
+
+template <int T>
+struct Queries {
+    q38_u32x4 part[kTiles][kParts<T>][8][64];
+    float unscale[Q38_OBSERVE_COLS];
+};
+
+/* The group's queries as operands: columns 6 u + h, zero past the last query. */
+template <int T>
+Q38_DEV void load_queries(Queries<T> &q, const q38_observe_args &a, int group, int j, int lane, int wave) {
+    const int d = 4 * lane;
+    const int i = T == Q38_KV_Q8 ? 2 * (d >> 6) + ((d >> 3) & 1) : d >> 5;
+    const int g = T == Q38_KV_Q8 ? (d >> 4) & 3 : (d >> 3) & 3;
+#pragma unroll 4
+    for (int n = 0; n < Q38_OBSERVE_COLS / kWaves; ++n) {
+        const int col = n * kWaves + wave, u = group * Q38_OBSERVE_QUERIES + col / kGroup, h = j * kGroup + col % kGroup;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        if (u < a.n_tokens) x = q38_ld4(a.q + ((size_t)u * Q38_ATTN_HEADS + h) * Q38_ATTN_HEAD_DIM + d) * Q38_SCORE_LOG2;
+        float unscale = 1.0f;
+        if (!kInBf16<T>) {
+            /* as the decode scales a head: its largest value to 2^9..10 */
+            float big = column_max(q38_max16(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)))));
+            const int e = max((int)(__float_as_uint(big) >> 23) - 126, -116);
+            x *= __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+            unscale = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
+        }
+        if (lane == 0) q.unscale[col] = unscale;
+        uint16_t p[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (kInBf16<T>) {
+                const uint32_t hi = __float_as_uint(x[e]) & 0xFFFF0000u;
+                const float r = x[e] - __uint_as_float(hi);
+                const uint32_t mid = __float_as_uint(r) & 0xFFFF0000u;
+                p[0][e] = (uint16_t)(hi >> 16);
+                p[1][e] = (uint16_t)(mid >> 16);
+                p[2][e] = (uint16_t)(__float_as_uint(r - __uint_as_float(mid)) >> 16);
+            } else {
+                const _Float16 hi = (_Float16)x[e];
+                p[0][e] = __builtin_bit_cast(uint16_t, hi);
+                p[1][e] = __builtin_bit_cast(uint16_t, (_Float16)((x[e] - (float)hi) * kLowUnit<T>));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kParts<T>; ++k)
+            *(reinterpret_cast<q38_u32x2 *>(&q.part[col >> 4][k][i][16 * g + (col & 15)]) + ((d >> 2) & 1)) =
+                q38_u32x2{pack16(p[k][0], p[k][1]), pack16(p[k][2], p[k][3])};
+    }
+}
+
+/* A page's keys as operands, and 8-bit rows' scales of tokens 4 (lane / 16) .. + 3. */
+struct Keys {
+    q38_u32x4 a[8];
+    f32x4 scale;
+};
+template <int T>
+Q38_DEV void load_keys(Keys &k, const char *kpool, int page, int j, int lane) {
+    char *block = q38_kv_block<T>(const_cast<char *>(kpool), page, j);
+    const q38_u32x4 *in = reinterpret_cast<const q38_u32x4 *>(block) + lane;
+    if constexpr (T == Q38_KV_MX4) {
+        const q38_u32x4 u[2] = {in[0], in[64]};
+        const q38_u32x2 s = *reinterpret_cast<const q38_u32x2 *>(q38_mx4_scales(block, j) + 8 * (lane & 15));
+        auto step = [&](uint32_t codes, float scale) {
+            return q38_u32x4{bf16_pair<0>(codes, scale), bf16_pair<1>(codes, scale), bf16_pair<2>(codes, scale), bf16_pair<3>(codes, scale)};
+        };
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            k.a[4 * i] = step(u[i][0], scale_byte<0>(s[i]));
+            k.a[4 * i + 1] = step(u[i][1], scale_byte<1>(s[i]));
+            k.a[4 * i + 2] = step(u[i][2], scale_byte<2>(s[i]));
+            k.a[4 * i + 3] = step(u[i][3], scale_byte<3>(s[i]));
+        }
+    } else if constexpr (T == Q38_KV_Q8) {
+        q38_u32x4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = in[64 * i];
+        k.scale = q38_ld4(q38_kv_scales(block, j) + 4 * (lane >> 4));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t x = u[i >> 1][2 * (i & 1)], y = u[i >> 1][2 * (i & 1) + 1];
+            k.a[i] = q38_u32x4{halves_of<0x04010400u>(x), halves_of<0x04030402u>(x), halves_of<0x04010400u>(y), halves_of<0x04030402u>(y)};
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k.a[i] = in[64 * i];
+    }
+}
+
+/* Scores (log2 units) of kPages pages against a tile's 16 columns. */
+template <int T>
+Q38_DEV void scores_of(const Keys (&k)[kPages], const q38_u32x4 (*part)[8][64], float unscale, int lane, float (&s)[kPages][4]) {
+    /* (an index that the compiler cannot see through: it would keep the parts of
+     * all tiles in registers over the loop of pages) */
+    asm volatile("" : "+v"(lane));
+    f32x4 c[kPages][2];
+#pragma unroll
+    for (int p = 0; p < kPages; ++p) c[p][0] = c[p][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int n = 0; n < kParts<T>; ++n) {
+            const q38_u32x4 q = part[n][i][lane];
+#pragma unroll
+            for (int p = 0; p < kPages; ++p) c[p][n > 0] = mma_k<T>(k[p].a[i], q, c[p][n > 0]);
+        }
+#pragma unroll
+    for (int p = 0; p < kPages; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[p][i] = kInBf16<T> ? c[p][0][i] + c[p][1][i] : __builtin_fmaf(c[p][1][i], 1.0f / kLowUnit<T>, c[p][0][i]) * unscale;
+            if (T == Q38_KV_Q8) s[p][i] *= k[p].scale[i];
+        }
+}
+
+/* Scores past the column's own position do not count.  page: the first of kPages that lie kWaves apart. */
+Q38_DEV void mask(float (&s)[kPages][4], int page, int last, int g) {
+#pragma unroll
+    for (int p = 0; p < kPages; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (16 * (page + kWaves * p) + 4 * g + i > last) s[p][i] = -INFINITY;
+}
+
+struct Span {
+    int begin, end; /* pages of the split */
+    int last;       /* the cache's last page that a query sees */
+};
+Q38_DEV Span span_of(const q38_observe_args &a) {
+    const int last = (a.base_pos + a.n_tokens - 1) >> 4, begin = blockIdx.x * a.split_pages;
+    return {begin, min(begin + a.split_pages, last + 1), last};
+}
+
+template <int T>
+Q38_DEV void observe_stats(const q38_observe_args &a) {
+    __shared__ __attribute__((aligned(16))) Queries<T> q;
+    __shared__ float red[kWaves][Q38_OBSERVE_COLS][2];
+    const int j = blockIdx.y, group = blockIdx.z;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const Span sp = span_of(a);
+    load_queries<T>(q, a, group, j, lane, wave);
+    __syncthreads();
+    float M[kTiles], L[kTiles], unscale[kTiles];
+    int last[kTiles]; /* the column's own position */
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        const int u = group * Q38_OBSERVE_QUERIES + (16 * t + c) / kGroup;
+        M[t] = -INFINITY;
+        L[t] = 0.0f;
+        unscale[t] = q.unscale[16 * t + c];
+        last[t] = u < a.n_tokens ? a.base_pos + u : -1;
+    }
+    for (int page = sp.begin + wave; page < sp.end; page += kWaves * kPages) {
+        Keys k[kPages];
+#pragma unroll
+        for (int p = 0; p < kPages; ++p) load_keys<T>(k[p], a.kpool, a.page_row[min(page + kWaves * p, sp.end - 1)], j, lane);
+        /* pages past the split's end, and positions that some column does not see */
+        const bool masks = page + kWaves * (kPages - 1) >= sp.end ||
+                           16 * (page + kWaves * (kPages - 1)) + 15 > a.base_pos + group * Q38_OBSERVE_QUERIES;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            float s[kPages][4];
+            scores_of<T>(k, q.part[t], unscale[t], lane, s);
+            if (masks) mask(s, page, min(last[t], 16 * sp.end - 1), g);
+            float top = M[t];
+#pragma unroll
+            for (int p = 0; p < kPages; ++p) top = fmaxf(top, fmaxf(fmaxf(s[p][0], s[p][1]), fmaxf(s[p][2], s[p][3])));
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float sum = L[t] * q38_exp2(M[t] - ref);
+#pragma unroll
+            for (int p = 0; p < kPages; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum += q38_exp2(s[p][i] - ref);
+            M[t] = top;
+            L[t] = sum;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        const float top = column_max(M[t]);
+        const float sum = column_sum(M[t] == -INFINITY ? 0.0f : L[t] * q38_exp2(M[t] - top));
+        if (g == 0) {
+            red[wave][16 * t + c][0] = top;
+            red[wave][16 * t + c][1] = sum;
+        }
+    }
+    __syncthreads();
+    if (tid >= Q38_OBSERVE_COLS) return;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red[w][tid][0]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+        sum += red[w][tid][0] == -INFINITY ? 0.0f : red[w][tid][1] * q38_exp2(red[w][tid][0] - top);
+    float *out = a.part_ml + ((((size_t)group * Q38_ATTN_KV_HEADS + j) * a.n_splits + blockIdx.x) * Q38_OBSERVE_COLS + tid) * 2;
+    out[0] = top;
+    out[1] = sum;
+}
+
+template <int T>
+Q38_DEV void observe_sums(const q38_observe_args &a) {
+    __shared__ __attribute__((aligned(16))) Queries<T> q;
+    __shared__ float stat[Q38_OBSERVE_COLS][2]; /* a column's maximum, and one over its sum */
+    const int j = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const Span sp = span_of(a);
+    for (int group = 0; group < a.n_groups; ++group) {
+        const int u0 = group * Q38_OBSERVE_QUERIES;
+        /* (the same in every wave) a split that only later groups see */
+        if (16 * sp.begin > a.base_pos + min(u0 + Q38_OBSERVE_QUERIES, a.n_tokens) - 1) continue;
+        __syncthreads(); /* the group before is done with q and stat */
+        load_queries<T>(q, a, group, j, lane, wave);
+        if (tid < Q38_OBSERVE_COLS) {
+            const float *ml = a.part_ml + (((size_t)group * Q38_ATTN_KV_HEADS + j) * a.n_splits * Q38_OBSERVE_COLS + tid) * 2;
+            float M = -INFINITY, L = 0.0f;
+            for (int s = 0; s < a.n_splits; ++s) {
+                const float m = ml[(size_t)s * Q38_OBSERVE_COLS * 2], l = ml[(size_t)s * Q38_OBSERVE_COLS * 2 + 1];
+                const float top = fmaxf(M, m);
+                if (m == -INFINITY) continue; /* it sees nothing of that split */
+                L = (M == -INFINITY ? 0.0f : L * q38_exp2(M - top)) + l * q38_exp2(m - top);
+                M = top;
+            }
+            const bool in = u0 + tid / kGroup < a.n_tokens;
+            stat[tid][0] = in ? M : 0.0f;
+            stat[tid][1] = in ? 1.0f / L : 0.0f;
+        }
+        __syncthreads();
+        float M[kTiles], inverse[kTiles], unscale[kTiles];
+        int last[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const int u = u0 + (16 * t + c) / kGroup;
+            M[t] = stat[16 * t + c][0];
+            inverse[t] = stat[16 * t + c][1];
+            unscale[t] = q.unscale[16 * t + c];
+            last[t] = u < a.n_tokens ? a.base_pos + u : -1;
+        }
+        for (int page = sp.begin + wave; page < sp.end; page += kWaves * kPages) {
+            Keys k[kPages];
+            int id[kPages];
+#pragma unroll
+            for (int p = 0; p < kPages; ++p) {
+                id[p] = a.page_row[min(page + kWaves * p, sp.end - 1)];
+                load_keys<T>(k[p], a.kpool, id[p], j, lane);
+            }
+            const bool masks = page + kWaves * (kPages - 1) >= sp.end || 16 * (page + kWaves * (kPages - 1)) + 15 > a.base_pos + u0;
+            float w[kPages][4] = {};
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                float s[kPages][4];
+                scores_of<T>(k, q.part[t], unscale[t], lane, s);
+                if (masks) mask(s, page, min(last[t], 16 * sp.end - 1), g);
+#pragma unroll
+                for (int p = 0; p < kPages; ++p)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[p][i] = __builtin_fmaf(q38_exp2(s[p][i] - M[t]), inverse[t], w[p][i]);
+            }
+#pragma unroll
+            for (int p = 0; p < kPages; ++p) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[p][i] = q38_sum16(w[p][i]);
+                const int t0 = 16 * (page + kWaves * p) + 4 * g, end = min(a.base_pos + a.n_tokens, 16 * sp.end);
+                float *to = a.weights + (size_t)id[p] * Q38_WEIGHTS_PAGE + j * Q38_PAGE_TOKENS + 4 * g;
+                if (c == 0)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (t0 + i < end) to[i] += w[p][i];
+            }
+        }
+    }
+}
+
+}  // namespace
+
+#define Q38_OBSERVE_KERNELS(name, T)                                                                                       \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_stats_##name(q38_observe_args a) { observe_stats<T>(a); } \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_sums_##name(q38_observe_args a) { observe_sums<T>(a); }
+Q38_OBSERVE_KERNELS(f16, Q38_KV_F16)
+Q38_OBSERVE_KERNELS(bf16, Q38_KV_BF16)
+Q38_OBSERVE_KERNELS(q8k, Q38_KV_Q8)
+Q38_OBSERVE_KERNELS(mxfp4, Q38_KV_MX4)

@@ -157,9 +157,9 @@ Q38_DEV uint32_t pack16(uint16_t lo, uint16_t hi) { return (uint32_t)hi << 16 | 
 /* Scores of a page's tokens, the softmax update, the weighted sum of its
  * values.  valid: tokens of the page that count (16 but for the sequence's
  * last page); first: nothing is summed yet. */
-template <int T>
+template <int T, bool kWeigh = false>
 Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64], float unscale, int valid, bool first,
-                       int lane) {
+                       int lane, float *scores = nullptr) {
     const int c = lane & 15, g = lane >> 4;
     f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
     /* the queries are read from LDS at every page: an index that the compiler
@@ -213,6 +213,8 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
             if constexpr (T == Q38_KV_Q8) vs[i] = 0.0f;
         }
     }
+    /* kept for the sums of weights, which need the whole context's maximum and sum first */
+    if (kWeigh && c < kGroup) q38_st4(scores + c * Q38_PAGE_TOKENS + 4 * g, f32x4{s[0], s[1], s[2], s[3]});
     const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     auto scale_heads = [&](float f) { /* o by each head's factor */
         float fr[4];
@@ -515,8 +517,12 @@ Q38_DEV Where find(const q38_decode_typed_args &a, int g) {
     return {b, a.seq[b], a.pos[b], a.split_base[b], a.split_base[b + 1] - a.split_base[b]};
 }
 
-template <int T, bool kPre, typename Args>
-Q38_DEV void decode_typed(const Args &a) {
+/* Nothing beside the attention (q38_weigh_args: the scores too). */
+struct NoSums {};
+
+template <int T, bool kPre, typename Args, typename Sums = NoSums>
+Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
+    constexpr bool kWeigh = !std::is_same_v<Sums, NoSums>;
     constexpr int kQSets = kInBf16<T> ? 2 : 1;
     /* pages of a wave in registers: two 16-bit ones leave too few for the rest
      * (128K tokens 95 us against 85), 8-bit ones are half as large (1 / 2 / 3
@@ -581,7 +587,9 @@ Q38_DEV void decode_typed(const Args &a) {
     if (kPre) {
         /* (every wave, so that the weights' load above stays before the pages':
          * under a branch it would sink into it) */
-        q38_rope_table_half(rope_cs[wave], lane & 31, pos, a.theta_scale);
+        int rope_pos = pos;
+        if constexpr (kWeigh) rope_pos += sums.evicted[b];
+        q38_rope_table_half(rope_cs[wave], lane & 31, rope_pos, a.theta_scale);
         /* the lanes read each other's entries below: LDS serves a wave in
          * order, the fence keeps the compiler to it */
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -665,7 +673,10 @@ Q38_DEV void decode_typed(const Args &a) {
                             put_new_token<T>(buf[u], new_rows, valid - 1, lane);
                     }
                 }
-                page_step<T>(st, buf[u], q_frag, unscale, valid, at == wave, lane);
+                float *scores = nullptr;
+                if constexpr (kWeigh)
+                    scores = sums.scores + (((size_t)g_split * (a.split_tokens >> 4) + at) * Q38_ATTN_KV_HEADS + j) * Q38_SCORES_PAGE;
+                page_step<T, kWeigh>(st, buf[u], q_frag, unscale, valid, at == wave, lane, scores);
                 fetch(buf[u], at + kWaves * kDepth);
             }
         }
@@ -722,6 +733,10 @@ Q38_DEV void decode_typed(const Args &a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) O[e] = w < n_pages ? __builtin_fmaf(fu, o[w][e], O[e]) : O[e];
         }
+    }
+    if (kWeigh && nsplit == 1 && lane == 0) {
+        a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 0] = M;
+        a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 1] = L;
     }
     if (nsplit == 1) {
         f32x4 r = O / L;

@@ -578,4 +578,102 @@ typedef struct {
 } q38_merge_one_args;
 #define Q38_MERGE_ONE_PARAMS q38_u64x4 p, q38_i32x2 n
 
+/* ------------------------------------------------ sums of attention weights */
+
+/* A tracking cache keeps, beside each page of a slot, the sum of the softmax
+ * weights that its tokens were given and the tokens' own positions:
+ * [max_pages][4 kv heads][16 tokens], f32 and int32. */
+#define Q38_WEIGHTS_PAGE (Q38_ATTN_KV_HEADS * Q38_PAGE_TOKENS)
+
+/* What a decode launch over such a cache takes beside q38_decode_typed_args.  The
+ * scores (log2 units) of split g's page p, kv head j: at ((g * split_tokens / 16 +
+ * p) * 4 + j) * Q38_SCORES_PAGE, [6 query heads][16 tokens]; each split's
+ * part_ml is written, a sequence's only one too. */
+#define Q38_SCORES_PAGE (Q38_ATTN_GROUP * Q38_PAGE_TOKENS)
+typedef struct {
+    float *scores;
+    int32_t evicted[Q38_MAX_BATCH]; /* tokens evicted before: the new one is that much further on */
+} q38_weigh_args;
+/* The merge after it: grid (96 n_seq + 4 total_splits), 256 threads; the first
+ * workgroups join the splits' outputs (q38_attn_decode_merge's), the others add the
+ * weights of a (split, kv head) to the sums. */
+typedef struct {
+    const float *scores;
+    const int32_t *page_table;
+    float *weights;  /* this layer's sums */
+    int32_t *tokens; /* and own positions */
+    int32_t pt_stride;
+    int32_t split_tokens;
+    int32_t appended; /* the call stored a row at pos[b]: its sum starts here */
+    int32_t pad_;
+    int32_t seq[Q38_MAX_BATCH];
+    int32_t pos[Q38_MAX_BATCH];
+    int32_t evicted[Q38_MAX_BATCH];
+} q38_weigh_merge_args;
+
+/* Sums and own positions of a ragged batch between the pages and rows
+ * [rows][4 kv heads]: grid (ceil(page_base[n_seq] / 4)), 256 threads, a wave a page. */
+typedef struct {
+    float *weights;
+    int32_t *tokens;
+    const int32_t *page_table;
+    float *weight_rows; /* NULL: to the pages zeros, from them nothing */
+    int32_t *token_rows; /* NULL: to the pages the positions + evicted, from them nothing */
+    int32_t pt_stride;
+    int32_t to_pages;
+    int32_t n_seq;
+    int32_t pad_;
+    int32_t seq[Q38_MAX_BATCH];
+    int32_t pos0[Q38_MAX_BATCH];
+    int32_t evicted[Q38_MAX_BATCH];
+    int32_t row_base[Q38_MAX_BATCH + 1];
+    int32_t page_base[Q38_MAX_BATCH + 8]; /* past n_seq: INT_MAX */
+} q38_kv_weights_args;
+
+/* Eviction.  The choice: grid (4 n_slots, n_seq), 1024 threads, a workgroup for a
+ * (slot, kv head) of a sequence; it leaves, at moves + (blockIdx.y * 4 n_slots +
+ * blockIdx.x) * 2 max_moves, the evicted positions below n_keep, and max_moves
+ * further the kept ones from n_keep on, both rising, as many of each as counts
+ * says.  The moves: grid (ceil(max_moves / Q38_EVICT_ROWS), 4 n_slots, n_seq),
+ * 256 threads. */
+#define Q38_EVICT_ROWS 16
+typedef struct {
+    char *kpool;
+    char *vpool;
+    float *weights;  /* every slot's: [n_slots][max_pages][4][16] */
+    int32_t *tokens;
+    const int32_t *page_table;
+    int32_t *moves;
+    int32_t *counts; /* [n_seq][4 n_slots] */
+    int64_t slot_bytes;   /* of a pool */
+    int64_t slot_weights; /* sums of a slot */
+    int32_t pt_stride;
+    int32_t max_moves;
+    int32_t seq[Q38_MAX_BATCH];
+    int32_t n_tokens[Q38_MAX_BATCH];
+    int32_t n_keep[Q38_MAX_BATCH];
+    int32_t first_recent[Q38_MAX_BATCH]; /* tokens whose own position is this or later stay */
+} q38_evict_args;
+
+/* Weights that queries of a prompt give: columns are (query, head of the group)
+ * of one kv head, Q38_OBSERVE_QUERIES queries a group.  Statistics: grid
+ * (n_splits, 4, n_groups), 512 threads, the columns' maximum (log2 units) and sum
+ * over a split's positions; sums: grid (n_splits, 4), 512 threads. */
+#define Q38_OBSERVE_QUERIES 16
+#define Q38_OBSERVE_PAGES 2 /* of keys that a wave holds */
+#define Q38_OBSERVE_COLS (Q38_OBSERVE_QUERIES * Q38_ATTN_GROUP)
+typedef struct {
+    const char *kpool; /* this layer's */
+    float *weights;
+    const int32_t *page_row; /* the sequence's page table */
+    const float *q;          /* [n_tokens][24][256] */
+    float *part_ml;          /* [n_groups][4][n_splits][Q38_OBSERVE_COLS][2] */
+    int32_t base_pos;
+    int32_t n_tokens;
+    int32_t split_pages;
+    int32_t n_splits;
+    int32_t n_groups;
+    int32_t pad_;
+} q38_observe_args;
+
 #endif
