@@ -199,7 +199,7 @@ struct q38_ctx {
     hipFunction_t f_weights_copy = nullptr;
     hipFunction_t f_evict_select = nullptr;
     hipFunction_t f_evict_move[kKvTypeCount] = {};
-    hipFunction_t f_observe_stats[kKvTypeCount] = {}, f_observe_sums[kKvTypeCount] = {};
+    hipFunction_t f_observe_stats[kKvTypeCount][2] = {}, f_observe_sums[kKvTypeCount][2] = {}; /* [1]: a short context */
     hipModule_t mod_rows_own[kKvTypeCount] = {}, mod_decode_own[kKvTypeCount] = {}; /* types with own_objects */
     hipFunction_t f_decode_typed[kKvTypeCount][2] = {}; /* from index 1 on; [1]: the pre step fused */
     hipFunction_t f_decode_typed_one[kKvTypeCount][2] = {};
@@ -558,8 +558,11 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
             Q38_HIP(hipModuleGetFunction(&ctx->f_weigh[i][pre], ctx->mod_weigh, ("q38_attn_weigh_" + ty + (pre ? "_pre" : "")).c_str()));
         }
         Q38_HIP(hipModuleGetFunction(&ctx->f_evict_move[i], ctx->mod_weights, ("q38_kv_evict_move_" + ty).c_str()));
-        Q38_HIP(hipModuleGetFunction(&ctx->f_observe_stats[i], ctx->mod_observe, ("q38_observe_stats_" + ty).c_str()));
-        Q38_HIP(hipModuleGetFunction(&ctx->f_observe_sums[i], ctx->mod_observe, ("q38_observe_sums_" + ty).c_str()));
+        for (int few = 0; few < 2; ++few) {
+            const std::string name = ty + (few ? "_short" : "");
+            Q38_HIP(hipModuleGetFunction(&ctx->f_observe_stats[i][few], ctx->mod_observe, ("q38_observe_stats_" + name).c_str()));
+            Q38_HIP(hipModuleGetFunction(&ctx->f_observe_sums[i][few], ctx->mod_observe, ("q38_observe_sums_" + name).c_str()));
+        }
     }
     const std::string p_proj = dir + "/proj.hsaco";
     Q38_HIP(hipModuleLoad(&ctx->mod_proj, p_proj.c_str()));
@@ -1379,9 +1382,12 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     memset(&a, 0, sizeof(a));
     a.n_groups = (n_tokens + Q38_OBSERVE_QUERIES - 1) / Q38_OBSERVE_QUERIES;
     if (a.n_groups > 65535) return fail("%d tokens: at most %d a call", n_tokens, 65535 * Q38_OBSERVE_QUERIES);
-    /* a workgroup a CU, each of its waves with whole sets of pages */
-    const int pages = (int)((end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS), step = Q38_DECODE_TYPED_WAVES * Q38_OBSERVE_PAGES;
-    const int slots = std::max(ctx->cu_count / Q38_ATTN_KV_HEADS, 1);
+    /* a workgroup a CU (64 splits at most: a lane each where they are joined), each of its waves with whole sets of
+     * pages: several at a time where every CU has that many, else one */
+    const int pages = (int)((end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS);
+    const int slots = std::min(std::max(ctx->cu_count / Q38_ATTN_KV_HEADS, 1), 64);
+    const int few = pages < slots * Q38_DECODE_TYPED_WAVES * Q38_OBSERVE_PAGES ? 1 : 0;
+    const int step = Q38_DECODE_TYPED_WAVES * (few ? 1 : Q38_OBSERVE_PAGES);
     a.split_pages = ((pages + slots - 1) / slots + step - 1) / step * step;
     a.n_splits = (pages + a.split_pages - 1) / a.split_pages;
     const size_t stats = (size_t)a.n_groups * Q38_ATTN_KV_HEADS * a.n_splits * Q38_OBSERVE_COLS * 2 * sizeof(float);
@@ -1394,8 +1400,8 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     a.base_pos = base_pos;
     a.n_tokens = n_tokens;
     const unsigned block = 64 * Q38_DECODE_TYPED_WAVES;
-    if (ctx->launch(ctx->f_observe_stats[kv->type], a.n_splits, Q38_ATTN_KV_HEADS, a.n_groups, block, &a)) return -1;
-    return ctx->launch(ctx->f_observe_sums[kv->type], a.n_splits, Q38_ATTN_KV_HEADS, 1, block, &a);
+    if (ctx->launch(ctx->f_observe_stats[kv->type][few], a.n_splits, Q38_ATTN_KV_HEADS, a.n_groups, block, &a)) return -1;
+    return ctx->launch(ctx->f_observe_sums[kv->type][few], a.n_splits, Q38_ATTN_KV_HEADS, 1, block, &a);
 }
 
 int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n_tokens, const int32_t *n_keep,

@@ -12,9 +12,12 @@
  *
  * S^T = K Q^T as in the decode (q38_decode_typed.h: a cached value is an operand
  * as it stands, a query is split into parts whose sum it is), but with 16 real
- * columns a product.  A workgroup keeps the parts of 16 queries' 96 columns in
- * LDS; a wave holds kPages pages of keys as operands and reads each part once for
- * all of them.  Groups of queries come one after the other in a workgroup of the
+ * columns a product, and with two parts of a query for every type: bf16 ones
+ * rounded to nearest leave 2^-17 of it, as the prefill's products do (the decode
+ * keeps a third), and the sums over many queries hardly see it: 32 queries over 32K
+ * tokens are within 3e-7 of 64 bits, 7 over 1000 within 7e-7.  A workgroup keeps the parts of 16 queries' 96
+ * columns in LDS; a wave holds kPages pages of keys as operands and reads each
+ * part once for all of them.  Groups of queries come one after the other in a workgroup of the
  * second launch, so that every sum has one owner and a fixed order.
  */
 #include "q38_decode_typed.h"
@@ -22,14 +25,12 @@
 namespace {
 
 constexpr int kTiles = Q38_OBSERVE_COLS / 16;
-constexpr int kPages = Q38_OBSERVE_PAGES;
-template <int T>
-constexpr int kParts = kInBf16<T> ? 3 : 2;
+constexpr int kParts = 2;
 static_assert(kTiles * 16 == Q38_OBSERVE_COLS, "whole tiles");
 
 template <int T>
 struct Queries {
-    q38_u32x4 part[kTiles][kParts<T>][8][64];
+    q38_u32x4 part[kTiles][kParts][8][64];
     float unscale[Q38_OBSERVE_COLS];
 };
 
@@ -39,38 +40,42 @@ Q38_DEV void load_queries(Queries<T> &q, const q38_observe_args &a, int group, i
     const int d = 4 * lane;
     const int i = T == Q38_KV_Q8 ? 2 * (d >> 6) + ((d >> 3) & 1) : d >> 5;
     const int g = T == Q38_KV_Q8 ? (d >> 4) & 3 : (d >> 3) & 3;
-#pragma unroll 4
-    for (int n = 0; n < Q38_OBSERVE_COLS / kWaves; ++n) {
+    constexpr int kRows = Q38_OBSERVE_COLS / kWaves;
+    f32x4 x[kRows];
+#pragma unroll
+    for (int n = 0; n < kRows; ++n) {
         const int col = n * kWaves + wave, u = group * Q38_OBSERVE_QUERIES + col / kGroup, h = j * kGroup + col % kGroup;
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
-        if (u < a.n_tokens) x = q38_ld4(a.q + ((size_t)u * Q38_ATTN_HEADS + h) * Q38_ATTN_HEAD_DIM + d) * Q38_SCORE_LOG2;
+        x[n] = q38_ld4(a.q + ((size_t)min(u, a.n_tokens - 1) * Q38_ATTN_HEADS + h) * Q38_ATTN_HEAD_DIM + d);
+        if (u >= a.n_tokens) x[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int n = 0; n < kRows; ++n) {
+        const int col = n * kWaves + wave;
+        f32x4 y = x[n] * Q38_SCORE_LOG2;
         float unscale = 1.0f;
         if (!kInBf16<T>) {
             /* as the decode scales a head: its largest value to 2^9..10 */
-            float big = column_max(q38_max16(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)))));
+            const float big = column_max(q38_max16(fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
             const int e = max((int)(__float_as_uint(big) >> 23) - 126, -116);
-            x *= __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+            y *= __uint_as_float((uint32_t)(127 + 10 - e) << 23);
             unscale = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
         }
         if (lane == 0) q.unscale[col] = unscale;
-        uint16_t p[3][4];
+        uint16_t p[kParts][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (kInBf16<T>) {
-                const uint32_t hi = __float_as_uint(x[e]) & 0xFFFF0000u;
-                const float r = x[e] - __uint_as_float(hi);
-                const uint32_t mid = __float_as_uint(r) & 0xFFFF0000u;
-                p[0][e] = (uint16_t)(hi >> 16);
-                p[1][e] = (uint16_t)(mid >> 16);
-                p[2][e] = (uint16_t)(__float_as_uint(r - __uint_as_float(mid)) >> 16);
-            } else {
-                const _Float16 hi = (_Float16)x[e];
+                const __bf16 hi = (__bf16)y[e];
                 p[0][e] = __builtin_bit_cast(uint16_t, hi);
-                p[1][e] = __builtin_bit_cast(uint16_t, (_Float16)((x[e] - (float)hi) * kLowUnit<T>));
+                p[1][e] = __builtin_bit_cast(uint16_t, (__bf16)(y[e] - (float)hi));
+            } else {
+                const _Float16 hi = (_Float16)y[e];
+                p[0][e] = __builtin_bit_cast(uint16_t, hi);
+                p[1][e] = __builtin_bit_cast(uint16_t, (_Float16)((y[e] - (float)hi) * kLowUnit<T>));
             }
         }
 #pragma unroll
-        for (int k = 0; k < kParts<T>; ++k)
+        for (int k = 0; k < kParts; ++k)
             *(reinterpret_cast<q38_u32x2 *>(&q.part[col >> 4][k][i][16 * g + (col & 15)]) + ((d >> 2) & 1)) =
                 q38_u32x2{pack16(p[k][0], p[k][1]), pack16(p[k][2], p[k][3])};
     }
@@ -115,7 +120,7 @@ Q38_DEV void load_keys(Keys &k, const char *kpool, int page, int j, int lane) {
 }
 
 /* Scores (log2 units) of kPages pages against a tile's 16 columns. */
-template <int T>
+template <int T, int kPages>
 Q38_DEV void scores_of(const Keys (&k)[kPages], const q38_u32x4 (*part)[8][64], float unscale, int lane, float (&s)[kPages][4]) {
     /* (an index that the compiler cannot see through: it would keep the parts of
      * all tiles in registers over the loop of pages) */
@@ -126,7 +131,7 @@ Q38_DEV void scores_of(const Keys (&k)[kPages], const q38_u32x4 (*part)[8][64], 
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int n = 0; n < kParts<T>; ++n) {
+        for (int n = 0; n < kParts; ++n) {
             const q38_u32x4 q = part[n][i][lane];
 #pragma unroll
             for (int p = 0; p < kPages; ++p) c[p][n > 0] = mma_k<T>(k[p].a[i], q, c[p][n > 0]);
@@ -141,6 +146,7 @@ Q38_DEV void scores_of(const Keys (&k)[kPages], const q38_u32x4 (*part)[8][64], 
 }
 
 /* Scores past the column's own position do not count.  page: the first of kPages that lie kWaves apart. */
+template <int kPages>
 Q38_DEV void mask(float (&s)[kPages][4], int page, int last, int g) {
 #pragma unroll
     for (int p = 0; p < kPages; ++p)
@@ -158,13 +164,19 @@ Q38_DEV Span span_of(const q38_observe_args &a) {
     return {begin, min(begin + a.split_pages, last + 1), last};
 }
 
-template <int T>
+/* Tiles of a group that hold a query. */
+Q38_DEV int tiles_of(const q38_observe_args &a, int group) {
+    return (min(a.n_tokens - group * Q38_OBSERVE_QUERIES, Q38_OBSERVE_QUERIES) * kGroup + 15) >> 4;
+}
+
+template <int T, int kPages>
 Q38_DEV void observe_stats(const q38_observe_args &a) {
     __shared__ __attribute__((aligned(16))) Queries<T> q;
     __shared__ float red[kWaves][Q38_OBSERVE_COLS][2];
     const int j = blockIdx.y, group = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const Span sp = span_of(a);
+    const int tiles = tiles_of(a, group);
     load_queries<T>(q, a, group, j, lane, wave);
     __syncthreads();
     float M[kTiles], L[kTiles], unscale[kTiles];
@@ -186,6 +198,7 @@ Q38_DEV void observe_stats(const q38_observe_args &a) {
                            16 * (page + kWaves * (kPages - 1)) + 15 > a.base_pos + group * Q38_OBSERVE_QUERIES;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
+            if (t >= tiles) continue;
             float s[kPages][4];
             scores_of<T>(k, q.part[t], unscale[t], lane, s);
             if (masks) mask(s, page, min(last[t], 16 * sp.end - 1), g);
@@ -219,12 +232,12 @@ Q38_DEV void observe_stats(const q38_observe_args &a) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
         sum += red[w][tid][0] == -INFINITY ? 0.0f : red[w][tid][1] * q38_exp2(red[w][tid][0] - top);
-    float *out = a.part_ml + ((((size_t)group * Q38_ATTN_KV_HEADS + j) * a.n_splits + blockIdx.x) * Q38_OBSERVE_COLS + tid) * 2;
+    float *out = a.part_ml + ((((size_t)group * Q38_ATTN_KV_HEADS + j) * Q38_OBSERVE_COLS + tid) * a.n_splits + blockIdx.x) * 2;
     out[0] = top;
     out[1] = sum;
 }
 
-template <int T>
+template <int T, int kPages>
 Q38_DEV void observe_sums(const q38_observe_args &a) {
     __shared__ __attribute__((aligned(16))) Queries<T> q;
     __shared__ float stat[Q38_OBSERVE_COLS][2]; /* a column's maximum, and one over its sum */
@@ -232,36 +245,33 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const Span sp = span_of(a);
     for (int group = 0; group < a.n_groups; ++group) {
-        const int u0 = group * Q38_OBSERVE_QUERIES;
+        const int u0 = group * Q38_OBSERVE_QUERIES, tiles = tiles_of(a, group);
         /* (the same in every wave) a split that only later groups see */
         if (16 * sp.begin > a.base_pos + min(u0 + Q38_OBSERVE_QUERIES, a.n_tokens) - 1) continue;
         __syncthreads(); /* the group before is done with q and stat */
         load_queries<T>(q, a, group, j, lane, wave);
-        if (tid < Q38_OBSERVE_COLS) {
-            const float *ml = a.part_ml + (((size_t)group * Q38_ATTN_KV_HEADS + j) * a.n_splits * Q38_OBSERVE_COLS + tid) * 2;
-            float M = -INFINITY, L = 0.0f;
-            for (int s = 0; s < a.n_splits; ++s) {
-                const float m = ml[(size_t)s * Q38_OBSERVE_COLS * 2], l = ml[(size_t)s * Q38_OBSERVE_COLS * 2 + 1];
-                const float top = fmaxf(M, m);
-                if (m == -INFINITY) continue; /* it sees nothing of that split */
-                L = (M == -INFINITY ? 0.0f : L * q38_exp2(M - top)) + l * q38_exp2(m - top);
-                M = top;
+        /* the splits' maxima and sums joined, a lane a split */
+        const float *ml = a.part_ml + (((size_t)group * Q38_ATTN_KV_HEADS + j) * Q38_OBSERVE_COLS * a.n_splits + min(lane, a.n_splits - 1)) * 2;
+        float m[Q38_OBSERVE_COLS / kWaves], l[Q38_OBSERVE_COLS / kWaves];
+#pragma unroll
+        for (int n = 0; n < Q38_OBSERVE_COLS / kWaves; ++n) {
+            const float *at = ml + (size_t)(n * kWaves + wave) * a.n_splits * 2;
+            m[n] = at[0];
+            l[n] = at[1];
+        }
+#pragma unroll
+        for (int n = 0; n < Q38_OBSERVE_COLS / kWaves; ++n) {
+            const int col = n * kWaves + wave;
+            const float top = column_max(q38_max16(m[n]));
+            /* a split that the column sees nothing of has a maximum of -inf */
+            const float sum = column_sum(q38_sum16(lane < a.n_splits && m[n] != -INFINITY ? l[n] * q38_exp2(m[n] - top) : 0.0f));
+            const bool in = u0 + col / kGroup < a.n_tokens;
+            if (lane == 0) {
+                stat[col][0] = in ? top : 0.0f;
+                stat[col][1] = in ? 1.0f / sum : 0.0f;
             }
-            const bool in = u0 + tid / kGroup < a.n_tokens;
-            stat[tid][0] = in ? M : 0.0f;
-            stat[tid][1] = in ? 1.0f / L : 0.0f;
         }
         __syncthreads();
-        float M[kTiles], inverse[kTiles], unscale[kTiles];
-        int last[kTiles];
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            const int u = u0 + (16 * t + c) / kGroup;
-            M[t] = stat[16 * t + c][0];
-            inverse[t] = stat[16 * t + c][1];
-            unscale[t] = q.unscale[16 * t + c];
-            last[t] = u < a.n_tokens ? a.base_pos + u : -1;
-        }
         for (int page = sp.begin + wave; page < sp.end; page += kWaves * kPages) {
             Keys k[kPages];
             int id[kPages];
@@ -274,13 +284,21 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
             float w[kPages][4] = {};
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) {
+                if (t >= tiles) continue;
                 float s[kPages][4];
-                scores_of<T>(k, q.part[t], unscale[t], lane, s);
-                if (masks) mask(s, page, min(last[t], 16 * sp.end - 1), g);
+                /* (read from LDS for each set of pages: six tiles' are too many registers) */
+                int col = 16 * t + c;
+                asm volatile("" : "+v"(col));
+                scores_of<T>(k, q.part[t], q.unscale[col], lane, s);
+                if (masks) {
+                    const int u = u0 + col / kGroup;
+                    mask(s, page, min(u < a.n_tokens ? a.base_pos + u : -1, 16 * sp.end - 1), g);
+                }
+                const float M = stat[col][0], inverse = stat[col][1];
 #pragma unroll
                 for (int p = 0; p < kPages; ++p)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[p][i] = __builtin_fmaf(q38_exp2(s[p][i] - M[t]), inverse[t], w[p][i]);
+                    for (int i = 0; i < 4; ++i) w[p][i] = __builtin_fmaf(q38_exp2(s[p][i] - M), inverse, w[p][i]);
             }
 #pragma unroll
             for (int p = 0; p < kPages; ++p) {
@@ -299,9 +317,16 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
 
 }  // namespace
 
-#define Q38_OBSERVE_KERNELS(name, T)                                                                                       \
-    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_stats_##name(q38_observe_args a) { observe_stats<T>(a); } \
-    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_sums_##name(q38_observe_args a) { observe_sums<T>(a); }
+#define Q38_OBSERVE_KERNEL(name, T, PAGES)                                                                        \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_stats_##name(q38_observe_args a) {     \
+        observe_stats<T, PAGES>(a);                                                                              \
+    }                                                                                                            \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_sums_##name(q38_observe_args a) {      \
+        observe_sums<T, PAGES>(a);                                                                               \
+    }
+#define Q38_OBSERVE_KERNELS(name, T)                   \
+    Q38_OBSERVE_KERNEL(name, T, Q38_OBSERVE_PAGES)     \
+    Q38_OBSERVE_KERNEL(name##_short, T, 1)
 Q38_OBSERVE_KERNELS(f16, Q38_KV_F16)
 Q38_OBSERVE_KERNELS(bf16, Q38_KV_BF16)
 Q38_OBSERVE_KERNELS(q8k, Q38_KV_Q8)

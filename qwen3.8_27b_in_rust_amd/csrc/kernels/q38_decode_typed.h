@@ -18,6 +18,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
+#ifndef Q38_MX4_DEPTH
+#define Q38_MX4_DEPTH 1
+#endif
 constexpr int kWaves = Q38_DECODE_TYPED_WAVES;
 constexpr int kGroup = Q38_ATTN_GROUP;
 /* A head's reference lies kRefBelow under the score that set it, and is raised
@@ -110,7 +113,13 @@ Q38_DEV uint32_t bf16_pair(uint32_t codes, float scale) {
 }
 template <int B>
 Q38_DEV float scale_byte(uint32_t e) {
-    return __uint_as_float((B == 0 ? e << 23 : B == 3 ? e >> 1 : B == 1 ? e << 15 : e << 7) & 0x7F800000u);
+    float r; /* (byte B << 23 in one operation; from C++ it is a shift and a mask) */
+    static_assert(B >= 0 && B < 4, "a byte of a word");
+    if (B == 0) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(23), "v"(e));
+    if (B == 1) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(23), "v"(e));
+    if (B == 2) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(23), "v"(e));
+    if (B == 3) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(23), "v"(e));
+    return r;
 }
 
 Q38_DEV float row_ror8(float x) {
@@ -167,20 +176,7 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
      * which the pages in flight need (8-bit pages leave room) */
     int ql = lane;
     if (T != Q38_KV_Q8) asm volatile("" : "+v"(ql));
-    if constexpr (T == Q38_KV_MX4) {
-        auto step = [&](uint32_t codes, float scale, int i) {
-            const q38_u32x4 a = {bf16_pair<0>(codes, scale), bf16_pair<1>(codes, scale), bf16_pair<2>(codes, scale), bf16_pair<3>(codes, scale)};
-            s0 = mma_k<T>(a, q[0][i][ql], s0);
-            s1 = mma_k<T>(a, q[1][i][ql], s1);
-        };
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            step(p.k[i][0], scale_byte<0>(p.ks[i]), 4 * i);
-            step(p.k[i][1], scale_byte<1>(p.ks[i]), 4 * i + 1);
-            step(p.k[i][2], scale_byte<2>(p.ks[i]), 4 * i + 2);
-            step(p.k[i][3], scale_byte<3>(p.ks[i]), 4 * i + 3);
-        }
-    } else if constexpr (T == Q38_KV_Q8) {
+    if (T == Q38_KV_Q8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const q38_u32x4 u = p.k[i];
@@ -200,8 +196,7 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         }
     }
     float s[4];
-    f32x4 ks, vs;
-    if constexpr (T != Q38_KV_MX4) ks = p.ks, vs = p.vs;
+    f32x4 ks = p.ks, vs = p.vs;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float x = s0[i] + s1[i];
@@ -210,7 +205,7 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         if (T == Q38_KV_Q8) s[i] *= ks[i];
         if (valid < 16 && 4 * g + i >= valid) {
             s[i] = -INFINITY;
-            if constexpr (T == Q38_KV_Q8) vs[i] = 0.0f;
+            vs[i] = 0.0f;
         }
     }
     /* kept for the sums of weights, which need the whole context's maximum and sum first */
@@ -303,25 +298,6 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         }
         a0 = q38_u32x2{pack16(x[0], x[1]), pack16(x[2], x[3])};
     }
-    if constexpr (T == Q38_KV_MX4) {
-        /* bytes of tokens that do not count are cleared, scales with codes */
-        const int n = min(max(valid - 4 * g, 0), 4);
-        const uint32_t bytes = n == 4 ? ~0u : (1u << (8 * n)) - 1u;
-        auto tiles = [&](uint32_t codes, uint32_t scales, int n) {
-            codes &= bytes, scales &= bytes;
-            const uint32_t t0 = bf16_pair<0>(codes, scale_byte<0>(scales)), t1 = bf16_pair<1>(codes, scale_byte<1>(scales)),
-                           t2 = bf16_pair<2>(codes, scale_byte<2>(scales)), t3 = bf16_pair<3>(codes, scale_byte<3>(scales));
-            const q38_u32x2 v0 = {__builtin_amdgcn_perm(t1, t0, 0x05040100u), __builtin_amdgcn_perm(t3, t2, 0x05040100u)};
-            const q38_u32x2 v1 = {__builtin_amdgcn_perm(t1, t0, 0x07060302u), __builtin_amdgcn_perm(t3, t2, 0x07060302u)};
-            st.o[n] = mma_v<T>(a0, v0, st.o[n]);
-            st.o[n + 1] = mma_v<T>(a0, v1, st.o[n + 1]);
-            st.o[n] = mma_v<T>(a1, v0, st.o[n]);
-            st.o[n + 1] = mma_v<T>(a1, v1, st.o[n + 1]);
-        };
-#pragma unroll
-        for (int i = 0; i < 8; ++i) tiles(p.v[i >> 2][i & 3], p.vs[i >> 2][i & 3], 2 * i);
-        return;
-    }
     /* values of tokens that do not count are cleared (8-bit ones are finite) */
     q38_u32x2 keep = {~0u, ~0u};
     if (T != Q38_KV_Q8 && valid < 16) {
@@ -331,9 +307,7 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
 #pragma unroll
     for (int n = 0; n < 16; ++n) {
         q38_u32x2 v;
-        if constexpr (T == Q38_KV_MX4) {
-            continue;
-        } else if (T == Q38_KV_Q8) {
+        if (T == Q38_KV_Q8) {
             const uint32_t u = p.v[n >> 2][n & 3];
             v = q38_u32x2{halves_of<0x04010400u>(u), halves_of<0x04030402u>(u)};
         } else {
@@ -342,6 +316,129 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         st.o[n] = mma_v<T>(a0, v, st.o[n]);
         if (T == Q38_KV_BF16) st.o[n] = mma_v<T>(a1, v, st.o[n]);
     }
+}
+
+/* The same for two pages of 4-bit rows at once, whose 32 tokens are the k of one
+ * product: half the products of O, and one look at the running maxima for both.
+ * valid: tokens of each that count; the bytes of the others are 0. */
+Q38_DEV uint32_t upper_halves(float lo, float hi) {
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+template <bool kWeigh>
+Q38_DEV void pair_step(State &st, const Page<Q38_KV_MX4> (&p)[2], const q38_u32x4 (*q)[8][64], int valid0, int valid1, bool first,
+                       int lane, float *scores0, float *scores1) {
+    constexpr int T = Q38_KV_MX4;
+    const int c = lane & 15, g = lane >> 4;
+    int ql = lane;
+    asm volatile("" : "+v"(ql)); /* (as in page_step) */
+    f32x4 s0[2] = {}, s1[2] = {};
+    auto step = [&](auto b, int i) {
+        constexpr int B = decltype(b)::value;
+        const q38_u32x4 q0 = q[0][4 * i + B][ql], q1 = q[1][4 * i + B][ql];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint32_t u = p[x].k[i][B];
+            const float scale = scale_byte<B>(p[x].ks[i]);
+            const q38_u32x4 a = {bf16_pair<0>(u, scale), bf16_pair<1>(u, scale), bf16_pair<2>(u, scale), bf16_pair<3>(u, scale)};
+            s0[x] = mma_k<T>(a, q0, s0[x]);
+            s1[x] = mma_k<T>(a, q1, s1[x]);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        step(std::integral_constant<int, 0>(), i);
+        step(std::integral_constant<int, 1>(), i);
+        step(std::integral_constant<int, 2>(), i);
+        step(std::integral_constant<int, 3>(), i);
+    }
+    float s[2][4];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float y = s0[x][i] + s1[x][i];
+            s[x][i] = y + row_ror8(y);
+        }
+    if (valid0 + valid1 < 32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (4 * g + i >= valid0) s[0][i] = -INFINITY;
+            if (4 * g + i >= valid1) s[1][i] = -INFINITY;
+        }
+    }
+    if (kWeigh && c < kGroup) {
+        q38_st4(scores0 + c * Q38_PAGE_TOKENS + 4 * g, f32x4{s[0][0], s[0][1], s[0][2], s[0][3]});
+        if (valid1 > 0) q38_st4(scores1 + c * Q38_PAGE_TOKENS + 4 * g, f32x4{s[1][0], s[1][1], s[1][2], s[1][3]});
+    }
+    const float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    if (__any(mx > st.ref + kRefSlack)) {
+        const float ref = fmaxf(st.ref, column_max(mx));
+        const float f = st.ref == -INFINITY ? 0.0f : q38_exp2(st.ref - ref);
+        st.l *= f;
+        st.ref = ref;
+        if (!first) {
+            float fr[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * g + i, 64);
+#pragma unroll
+            for (int n = 0; n < 16; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st.o[n][i] *= fr[i];
+        }
+    }
+    /* the weights' parts: rows 0-5 the first and, in a product of its own, the third, rows 8-13 the second */
+    q38_u32x4 a0, a1;
+    const bool upper = c >= 8;
+    float sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        float w[4], r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float e = q38_exp2(s[x][i] - st.ref);
+            sum += e;
+            const float rest = e - __uint_as_float(__float_as_uint(e) & 0xFFFF0000u);
+            const float last = rest - __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u);
+            w[i] = upper ? rest : e;
+            r[i] = upper ? 0.0f : last;
+        }
+        a0[2 * x] = upper_halves(w[0], w[1]);
+        a0[2 * x + 1] = upper_halves(w[2], w[3]);
+        a1[2 * x] = upper_halves(r[0], r[1]);
+        a1[2 * x + 1] = upper_halves(r[2], r[3]);
+    }
+    st.l += sum;
+    /* a byte's two values are dims of two tiles: tokens are paired up for each */
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        q38_u32x4 v0, v1;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint32_t u = p[x].v[i >> 2][i & 3], e = p[x].vs[i >> 2][i & 3];
+            const uint32_t t0 = bf16_pair<0>(u, scale_byte<0>(e)), t1 = bf16_pair<1>(u, scale_byte<1>(e)),
+                           t2 = bf16_pair<2>(u, scale_byte<2>(e)), t3 = bf16_pair<3>(u, scale_byte<3>(e));
+            v0[2 * x] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
+            v0[2 * x + 1] = __builtin_amdgcn_perm(t3, t2, 0x05040100u);
+            v1[2 * x] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
+            v1[2 * x + 1] = __builtin_amdgcn_perm(t3, t2, 0x07060302u);
+        }
+        st.o[2 * i] = mma_k<T>(a0, v0, st.o[2 * i]);
+        st.o[2 * i + 1] = mma_k<T>(a0, v1, st.o[2 * i + 1]);
+        st.o[2 * i] = mma_k<T>(a1, v0, st.o[2 * i]);
+        st.o[2 * i + 1] = mma_k<T>(a1, v1, st.o[2 * i + 1]);
+    }
+}
+/* The values of tokens from `valid` on as 0. */
+Q38_DEV void clear_tail(Page<Q38_KV_MX4> &p, int valid, int lane) {
+    const int n = min(max(valid - 4 * (lane >> 4), 0), 4);
+    const uint32_t bytes = n == 4 ? ~0u : (1u << (8 * n)) - 1u;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            p.v[s][w] &= bytes;
+            p.vs[s][w] &= bytes;
+        }
 }
 
 /* The new token's rows in LDS as they are stored: the key's elements in order
@@ -527,7 +624,8 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
     /* pages of a wave in registers: two 16-bit ones leave too few for the rest
      * (128K tokens 95 us against 85), 8-bit ones are half as large (1 / 2 / 3
      * pages: 49.9 / 47.5 / 48.8 us) */
-    constexpr int kDepth = T == Q38_KV_MX4 ? 3 : T == Q38_KV_Q8 ? 2 : 1;
+    constexpr int kDepth = T == Q38_KV_MX4 ? Q38_MX4_DEPTH : T == Q38_KV_Q8 ? 2 : 1;
+    constexpr int kPer = T == Q38_KV_MX4 ? 2 : 1; /* pages of a step */
     __shared__ q38_u32x4 q_frag[kQSets][8][64];
     __shared__ float q_unscale[8];
     __shared__ __attribute__((aligned(16))) std::conditional_t<T == Q38_KV_MX4, NewRowsMx4, NewRows> new_rows;
@@ -573,8 +671,8 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
     /* the wave's first pages: no load from here to the first score sits under
      * a branch, so the rows above are waited for alone and the pages come in
      * while the queries are formed */
-    Page<T> buf[kDepth];
-    load_page<T>(buf[0], a, first_page, wave < n_pages, j, lane);
+    Page<T> buf[kDepth][kPer];
+    load_page<T>(buf[0][0], a, first_page, wave < n_pages, j, lane);
     /* all of its page ids, the i-th in lane i: pages wave, wave + 8, ... (64 of
      * them cover the largest split) */
     const int my_pages = pt[min(wave + kWaves * lane, n_pages - 1)];
@@ -582,7 +680,7 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
         load_page<T>(p, a, __builtin_amdgcn_readlane(my_pages, (at / kWaves) & 63), at < n_pages, j, lane);
     };
 #pragma unroll
-    for (int u = 1; u < kDepth; ++u) fetch(buf[u], wave + kWaves * u);
+    for (int u = 1; u < kDepth * kPer; ++u) fetch(buf[u / kPer][u % kPer], wave + kWaves * u);
 
     if (kPre) {
         /* (every wave, so that the weights' load above stays before the pages':
@@ -658,26 +756,40 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
         for (int n = 0; n < 16; ++n) st.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
         /* the only ways out are the gotos: a page's loads are behind the same
          * number of younger ones on every path, and are waited for alone */
-        for (int i = wave;; i += kWaves * kDepth) {
+        for (int i = wave;; i += kWaves * kDepth * kPer) {
 #pragma unroll
             for (int u = 0; u < kDepth; ++u) {
-                const int at = i + kWaves * u;
+                const int at = i + kWaves * kPer * u;
                 if (at >= n_pages) goto done;
-                int valid = Q38_PAGE_TOKENS;
-                if (at == n_pages - 1) {
-                    valid = t_end - t_begin - Q38_PAGE_TOKENS * at;
-                    if (has_pos && a.k_new != nullptr) {
-                        if constexpr (T == Q38_KV_MX4)
-                            put_new_token(buf[u], new_rows, valid - 1, lane);
-                        else
-                            put_new_token<T>(buf[u], new_rows, valid - 1, lane);
-                    }
-                }
                 float *scores = nullptr;
                 if constexpr (kWeigh)
                     scores = sums.scores + (((size_t)g_split * (a.split_tokens >> 4) + at) * Q38_ATTN_KV_HEADS + j) * Q38_SCORES_PAGE;
-                page_step<T, kWeigh>(st, buf[u], q_frag, unscale, valid, at == wave, lane, scores);
-                fetch(buf[u], at + kWaves * kDepth);
+                if constexpr (T == Q38_KV_MX4) {
+                    int valid[2] = {Q38_PAGE_TOKENS, Q38_PAGE_TOKENS};
+                    if (at + kWaves >= n_pages - 1) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int page = at + kWaves * x;
+                            if (page >= n_pages) valid[x] = 0; /* (it was loaded as zeros) */
+                            if (page != n_pages - 1) continue;
+                            valid[x] = t_end - t_begin - Q38_PAGE_TOKENS * page;
+                            if (has_pos && a.k_new != nullptr) put_new_token(buf[u][x], new_rows, valid[x] - 1, lane);
+                            clear_tail(buf[u][x], valid[x], lane);
+                        }
+                    }
+                    pair_step<kWeigh>(st, buf[u], q_frag, valid[0], valid[1], at == wave, lane, scores,
+                                      scores + kWaves * Q38_ATTN_KV_HEADS * Q38_SCORES_PAGE);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) fetch(buf[u][x], at + kWaves * (kPer * kDepth + x));
+                } else {
+                    int valid = Q38_PAGE_TOKENS;
+                    if (at == n_pages - 1) {
+                        valid = t_end - t_begin - Q38_PAGE_TOKENS * at;
+                        if (has_pos && a.k_new != nullptr) put_new_token<T>(buf[u][0], new_rows, valid - 1, lane);
+                    }
+                    page_step<T, kWeigh>(st, buf[u][0], q_frag, unscale, valid, at == wave, lane, scores);
+                    fetch(buf[u][0], at + kWaves * kDepth);
+                }
             }
         }
     done:

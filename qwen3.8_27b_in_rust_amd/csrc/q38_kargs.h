@@ -660,18 +660,18 @@ typedef struct {
  * (n_splits, 4, n_groups), 512 threads, the columns' maximum (log2 units) and sum
  * over a split's positions; sums: grid (n_splits, 4), 512 threads. */
 #define Q38_OBSERVE_QUERIES 16
-#define Q38_OBSERVE_PAGES 2 /* of keys that a wave holds */
+#define Q38_OBSERVE_PAGES 4 /* of keys that a wave holds, or one (a short context) */
 #define Q38_OBSERVE_COLS (Q38_OBSERVE_QUERIES * Q38_ATTN_GROUP)
 typedef struct {
     const char *kpool; /* this layer's */
     float *weights;
     const int32_t *page_row; /* the sequence's page table */
     const float *q;          /* [n_tokens][24][256] */
-    float *part_ml;          /* [n_groups][4][n_splits][Q38_OBSERVE_COLS][2] */
+    float *part_ml;          /* [n_groups][4][Q38_OBSERVE_COLS][n_splits][2] */
     int32_t base_pos;
     int32_t n_tokens;
     int32_t split_pages;
-    int32_t n_splits;
+    int32_t n_splits; /* 64 at most */
     int32_t n_groups;
     int32_t pad_;
 } q38_observe_args;
