@@ -11,6 +11,7 @@ __graft_entry__.py), or call the library through any FFI directly.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 import struct
@@ -179,8 +180,14 @@ def _i32(seq) -> bytes:
     """Host integers as the int32 array that a call reads (and does not keep)."""
     try:
         return _PACK[len(seq)](*seq)
-    except (IndexError, struct.error):  # more of them, or values that convert to int
-        return bytes((c_int32 * len(seq))(*map(int, seq)))
+    except IndexError:  # more of them
+        try:
+            return array.array("i", seq).tobytes()
+        except (TypeError, OverflowError):
+            pass
+    except struct.error:
+        pass
+    return bytes((c_int32 * len(seq))(*map(int, seq)))  # values that convert to int
 
 
 class DeviceArray:

@@ -333,11 +333,10 @@ struct q38_kv {
     };
     std::vector<Images> images; /* [max_seqs][n_slots] */
     bool image_cache = true;
-    /* A tracking cache's sums of attention weights and own positions, [n_slots][max_pages][4][16] as the pages
-     * lie, and what each sequence has lost: */
+    /* A tracking cache's sums of attention weights and own positions, [n_slots][max_pages] x Q38_WEIGHTS_PAGE, and
+     * what each sequence has lost: */
     bool tracks = false;
     float *weights = nullptr;
-    int32_t *tokens = nullptr;
     struct Evicted {
         int32_t tokens = 0; /* so far: a position's row is that much further on */
         int32_t kept = 0;   /* by the last eviction: positions before are in no order */
@@ -345,6 +344,8 @@ struct q38_kv {
     std::vector<Evicted> evicted;
 
     size_t slot_sums() const { return (size_t)max_pages * Q38_WEIGHTS_PAGE; }
+    float *weights_of(int slot) const { return weights + (size_t)slot * slot_sums(); }
+    int32_t *tokens_of(int slot) const { return reinterpret_cast<int32_t *>(weights_of(slot)) + Q38_PAGE_TOKENS; }
     int32_t evicted_of(int seq) const { return tracks ? evicted[seq].tokens : 0; }
     void forget_evicted(int seq) {
         if (tracks) evicted[seq] = Evicted();
@@ -947,7 +948,6 @@ int q38_kv_destroy(q38_kv *kv) {
     (void)hipFree(kv->vpool);
     (void)hipFree(kv->d_page_table);
     (void)hipFree(kv->weights);
-    (void)hipFree(kv->tokens);
     (void)hipHostFree(kv->staging);
     delete kv;
     return 0;
@@ -1157,8 +1157,8 @@ int launch_weights(q38_kv *kv, int slot, bool to_pages, int n_seq, const int32_t
     for (int b = 0; b < n_seq;) {
         q38_kv_weights_args a;
         memset(&a, 0, sizeof(a));
-        a.weights = kv->weights + (size_t)slot * kv->slot_sums();
-        a.tokens = kv->tokens + (size_t)slot * kv->slot_sums();
+        a.weights = kv->weights_of(slot);
+        a.tokens = kv->tokens_of(slot);
         a.page_table = kv->d_page_table;
         a.weight_rows = d_weights != nullptr ? d_weights + row * Q38_ATTN_KV_HEADS : nullptr;
         a.token_rows = d_tokens != nullptr ? d_tokens + row * Q38_ATTN_KV_HEADS : nullptr;
@@ -1303,22 +1303,18 @@ int q38_kv_track_weights(q38_kv *kv, int enable) {
             if (kv->seq_live[s] && kv->evicted[s].tokens > 0) return fail("sequence %d has evicted tokens", s);
         Q38_HIP(hipStreamSynchronize(kv->ctx->stream));
         (void)hipFree(kv->weights);
-        (void)hipFree(kv->tokens);
         kv->weights = nullptr;
-        kv->tokens = nullptr;
         kv->tracks = false;
         return 0;
     }
     if (kv->type == 0) return fail("a cache of F32 rows tracks no weights: F16, BF16, Q8_K or MXFP4 rows do");
     const size_t bytes = kv->slot_sums() * kv->n_slots * sizeof(float);
-    if (hipMalloc(&kv->weights, bytes) != hipSuccess || hipMalloc(&kv->tokens, bytes) != hipSuccess) {
+    if (hipMalloc(&kv->weights, bytes) != hipSuccess) {
         (void)hipGetLastError();
-        (void)hipFree(kv->weights);
         kv->weights = nullptr;
-        return fail("cannot allocate %zu bytes for the sums of weights", 2 * bytes);
+        return fail("cannot allocate %zu bytes for the sums of weights", bytes);
     }
     Q38_HIP(hipMemsetAsync(kv->weights, 0, bytes, kv->ctx->stream));
-    Q38_HIP(hipMemsetAsync(kv->tokens, 0, bytes, kv->ctx->stream));
     kv->evicted.assign(kv->max_seqs, q38_kv::Evicted());
     kv->tracks = true;
     /* tokens that are there already */
@@ -1393,7 +1389,7 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     const size_t stats = (size_t)a.n_groups * Q38_ATTN_KV_HEADS * a.n_splits * Q38_OBSERVE_COLS * 2 * sizeof(float);
     if (ctx->ensure_work(stats)) return -1;
     a.kpool = reinterpret_cast<const char *>(kv->kslot(slot));
-    a.weights = kv->weights + (size_t)slot * kv->slot_sums();
+    a.weights = kv->weights_of(slot);
     a.page_row = kv->d_page_table + (size_t)seq * kv->pt_stride;
     a.q = d_q;
     a.part_ml = static_cast<float *>(ctx->work);
@@ -1438,8 +1434,8 @@ int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n
         memset(&a, 0, sizeof(a));
         a.kpool = reinterpret_cast<char *>(kv->kpool);
         a.vpool = reinterpret_cast<char *>(kv->vpool);
-        a.weights = kv->weights;
-        a.tokens = kv->tokens;
+        a.weights = kv->weights_of(0);
+        a.tokens = kv->tokens_of(0);
         a.page_table = kv->d_page_table;
         a.counts = static_cast<int32_t *>(ctx->work);
         a.moves = reinterpret_cast<int32_t *>(static_cast<char *>(ctx->work) + counts);
@@ -1723,8 +1719,8 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
         L->w.scores = scores;
         L->mw.scores = scores;
         L->mw.page_table = a.page_table;
-        L->mw.weights = kv->weights + (size_t)slot * kv->slot_sums();
-        L->mw.tokens = kv->tokens + (size_t)slot * kv->slot_sums();
+        L->mw.weights = kv->weights_of(slot);
+        L->mw.tokens = kv->tokens_of(slot);
         L->mw.pt_stride = kv->pt_stride;
         L->mw.split_tokens = split_tokens;
         L->mw.appended = d_k_new != nullptr ? 1 : 0;

@@ -305,7 +305,7 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[p][i] = q38_sum16(w[p][i]);
                 const int t0 = 16 * (page + kWaves * p) + 4 * g, end = min(a.base_pos + a.n_tokens, 16 * sp.end);
-                float *to = a.weights + (size_t)id[p] * Q38_WEIGHTS_PAGE + j * Q38_PAGE_TOKENS + 4 * g;
+                float *to = a.weights + (size_t)id[p] * Q38_WEIGHTS_PAGE + j * Q38_WEIGHTS_HEAD + 4 * g;
                 if (c == 0)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)

@@ -57,7 +57,7 @@ Q38_DEV void add_weights(const q38_merge_args &m, const q38_weigh_merge_args &a,
     const float *scores = a.scores + ((size_t)g * (a.split_tokens >> 4) * Q38_ATTN_KV_HEADS + j) * Q38_SCORES_PAGE;
     for (int t = 4 * tid; t < t_end - t_begin; t += 4 * 256) {
         const float *sc = scores + (size_t)(t >> 4) * Q38_ATTN_KV_HEADS * Q38_SCORES_PAGE + (t & 15);
-        const size_t at = (size_t)pt[t >> 4] * Q38_WEIGHTS_PAGE + j * Q38_PAGE_TOKENS + (t & 15);
+        const size_t at = (size_t)pt[t >> 4] * Q38_WEIGHTS_PAGE + j * Q38_WEIGHTS_HEAD + (t & 15);
         f32x4 s[kGroup];
 #pragma unroll
         for (int h = 0; h < kGroup; ++h) s[h] = q38_ld4(sc + h * Q38_PAGE_TOKENS);

@@ -2,6 +2,8 @@
  * The sums of attention weights of a tracking cache: in and out of its pages,
  * and the eviction of the tokens that have the least.
  */
+#include <type_traits>
+
 #include "q38_kv_types.h"
 
 namespace {
@@ -17,7 +19,7 @@ Q38_DEV void copy_weights(const q38_kv_weights_args &a) {
     const int first = a.pos0[b], n = a.row_base[b + 1] - a.row_base[b];
     const int lp = (first >> 4) + x - a.page_base[b], t = lane >> 2, j = lane & 3, p = lp * Q38_PAGE_TOKENS + t;
     if (p < first || p >= first + n) return;
-    const size_t at = (size_t)a.page_table[(size_t)a.seq[b] * a.pt_stride + lp] * Q38_WEIGHTS_PAGE + j * Q38_PAGE_TOKENS + t;
+    const size_t at = (size_t)a.page_table[(size_t)a.seq[b] * a.pt_stride + lp] * Q38_WEIGHTS_PAGE + j * Q38_WEIGHTS_HEAD + t;
     const size_t row = (size_t)(a.row_base[b] + p - first) * Q38_ATTN_KV_HEADS + j;
     if (a.to_pages) {
         a.weights[at] = a.weight_rows != nullptr ? a.weight_rows[row] : 0.0f;
@@ -39,171 +41,313 @@ Q38_DEV uint32_t rank_of(float w, int token, int first_recent) {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 
-/* Exclusive sum over the workgroup's threads, and the total. */
-Q38_DEV uint32_t scan(uint32_t x, uint32_t *lds, uint32_t &total) {
+/* Inclusive sum over the wave's lanes: within each row of 16, then a row's last
+ * lane to the row after it, then the lower half's last to the upper half. */
+template <int CTRL, int ROWS>
+Q38_DEV uint32_t moved(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false);
+}
+Q38_DEV uint32_t wave_sum_to(uint32_t x) {
+    x += moved<0x111, 0xF>(x); /* row_shr 1, 2, 4, 8 */
+    x += moved<0x112, 0xF>(x);
+    x += moved<0x114, 0xF>(x);
+    x += moved<0x118, 0xF>(x);
+    x += moved<0x142, 0xA>(x); /* row_bcast 15, 31 */
+    return x + moved<0x143, 0xC>(x);
+}
+/* Exclusive sum over the workgroup's threads. */
+Q38_DEV uint32_t scan(uint32_t x, uint32_t *lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t sum = x;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t y = __shfl_up(sum, d, 64);
-        if (lane >= d) sum += y;
-    }
+    const uint32_t sum = wave_sum_to(x);
     __syncthreads(); /* lds may still be read from the call before */
     if (lane == 63) lds[wave] = sum;
     __syncthreads();
     uint32_t before = 0;
-    total = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        const uint32_t y = lds[w];
-        before += w < wave ? y : 0;
-        total += y;
-    }
+    for (int w = 0; w < kWaves; ++w) before += w < wave ? lds[w] : 0;
     return before + sum - x;
 }
 
+/* The same for kRounds values of each thread, all of a round before the next's:
+ * x becomes the exclusive sums, and the total is returned.  (rounds: those that hold
+ * anything but 0.) */
+constexpr int kRounds = 8;
+Q38_DEV uint32_t scan_rounds(uint32_t (&x)[kRounds], int rounds, uint32_t *lds) {
+    static_assert(kRounds * kWaves == 128, "two a lane");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t sum[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) sum[r] = r < rounds ? wave_sum_to(x[r]) : 0;
+    __syncthreads();
+    if (lane == 63)
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) lds[r * kWaves + wave] = sum[r];
+    __syncthreads();
+    if (wave == 0) {
+        const uint32_t a = lds[2 * lane], b = lds[2 * lane + 1], to = wave_sum_to(a + b);
+        lds[2 * lane] = to - a - b;
+        lds[2 * lane + 1] = to - b;
+        if (lane == 63) lds[128] = to;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) x[r] = lds[r * kWaves + wave] + sum[r] - x[r];
+    return lds[128];
+}
+
 /* The n_keep ranks that stay of n: the n_keep-th largest found digit by digit
- * (eight bits a pass over the sums), then in one more pass which tokens those are --
- * all above it, and of those that equal it the first -- and where the holes below
- * n_keep and the tokens that fill them lie.  A thread has a page's 16 tokens. */
+ * (11, 11 and 10 bits, so that weights of one size spread over the bins), then in
+ * one more pass which tokens those are -- all above it, and of those that equal it
+ * the first -- and where the holes below n_keep and the tokens that fill them lie.
+ * A block of 32768 tokens at a time, kRounds of four tokens to a thread (a page to
+ * four of them: a thread a page read a line each, 64 to an instruction, and took
+ * 32 us where this takes KSELECT); the first block's ranks stay in registers, a longer
+ * context's others are formed again for each pass.  After the first digit few ranks
+ * are left as a rule: up to kList of them are put together in LDS for the other two.
+ * Tokens past the last one have rank 0, which none is below, and come after every
+ * other of rank 0. */
+constexpr int kBins = 2048, kList = 8192, kBlock = 4 * kRounds * kThreads;
+typedef uint32_t Ranks[kRounds][4];
 Q38_DEV void select(const q38_evict_args &a) {
-    __shared__ uint32_t hist[kWaves][256];
-    __shared__ uint32_t lds[kWaves], found[2];
-    const int x = blockIdx.x, b = blockIdx.y, slot = x >> 2, j = x & 3, tid = threadIdx.x, wave = tid >> 6;
+    __shared__ uint32_t hist[kBins], list[kList];
+    __shared__ uint32_t lds[kRounds * kWaves + 1], found[4], listed;
+    const int x = blockIdx.x, b = blockIdx.y, slot = x >> 2, j = x & 3, tid = threadIdx.x;
     const int n = a.n_tokens[b], keep = a.n_keep[b], recent = a.first_recent[b], pages = (n + 15) >> 4;
-    if (keep >= n) {
+    if (keep >= n || keep == 0) {
         if (tid == 0) a.counts[(size_t)b * gridDim.x + x] = 0;
         return;
     }
     const int32_t *pt = a.page_table + (size_t)a.seq[b] * a.pt_stride;
-    const float *weights = a.weights + (size_t)slot * a.slot_weights + j * Q38_PAGE_TOKENS;
-    const int32_t *tokens = a.tokens + (size_t)slot * a.slot_weights + j * Q38_PAGE_TOKENS;
-    auto load = [&](int page, uint32_t (&rank)[16]) {
-        const size_t at = (size_t)pt[page] * Q38_WEIGHTS_PAGE;
+    const float *weights = a.weights + (size_t)slot * a.slot_weights + j * Q38_WEIGHTS_HEAD;
+    const int32_t *tokens = a.tokens + (size_t)slot * a.slot_weights + j * Q38_WEIGHTS_HEAD;
+    auto first_of = [&](int block, int r) { return block * kBlock + 4 * (r * kThreads + tid); }; /* a thread's four tokens */
+    auto rounds_of = [&](int block) { return min((n - block * kBlock + 4 * kThreads - 1) / (4 * kThreads), kRounds); };
+    auto load = [&](int block, Ranks &rank) {
+        size_t at[kRounds];
+        const int rounds = rounds_of(block);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4 w = q38_ld4(weights + at + 4 * i);
-            const q38_i32x4 t = *reinterpret_cast<const q38_i32x4 *>(tokens + at + 4 * i);
+        for (int r = 0; r < kRounds; ++r) {
+            const int t = first_of(block, r);
+            if (r < rounds) at[r] = (size_t)pt[min(t >> 4, pages - 1)] * Q38_WEIGHTS_PAGE + (t & 15);
+        }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) rank[4 * i + e] = rank_of(w[e], t[e], recent);
+        for (int r = 0; r < kRounds; ++r) {
+            if (r >= rounds) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) rank[r][e] = 0;
+                continue;
+            }
+            const f32x4 w = q38_ld4(weights + at[r]);
+            const q38_i32x4 own = *reinterpret_cast<const q38_i32x4 *>(tokens + at[r]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rank[r][e] = first_of(block, r) + e < n ? rank_of(w[e], own[e], recent) : 0;
+        }
+    };
+    Ranks held;
+    load(0, held);
+    auto each = [&](auto use) {
+        use(0, held);
+        for (int block = 1; block * kBlock < n; ++block) {
+            Ranks rank;
+            load(block, rank);
+            use(block, rank);
         }
     };
     uint32_t prefix = 0, left = (uint32_t)keep; /* the largest digits so far, and ranks to take among those that share them */
-    for (int shift = 24; keep > 0 && shift >= 0; shift -= 8) {
-        for (int i = tid; i < kWaves * 256; i += kThreads) (&hist[0][0])[i] = 0;
+    uint32_t known = 0;                         /* their bits */
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digit = pass == 2 ? 1023u : 2047u;
+        for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+        if (pass == 1 && tid == 0) listed = 0;
         __syncthreads();
-        for (int page = tid; page < pages; page += kThreads) {
-            uint32_t rank[16];
-            load(page, rank);
+        /* every rank that has a token, and that shares the digits known so far */
+        auto ranks = [&](auto use) {
+            each([&](int block, const Ranks &rank) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (16 * page + i < n && (shift == 24 || rank[i] >> (shift + 8) == prefix >> (shift + 8)))
-                    atomicAdd(&hist[wave][(rank[i] >> shift) & 255u], 1u);
+                for (int r = 0; r < kRounds; ++r)
+                    if (first_of(block, r) < n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (pass == 0 || (rank[r][e] & known) == prefix) use(rank[r][e]);
+            });
+        };
+        if (pass == 0 || found[2] > kList) {
+            ranks([&](uint32_t rank) { atomicAdd(&hist[(rank >> shift) & digit], 1u); });
+        } else {
+            if (pass == 1) {
+                /* a wave's at once (one by one took 2.5 us longer) */
+                uint32_t mine = 0;
+                ranks([&](uint32_t) { ++mine; });
+                const uint32_t to = wave_sum_to(mine);
+                uint32_t at = 0;
+                if ((tid & 63) == 63) at = atomicAdd(&listed, to);
+                at = __builtin_amdgcn_readlane(at, 63) + to - mine;
+                ranks([&](uint32_t rank) { list[at++] = rank; });
+                __syncthreads();
+            }
+            for (uint32_t i = tid; i < listed; i += kThreads)
+                if ((list[i] & known) == prefix) atomicAdd(&hist[(list[i] >> shift) & digit], 1u);
         }
         __syncthreads();
-        /* thread d: how many have digit 255 - d */
-        uint32_t count = 0, total;
-        if (tid < 256)
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) count += hist[w][255 - tid];
-        const uint32_t above = scan(count, lds, total);
-        if (tid < 256 && above < left && above + count >= left) {
-            found[0] = 255 - tid;
-            found[1] = left - above;
+        /* thread t: the bins kBins - 1 - 2 t and the one below it */
+        const uint32_t c0 = hist[kBins - 1 - 2 * tid], c1 = hist[kBins - 2 - 2 * tid];
+        const uint32_t above = scan(c0 + c1, lds);
+        if (above < left && above + c0 + c1 >= left) {
+            const bool upper = above + c0 >= left;
+            found[0] = kBins - (upper ? 1 : 2) - 2 * tid;
+            found[1] = left - above - (upper ? 0 : c0);
+            if (pass == 0) found[2] = upper ? c0 : c1; /* ranks that share the first digit, */
+            if (pass == 2) found[3] = upper ? c0 : c1; /* and all */
         }
         __syncthreads();
         prefix |= found[0] << shift;
+        known |= digit << shift;
         left = found[1];
     }
     /* prefix: the smallest rank that stays; left of those that equal it do */
     int32_t *holes = a.moves + ((size_t)b * gridDim.x + x) * 2 * a.max_moves, *sources = holes + a.max_moves;
+    const bool some = left < found[3];
     uint32_t equal_before = 0, holes_before = 0, sources_before = 0;
-    for (int page0 = 0; page0 < pages; page0 += kThreads) {
-        const int page = page0 + tid;
-        uint32_t above = 0, equal = 0, total;
-        if (page < pages) {
-            uint32_t rank[16];
-            load(page, rank);
+    each([&](int block, const Ranks &rank) {
+        uint32_t stays[kRounds], count[kRounds];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const bool in = 16 * page + i < n && keep > 0;
-                above |= (in && rank[i] > prefix ? 1u : 0u) << i;
-                equal |= (in && rank[i] == prefix ? 1u : 0u) << i;
+        for (int r = 0; r < kRounds; ++r) {
+            stays[r] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) stays[r] |= (rank[r][e] >= prefix ? 1u : 0u) << e;
+        }
+        if (some) { /* not all that equal it stay: the first ones do */
+            uint32_t equal[kRounds];
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                equal[r] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) equal[r] |= (rank[r][e] == prefix ? 1u : 0u) << e;
+                count[r] = __popc(equal[r]);
+            }
+            const uint32_t total = scan_rounds(count, rounds_of(block), lds);
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                uint32_t at = equal_before + count[r];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (equal[r] >> e & 1u) {
+                        if (at >= left) stays[r] &= ~(1u << e);
+                        ++at;
+                    }
+            }
+            equal_before += total;
+        }
+        /* holes below n_keep and tokens that stay from there on, 32768 of either at most */
+        uint32_t holes_of[kRounds];
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            const int t = first_of(block, r);
+            const uint32_t low = (1u << min(max(keep - t, 0), 4)) - 1u, in = (1u << min(max(n - t, 0), 4)) - 1u;
+            holes_of[r] = ~stays[r] & low;
+            stays[r] &= in & ~low;
+            count[r] = __popc(holes_of[r]) | __popc(stays[r]) << 16;
+        }
+        const uint32_t total = scan_rounds(count, rounds_of(block), lds);
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            /* a token is in the one list or in the other, by its side of n_keep: four are on one side but where
+             * n_keep lies among them */
+            const int t = first_of(block, r);
+            int32_t *h = holes + holes_before + (count[r] & 0xFFFFu), *f = sources + sources_before + (count[r] >> 16);
+            int32_t *out = t < keep ? h : f;
+            const uint32_t listed_here = holes_of[r] | stays[r];
+            if (__ballot(listed_here != 0) == 0) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (t + e == keep) out = f;
+                if (listed_here >> e & 1u) *out++ = t + e;
             }
         }
-        uint32_t rest = equal_before + scan((uint32_t)__popc(equal), lds, total);
-        equal_before += total;
-        uint32_t stays = above;
-        for (uint32_t e = equal; e != 0 && rest < left; ++rest, e &= e - 1) stays |= e & (0u - e);
-        const int below = min(max(keep - 16 * page, 0), 16), count = min(max(n - 16 * page, 0), 16);
-        const uint32_t low = (1u << below) - 1u, all = (1u << count) - 1u;
-        uint32_t hole = ~stays & low & all, source = stays & ~low & all;
-        const uint32_t h = scan((uint32_t)__popc(hole), lds, total);
-        int at = (int)(holes_before + h);
-        holes_before += total;
-        for (; hole != 0; hole &= hole - 1) holes[at++] = 16 * page + __builtin_ctz(hole);
-        const uint32_t s = scan((uint32_t)__popc(source), lds, total);
-        at = (int)(sources_before + s);
-        sources_before += total;
-        for (; source != 0; source &= source - 1) sources[at++] = 16 * page + __builtin_ctz(source);
-    }
+        holes_before += total & 0xFFFFu;
+        sources_before += total >> 16;
+    });
     if (tid == 0) a.counts[(size_t)b * gridDim.x + x] = (int32_t)holes_before;
 }
 
-/* A row of one kv head from one place to another: a wave.  K moves in its 16-byte
- * pieces, V in the units that hold one token's values alone. */
+/* A row of one kv head on its way: what a wave's lane holds of it.  K goes in its
+ * 16-byte pieces, V in the units that hold one token's values alone. */
 template <int T>
-Q38_DEV void move_row(const char *from, int t0, char *to, int t1, bool key, int head, int lane) {
-    if (key) {
-        constexpr int kPieces = T == Q38_KV_MX4 ? 8 : T == Q38_KV_Q8 ? 16 : 32;
-        if (lane < kPieces)
-            reinterpret_cast<q38_u32x4 *>(to)[lane * 16 + t1] = reinterpret_cast<const q38_u32x4 *>(from)[lane * 16 + t0];
-    } else {
+struct Row {
+    static constexpr int kPieces = T == Q38_KV_MX4 ? 8 : T == Q38_KV_Q8 ? 16 : 32;
+    static constexpr int kUnits = T == Q38_KV_MX4 ? 2 : 4; /* of V, a lane */
+    typedef std::conditional_t<T == Q38_KV_F16 || T == Q38_KV_BF16, uint16_t, uint8_t> Unit;
+    q38_u32x4 k;
+    Unit v[kUnits];
+    uint32_t scale; /* lane 0 K's and lane 1 V's of 8-bit rows; of 4-bit ones lanes 0 .. 7 and 8 .. 15 */
+
+    static Q38_DEV int unit(int i, int t, int lane) {
+        if (T == Q38_KV_MX4) {
+            const int u = 64 * i + lane;
+            return q38_v_index<T>(t, (u >> 4) * 32 + (u & 15)) >> 1;
+        }
+        return q38_v_index<T>(t, 64 * i + lane);
+    }
+    Q38_DEV void load(char *kb, char *vb, int t, int head, int lane) {
+        k = reinterpret_cast<const q38_u32x4 *>(kb)[min(lane, kPieces - 1) * 16 + t];
 #pragma unroll
-        for (int i = 0; i < (T == Q38_KV_MX4 ? 2 : 4); ++i) {
-            if constexpr (T == Q38_KV_MX4) {
-                const int u = 64 * i + lane, d = (u >> 4) * 32 + (u & 15);
-                to[q38_v_index<T>(t1, d) >> 1] = from[q38_v_index<T>(t0, d) >> 1];
-            } else if constexpr (T == Q38_KV_Q8) {
-                to[q38_v_index<T>(t1, 64 * i + lane)] = from[q38_v_index<T>(t0, 64 * i + lane)];
-            } else {
-                reinterpret_cast<uint16_t *>(to)[q38_v_index<T>(t1, 64 * i + lane)] =
-                    reinterpret_cast<const uint16_t *>(from)[q38_v_index<T>(t0, 64 * i + lane)];
-            }
+        for (int i = 0; i < kUnits; ++i) v[i] = reinterpret_cast<const Unit *>(vb)[unit(i, t, lane)];
+        if constexpr (T == Q38_KV_Q8) scale = __float_as_uint(q38_kv_scales(lane & 1 ? vb : kb, head)[t]);
+        if constexpr (T == Q38_KV_MX4)
+            scale = lane & 8 ? q38_mx4_scales(vb, head)[q38_mx4_v_scale(t, 32 * (lane & 7))] : q38_mx4_scales(kb, head)[q38_mx4_k_scale(t, 32 * (lane & 7))];
+    }
+    Q38_DEV void store(char *kb, char *vb, int t, int head, int lane) const {
+        if (lane < kPieces) reinterpret_cast<q38_u32x4 *>(kb)[lane * 16 + t] = k;
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) reinterpret_cast<Unit *>(vb)[unit(i, t, lane)] = v[i];
+        if constexpr (T == Q38_KV_Q8) {
+            if (lane < 2) q38_kv_scales(lane & 1 ? vb : kb, head)[t] = __uint_as_float(scale);
+        }
+        if constexpr (T == Q38_KV_MX4) {
+            if (lane < 8) q38_mx4_scales(kb, head)[q38_mx4_k_scale(t, 32 * lane)] = (uint8_t)scale;
+            else if (lane < 16) q38_mx4_scales(vb, head)[q38_mx4_v_scale(t, 32 * (lane & 7))] = (uint8_t)scale;
         }
     }
-    if constexpr (T == Q38_KV_Q8) {
-        if (lane == 0) q38_kv_scales(to, head)[t1] = q38_kv_scales(const_cast<char *>(from), head)[t0];
-    }
-    if constexpr (T == Q38_KV_MX4) {
-        const uint8_t *s = q38_mx4_scales(const_cast<char *>(from), head);
-        uint8_t *r = q38_mx4_scales(to, head);
-        if (lane < 8)
-            r[key ? q38_mx4_k_scale(t1, 32 * lane) : q38_mx4_v_scale(t1, 32 * lane)] =
-                s[key ? q38_mx4_k_scale(t0, 32 * lane) : q38_mx4_v_scale(t0, 32 * lane)];
-    }
-}
+};
 
 /* Holes lie below n_keep and the rows that fill them from there on: no row is read
- * that another move writes, so the moves run in any order, in place. */
+ * that another move writes, so the moves run in any order, in place.  A wave has
+ * kRows of them in flight. */
+constexpr int kRows = Q38_EVICT_ROWS / 4;
 template <int T>
 Q38_DEV void move_rows(const q38_evict_args &a) {
     const int x = blockIdx.y, b = blockIdx.z, slot = x >> 2, j = x & 3;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int count = a.counts[(size_t)b * gridDim.y + x], begin = blockIdx.x * Q38_EVICT_ROWS;
-    const int32_t *holes = a.moves + ((size_t)b * gridDim.y + x) * 2 * a.max_moves, *sources = holes + a.max_moves;
+    const int begin = blockIdx.x * Q38_EVICT_ROWS + kRows * wave;
+    const int count = min(a.counts[(size_t)b * gridDim.y + x] - begin, kRows);
+    if (count <= 0) return;
+    const int32_t *holes = a.moves + ((size_t)b * gridDim.y + x) * 2 * a.max_moves + begin, *sources = holes + a.max_moves;
     const int32_t *pt = a.page_table + (size_t)a.seq[b] * a.pt_stride;
     char *k = a.kpool + (size_t)slot * a.slot_bytes, *v = a.vpool + (size_t)slot * a.slot_bytes;
-    for (int i = begin + wave; i < min(begin + Q38_EVICT_ROWS, count); i += 4) {
-        const int p1 = holes[i], p0 = sources[i], g0 = pt[p0 >> 4], g1 = pt[p1 >> 4], t0 = p0 & 15, t1 = p1 & 15;
-        move_row<T>(q38_kv_block<T>(k, g0, j), t0, q38_kv_block<T>(k, g1, j), t1, true, j, lane);
-        move_row<T>(q38_kv_block<T>(v, g0, j), t0, q38_kv_block<T>(v, g1, j), t1, false, j, lane);
-        if (lane == 0) {
-            const size_t from = (size_t)slot * a.slot_weights + (size_t)g0 * Q38_WEIGHTS_PAGE + j * Q38_PAGE_TOKENS + t0;
-            const size_t to = (size_t)slot * a.slot_weights + (size_t)g1 * Q38_WEIGHTS_PAGE + j * Q38_PAGE_TOKENS + t1;
-            a.weights[to] = a.weights[from];
-            a.tokens[to] = a.tokens[from];
-        }
+    /* lane i: move i's place, lane 32 + i its source (past the last move the last one again) */
+    const int i = min(lane & 31, count - 1);
+    const int p = (lane & 32 ? sources : holes)[i], page = pt[p >> 4];
+    const size_t sum = (size_t)slot * a.slot_weights + (size_t)page * Q38_WEIGHTS_PAGE + j * Q38_WEIGHTS_HEAD + (p & 15);
+    const float weight = a.weights[sum];
+    const int token = a.tokens[sum];
+    Row<T> row[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        const int from = __builtin_amdgcn_readlane(page, 32 + r), t = __builtin_amdgcn_readlane(p, 32 + r) & 15;
+        row[r].load(q38_kv_block<T>(k, from, j), q38_kv_block<T>(v, from, j), t, j, lane);
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        if (r >= count) break;
+        const int to = __builtin_amdgcn_readlane(page, r), t = __builtin_amdgcn_readlane(p, r) & 15;
+        row[r].store(q38_kv_block<T>(k, to, j), q38_kv_block<T>(v, to, j), t, j, lane);
+    }
+    const float w = __shfl(weight, 32 + (lane & 31), 64);
+    const int tok = __shfl(token, 32 + (lane & 31), 64);
+    if (lane < count) {
+        a.weights[sum] = w;
+        a.tokens[sum] = tok;
     }
 }
 

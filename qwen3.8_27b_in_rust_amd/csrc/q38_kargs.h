@@ -580,10 +580,11 @@ typedef struct {
 
 /* ------------------------------------------------ sums of attention weights */
 
-/* A tracking cache keeps, beside each page of a slot, the sum of the softmax
- * weights that its tokens were given and the tokens' own positions:
- * [max_pages][4 kv heads][16 tokens], f32 and int32. */
-#define Q38_WEIGHTS_PAGE (Q38_ATTN_KV_HEADS * Q38_PAGE_TOKENS)
+/* A tracking cache keeps, for each page of a slot and kv head, the sums of the
+ * softmax weights that its 16 tokens were given (f32) and after them the tokens' own
+ * positions (int32): a cache line, as the eviction's choice reads both. */
+#define Q38_WEIGHTS_HEAD (2 * Q38_PAGE_TOKENS)
+#define Q38_WEIGHTS_PAGE (Q38_ATTN_KV_HEADS * Q38_WEIGHTS_HEAD)
 
 /* What a decode launch over such a cache takes beside q38_decode_typed_args.  The
  * scores (log2 units) of split g's page p, kv head j: at ((g * split_tokens / 16 +
@@ -601,7 +602,7 @@ typedef struct {
     const float *scores;
     const int32_t *page_table;
     float *weights;  /* this layer's sums */
-    int32_t *tokens; /* and own positions */
+    int32_t *tokens; /* and own positions: the same lines, past the sums */
     int32_t pt_stride;
     int32_t split_tokens;
     int32_t appended; /* the call stored a row at pos[b]: its sum starts here */
@@ -640,7 +641,7 @@ typedef struct {
 typedef struct {
     char *kpool;
     char *vpool;
-    float *weights;  /* every slot's: [n_slots][max_pages][4][16] */
+    float *weights;  /* every slot's: [n_slots][max_pages] x Q38_WEIGHTS_PAGE */
     int32_t *tokens;
     const int32_t *page_table;
     int32_t *moves;
