@@ -1384,7 +1384,9 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     const int slots = std::min(std::max(ctx->cu_count / Q38_ATTN_KV_HEADS, 1), 64);
     const int few = pages < slots * Q38_DECODE_TYPED_WAVES * Q38_OBSERVE_PAGES ? 1 : 0;
     const int step = Q38_DECODE_TYPED_WAVES * (few ? 1 : Q38_OBSERVE_PAGES);
-    a.split_pages = ((pages + slots - 1) / slots + step - 1) / step * step;
+    auto split_for = [&](int wanted) { return ((pages + wanted - 1) / wanted + step - 1) / step * step; };
+    /* the statistics of all groups at once */
+    a.split_pages = split_for(std::max(slots / a.n_groups, 1));
     a.n_splits = (pages + a.split_pages - 1) / a.split_pages;
     const size_t stats = (size_t)a.n_groups * Q38_ATTN_KV_HEADS * a.n_splits * Q38_OBSERVE_COLS * 2 * sizeof(float);
     if (ctx->ensure_work(stats)) return -1;
@@ -1397,7 +1399,8 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     a.n_tokens = n_tokens;
     const unsigned block = 64 * Q38_DECODE_TYPED_WAVES;
     if (ctx->launch(ctx->f_observe_stats[kv->type][few], a.n_splits, Q38_ATTN_KV_HEADS, a.n_groups, block, &a)) return -1;
-    return ctx->launch(ctx->f_observe_sums[kv->type][few], a.n_splits, Q38_ATTN_KV_HEADS, 1, block, &a);
+    a.split_pages = split_for(slots);
+    return ctx->launch(ctx->f_observe_sums[kv->type][few], (pages + a.split_pages - 1) / a.split_pages, Q38_ATTN_KV_HEADS, 1, block, &a);
 }
 
 int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n_tokens, const int32_t *n_keep,

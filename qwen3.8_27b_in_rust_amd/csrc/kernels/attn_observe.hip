@@ -28,9 +28,13 @@ constexpr int kTiles = Q38_OBSERVE_COLS / 16;
 constexpr int kParts = 2;
 static_assert(kTiles * 16 == Q38_OBSERVE_COLS, "whole tiles");
 
+/* A step's operand of a tile, its four groups of 16 lanes 16 bytes further apart than
+ * they are long: a wave stores one column of every step and group at once, which
+ * would all lie in two banks. */
+typedef q38_u32x4 Step[4][17];
 template <int T>
 struct Queries {
-    q38_u32x4 part[kTiles][kParts][8][64];
+    Step part[kTiles][kParts][8];
     float unscale[Q38_OBSERVE_COLS];
 };
 
@@ -76,7 +80,7 @@ Q38_DEV void load_queries(Queries<T> &q, const q38_observe_args &a, int group, i
         }
 #pragma unroll
         for (int k = 0; k < kParts; ++k)
-            *(reinterpret_cast<q38_u32x2 *>(&q.part[col >> 4][k][i][16 * g + (col & 15)]) + ((d >> 2) & 1)) =
+            *(reinterpret_cast<q38_u32x2 *>(&q.part[col >> 4][k][i][g][col & 15]) + ((d >> 2) & 1)) =
                 q38_u32x2{pack16(p[k][0], p[k][1]), pack16(p[k][2], p[k][3])};
     }
 }
@@ -119,29 +123,38 @@ Q38_DEV void load_keys(Keys &k, const char *kpool, int page, int j, int lane) {
     }
 }
 
-/* Scores (log2 units) of kPages pages against a tile's 16 columns. */
+/* Scores (log2 units) less `base` of kPages pages against a tile's 16 columns.
+ * bf16 operands: both parts' products go into one sum that starts at -base. */
 template <int T, int kPages>
-Q38_DEV void scores_of(const Keys (&k)[kPages], const q38_u32x4 (*part)[8][64], float unscale, int lane, float (&s)[kPages][4]) {
+Q38_DEV void scores_of(const Keys (&k)[kPages], const Step (*part)[8], float unscale, float base, int lane, float (&s)[kPages][4]) {
     /* (an index that the compiler cannot see through: it would keep the parts of
      * all tiles in registers over the loop of pages) */
     asm volatile("" : "+v"(lane));
-    f32x4 c[kPages][2];
+    constexpr int kSums = kInBf16<T> ? 1 : 2;
+    const float first = kInBf16<T> ? -base : 0.0f;
+    f32x4 c[kPages][kSums];
 #pragma unroll
-    for (int p = 0; p < kPages; ++p) c[p][0] = c[p][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < kPages; ++p)
+#pragma unroll
+        for (int n = 0; n < kSums; ++n) c[p][n] = f32x4{first, first, first, first};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int n = 0; n < kParts; ++n) {
-            const q38_u32x4 q = part[n][i][lane];
+            const q38_u32x4 q = part[n][i][0][lane + (lane >> 4)];
 #pragma unroll
-            for (int p = 0; p < kPages; ++p) c[p][n > 0] = mma_k<T>(k[p].a[i], q, c[p][n > 0]);
+            for (int p = 0; p < kPages; ++p) c[p][n % kSums] = mma_k<T>(k[p].a[i], q, c[p][n % kSums]);
         }
 #pragma unroll
     for (int p = 0; p < kPages; ++p)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            s[p][i] = kInBf16<T> ? c[p][0][i] + c[p][1][i] : __builtin_fmaf(c[p][1][i], 1.0f / kLowUnit<T>, c[p][0][i]) * unscale;
-            if (T == Q38_KV_Q8) s[p][i] *= k[p].scale[i];
+            if constexpr (kInBf16<T>) {
+                s[p][i] = c[p][0][i];
+            } else {
+                const float x = __builtin_fmaf(c[p][kSums - 1][i], 1.0f / kLowUnit<T>, c[p][0][i]);
+                s[p][i] = __builtin_fmaf(x, T == Q38_KV_Q8 ? unscale * k[p].scale[i] : unscale, -base);
+            }
         }
 }
 
@@ -199,20 +212,31 @@ Q38_DEV void observe_stats(const q38_observe_args &a) {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
             if (t >= tiles) continue;
+            /* against the column's reference so far, which is raised, as the decode's is, once a score passes it by
+             * kRefSlack */
             float s[kPages][4];
-            scores_of<T>(k, q.part[t], unscale[t], lane, s);
+            const bool none = M[t] == -INFINITY;
+            const float base = none ? 0.0f : M[t];
+            scores_of<T>(k, q.part[t], unscale[t], base, lane, s);
             if (masks) mask(s, page, min(last[t], 16 * sp.end - 1), g);
-            float top = M[t];
+            float top = -INFINITY;
 #pragma unroll
             for (int p = 0; p < kPages; ++p) top = fmaxf(top, fmaxf(fmaxf(s[p][0], s[p][1]), fmaxf(s[p][2], s[p][3])));
-            const float ref = top == -INFINITY ? 0.0f : top;
-            float sum = L[t] * q38_exp2(M[t] - ref);
+            if (__any(top > (none ? -INFINITY : kRefSlack))) {
+                const float by = none ? (top == -INFINITY ? 0.0f : top) : fmaxf(top, 0.0f);
+                if (!none || top != -INFINITY) M[t] = base + by;
+                L[t] *= q38_exp2(-by); /* (nothing where there is no reference yet) */
+#pragma unroll
+                for (int p = 0; p < kPages; ++p)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[p][i] -= by;
+            }
+            float sum = 0.0f;
 #pragma unroll
             for (int p = 0; p < kPages; ++p)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum += q38_exp2(s[p][i] - ref);
-            M[t] = top;
-            L[t] = sum;
+                for (int i = 0; i < 4; ++i) sum += q38_exp2(s[p][i]);
+            L[t] += sum;
         }
     }
 #pragma unroll
@@ -274,12 +298,8 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
         __syncthreads();
         for (int page = sp.begin + wave; page < sp.end; page += kWaves * kPages) {
             Keys k[kPages];
-            int id[kPages];
 #pragma unroll
-            for (int p = 0; p < kPages; ++p) {
-                id[p] = a.page_row[min(page + kWaves * p, sp.end - 1)];
-                load_keys<T>(k[p], a.kpool, id[p], j, lane);
-            }
+            for (int p = 0; p < kPages; ++p) load_keys<T>(k[p], a.kpool, a.page_row[min(page + kWaves * p, sp.end - 1)], j, lane);
             const bool masks = page + kWaves * (kPages - 1) >= sp.end || 16 * (page + kWaves * (kPages - 1)) + 15 > a.base_pos + u0;
             float w[kPages][4] = {};
 #pragma unroll
@@ -289,27 +309,38 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
                 /* (read from LDS for each set of pages: six tiles' are too many registers) */
                 int col = 16 * t + c;
                 asm volatile("" : "+v"(col));
-                scores_of<T>(k, q.part[t], q.unscale[col], lane, s);
+                scores_of<T>(k, q.part[t], q.unscale[col], stat[col][0], lane, s);
                 if (masks) {
                     const int u = u0 + col / kGroup;
                     mask(s, page, min(u < a.n_tokens ? a.base_pos + u : -1, 16 * sp.end - 1), g);
                 }
-                const float M = stat[col][0], inverse = stat[col][1];
+                const float inverse = stat[col][1];
 #pragma unroll
                 for (int p = 0; p < kPages; ++p)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[p][i] = __builtin_fmaf(q38_exp2(s[p][i] - M), inverse, w[p][i]);
+                    for (int i = 0; i < 4; ++i) w[p][i] = __builtin_fmaf(q38_exp2(s[p][i]), inverse, w[p][i]);
             }
 #pragma unroll
             for (int p = 0; p < kPages; ++p) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[p][i] = q38_sum16(w[p][i]);
-                const int t0 = 16 * (page + kWaves * p) + 4 * g, end = min(a.base_pos + a.n_tokens, 16 * sp.end);
-                float *to = a.weights + (size_t)id[p] * Q38_WEIGHTS_PAGE + j * Q38_WEIGHTS_HEAD + 4 * g;
-                if (c == 0)
+            }
+            /* lane 16 g + p adds page p's tokens 4 g .. + 3 (all at once: one after the other each waits for its sum) */
+            f32x4 add = {w[0][0], w[0][1], w[0][2], w[0][3]};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (t0 + i < end) to[i] += w[p][i];
+            for (int p = 1; p < kPages; ++p)
+                if (c == p) add = f32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
+            const int t0 = 16 * (page + kWaves * c) + 4 * g, end = min(a.base_pos + a.n_tokens, 16 * sp.end);
+            if (c < kPages && t0 < end) {
+                float *sums = a.weights + (size_t)a.page_row[page + kWaves * c] * Q38_WEIGHTS_PAGE + j * Q38_WEIGHTS_HEAD + 4 * g;
+                const f32x4 now = q38_ld4(sums) + add;
+                if (t0 + 4 <= end) {
+                    q38_st4(sums, now);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                        if (t0 + i < end) sums[i] = now[i];
+                }
             }
         }
     }

@@ -101,7 +101,7 @@ Q38_DEV uint32_t scan_rounds(uint32_t (&x)[kRounds], int rounds, uint32_t *lds) 
  * the first -- and where the holes below n_keep and the tokens that fill them lie.
  * A block of 32768 tokens at a time, kRounds of four tokens to a thread (a page to
  * four of them: a thread a page read a line each, 64 to an instruction, and took
- * 32 us where this takes KSELECT); the first block's ranks stay in registers, a longer
+ * 32 us of 32K tokens where this takes 22); the first block's ranks stay in registers, a longer
  * context's others are formed again for each pass.  After the first digit few ranks
  * are left as a rule: up to kList of them are put together in LDS for the other two.
  * Tokens past the last one have rank 0, which none is below, and come after every

@@ -659,7 +659,8 @@ typedef struct {
 /* Weights that queries of a prompt give: columns are (query, head of the group)
  * of one kv head, Q38_OBSERVE_QUERIES queries a group.  Statistics: grid
  * (n_splits, 4, n_groups), 512 threads, the columns' maximum (log2 units) and sum
- * over a split's positions; sums: grid (n_splits, 4), 512 threads. */
+ * over a split's positions; sums: grid (splits of its own split_pages, 4), 512
+ * threads. */
 #define Q38_OBSERVE_QUERIES 16
 #define Q38_OBSERVE_PAGES 4 /* of keys that a wave holds, or one (a short context) */
 #define Q38_OBSERVE_COLS (Q38_OBSERVE_QUERIES * Q38_ATTN_GROUP)
@@ -672,7 +673,7 @@ typedef struct {
     int32_t base_pos;
     int32_t n_tokens;
     int32_t split_pages;
-    int32_t n_splits; /* 64 at most */
+    int32_t n_splits; /* of the statistics, 64 at most */
     int32_t n_groups;
     int32_t pad_;
 } q38_observe_args;
