@@ -1378,12 +1378,15 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     memset(&a, 0, sizeof(a));
     a.n_groups = (n_tokens + Q38_OBSERVE_QUERIES - 1) / Q38_OBSERVE_QUERIES;
     if (a.n_groups > 65535) return fail("%d tokens: at most %d a call", n_tokens, 65535 * Q38_OBSERVE_QUERIES);
-    /* a workgroup a CU (64 splits at most: a lane each where they are joined), each of its waves with whole sets of
-     * pages: several at a time where every CU has that many, else one */
+    /* a workgroup a CU (64 splits at most, which are joined four lanes to a column), each of its waves with whole sets of
+     * pages: several at a time where half the CUs have that many, else one (us, several against one: 32 queries over 8K / 16K /
+     * 24K tokens of MXFP4 42.7 / 44.5 / 52.6 against 31.9 / 48.0 / 64.7, of bf16 44.0 / 49.4 / 60.9 against 33.0 / 52.0 /
+     * 68.2; one query 16.7 / 17.0 / 17.4 against 14.7 / 17.1 / 19.3) */
     const int pages = (int)((end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS);
     const int slots = std::min(std::max(ctx->cu_count / Q38_ATTN_KV_HEADS, 1), 64);
-    const int few = pages < slots * Q38_DECODE_TYPED_WAVES * Q38_OBSERVE_PAGES ? 1 : 0;
-    const int step = Q38_DECODE_TYPED_WAVES * (few ? 1 : Q38_OBSERVE_PAGES);
+    const int held = kKvTypes[kv->type].ggml_type == Q38_GGML_Q8_K ? Q38_OBSERVE_PAGES_Q8 : Q38_OBSERVE_PAGES;
+    const int few = 2 * pages < slots * Q38_DECODE_TYPED_WAVES * held ? 1 : 0;
+    const int step = Q38_DECODE_TYPED_WAVES * (few ? 1 : held);
     auto split_for = [&](int wanted) { return ((pages + wanted - 1) / wanted + step - 1) / step * step; };
     /* the statistics of all groups at once */
     a.split_pages = split_for(std::max(slots / a.n_groups, 1));

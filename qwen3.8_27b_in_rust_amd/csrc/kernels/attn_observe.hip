@@ -26,6 +26,8 @@ namespace {
 
 constexpr int kTiles = Q38_OBSERVE_COLS / 16;
 constexpr int kParts = 2;
+template <int T>
+constexpr int kPagesOf = T == Q38_KV_Q8 ? Q38_OBSERVE_PAGES_Q8 : Q38_OBSERVE_PAGES;
 static_assert(kTiles * 16 == Q38_OBSERVE_COLS, "whole tiles");
 
 /* A step's operand of a tile, its four groups of 16 lanes 16 bytes further apart than
@@ -274,23 +276,34 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
         if (16 * sp.begin > a.base_pos + min(u0 + Q38_OBSERVE_QUERIES, a.n_tokens) - 1) continue;
         __syncthreads(); /* the group before is done with q and stat */
         load_queries<T>(q, a, group, j, lane, wave);
-        /* the splits' maxima and sums joined, a lane a split */
-        const float *ml = a.part_ml + (((size_t)group * Q38_ATTN_KV_HEADS + j) * Q38_OBSERVE_COLS * a.n_splits + min(lane, a.n_splits - 1)) * 2;
-        float m[Q38_OBSERVE_COLS / kWaves], l[Q38_OBSERVE_COLS / kWaves];
+        /* the splits' maxima and sums joined, four threads a column (a wave a column
+         * took 2 us longer a group) */
+        const int col = tid >> 2;
+        if (col < Q38_OBSERVE_COLS) {
+            constexpr int kEach = 64 / 4;
+            const float *ml = a.part_ml + (((size_t)group * Q38_ATTN_KV_HEADS + j) * Q38_OBSERVE_COLS + col) * a.n_splits * 2;
+            float m[kEach], l[kEach], top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int n = 0; n < Q38_OBSERVE_COLS / kWaves; ++n) {
-            const float *at = ml + (size_t)(n * kWaves + wave) * a.n_splits * 2;
-            m[n] = at[0];
-            l[n] = at[1];
-        }
+            for (int n = 0; n < kEach; ++n) {
+                const int at = 4 * n + (tid & 3);
+                m[n] = -INFINITY;
+                l[n] = 0.0f;
+                if (at < a.n_splits) {
+                    m[n] = ml[2 * at];
+                    l[n] = ml[2 * at + 1];
+                }
+            }
 #pragma unroll
-        for (int n = 0; n < Q38_OBSERVE_COLS / kWaves; ++n) {
-            const int col = n * kWaves + wave;
-            const float top = column_max(q38_max16(m[n]));
+            for (int n = 0; n < kEach; ++n) top = fmaxf(top, m[n]);
+            top = fmaxf(top, q38_dpp<0xB1>(top));
+            top = fmaxf(top, q38_dpp<0x4E>(top));
             /* a split that the column sees nothing of has a maximum of -inf */
-            const float sum = column_sum(q38_sum16(lane < a.n_splits && m[n] != -INFINITY ? l[n] * q38_exp2(m[n] - top) : 0.0f));
+#pragma unroll
+            for (int n = 0; n < kEach; ++n) sum += m[n] != -INFINITY ? l[n] * q38_exp2(m[n] - top) : 0.0f;
+            sum += q38_dpp<0xB1>(sum);
+            sum += q38_dpp<0x4E>(sum);
             const bool in = u0 + col / kGroup < a.n_tokens;
-            if (lane == 0) {
+            if ((tid & 3) == 0) {
                 stat[col][0] = in ? top : 0.0f;
                 stat[col][1] = in ? 1.0f / sum : 0.0f;
             }
@@ -356,7 +369,7 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
         observe_sums<T, PAGES>(a);                                                                               \
     }
 #define Q38_OBSERVE_KERNELS(name, T)                   \
-    Q38_OBSERVE_KERNEL(name, T, Q38_OBSERVE_PAGES)     \
+    Q38_OBSERVE_KERNEL(name, T, kPagesOf<T>)           \
     Q38_OBSERVE_KERNEL(name##_short, T, 1)
 Q38_OBSERVE_KERNELS(f16, Q38_KV_F16)
 Q38_OBSERVE_KERNELS(bf16, Q38_KV_BF16)

@@ -663,6 +663,7 @@ typedef struct {
  * threads. */
 #define Q38_OBSERVE_QUERIES 16
 #define Q38_OBSERVE_PAGES 4 /* of keys that a wave holds, or one (a short context) */
+#define Q38_OBSERVE_PAGES_Q8 3 /* of 8-bit rows, whose scales take registers too */
 #define Q38_OBSERVE_COLS (Q38_OBSERVE_QUERIES * Q38_ATTN_GROUP)
 typedef struct {
     const char *kpool; /* this layer's */
