@@ -196,7 +196,8 @@ int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
  * q38_kv_write and q38_attn_prefill, which take cache positions as ever;
  * q38_kv_append refuses a sequence that has evicted tokens.  Rows that stay keep
  * the turn that they were stored with.  Positions below the last eviction's n_keep are
- * in no order: q38_seq_truncate goes back to n_keep or to 0, not between.
+ * in no order: rows are stored from n_keep on (others fail with -1), and
+ * q38_seq_truncate goes back to n_keep or to 0, not between.
  * q38_seq_reset, a truncate to 0 and q38_seq_set_pages begin anew, with none
  * evicted. */
 
@@ -206,7 +207,8 @@ int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
  * graphs on a tracking cache adds its weights to the positions that it reads,
  * and takes a sequence once a call; a stored row, whichever call stores it,
  * starts at 0 (in a decode call that appends it, at the weight it gives itself).
- * Such a call needs 24 f32 scores a token in its workspace.  A graph is recorded with tracking
+ * A score that is not finite spoils its kv head's sums.  Such a call needs 24 f32 scores a
+ * token in its workspace.  A graph is recorded with tracking
  * on or off, and its positions are set anew after an eviction. */
 int q38_kv_track_weights(q38_kv *kv, int enable);
 /* Tokens of the sequence that evictions have taken out so far. */

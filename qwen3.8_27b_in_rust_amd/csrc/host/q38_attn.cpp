@@ -347,6 +347,12 @@ struct q38_kv {
     float *weights_of(int slot) const { return weights + (size_t)slot * slot_sums(); }
     int32_t *tokens_of(int slot) const { return reinterpret_cast<int32_t *>(weights_of(slot)) + Q38_PAGE_TOKENS; }
     int32_t evicted_of(int seq) const { return tracks ? evicted[seq].tokens : 0; }
+    /* Rows are stored past what the last eviction has left. */
+    int check_store(int seq, long pos) const {
+        if (tracks && pos < evicted[seq].kept)
+            return fail("sequence %d: positions before %d have been in no order since the last eviction", seq, evicted[seq].kept);
+        return 0;
+    }
     void forget_evicted(int seq) {
         if (tracks) evicted[seq] = Evicted();
     }
@@ -842,11 +848,20 @@ int q38_kernel_timer_start(q38_ctx *ctx, const char *kernel_name, int max_launch
                 const std::string decode = "q38_attn_decode_" + ty + (pre ? "_pre" : "");
                 if (name == decode) f = ctx->f_decode_typed[i][pre];
                 if (name == decode + "_one") f = ctx->f_decode_typed_one[i][pre];
+                if (name == "q38_attn_weigh_" + ty + (pre ? "_pre" : "")) f = ctx->f_weigh[i][pre];
             }
+            for (int few = 0; i > 0 && few < 2; ++few) {
+                if (name == "q38_observe_stats_" + ty + (few ? "_short" : "")) f = ctx->f_observe_stats[i][few];
+                if (name == "q38_observe_sums_" + ty + (few ? "_short" : "")) f = ctx->f_observe_sums[i][few];
+            }
+            if (i > 0 && name == "q38_kv_evict_move_" + ty) f = ctx->f_evict_move[i];
         }
         for (int v = 0; v < kNormVectors; ++v)
             for (int w = 0; w < 2; ++w)
                 if (name == norm_kernel_name(w, v)) f = ctx->f_norm[w][v];
+        if (name == "q38_attn_weigh_merge") f = ctx->f_weigh_merge;
+        if (name == "q38_kv_weights_copy") f = ctx->f_weights_copy;
+        if (name == "q38_kv_evict_select") f = ctx->f_evict_select;
         if (name == "q38_add_rms_norm_any") f = ctx->f_norm_any;
         if (name == "q38_dequantize_q8k") f = ctx->f_dequantize_q8k;
         for (int i = 0; i < kGemvTypes; ++i) {
@@ -1003,11 +1018,10 @@ int q38_seq_truncate(q38_kv *kv, int seq, int n_tokens) {
     if (kv == nullptr) return fail("kv is NULL");
     if (kv->check_seq(seq)) return -1;
     if (n_tokens < 0) return fail("negative token count");
-    if (kv->tracks && n_tokens < kv->evicted[seq].kept) {
-        if (n_tokens > 0)
-            return fail("sequence %d: positions before %d have been in no order since the last eviction", seq, kv->evicted[seq].kept);
+    if (n_tokens == 0)
         kv->forget_evicted(seq);
-    }
+    else if (kv->check_store(seq, n_tokens))
+        return -1;
     kv->release_from(seq, (n_tokens + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS);
     return 0;
 }
@@ -1196,6 +1210,7 @@ static int kv_copy(q38_kv *kv, int layer, int seq, int pos0, int n_tokens, float
     if (pos0 < 0 || n_tokens < 0) return fail("negative position or count");
     if (n_tokens == 0) return 0;
     if (to_pages) {
+        if (kv->check_store(seq, pos0)) return -1;
         if (kv->reserve(seq, pos0 + n_tokens)) return -1;
         kv->images_from(seq, slot, pos0);
     } else if (pos0 + n_tokens > kv->seq_pages[seq] * Q38_PAGE_TOKENS) {
@@ -1431,11 +1446,14 @@ int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n
     }
     if (check_not_capturing(kv, "an eviction")) return -1;
     q38_ctx *ctx = kv->ctx;
-    const int lists = Q38_ATTN_KV_HEADS * kv->n_slots, batch = std::min(n_seq, Q38_MAX_BATCH);
+    const int lists = Q38_ATTN_KV_HEADS * kv->n_slots;
+    /* as many sequences a launch as 256 MB of moves hold (one at least) */
+    const size_t each = (size_t)lists * 2 * max_moves * sizeof(int32_t);
+    const int batch = (int)std::min<size_t>(std::min(n_seq, Q38_MAX_BATCH), std::max<size_t>((256u << 20) / std::max<size_t>(each, 1), 1));
     const size_t counts = ((size_t)batch * lists * sizeof(int32_t) + 15) / 16 * 16;
-    if (max_moves > 0 && ctx->ensure_work(counts + (size_t)batch * lists * 2 * max_moves * sizeof(int32_t))) return -1;
-    for (int b0 = 0; b0 < n_seq && max_moves > 0; b0 += Q38_MAX_BATCH) {
-        const int n = std::min(Q38_MAX_BATCH, n_seq - b0);
+    if (max_moves > 0 && ctx->ensure_work(counts + batch * each)) return -1;
+    for (int b0 = 0; b0 < n_seq && max_moves > 0; b0 += batch) {
+        const int n = std::min(batch, n_seq - b0);
         q38_evict_args a;
         memset(&a, 0, sizeof(a));
         a.kpool = reinterpret_cast<char *>(kv->kpool);
@@ -1801,6 +1819,7 @@ int validate_decode(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, co
             if (seq_ids[c] == s && (appends || kv->tracks)) return fail("sequence %d appears twice", s);
         const int need = positions[b] / Q38_PAGE_TOKENS + 1;
         if (appends) {
+            if (kv->check_store(s, positions[b])) return -1;
             pages_needed += std::max(0, need - kv->seq_pages[s]);
         } else if (need > kv->seq_pages[s]) {
             return fail("sequence %d: position %d is not reserved", s, positions[b]);
@@ -2394,6 +2413,7 @@ int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
                     kv->pt_stride * Q38_PAGE_TOKENS);
     const long need = (end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS - kv->seq_pages[seq];
     if (d_k == nullptr && need > 0) return fail("positions %d..%ld are not reserved", base_pos, end - 1);
+    if (d_k != nullptr && kv->check_store(seq, base_pos)) return -1;
     if (need > (long)kv->free_pages.size())
         return fail("KV pool exhausted: need %ld pages, %zu free", need, kv->free_pages.size());
     q38_ctx *ctx = kv->ctx;

@@ -13,8 +13,8 @@
  * S^T = K Q^T as in the decode (q38_decode_typed.h: a cached value is an operand
  * as it stands, a query is split into parts whose sum it is), but with 16 real
  * columns a product, and with two parts of a query for every type: bf16 ones
- * rounded to nearest leave 2^-17 of it, as the prefill's products do (the decode
- * keeps a third), and the sums over many queries hardly see it: 32 queries over 32K
+ * rounded to nearest leave 2^-16 of it at most, as the prefill's do (the decode
+ * keeps a third part, for half as many products again), and the sums over many queries hardly see it: 32 queries over 32K
  * tokens are within 3e-7 of 64 bits, 7 over 1000 within 7e-7.  A workgroup keeps the parts of 16 queries' 96
  * columns in LDS; a wave holds kPages pages of keys as operands and reads each
  * part once for all of them.  Groups of queries come one after the other in a workgroup of the

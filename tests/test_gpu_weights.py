@@ -18,12 +18,18 @@ def stored(x, ty):
     return stored4(x) if ty == "mxfp4" else typed_rows.stored(x, TYPES[ty])
 
 
-def weights_of(q, k):
+#: What a query's parts leave of it: 22 bits in a decode; where a prompt's queries are observed over bf16 operands, two parts
+#: rounded to nearest, each off by 2^-8 of what it stands for.
+DECODE = 2.0 ** -22
+OBSERVE = {"f16": 2.0 ** -22, "q8_k": 2.0 ** -22, "bf16": 2.0 ** -16, "mxfp4": 2.0 ** -16}
+
+
+def weights_of(q, k, query=DECODE):
     """One token's softmax weights in 64 bits per kv head, [n][4], and a bound on what a kernel may be off.
 
     A score is off by (264 S + |s|) u at most (typed_rows.attend), S = sum |q k| / 16 over its row; a weight by that much
     of itself, by the denominator's own error (the largest score's, and (n + 16) u for the sum's order), 4 u for the exponential
-    and its argument and 4 u for the division and the sum over heads; 2^-21 for a query's 22 bits."""
+    and its argument and 4 u for the division and the sum over heads; what a query's parts leave, `query` of S, in both."""
     n = k.shape[0]
     out, bound = np.zeros((n, 4)), np.zeros((n, 4))
     q, k = q.reshape(24, 256).astype(np.float64), k.astype(np.float64)
@@ -33,7 +39,7 @@ def weights_of(q, k):
         size = np.abs(kk) @ np.abs(q[h]) / 16.0
         p = np.exp(s - s.max())
         p /= p.sum()
-        e = (264 * size + np.abs(s) + 264 * size.max() + np.abs(s).max() + n + 24) * U + 2.0 ** -21
+        e = (264 * size + np.abs(s) + 264 * size.max() + np.abs(s).max() + n + 24) * U + query * (size + size.max())
         out[:, h // 6] += p
         bound[:, h // 6] += 1.01 * e * p + 1e-37
     return out, bound
@@ -262,7 +268,7 @@ def test_observe(pkg, ctx, ty, base, n):
         k = stored(K, ty)
         want, bound = mark[:P].astype(np.float64), np.zeros((P, 4))
         for u in range(n):
-            w, e = weights_of(Q[u], k[:base + u + 1])
+            w, e = weights_of(Q[u], k[:base + u + 1], OBSERVE[ty])
             want[:base + u + 1] += w
             bound[:base + u + 1] += e
         bound += (n + 6 * n) * U * want  # its own sum's order
@@ -293,7 +299,7 @@ def test_observe_equals_decode_steps(pkg, ctx, ty):
         steps, _ = c.weights(s, P)
         k, bound = stored(K, ty), np.zeros((P, 4))
         for u in range(n):
-            bound[:P - n + u + 1] += weights_of(Q[u], k[:P - n + u + 1])[1]
+            bound[:P - n + u + 1] += weights_of(Q[u], k[:P - n + u + 1], OBSERVE[ty])[1]
         _held(got, steps.astype(np.float64), 2 * bound + 14 * n * U * np.maximum(got, steps))
         assert abs(float(got.astype(np.float64).sum()) - 24 * n) < 1e-2
 
@@ -529,3 +535,95 @@ def test_graph_recorded_before_tracking_is_refused(pkg, ctx):
         graph.launch()
         ctx.sync()
     kv.close()
+
+
+def test_prefill_and_images_follow_an_eviction(pkg, ctx):
+    """Prompt pieces before and after an eviction: the block images of what moved are formed anew."""
+    rng = np.random.default_rng(31)
+    for ty in sorted(TYPES):
+        with Cache(pkg, ctx, ty, [200]) as c:
+            s = c.seqs[0]
+            K, V, Q = _rows(rng, 230), _rows(rng, 230), _q(rng, 200)
+            out, out2 = ctx.empty((200, 24, 256)), ctx.empty((200, 24, 256))
+            c.kv.attn_prefill(3, s, 0, 200, ctx.array(Q), ctx.array(K[:200]), ctx.array(V[:200]), out)
+            c.kv.attn_observe(3, s, 180, 20, ctx.array(Q[180:]))
+            c.kv.evict([s], [200], [77], [9])
+            c.kv.attn_prefill(3, s, 77, 30, ctx.array(Q), ctx.array(K[200:]), ctx.array(V[200:]), out)
+            got = out.download(30)
+            c.kv.set_prefill_cache(False)
+            c.kv.attn_prefill(3, s, 77, 30, ctx.array(Q), None, None, out2)
+            assert np.array_equal(_bits(got), _bits(out2.download(30)))
+            k, v = c.rows(s, 107)
+            assert np.array_equal(_bits(v[77:]), _bits(stored(V[200:], ty)))
+            for t in (0, 13, 29):
+                want, bound = attend(Q[t], k[:78 + t], v[:78 + t])
+                assert np.all(np.abs(got[t] - want) <= bound * 2.0 ** 7)
+
+
+def test_two_graphs_two_layers(pkg, ctx):
+    """Two recorded graphs of two layers each on one tracking cache, replayed in turn with eager steps between: outputs and
+    sums equal those of plain calls on another cache, bit for bit."""
+    rng = np.random.default_rng(37)
+    lengths = [90, 300]
+    with Cache(pkg, ctx, "mxfp4", lengths, slots=2) as c, Cache(pkg, ctx, "mxfp4", lengths, slots=2, seed=8) as e:
+        for n, a, b in zip(lengths, c.seqs, e.seqs):
+            K = ctx.array(_rows(rng, n))
+            for layer in (3, 7):
+                c.kv.write(layer, a, 0, n, K, K)
+                e.kv.write(layer, b, 0, n, K, K)
+        q1, q2 = ctx.array(_q(rng, 2)), ctx.array(_q(rng, 2))
+        k = ctx.array(_rows(rng, 2))
+        o = [ctx.empty((2, 24, 256)) for _ in range(6)]
+        calls = lambda a, b: [{"layer": 3, "q": q1, "out": a}, {"layer": 7, "q": q2, "k_new": k, "v_new": k, "out": b}]  # noqa: E731
+        with c.kv.decode_graph(c.seqs, [80, 250], calls(o[0], o[1])) as g, c.kv.decode_graph(c.seqs, [40, 290], calls(o[2], o[3])) as h:
+            for pos in ([80, 250], [89, 299], [15, 16]):
+                for graph, x, at in ((g, o[0:2], pos), (h, o[2:4], [p // 2 for p in pos])):
+                    graph.set_positions(at)
+                    for _ in range(2):
+                        graph.launch()
+                        e.kv.attn_decode(3, e.seqs, at, q1, o[4])
+                        e.kv.attn_decode(7, e.seqs, at, q2, o[5], k_new=k, v_new=k)
+                        assert np.array_equal(_bits(x[0].download()), _bits(o[4].download()))
+                        assert np.array_equal(_bits(x[1].download()), _bits(o[5].download()))
+                c.kv.attn_decode(3, c.seqs, pos, q2, o[4])
+                e.kv.attn_decode(3, e.seqs, pos, q2, o[5])
+            for n, a, b in zip(lengths, c.seqs, e.seqs):
+                for layer in (3, 7):
+                    assert np.array_equal(_bits(c.weights(a, n, layer)[0]), _bits(e.weights(b, n, layer)[0]))
+
+
+def test_sums_of_large_contexts_past_2_32_bytes(pkg, ctx):
+    """Pages at the end of a pool whose sums' and rows' offsets pass 2^32 bytes: decode, observe and eviction there."""
+    n_pages = 4300000 // 2
+    kv = pkg.KVCache(ctx, 2, n_pages, 1, 16 * 200, ggml_type=MXFP4)
+    try:
+        kv.track_weights(True)
+        s = kv.seq_create()
+        kv.seq_set_pages(s, [n_pages - 1 - i for i in range(20)])
+        rng = np.random.default_rng(4)
+        P = 315
+        K, V, Q = _rows(rng, P), _rows(rng, P), _q(rng, 5)
+        kv.write(7, s, 0, P, ctx.array(K), ctx.array(V))
+        o = ctx.empty((24, 256))
+        kv.attn_decode(7, [s], [P - 1], ctx.array(Q[0]), o)
+        kv.attn_observe(7, s, P - 4, 4, ctx.array(Q[1:]))
+        w, t = ctx.empty((P, 4)), ctx.empty((P, 4), np.int32)
+        kv.weights_get(7, [s], [0], [P], w, t)
+        k = stored(K, "mxfp4")
+        want, off = weights_of(Q[0], k)
+        for u in range(4):
+            a, e = weights_of(Q[1 + u], k[:P - 3 + u], OBSERVE["mxfp4"])
+            want[:P - 3 + u] += a
+            off[:P - 3 + u] += e + 40 * U * want[:P - 3 + u]
+        w0, t0 = w.download(), t.download()
+        _held(w0, want, off)
+        kv.evict([s], [P], [100], [10])
+        k1, v1 = ctx.empty((100, 1024)), ctx.empty((100, 1024))
+        kv.read(7, s, 0, 100, k1, v1)
+        for j in range(4):
+            at = chosen(w0[:, j], t0[:, j], P, 100, P - 10)
+            dims = slice(256 * j, 256 * j + 256)
+            assert np.array_equal(k1.download()[:, dims], k[at][:, dims])
+            assert np.array_equal(v1.download()[:, dims], stored(V, "mxfp4")[at][:, dims])
+    finally:
+        kv.close()
