@@ -140,6 +140,13 @@ constexpr KvType kKvTypes[] = {
     {Q38_GGML_MXFP4, Q38_KV_PAGE_MX4, "mxfp4", true},
 };
 constexpr int kKvTypeCount = (int)(sizeof(kKvTypes) / sizeof(kKvTypes[0]));
+/* q38_attn_observe's kernels over rows of a type, for a short context and for few queries (bf16 operands, which take
+ * a third part of theirs then). */
+std::string observe_name(int type, int short_context, int few) {
+    const int ty = kKvTypes[type].ggml_type;
+    const bool third = few && (ty == Q38_GGML_BF16 || ty == Q38_GGML_MXFP4);
+    return std::string(kKvTypes[type].suffix) + (short_context ? "_short" : "") + (third ? "_few" : "");
+}
 /* q38_add_rms_norm's kernels that hold a row in registers: 256 or 1024
  * threads, 1 .. kNormVectors vectors of 4 values a thread. */
 constexpr int kNormVectors = 5;
@@ -199,7 +206,8 @@ struct q38_ctx {
     hipFunction_t f_weights_copy = nullptr;
     hipFunction_t f_evict_select = nullptr;
     hipFunction_t f_evict_move[kKvTypeCount] = {};
-    hipFunction_t f_observe_stats[kKvTypeCount][2] = {}, f_observe_sums[kKvTypeCount][2] = {}; /* [1]: a short context */
+    /* [1]: a short context; [][1]: few queries */
+    hipFunction_t f_observe_stats[kKvTypeCount][2][2] = {}, f_observe_sums[kKvTypeCount][2][2] = {};
     hipModule_t mod_rows_own[kKvTypeCount] = {}, mod_decode_own[kKvTypeCount] = {}; /* types with own_objects */
     hipFunction_t f_decode_typed[kKvTypeCount][2] = {}; /* from index 1 on; [1]: the pre step fused */
     hipFunction_t f_decode_typed_one[kKvTypeCount][2] = {};
@@ -565,10 +573,10 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
             Q38_HIP(hipModuleGetFunction(&ctx->f_weigh[i][pre], ctx->mod_weigh, ("q38_attn_weigh_" + ty + (pre ? "_pre" : "")).c_str()));
         }
         Q38_HIP(hipModuleGetFunction(&ctx->f_evict_move[i], ctx->mod_weights, ("q38_kv_evict_move_" + ty).c_str()));
-        for (int few = 0; few < 2; ++few) {
-            const std::string name = ty + (few ? "_short" : "");
-            Q38_HIP(hipModuleGetFunction(&ctx->f_observe_stats[i][few], ctx->mod_observe, ("q38_observe_stats_" + name).c_str()));
-            Q38_HIP(hipModuleGetFunction(&ctx->f_observe_sums[i][few], ctx->mod_observe, ("q38_observe_sums_" + name).c_str()));
+        for (int v = 0; v < 4; ++v) {
+            const std::string name = observe_name(i, v >> 1, v & 1);
+            Q38_HIP(hipModuleGetFunction(&ctx->f_observe_stats[i][v >> 1][v & 1], ctx->mod_observe, ("q38_observe_stats_" + name).c_str()));
+            Q38_HIP(hipModuleGetFunction(&ctx->f_observe_sums[i][v >> 1][v & 1], ctx->mod_observe, ("q38_observe_sums_" + name).c_str()));
         }
     }
     const std::string p_proj = dir + "/proj.hsaco";
@@ -850,9 +858,9 @@ int q38_kernel_timer_start(q38_ctx *ctx, const char *kernel_name, int max_launch
                 if (name == decode + "_one") f = ctx->f_decode_typed_one[i][pre];
                 if (name == "q38_attn_weigh_" + ty + (pre ? "_pre" : "")) f = ctx->f_weigh[i][pre];
             }
-            for (int few = 0; i > 0 && few < 2; ++few) {
-                if (name == "q38_observe_stats_" + ty + (few ? "_short" : "")) f = ctx->f_observe_stats[i][few];
-                if (name == "q38_observe_sums_" + ty + (few ? "_short" : "")) f = ctx->f_observe_sums[i][few];
+            for (int v = 0; i > 0 && v < 4; ++v) {
+                if (name == "q38_observe_stats_" + observe_name(i, v >> 1, v & 1)) f = ctx->f_observe_stats[i][v >> 1][v & 1];
+                if (name == "q38_observe_sums_" + observe_name(i, v >> 1, v & 1)) f = ctx->f_observe_sums[i][v >> 1][v & 1];
             }
             if (i > 0 && name == "q38_kv_evict_move_" + ty) f = ctx->f_evict_move[i];
         }
@@ -1400,8 +1408,9 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     const int pages = (int)((end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS);
     const int slots = std::min(std::max(ctx->cu_count / Q38_ATTN_KV_HEADS, 1), 64);
     const int held = kKvTypes[kv->type].ggml_type == Q38_GGML_Q8_K ? Q38_OBSERVE_PAGES_Q8 : Q38_OBSERVE_PAGES;
-    const int few = 2 * pages < slots * Q38_DECODE_TYPED_WAVES * held ? 1 : 0;
-    const int step = Q38_DECODE_TYPED_WAVES * (few ? 1 : held);
+    const int is_short = 2 * pages < slots * Q38_DECODE_TYPED_WAVES * held ? 1 : 0;
+    const int step = Q38_DECODE_TYPED_WAVES * (is_short ? 1 : held);
+    const int few = a.n_groups == 1 ? 1 : 0;
     auto split_for = [&](int wanted) { return ((pages + wanted - 1) / wanted + step - 1) / step * step; };
     /* the statistics of all groups at once */
     a.split_pages = split_for(std::max(slots / a.n_groups, 1));
@@ -1416,9 +1425,9 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     a.base_pos = base_pos;
     a.n_tokens = n_tokens;
     const unsigned block = 64 * Q38_DECODE_TYPED_WAVES;
-    if (ctx->launch(ctx->f_observe_stats[kv->type][few], a.n_splits, Q38_ATTN_KV_HEADS, a.n_groups, block, &a)) return -1;
+    if (ctx->launch(ctx->f_observe_stats[kv->type][is_short][few], a.n_splits, Q38_ATTN_KV_HEADS, a.n_groups, block, &a)) return -1;
     a.split_pages = split_for(slots);
-    return ctx->launch(ctx->f_observe_sums[kv->type][few], (pages + a.split_pages - 1) / a.split_pages, Q38_ATTN_KV_HEADS, 1, block, &a);
+    return ctx->launch(ctx->f_observe_sums[kv->type][is_short][few], (pages + a.split_pages - 1) / a.split_pages, Q38_ATTN_KV_HEADS, 1, block, &a);
 }
 
 int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n_tokens, const int32_t *n_keep,

@@ -12,20 +12,21 @@
  *
  * S^T = K Q^T as in the decode (q38_decode_typed.h: a cached value is an operand
  * as it stands, a query is split into parts whose sum it is), but with 16 real
- * columns a product, and with two parts of a query for every type: bf16 ones
- * rounded to nearest leave 2^-16 of it at most, as the prefill's do (the decode
- * keeps a third part, for half as many products again), and the sums over many queries hardly see it: 32 queries over 32K
- * tokens are within 3e-7 of 64 bits, 7 over 1000 within 7e-7.  A workgroup keeps the parts of 16 queries' 96
- * columns in LDS; a wave holds kPages pages of keys as operands and reads each
- * part once for all of them.  Groups of queries come one after the other in a workgroup of the
- * second launch, so that every sum has one owner and a fixed order.
+ * columns a product.  f16 operands take a query's two parts (22 bits), bf16 ones
+ * three (24) for up to 16 queries and two for more: rounded to nearest they leave
+ * 2^-16 of it at most, as the prefill's do, which half as many products again would
+ * keep, and which sums over more than 16 queries hardly see (32 queries over 32K
+ * tokens lie within 3e-7 of 64 bits; 7 over 1000 would within 6e-7, one within 2e-6).
+ * A workgroup keeps the parts of 16 queries' 96 columns in LDS; a wave holds kPages
+ * pages of keys as operands and reads each part once for all of them.  Groups of
+ * queries come one after the other in a workgroup of the second launch, so that
+ * every sum has one owner and a fixed order.
  */
 #include "q38_decode_typed.h"
 
 namespace {
 
 constexpr int kTiles = Q38_OBSERVE_COLS / 16;
-constexpr int kParts = 2;
 template <int T>
 constexpr int kPagesOf = T == Q38_KV_Q8 ? Q38_OBSERVE_PAGES_Q8 : Q38_OBSERVE_PAGES;
 static_assert(kTiles * 16 == Q38_OBSERVE_COLS, "whole tiles");
@@ -34,28 +35,35 @@ static_assert(kTiles * 16 == Q38_OBSERVE_COLS, "whole tiles");
  * they are long: a wave stores one column of every step and group at once, which
  * would all lie in two banks. */
 typedef q38_u32x4 Step[4][17];
-template <int T>
+template <int kParts>
 struct Queries {
     Step part[kTiles][kParts][8];
     float unscale[Q38_OBSERVE_COLS];
 };
 
+/* Tiles of a group that hold a query. */
+Q38_DEV int tiles_of(const q38_observe_args &a, int group) {
+    return (min(a.n_tokens - group * Q38_OBSERVE_QUERIES, Q38_OBSERVE_QUERIES) * kGroup + 15) >> 4;
+}
+
 /* The group's queries as operands: columns 6 u + h, zero past the last query. */
-template <int T>
-Q38_DEV void load_queries(Queries<T> &q, const q38_observe_args &a, int group, int j, int lane, int wave) {
+template <int T, int kParts>
+Q38_DEV void load_queries(Queries<kParts> &q, const q38_observe_args &a, int group, int j, int lane, int wave) {
     const int d = 4 * lane;
     const int i = T == Q38_KV_Q8 ? 2 * (d >> 6) + ((d >> 3) & 1) : d >> 5;
     const int g = T == Q38_KV_Q8 ? (d >> 4) & 3 : (d >> 3) & 3;
     constexpr int kRows = Q38_OBSERVE_COLS / kWaves;
+    const int rows = tiles_of(a, group) * 16 / kWaves; /* of tiles that hold a query */
     f32x4 x[kRows];
 #pragma unroll
-    for (int n = 0; n < kRows; ++n) {
+    for (int n = 0; n < kRows; ++n) { /* (a branch a load would hold the loads up) */
         const int col = n * kWaves + wave, u = group * Q38_OBSERVE_QUERIES + col / kGroup, h = j * kGroup + col % kGroup;
         x[n] = q38_ld4(a.q + ((size_t)min(u, a.n_tokens - 1) * Q38_ATTN_HEADS + h) * Q38_ATTN_HEAD_DIM + d);
         if (u >= a.n_tokens) x[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
     for (int n = 0; n < kRows; ++n) {
+        if (n >= rows) continue;
         const int col = n * kWaves + wave;
         f32x4 y = x[n] * Q38_SCORE_LOG2;
         float unscale = 1.0f;
@@ -71,9 +79,13 @@ Q38_DEV void load_queries(Queries<T> &q, const q38_observe_args &a, int group, i
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (kInBf16<T>) {
-                const __bf16 hi = (__bf16)y[e];
-                p[0][e] = __builtin_bit_cast(uint16_t, hi);
-                p[1][e] = __builtin_bit_cast(uint16_t, (__bf16)(y[e] - (float)hi));
+                float rest = y[e];
+#pragma unroll
+                for (int k = 0; k < kParts; ++k) {
+                    const __bf16 part = (__bf16)rest;
+                    p[k][e] = __builtin_bit_cast(uint16_t, part);
+                    rest -= (float)part;
+                }
             } else {
                 const _Float16 hi = (_Float16)y[e];
                 p[0][e] = __builtin_bit_cast(uint16_t, hi);
@@ -126,9 +138,9 @@ Q38_DEV void load_keys(Keys &k, const char *kpool, int page, int j, int lane) {
 }
 
 /* Scores (log2 units) less `base` of kPages pages against a tile's 16 columns.
- * bf16 operands: both parts' products go into one sum that starts at -base. */
-template <int T, int kPages>
-Q38_DEV void scores_of(const Keys (&k)[kPages], const Step (*part)[8], float unscale, float base, int lane, float (&s)[kPages][4]) {
+ * bf16 operands: all parts' products go into one sum that starts at -base. */
+template <int T, int kPages, int kParts>
+Q38_DEV void scores_of(const Keys (&k)[kPages], const Step (&part)[kParts][8], float unscale, float base, int lane, float (&s)[kPages][4]) {
     /* (an index that the compiler cannot see through: it would keep the parts of
      * all tiles in registers over the loop of pages) */
     asm volatile("" : "+v"(lane));
@@ -179,15 +191,9 @@ Q38_DEV Span span_of(const q38_observe_args &a) {
     return {begin, min(begin + a.split_pages, last + 1), last};
 }
 
-/* Tiles of a group that hold a query. */
-Q38_DEV int tiles_of(const q38_observe_args &a, int group) {
-    return (min(a.n_tokens - group * Q38_OBSERVE_QUERIES, Q38_OBSERVE_QUERIES) * kGroup + 15) >> 4;
-}
-
-template <int T, int kPages>
+template <int T, int kPages, int kParts>
 Q38_DEV void observe_stats(const q38_observe_args &a) {
-    __shared__ __attribute__((aligned(16))) Queries<T> q;
-    __shared__ float red[kWaves][Q38_OBSERVE_COLS][2];
+    __shared__ __attribute__((aligned(16))) Queries<kParts> q;
     const int j = blockIdx.y, group = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const Span sp = span_of(a);
@@ -241,6 +247,10 @@ Q38_DEV void observe_stats(const q38_observe_args &a) {
             L[t] += sum;
         }
     }
+    /* the waves' in the queries' place */
+    __syncthreads();
+    float(*red)[Q38_OBSERVE_COLS][2] = reinterpret_cast<float(*)[Q38_OBSERVE_COLS][2]>(&q);
+    static_assert(sizeof(float) * kWaves * Q38_OBSERVE_COLS * 2 <= sizeof(q), "the waves' columns fit");
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
         const float top = column_max(M[t]);
@@ -263,9 +273,9 @@ Q38_DEV void observe_stats(const q38_observe_args &a) {
     out[1] = sum;
 }
 
-template <int T, int kPages>
+template <int T, int kPages, int kParts>
 Q38_DEV void observe_sums(const q38_observe_args &a) {
-    __shared__ __attribute__((aligned(16))) Queries<T> q;
+    __shared__ __attribute__((aligned(16))) Queries<kParts> q;
     __shared__ float stat[Q38_OBSERVE_COLS][2]; /* a column's maximum, and one over its sum */
     const int j = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
@@ -361,17 +371,23 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
 
 }  // namespace
 
-#define Q38_OBSERVE_KERNEL(name, T, PAGES)                                                                        \
+#define Q38_OBSERVE_KERNEL(name, T, PAGES, PARTS)                                                                 \
     extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_stats_##name(q38_observe_args a) {     \
-        observe_stats<T, PAGES>(a);                                                                              \
+        observe_stats<T, PAGES, PARTS>(a);                                                                       \
     }                                                                                                            \
     extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_sums_##name(q38_observe_args a) {      \
-        observe_sums<T, PAGES>(a);                                                                               \
+        observe_sums<T, PAGES, PARTS>(a);                                                                        \
     }
-#define Q38_OBSERVE_KERNELS(name, T)                   \
-    Q38_OBSERVE_KERNEL(name, T, kPagesOf<T>)           \
-    Q38_OBSERVE_KERNEL(name##_short, T, 1)
+#define Q38_OBSERVE_KERNELS(name, T)                      \
+    Q38_OBSERVE_KERNEL(name, T, kPagesOf<T>, 2)           \
+    Q38_OBSERVE_KERNEL(name##_short, T, 1, 2)
+/* few queries */
+#define Q38_OBSERVE_FEW(name, T)                          \
+    Q38_OBSERVE_KERNEL(name##_few, T, kPagesOf<T>, 3)     \
+    Q38_OBSERVE_KERNEL(name##_short_few, T, 1, 3)
 Q38_OBSERVE_KERNELS(f16, Q38_KV_F16)
 Q38_OBSERVE_KERNELS(bf16, Q38_KV_BF16)
+Q38_OBSERVE_FEW(bf16, Q38_KV_BF16)
 Q38_OBSERVE_KERNELS(q8k, Q38_KV_Q8)
 Q38_OBSERVE_KERNELS(mxfp4, Q38_KV_MX4)
+Q38_OBSERVE_FEW(mxfp4, Q38_KV_MX4)

@@ -127,10 +127,10 @@ struct Cache {
         ctx.f_weigh_merge = kWeighMerge;
         for (int i = 0; i < kKvTypeCount; ++i) {
             ctx.f_evict_move[i] = kMove;
-            for (int few = 0; few < 2; ++few) {
-                ctx.f_observe_stats[i][few] = kStats;
-                ctx.f_observe_sums[i][few] = kSums;
-                ctx.f_weigh[i][few] = kWeigh;
+            for (int v = 0; v < 2; ++v) {
+                ctx.f_observe_stats[i][v][0] = ctx.f_observe_stats[i][v][1] = kStats;
+                ctx.f_observe_sums[i][v][0] = ctx.f_observe_sums[i][v][1] = kSums;
+                ctx.f_weigh[i][v] = kWeigh;
             }
             for (q38_ctx::RowsKernel *k : {&ctx.f_kv_append[i], &ctx.f_kv_gather[i]}) k->many = k->few = kRows;
         }
