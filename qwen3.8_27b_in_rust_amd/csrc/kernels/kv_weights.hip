@@ -312,42 +312,28 @@ struct Row {
 };
 
 /* Holes lie below n_keep and the rows that fill them from there on: no row is read
- * that another move writes, so the moves run in any order, in place.  A wave has
- * kRows of them in flight. */
-constexpr int kRows = Q38_EVICT_ROWS / 4;
+ * that another move writes, so the moves run in any order, in place.  A wave a move:
+ * 24K rows of bf16, a quarter of what they lie among, 32.6 us, with two a wave 33.9,
+ * four 37.1; Q8_K rows of eight sequences 15.5, 16.9 and 17.3.  A row's elements lie
+ * among its page's (q38_kv_layout.h), so a line comes in for each sixteenth of a key
+ * and each 64 bytes of a value that move. */
 template <int T>
 Q38_DEV void move_rows(const q38_evict_args &a) {
     const int x = blockIdx.y, b = blockIdx.z, slot = x >> 2, j = x & 3;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int begin = blockIdx.x * Q38_EVICT_ROWS + kRows * wave;
-    const int count = min(a.counts[(size_t)b * gridDim.y + x] - begin, kRows);
-    if (count <= 0) return;
-    const int32_t *holes = a.moves + ((size_t)b * gridDim.y + x) * 2 * a.max_moves + begin, *sources = holes + a.max_moves;
+    const int tid = threadIdx.x, lane = tid & 63, i = blockIdx.x * Q38_EVICT_ROWS + __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (i >= a.counts[(size_t)b * gridDim.y + x]) return;
+    const int32_t *holes = a.moves + ((size_t)b * gridDim.y + x) * 2 * a.max_moves, *sources = holes + a.max_moves;
     const int32_t *pt = a.page_table + (size_t)a.seq[b] * a.pt_stride;
     char *k = a.kpool + (size_t)slot * a.slot_bytes, *v = a.vpool + (size_t)slot * a.slot_bytes;
-    /* lane i: move i's place, lane 32 + i its source (past the last move the last one again) */
-    const int i = min(lane & 31, count - 1);
-    const int p = (lane & 32 ? sources : holes)[i], page = pt[p >> 4];
-    const size_t sum = (size_t)slot * a.slot_weights + (size_t)page * Q38_WEIGHTS_PAGE + j * Q38_WEIGHTS_HEAD + (p & 15);
-    const float weight = a.weights[sum];
-    const int token = a.tokens[sum];
-    Row<T> row[kRows];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-        const int from = __builtin_amdgcn_readlane(page, 32 + r), t = __builtin_amdgcn_readlane(p, 32 + r) & 15;
-        row[r].load(q38_kv_block<T>(k, from, j), q38_kv_block<T>(v, from, j), t, j, lane);
-    }
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-        if (r >= count) break;
-        const int to = __builtin_amdgcn_readlane(page, r), t = __builtin_amdgcn_readlane(p, r) & 15;
-        row[r].store(q38_kv_block<T>(k, to, j), q38_kv_block<T>(v, to, j), t, j, lane);
-    }
-    const float w = __shfl(weight, 32 + (lane & 31), 64);
-    const int tok = __shfl(token, 32 + (lane & 31), 64);
-    if (lane < count) {
-        a.weights[sum] = w;
-        a.tokens[sum] = tok;
+    const int to = holes[i], from = sources[i], page1 = pt[to >> 4], page0 = pt[from >> 4], t1 = to & 15, t0 = from & 15;
+    Row<T> row;
+    row.load(q38_kv_block<T>(k, page0, j), q38_kv_block<T>(v, page0, j), t0, j, lane);
+    row.store(q38_kv_block<T>(k, page1, j), q38_kv_block<T>(v, page1, j), t1, j, lane);
+    if (lane == 0) {
+        const size_t first = (size_t)slot * a.slot_weights + j * Q38_WEIGHTS_HEAD;
+        const size_t source = first + (size_t)page0 * Q38_WEIGHTS_PAGE + t0, hole = first + (size_t)page1 * Q38_WEIGHTS_PAGE + t1;
+        a.weights[hole] = a.weights[source];
+        a.tokens[hole] = a.tokens[source];
     }
 }
 
@@ -355,7 +341,7 @@ Q38_DEV void move_rows(const q38_evict_args &a) {
 
 extern "C" __global__ __launch_bounds__(256) void q38_kv_weights_copy(q38_kv_weights_args a) { copy_weights(a); }
 extern "C" __global__ __launch_bounds__(kThreads) void q38_kv_evict_select(q38_evict_args a) { select(a); }
-extern "C" __global__ __launch_bounds__(256) void q38_kv_evict_move_f16(q38_evict_args a) { move_rows<Q38_KV_F16>(a); }
-extern "C" __global__ __launch_bounds__(256) void q38_kv_evict_move_bf16(q38_evict_args a) { move_rows<Q38_KV_BF16>(a); }
-extern "C" __global__ __launch_bounds__(256) void q38_kv_evict_move_q8k(q38_evict_args a) { move_rows<Q38_KV_Q8>(a); }
-extern "C" __global__ __launch_bounds__(256) void q38_kv_evict_move_mxfp4(q38_evict_args a) { move_rows<Q38_KV_MX4>(a); }
+extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_ROWS) void q38_kv_evict_move_f16(q38_evict_args a) { move_rows<Q38_KV_F16>(a); }
+extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_ROWS) void q38_kv_evict_move_bf16(q38_evict_args a) { move_rows<Q38_KV_BF16>(a); }
+extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_ROWS) void q38_kv_evict_move_q8k(q38_evict_args a) { move_rows<Q38_KV_Q8>(a); }
+extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_ROWS) void q38_kv_evict_move_mxfp4(q38_evict_args a) { move_rows<Q38_KV_MX4>(a); }

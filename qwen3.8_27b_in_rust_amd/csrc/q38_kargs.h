@@ -636,8 +636,8 @@ typedef struct {
  * blockIdx.x) * 2 max_moves, the evicted positions below n_keep, and max_moves
  * further the kept ones from n_keep on, both rising, as many of each as counts
  * says.  The moves: grid (ceil(max_moves / Q38_EVICT_ROWS), 4 n_slots, n_seq),
- * 256 threads. */
-#define Q38_EVICT_ROWS 16
+ * 64 Q38_EVICT_ROWS threads. */
+#define Q38_EVICT_ROWS 8 /* a wave each */
 typedef struct {
     char *kpool;
     char *vpool;
