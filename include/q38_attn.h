@@ -208,8 +208,9 @@ int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
  * and takes a sequence once a call; a stored row, whichever call stores it,
  * starts at 0 (in a decode call that appends it, at the weight it gives itself).
  * A score that is not finite spoils its kv head's sums.  Such a call needs 24 f32 scores a
- * token in its workspace.  A graph is recorded with tracking
- * on or off, and its positions are set anew after an eviction. */
+ * token in its workspace.  A graph is recorded with tracking on or off, and its
+ * positions are set anew after an eviction.  The sums' memory is kept, tracking or
+ * not, until the cache is destroyed.  A change of tracking cannot be captured. */
 int q38_kv_track_weights(q38_kv *kv, int enable);
 /* Tokens of the sequence that evictions have taken out so far. */
 int q38_seq_evicted(q38_kv *kv, int seq, int *n_tokens);
@@ -228,7 +229,7 @@ int q38_kv_weights_get(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids,
  * that the queries d_q [n_tokens][24][256] (post-norm, post-RoPE, 16-byte
  * aligned) of positions base_pos .. base_pos + n_tokens - 1, whose rows are in
  * the cache, give causally to all positions up to their own.  All of a prompt's
- * queries, or its last ones, as the caller wants them to count. */
+ * queries, or its last ones, as the caller wants them to count.  It cannot be captured. */
 int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens, const float *d_q);
 
 /* Of the n_tokens[b] tokens that sequence seq_ids[b] holds (positions 0 ..

@@ -344,7 +344,7 @@ struct q38_kv {
     /* A tracking cache's sums of attention weights and own positions, [n_slots][max_pages] x Q38_WEIGHTS_PAGE, and
      * what each sequence has lost: */
     bool tracks = false;
-    float *weights = nullptr;
+    float *weights = nullptr; /* kept until the cache is destroyed: a graph's arguments name them */
     struct Evicted {
         int32_t tokens = 0; /* so far: a position's row is that much further on */
         int32_t kept = 0;   /* by the last eviction: positions before are in no order */
@@ -1324,15 +1324,12 @@ int q38_kv_track_weights(q38_kv *kv, int enable) {
     if (!enable) {
         for (int s = 0; s < kv->max_seqs; ++s)
             if (kv->seq_live[s] && kv->evicted[s].tokens > 0) return fail("sequence %d has evicted tokens", s);
-        Q38_HIP(hipStreamSynchronize(kv->ctx->stream));
-        (void)hipFree(kv->weights);
-        kv->weights = nullptr;
         kv->tracks = false;
         return 0;
     }
     if (kv->type == 0) return fail("a cache of F32 rows tracks no weights: F16, BF16, Q8_K or MXFP4 rows do");
     const size_t bytes = kv->slot_sums() * kv->n_slots * sizeof(float);
-    if (hipMalloc(&kv->weights, bytes) != hipSuccess) {
+    if (kv->weights == nullptr && hipMalloc(&kv->weights, bytes) != hipSuccess) {
         (void)hipGetLastError();
         kv->weights = nullptr;
         return fail("cannot allocate %zu bytes for the sums of weights", bytes);
@@ -1401,6 +1398,7 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     memset(&a, 0, sizeof(a));
     a.n_groups = (n_tokens + Q38_OBSERVE_QUERIES - 1) / Q38_OBSERVE_QUERIES;
     if (a.n_groups > 65535) return fail("%d tokens: at most %d a call", n_tokens, 65535 * Q38_OBSERVE_QUERIES);
+    if (check_not_capturing(kv, "a call whose workspace a later one may move")) return -1;
     /* a workgroup a CU (64 splits at most, which are joined four lanes to a column), each of its waves with whole sets of
      * pages: several at a time where half the CUs have that many, else one (us, several against one: 32 queries over 8K / 16K /
      * 24K tokens of MXFP4 42.7 / 44.5 / 52.6 against 31.9 / 48.0 / 64.7, of bf16 44.0 / 49.4 / 60.9 against 33.0 / 52.0 /
@@ -1980,7 +1978,7 @@ struct q38_decode_graph {
     hipGraphNode_t last = nullptr; /* the node the next step depends on */
     int steps = 0;
     bool tracks = false; /* recorded over a tracking cache */
-    int32_t evicted[Q38_MAX_BATCH] = {0}; /* each sequence's evicted tokens when the positions were set */
+    int32_t evicted[Q38_MAX_BATCH] = {0}; /* each sequence's evicted tokens when the arguments were made */
 
     ~q38_decode_graph() {
         if (exec != nullptr) (void)hipGraphExecDestroy(exec);
@@ -2138,6 +2136,7 @@ int q38_decode_graph_add_decode(q38_decode_graph *g, const q38_decode_call *call
         g->node_params(o, true, &p, arg);
         Q38_HIP(hipGraphKernelNodeSetParams(o.merge_node, &p));
     }
+    g->note_evicted();
     g->calls.push_back(k);
     q38_decode_graph::Call &kk = g->calls.back();
     hipKernelNodeParams p;

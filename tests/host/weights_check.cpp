@@ -386,6 +386,7 @@ int main() {
         g_capture = hipStreamCaptureStatusActive;
         refused(q38_kv_evict(kv, 2, s2, n, k, r), "cannot be captured");
         refused(q38_kv_track_weights(kv, 0), "cannot be captured");
+        refused(q38_attn_observe(kv, 3, a, 0, 3, f), "cannot be captured");
         g_capture = hipStreamCaptureStatusNone;
         refused(q38_kv_track_weights(kv, 0), "has evicted tokens");
         refused(q38_seq_truncate(kv, e, 39), "in no order");

@@ -534,6 +534,16 @@ def test_graph_recorded_before_tracking_is_refused(pkg, ctx):
         graph.set_positions([21])
         graph.launch()
         ctx.sync()
+    # tracking off and on again under a graph: its arguments still name the sums
+    kv.track_weights(True)
+    with kv.decode_graph([s], [20], [{"layer": 3, "q": q, "out": o}]) as graph:
+        graph.launch()
+        kv.track_weights(False)
+        kv.track_weights(True)
+        graph.launch()
+        w = ctx.empty((21, 4))
+        kv.weights_get(3, [s], [0], [21], w)
+        assert np.abs(w.download().sum(0) - 6).max() <= 6 * 40 * U
     kv.close()
 
 
