@@ -1546,7 +1546,7 @@ struct decode_plan {
     size_t part_bytes = 0; /* of work_bytes: the rest is a tracking cache's scores */
 };
 
-/* Tokens per split over 16- or 8-bit rows (unless q38_set_decode_split fixed
+/* Tokens per split over 16-, 8- or 4-bit rows (unless q38_set_decode_split fixed
  * it).  A workgroup there costs as much as streaming some hundreds of tokens
  * before its first and after its last page, and a CU holds one at a time, so
  * few rounds of large splits win: the fewest rounds that splits of at most

@@ -21,6 +21,14 @@
  * pages of keys as operands and reads each part once for all of them.  Groups of
  * queries come one after the other in a workgroup of the second launch, so that
  * every sum has one owner and a fixed order.
+ *
+ * Measured: 32 queries over 32K tokens of MXFP4 in 25.9 us for the statistics and 32.7
+ * for the sums.  The products of two parts are 25.8 GFLOP a launch, 20.5 us at the
+ * 1260 TFLOP/s of a large library product: 79 and 63% of that rate (the keys, 19 MB,
+ * would take 3); what is left is the vector unit's masks, exponentials and sums
+ * over columns, 57 and 67 instructions a page and tile beside 16 products.  7 queries over 1000 tokens of
+ * bf16 8.0 and 9.2: 32 workgroups, a wave a page or two, bound by the chain
+ * queries - parts in LDS - keys - join.
  */
 #include "q38_decode_typed.h"
 

@@ -18,9 +18,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
-#ifndef Q38_MX4_DEPTH
-#define Q38_MX4_DEPTH 1
-#endif
 constexpr int kWaves = Q38_DECODE_TYPED_WAVES;
 constexpr int kGroup = Q38_ATTN_GROUP;
 /* A head's reference lies kRefBelow under the score that set it, and is raised
@@ -623,8 +620,9 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
     constexpr int kQSets = kInBf16<T> ? 2 : 1;
     /* pages of a wave in registers: two 16-bit ones leave too few for the rest
      * (128K tokens 95 us against 85), 8-bit ones are half as large (1 / 2 / 3
-     * pages: 49.9 / 47.5 / 48.8 us) */
-    constexpr int kDepth = T == Q38_KV_MX4 ? Q38_MX4_DEPTH : T == Q38_KV_Q8 ? 2 : 1;
+     * pages: 49.9 / 47.5 / 48.8 us), 4-bit ones come in pairs (one / two of them:
+     * 29.6 / 30.2) */
+    constexpr int kDepth = T == Q38_KV_Q8 ? 2 : 1;
     constexpr int kPer = T == Q38_KV_MX4 ? 2 : 1; /* pages of a step */
     __shared__ q38_u32x4 q_frag[kQSets][8][64];
     __shared__ float q_unscale[8];

@@ -44,10 +44,10 @@
 #define Q38_MAX_SPLITS 4096 /* splits of one sequence in one decode launch */
 #define Q38_MAX_SPLIT_TOKENS 4096 /* context tokens one decode workgroup streams */
 #define Q38_DECODE_WAVES 4 /* waves of a decode workgroup */
-#define Q38_DECODE_TYPED_WAVES 8 /* waves of a decode workgroup over 16- or 8-bit rows */
+#define Q38_DECODE_TYPED_WAVES 8 /* waves of a decode workgroup over 16-, 8- or 4-bit rows */
 #define Q38_HEAD_PAGE_SPLITS 256 /* splits whose first page ids a decode launch can carry */
 
-/* Split-K paged decode: grid (total_splits, 4 kv heads).  Over 16- or 8-bit rows
+/* Split-K paged decode: grid (total_splits, 4 kv heads).  Over 16-, 8- or 4-bit rows
  * the pools are bytes (q38_kv_layout.h) and the launch carries no page ids. */
 typedef struct {
     float *kpool;              /* this layer's K pages: [max_pages][4][16][256] */
