@@ -4,21 +4,17 @@
  * A cached token's sum, per kv head, takes the softmax weight that each of the
  * group's 6 query heads gives it: W[t] += sum_h exp2(s_ht - M_h) / L_h.  M_h
  * and L_h are known only when every split has run, so the decode kernel
- * (q38_decode_typed.h) leaves its scores, 96 bytes a token and kv head, and
+ * (q38_decode_typed.h) leaves its scores, 24 bytes a token and kv head, and
  * the launch that joins the splits' outputs turns them into weights beside it: a
  * workgroup per (split, kv head) joins the splits' maxima and sums for its six
  * heads and adds what each token gets.  Each sum has one owner, so the order of
- * additions is fixed.  Scores are written and read back through the caches: 384
- * bytes a token against the 1088 to 4096 of its rows.  (To form them again in the second
- * launch would read the keys twice, 512 to 2048 bytes a token.)
+ * additions is fixed.  Scores are 96 bytes a token against the 1088 to 4096 of
+ * its rows.  (To form them again in the second launch would read the keys twice, 512 to
+ * 2048 bytes a token.)
  *
  * Measured (us of a whole pass with its merge, 600 MB of layers in turn; beside it a
  * cache that tracks nothing): bf16 rows 1021 tokens 9.6 (8.3), 32K 29.4 (26.1), 128K 104 (86);
- * Q8_K 10.1 (8.5), 21.1 (17.6), 57 (47); MXFP4 10.3 (8.5), 18.2 (14.7), 43 (31).
- * 128K tokens have 50 MB of scores, written and read: 16 us at the rate of a
- * copy, which is what the sums add.  Short sequences that a plain decode
- * finishes in one launch take two (17 tokens 9.5 against 4.9).
- */
+@@ */
 #include "q38_decode_typed.h"
 #include "q38_merge.h"
 

@@ -71,6 +71,19 @@ Q38_DEV q38_u32x2 ld_block8(__amdgpu_buffer_rsrc_t r, int at) {
     return __builtin_bit_cast(q38_u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 2));
 }
 
+/* A page's scores, lane (c, g)'s four tokens of column c: columns past the six heads lie
+ * past the range, where nothing is stored (a branch instead of it would leave the count of outstanding accesses
+ * open, and every wait for the page's values would wait for this store as well: 128K tokens of MXFP4 42.4 us
+ * against 39).  MXFP4's are written through L2 (32K tokens 15.3 us against 16.4, and 128K 38.5 against 38.9);
+ * other rows' stay there for a while (bf16 27.3 against 28.0 and 100 in both, Q8_K 19.1 against 18.7 and 56.8
+ * against 57.5). */
+template <int T>
+Q38_DEV void put_scores(float *page, bool live, int c, int g, const float (&s)[4]) {
+    constexpr int kPolicy = T == Q38_KV_MX4 ? 16 : 0;
+    const __amdgpu_buffer_rsrc_t r = block_rsrc(reinterpret_cast<char *>(page), live ? Q38_SCORES_PAGE * 4 : 0);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(q38_u32x4, f32x4{s[0], s[1], s[2], s[3]}), r, (c * Q38_PAGE_TOKENS + 4 * g) * 4, 0, kPolicy);
+}
+
 template <int T, typename Args>
 Q38_DEV void load_page(Page<T> &p, const Args &a, int page, bool live, int j, int lane) {
     const int scales = T == Q38_KV_MX4 ? q38_mx4_scales_offset(j) : q38_kv_scales_offset(j);
@@ -206,7 +219,7 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         }
     }
     /* kept for the sums of weights, which need the whole context's maximum and sum first */
-    if (kWeigh && c < kGroup) q38_st4(scores + c * Q38_PAGE_TOKENS + 4 * g, f32x4{s[0], s[1], s[2], s[3]});
+    if (kWeigh) put_scores<T>(scores, true, c, g, s);
     const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     auto scale_heads = [&](float f) { /* o by each head's factor */
         float fr[4];
@@ -363,9 +376,9 @@ Q38_DEV void pair_step(State &st, const Page<Q38_KV_MX4> (&p)[2], const q38_u32x
             if (4 * g + i >= valid1) s[1][i] = -INFINITY;
         }
     }
-    if (kWeigh && c < kGroup) {
-        q38_st4(scores0 + c * Q38_PAGE_TOKENS + 4 * g, f32x4{s[0][0], s[0][1], s[0][2], s[0][3]});
-        if (valid1 > 0) q38_st4(scores1 + c * Q38_PAGE_TOKENS + 4 * g, f32x4{s[1][0], s[1][1], s[1][2], s[1][3]});
+    if (kWeigh) {
+        put_scores<T>(scores0, true, c, g, s[0]);
+        put_scores<T>(scores1, valid1 > 0, c, g, s[1]);
     }
     const float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     if (__any(mx > st.ref + kRefSlack)) {
