@@ -1543,6 +1543,7 @@ struct decode_plan {
     int split_tokens = 0;
     int total_splits = 0;
     size_t work_bytes = 0;
+    bool merges = false;   /* some sequence has several splits */
     size_t part_bytes = 0; /* of work_bytes: the rest is a tracking cache's scores */
 };
 
@@ -1596,14 +1597,13 @@ int plan_decode(const q38_kv *kv, int n_seq, const int32_t *positions, decode_pl
     else if (choose_split_tokens(ctx, n_seq, total_tokens, max_tokens, &plan->split_tokens))
         return -1;
     int total = 0;
-    bool any_multi = false;
     for (int b = 0; b < n_seq; ++b) {
         const int ns = (positions[b] + plan->split_tokens) / plan->split_tokens; /* ceil((pos+1)/split) */
-        any_multi |= ns > 1;
+        plan->merges |= ns > 1;
         total += ns;
     }
     plan->total_splits = total;
-    plan->part_bytes = any_multi || kv->tracks ? (size_t)total * Q38_ATTN_HEADS * (Q38_ATTN_HEAD_DIM + 2) * sizeof(float) : 0;
+    plan->part_bytes = plan->merges || kv->tracks ? (size_t)total * Q38_ATTN_HEADS * (Q38_ATTN_HEAD_DIM + 2) * sizeof(float) : 0;
     const size_t pages = (size_t)total * (plan->split_tokens / Q38_PAGE_TOKENS);
     plan->work_bytes =
         plan->part_bytes + (kv->tracks ? pages * Q38_ATTN_KV_HEADS * Q38_SCORES_PAGE * sizeof(float) : 0);
@@ -1723,11 +1723,11 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
         }
     }
 
-    L->merge = plan.work_bytes > 0;
+    L->merge = plan.merges;
     if (work != nullptr) {
         a.part_o = static_cast<float *>(work);
         a.part_ml = a.part_o + (size_t)total * Q38_ATTN_HEADS * Q38_ATTN_HEAD_DIM;
-    } else if (L->merge) {
+    } else if (plan.work_bytes > 0) {
         return fail("decode workspace missing");
     }
     const bool one = arg_pages && n_seq == 1;
@@ -1748,6 +1748,8 @@ int build_decode(q38_kv *kv, int slot, int n_seq, const int32_t *seq_ids, const 
         memset(&L->w, 0, sizeof(L->w));
         memset(&L->mw, 0, sizeof(L->mw));
         L->w.scores = scores;
+        L->w.weights = kv->weights_of(slot);
+        L->w.tokens = kv->tokens_of(slot);
         L->mw.scores = scores;
         L->mw.page_table = a.page_table;
         L->mw.weights = kv->weights_of(slot);

@@ -7,14 +7,20 @@
  * (q38_decode_typed.h) leaves its scores, 24 bytes a token and kv head, and
  * the launch that joins the splits' outputs turns them into weights beside it: a
  * workgroup per (split, kv head) joins the splits' maxima and sums for its six
- * heads and adds what each token gets.  Each sum has one owner, so the order of
- * additions is fixed.  Scores are 96 bytes a token against the 1088 to 4096 of
- * its rows.  (To form them again in the second launch would read the keys twice, 512 to
- * 2048 bytes a token.)
+ * heads and adds what each token gets.  A sequence of one split has both at its
+ * workgroups' end, and they add there: where all sequences have one there is no
+ * second launch.  Each sum has one owner, so the order of additions is fixed.
+ * Scores are 96 bytes a token against the 1088 to 4096 of its rows.  (To form them
+ * again in the second launch would read the keys twice, 512 to 2048 bytes a token.)
  *
  * Measured (us of a whole pass with its merge, 600 MB of layers in turn; beside it a
- * cache that tracks nothing): bf16 rows 1021 tokens 9.6 (8.3), 32K 29.4 (26.1), 128K 104 (86);
-@@ */
+ * cache that tracks nothing): bf16 rows 17 tokens 6.2 (4.8), 1021 10.0 (8.3), 32K 29.2 (26.1), 128K 102 (86);
+ * Q8_K 6.7 (5.3), 10.3 (8.5), 21.2 (17.6), 57 (47); MXFP4 6.9 (4.9), 10.4 (8.5), 17.3 (14.7), 39 (31).
+ * (17 tokens with the sums in a launch of their own: 8.9, 9.5 and 10.0.)
+ * Of 128K tokens' 12.6 MB of scores most of what they cost is their writing between the
+ * pages' loads (bf16 86 us without; kept in LDS to the split's end 93, but 0.5 to 0.9
+ * longer up to 32K tokens, and nothing gained for MXFP4).
+ */
 #include "q38_decode_typed.h"
 #include "q38_merge.h"
 
@@ -35,11 +41,12 @@ Q38_WEIGH_KERNEL(mxfp4_pre, Q38_KV_MX4, true)
 namespace {
 
 /* Workgroup (split g, kv head j): the tokens of the split. */
-Q38_DEV void add_weights(const q38_merge_args &m, const q38_weigh_merge_args &a, int g, int j) {
+Q38_DEV void add_split(const q38_merge_args &m, const q38_weigh_merge_args &a, int g, int j) {
     __shared__ float top[kGroup], inverse[kGroup];
     int b = 0;
     while (b + 1 < m.n_seq && m.split_base[b + 1] <= g) ++b;
     const int base = m.split_base[b], n = m.split_base[b + 1] - base;
+    if (n == 1) return; /* the decode kernel has added them */
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     for (int h = wave; h < kGroup; h += 4) {
         /* the head's maximum and sum over all splits */
@@ -56,35 +63,11 @@ Q38_DEV void add_weights(const q38_merge_args &m, const q38_weigh_merge_args &a,
         }
     }
     __syncthreads();
-    const int pos = a.pos[b], t_begin = (g - base) * a.split_tokens, t_end = min(pos + 1, t_begin + a.split_tokens);
-    const int32_t *pt = a.page_table + (size_t)a.seq[b] * a.pt_stride + (t_begin >> 4);
-    const float *scores = a.scores + ((size_t)g * (a.split_tokens >> 4) * Q38_ATTN_KV_HEADS + j) * Q38_SCORES_PAGE;
-    for (int t = 4 * tid; t < t_end - t_begin; t += 4 * 256) {
-        const float *sc = scores + (size_t)(t >> 4) * Q38_ATTN_KV_HEADS * Q38_SCORES_PAGE + (t & 15);
-        const size_t at = (size_t)pt[t >> 4] * Q38_WEIGHTS_PAGE + j * Q38_WEIGHTS_HEAD + (t & 15);
-        f32x4 s[kGroup];
-#pragma unroll
-        for (int h = 0; h < kGroup; ++h) s[h] = q38_ld4(sc + h * Q38_PAGE_TOKENS);
-        const f32x4 old = q38_ld4(a.weights + at);
-        f32x4 w = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < kGroup; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __builtin_fmaf(q38_exp2(s[h][i] - top[h]), inverse[h], w[i]);
-        if (t_begin + t + 4 <= pos) {
-            q38_st4(a.weights + at, old + w);
-            continue;
-        }
-        /* the last tokens: none behind pos, and a new one starts its sum */
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = t_begin + t + i;
-            if (p > pos) break;
-            const bool starts = p == pos && a.appended;
-            a.weights[at + i] = starts ? w[i] : old[i] + w[i];
-            if (starts) a.tokens[at + i] = pos + a.evicted[b];
-        }
-    }
+    const int t_begin = (g - base) * a.split_tokens, last = a.pos[b] - t_begin;
+    const size_t head = (size_t)j * Q38_WEIGHTS_HEAD;
+    add_weights<256>(top, inverse, a.scores + ((size_t)g * (a.split_tokens >> 4) * Q38_ATTN_KV_HEADS + j) * Q38_SCORES_PAGE,
+                     a.page_table + (size_t)a.seq[b] * a.pt_stride + (t_begin >> 4), a.weights + head, a.tokens + head,
+                     min(last + 1, a.split_tokens), last, a.appended != 0, a.pos[b] + a.evicted[b]);
 }
 
 }  // namespace
@@ -94,7 +77,7 @@ extern "C" __global__ __launch_bounds__(256) void q38_attn_weigh_merge(q38_merge
     const int x = blockIdx.x;
     if (x >= m.n_seq * kMerges) {
         const int y = x - m.n_seq * kMerges;
-        add_weights(m, a, y >> 2, y & 3);
+        add_split(m, a, y >> 2, y & 3);
         return;
     }
     const int b = x / kMerges, rest = x - b * kMerges, base = m.split_base[b], n = m.split_base[b + 1] - base;

@@ -624,6 +624,40 @@ Q38_DEV Where find(const q38_decode_typed_args &a, int g) {
     return {b, a.seq[b], a.pos[b], a.split_base[b], a.split_base[b + 1] - a.split_base[b]};
 }
 
+/* What the weights of six heads, of whose scores over the whole context top is the maximum and
+ * inverse one over the sum, add to a split's n tokens.  pt: its first page's id;
+ * last: the sequence's last position among them (past them where a later split has it), which a row
+ * stored by the call starts anew as the sequence's token `token`. */
+template <int kThreads>
+Q38_DEV void add_weights(const float *top, const float *inverse, const float *scores, const int32_t *pt, float *weights, int32_t *tokens,
+                         int n, int last, bool stored, int token) {
+    for (int t = 4 * threadIdx.x; t < n; t += 4 * kThreads) {
+        const float *sc = scores + (size_t)(t >> 4) * Q38_ATTN_KV_HEADS * Q38_SCORES_PAGE + (t & 15);
+        const size_t at = (size_t)pt[t >> 4] * Q38_WEIGHTS_PAGE + (t & 15);
+        f32x4 s[kGroup];
+#pragma unroll
+        for (int h = 0; h < kGroup; ++h) s[h] = q38_ld4(sc + h * Q38_PAGE_TOKENS);
+        const f32x4 old = q38_ld4(weights + at);
+        f32x4 w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < kGroup; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __builtin_fmaf(q38_exp2(s[h][i] - top[h]), inverse[h], w[i]);
+        if (t + 4 <= last) {
+            q38_st4(weights + at, old + w);
+            continue;
+        }
+        /* the last tokens: none behind the last, and a new one starts its sum */
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (t + i > last) break;
+            const bool starts = t + i == last && stored;
+            weights[at + i] = starts ? w[i] : old[i] + w[i];
+            if (starts) tokens[at + i] = token;
+        }
+    }
+}
+
 /* Nothing beside the attention (q38_weigh_args: the scores too). */
 struct NoSums {};
 
@@ -644,6 +678,7 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
     __shared__ __attribute__((aligned(16))) float red_o[kWaves][kGroup][Q38_ATTN_HEAD_DIM];
     __shared__ __attribute__((aligned(16))) float red_m[8][kWaves], red_l[8][kWaves]; /* [column][wave] */
     __shared__ __attribute__((aligned(16))) float red_unit[8][kWaves]; /* of red_o */
+    __shared__ float head_top[kGroup], head_inverse[kGroup]; /* over the whole context */
     static_assert(kWaves == 8 && kGroup == 6, "a wave per query head, one for the key and one for the value");
 
     const int g_split = blockIdx.x, j = blockIdx.y, tid = threadIdx.x;
@@ -829,52 +864,63 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
     __syncthreads();
 
     /* a wave per head joins the waves' parts, lane l dims 4l .. 4l + 3 */
-    if (wave >= kGroup) return;
-    float M = -INFINITY, L = 0.0f;
-    f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    const int h = j * kGroup + wave;
-    const size_t at = (size_t)h * Q38_ATTN_HEAD_DIM + 4 * lane;
-    if (n_pages == 1) {
-        M = red_m[wave][0];
-        L = red_l[wave][0];
-        O = q38_ld4(&red_o[0][wave][4 * lane]) * red_unit[wave][0];
-    } else {
-        float m[kWaves], f[kWaves];
-        f32x4 o[kWaves];
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            m[w] = w < n_pages ? red_m[wave][w] : -INFINITY;
-            o[w] = q38_ld4(&red_o[w][wave][4 * lane]);
-            M = fmaxf(M, m[w]);
+    if (wave >= kGroup && !(kWeigh && nsplit == 1)) return;
+    if (wave < kGroup) {
+        float M = -INFINITY, L = 0.0f;
+        f32x4 O = {0.f, 0.f, 0.f, 0.f};
+        const int h = j * kGroup + wave;
+        const size_t at = (size_t)h * Q38_ATTN_HEAD_DIM + 4 * lane;
+        if (n_pages == 1) {
+            M = red_m[wave][0];
+            L = red_l[wave][0];
+            O = q38_ld4(&red_o[0][wave][4 * lane]) * red_unit[wave][0];
+        } else {
+            float m[kWaves], f[kWaves];
+            f32x4 o[kWaves];
+    #pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                m[w] = w < n_pages ? red_m[wave][w] : -INFINITY;
+                o[w] = q38_ld4(&red_o[w][wave][4 * lane]);
+                M = fmaxf(M, m[w]);
+            }
+    #pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                f[w] = q38_exp2(m[w] - M);
+                /* a wave without pages has left nothing there */
+                L += w < n_pages ? red_l[wave][w] * f[w] : 0.0f;
+                const float fu = f[w] * red_unit[wave][w];
+    #pragma unroll
+                for (int e = 0; e < 4; ++e) O[e] = w < n_pages ? __builtin_fmaf(fu, o[w][e], O[e]) : O[e];
+            }
         }
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            f[w] = q38_exp2(m[w] - M);
-            /* a wave without pages has left nothing there */
-            L += w < n_pages ? red_l[wave][w] * f[w] : 0.0f;
-            const float fu = f[w] * red_unit[wave][w];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) O[e] = w < n_pages ? __builtin_fmaf(fu, o[w][e], O[e]) : O[e];
+        if (nsplit == 1) {
+            f32x4 r = O / L;
+            if (a.gate != nullptr) {
+                const f32x4 gate = q38_ld4(a.gate + ((size_t)b * Q38_ATTN_HEADS + h) * a.gate_head_stride + 4 * lane);
+    #pragma unroll
+                for (int e = 0; e < 4; ++e) r[e] *= q38_sigmoid(gate[e]);
+            }
+            q38_st4(a.out + (size_t)b * Q38_ATTN_Q_DIM + at, r);
+            if (kWeigh && lane == 0) {
+                head_top[wave] = M;
+                head_inverse[wave] = 1.0f / L;
+            }
+        } else {
+            q38_st4(a.part_o + (size_t)g_split * Q38_ATTN_Q_DIM + at, O);
+            if (lane == 0) {
+                a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 0] = M;
+                a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 1] = L;
+            }
         }
     }
-    if (kWeigh && nsplit == 1 && lane == 0) {
-        a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 0] = M;
-        a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 1] = L;
-    }
-    if (nsplit == 1) {
-        f32x4 r = O / L;
-        if (a.gate != nullptr) {
-            const f32x4 gate = q38_ld4(a.gate + ((size_t)b * Q38_ATTN_HEADS + h) * a.gate_head_stride + 4 * lane);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r[e] *= q38_sigmoid(gate[e]);
-        }
-        q38_st4(a.out + (size_t)b * Q38_ATTN_Q_DIM + at, r);
-    } else {
-        q38_st4(a.part_o + (size_t)g_split * Q38_ATTN_Q_DIM + at, O);
-        if (lane == 0) {
-            a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 0] = M;
-            a.part_ml[((size_t)g_split * Q38_ATTN_HEADS + h) * 2 + 1] = L;
-        }
+    if constexpr (kWeigh) {
+        if (nsplit != 1) return;
+        /* the whole context: its sums without a second launch, once every wave's scores are stored */
+        __builtin_amdgcn_s_waitcnt(0x0f70); /* vmcnt(0) */
+        __syncthreads();
+        const size_t head = (size_t)j * Q38_WEIGHTS_HEAD;
+        add_weights<64 * kWaves>(head_top, head_inverse, sums.scores + ((size_t)g_split * (a.split_tokens >> 4) * Q38_ATTN_KV_HEADS + j) * Q38_SCORES_PAGE,
+                                 pt, sums.weights + head, sums.tokens + head, t_end, pos, a.k_new != nullptr, pos + sums.evicted[b]);
     }
 }
 

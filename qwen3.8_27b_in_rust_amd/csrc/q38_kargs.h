@@ -588,16 +588,18 @@ typedef struct {
 
 /* What a decode launch over such a cache takes beside q38_decode_typed_args.  The
  * scores (log2 units) of split g's page p, kv head j: at ((g * split_tokens / 16 +
- * p) * 4 + j) * Q38_SCORES_PAGE, [6 query heads][16 tokens]; each split's
- * part_ml is written, a sequence's only one too. */
+ * p) * 4 + j) * Q38_SCORES_PAGE, [6 query heads][16 tokens].  A sequence of one
+ * split adds its weights to the sums itself. */
 #define Q38_SCORES_PAGE (Q38_ATTN_GROUP * Q38_PAGE_TOKENS)
 typedef struct {
     float *scores;
+    float *weights;  /* this layer's sums */
+    int32_t *tokens; /* and own positions: the same lines, past the sums */
     int32_t evicted[Q38_MAX_BATCH]; /* tokens evicted before: the new one is that much further on */
 } q38_weigh_args;
 /* The merge after it: grid (96 n_seq + 4 total_splits), 256 threads; the first
  * workgroups join the splits' outputs (q38_attn_decode_merge's), the others add the
- * weights of a (split, kv head) to the sums. */
+ * weights of a (split, kv head) to the sums, where the sequence has several. */
 typedef struct {
     const float *scores;
     const int32_t *page_table;

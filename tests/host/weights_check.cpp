@@ -252,10 +252,19 @@ int main() {
             g_launches.clear();
             const float *q = reinterpret_cast<float *>(0x70000000000ull);
             REQUIRE(q38_attn_decode(kv, 3, 70, seq.data(), pos.data(), q, nullptr, nullptr, nullptr, const_cast<float *>(q)) == 0);
-            REQUIRE(g_launches.size() == 4);
-            for (int l = 0; l < 4; l += 2) {
+            size_t l = 0;
+            for (int b0 = 0; b0 < 70; b0 += Q38_MAX_BATCH) {
+                REQUIRE(l < g_launches.size() && g_launches[l].f == kWeigh);
                 const auto a = arg<q38_decode_typed_args>(g_launches[l]);
                 const auto w = arg<q38_weigh_args>(g_launches[l], 1);
+                REQUIRE(a.n_seq == std::min(70 - b0, Q38_MAX_BATCH) && w.weights == kv->weights_of(0) && w.tokens == kv->tokens_of(0));
+                /* sequences of one split add their weights themselves */
+                if (a.total_splits == a.n_seq) {
+                    ++l;
+                    REQUIRE(inside(w.scores, (size_t)a.total_splits * (a.split_tokens / 16) * 4 * Q38_SCORES_PAGE * 4));
+                    continue;
+                }
+                REQUIRE(l + 1 < g_launches.size());
                 const auto m = arg<q38_merge_args>(g_launches[l + 1]);
                 const auto mw = arg<q38_weigh_merge_args>(g_launches[l + 1], 1);
                 REQUIRE(g_launches[l].f == kWeigh && g_launches[l].gx == (unsigned)a.total_splits && g_launches[l].block == 512);
@@ -271,7 +280,9 @@ int main() {
                     REQUIRE(m.split_base[b] == a.split_base[b]);
                     REQUIRE((a.split_base[b + 1] - a.split_base[b]) == (a.pos[b] + a.split_tokens) / a.split_tokens);
                 }
+                l += 2;
             }
+            REQUIRE(l == g_launches.size());
         }
         c.ctx.split_tokens = 0;
         /* a prompt's queries: every page of every group in one split of either launch, statistics inside the workspace */
