@@ -1482,7 +1482,8 @@ int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n
             a.first_recent[i] = kv->evicted[seq_ids[b]].tokens + n_tokens[b] - n_recent[b];
         }
         if (ctx->launch(ctx->f_evict_select, lists, n, 1, 1024, &a)) return -1;
-        if (ctx->launch(ctx->f_evict_move[kv->type], (unsigned)((max_moves + Q38_EVICT_ROWS - 1) / Q38_EVICT_ROWS), lists, n, 64 * Q38_EVICT_ROWS, &a))
+        const long rows = 8 * Q38_EVICT_WAVES * (kKvTypes[kv->type].ggml_type == Q38_GGML_MXFP4 ? Q38_EVICT_MX4 : 1); /* of eight workgroups */
+        if (ctx->launch(ctx->f_evict_move[kv->type], (unsigned)((max_moves + rows - 1) / rows * 8), lists, n, 64 * Q38_EVICT_WAVES, &a))
             return -1;
     }
     for (int b = 0; b < n_seq; ++b) {

@@ -11,9 +11,9 @@
  *
  * Measured: a layer of 32K tokens to 8K, bf16: lists 22.3 us (four workgroups, one a kv head;
  * 16 layers' are 64 beside each other, in the same time), 24.6K rows moved in
- * 26-32, for 91 MB read and 39 written past L2, 4.1-5 TB/s.  (The rows have 25 MB: their bytes
+ * 24-30, for 81 MB read and 35 written past L2, 3.9-4.8 TB/s.  (The rows have 25 MB: their bytes
  * lie in nine of ten lines of the pages they come from.)  Eight sequences of 250 to
- * 4003 tokens of Q8_K to 60% of them 11.9 and 12.9.
+ * 4003 tokens of Q8_K to 60% of them 11.5 and 13.4.
  */
 #include <type_traits>
 
@@ -325,28 +325,58 @@ struct Row {
 };
 
 /* Holes lie below n_keep and the rows that fill them from there on: no row is read
- * that another move writes, so the moves run in any order, in place.  A wave a move:
- * 24K rows of bf16, a quarter of what they lie among, 32.6 us, with two a wave 33.9,
- * four 37.1; Q8_K rows of eight sequences 15.5, 16.9 and 17.3.  A row's elements lie
+ * that another move writes, so the moves run in any order, in place.  A wave a move,
+ * of 4-bit rows two: a wave's chain is count - move - pages - rows, and 4-bit ones are too few
+ * bytes to fill it (16 layers of 32K tokens to 8K: one / two / four / eight a wave 195 /
+ * 158 / 165 / 177 us, to 24K 209 / 164 / 195 / 202; of bf16 462 / 488 / - / -, 691 /
+ * 704, Q8_K 265 / 271, 354 / 366).  A row's elements lie
  * among its page's (q38_kv_layout.h), so a line comes in for each sixteenth of a key
- * and each 64 bytes of a value that move. */
+ * and each 64 bytes of a value that move; an XCD takes an eighth of a list in one
+ * piece, so that neighbours find their lines in its L2 (one layer of bf16 reads 81 MB and
+ * writes 35 against 91 and 39, of which a quarter as many requests for parts of 64 bytes; 16
+ * layers 462 us against 487, 691 against 753, Q8_K 265 against 278, 354 against 370). */
+template <int T>
+constexpr int kRowsOf = T == Q38_KV_MX4 ? Q38_EVICT_MX4 : 1;
 template <int T>
 Q38_DEV void move_rows(const q38_evict_args &a) {
     const int x = blockIdx.y, b = blockIdx.z, slot = x >> 2, j = x & 3;
-    const int tid = threadIdx.x, lane = tid & 63, i = blockIdx.x * Q38_EVICT_ROWS + __builtin_amdgcn_readfirstlane(tid >> 6);
-    if (i >= a.counts[(size_t)b * gridDim.y + x]) return;
+    const int tid = threadIdx.x, lane = tid & 63;
+    constexpr int kRows = kRowsOf<T>, kAll = Q38_EVICT_WAVES * kRows;
+    const int n = a.counts[(size_t)b * gridDim.y + x], each = (n + 8 * kAll - 1) / (8 * kAll), u = blockIdx.x >> 3;
+    const int i = ((blockIdx.x & 7) * each + u) * kAll + __builtin_amdgcn_readfirstlane(tid >> 6) * kRows;
+    if (u >= each || i >= n) return;
     const int32_t *holes = a.moves + ((size_t)b * gridDim.y + x) * 2 * a.max_moves, *sources = holes + a.max_moves;
     const int32_t *pt = a.page_table + (size_t)a.seq[b] * a.pt_stride;
     char *k = a.kpool + (size_t)slot * a.slot_bytes, *v = a.vpool + (size_t)slot * a.slot_bytes;
-    const int to = holes[i], from = sources[i], page1 = pt[to >> 4], page0 = pt[from >> 4], t1 = to & 15, t0 = from & 15;
-    Row<T> row;
-    row.load(q38_kv_block<T>(k, page0, j), q38_kv_block<T>(v, page0, j), t0, j, lane);
-    row.store(q38_kv_block<T>(k, page1, j), q38_kv_block<T>(v, page1, j), t1, j, lane);
-    if (lane == 0) {
-        const size_t first = (size_t)slot * a.slot_weights + j * Q38_WEIGHTS_HEAD;
-        const size_t source = first + (size_t)page0 * Q38_WEIGHTS_PAGE + t0, hole = first + (size_t)page1 * Q38_WEIGHTS_PAGE + t1;
-        a.weights[hole] = a.weights[source];
-        a.tokens[hole] = a.tokens[source];
+    Row<T> row[kRows];
+    int page1[kRows], page0[kRows], t1[kRows], t0[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) { /* (past the last: that one again, read but not stored) */
+        const int at = min(i + r, n - 1), to = holes[at], from = sources[at];
+        page1[r] = pt[to >> 4];
+        page0[r] = pt[from >> 4];
+        t1[r] = to & 15;
+        t0[r] = from & 15;
+    }
+    const size_t first = (size_t)slot * a.slot_weights + j * Q38_WEIGHTS_HEAD;
+    float weight[kRows];
+    int32_t token[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        row[r].load(q38_kv_block<T>(k, page0[r], j), q38_kv_block<T>(v, page0[r], j), t0[r], j, lane);
+        const size_t source = first + (size_t)page0[r] * Q38_WEIGHTS_PAGE + t0[r];
+        weight[r] = a.weights[source];
+        token[r] = a.tokens[source];
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        if (i + r >= n) return;
+        row[r].store(q38_kv_block<T>(k, page1[r], j), q38_kv_block<T>(v, page1[r], j), t1[r], j, lane);
+        if (lane == 0) {
+            const size_t hole = first + (size_t)page1[r] * Q38_WEIGHTS_PAGE + t1[r];
+            a.weights[hole] = weight[r];
+            a.tokens[hole] = token[r];
+        }
     }
 }
 
@@ -354,7 +384,7 @@ Q38_DEV void move_rows(const q38_evict_args &a) {
 
 extern "C" __global__ __launch_bounds__(256) void q38_kv_weights_copy(q38_kv_weights_args a) { copy_weights(a); }
 extern "C" __global__ __launch_bounds__(kThreads) void q38_kv_evict_select(q38_evict_args a) { select(a); }
-extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_ROWS) void q38_kv_evict_move_f16(q38_evict_args a) { move_rows<Q38_KV_F16>(a); }
-extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_ROWS) void q38_kv_evict_move_bf16(q38_evict_args a) { move_rows<Q38_KV_BF16>(a); }
-extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_ROWS) void q38_kv_evict_move_q8k(q38_evict_args a) { move_rows<Q38_KV_Q8>(a); }
-extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_ROWS) void q38_kv_evict_move_mxfp4(q38_evict_args a) { move_rows<Q38_KV_MX4>(a); }
+extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_WAVES) void q38_kv_evict_move_f16(q38_evict_args a) { move_rows<Q38_KV_F16>(a); }
+extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_WAVES) void q38_kv_evict_move_bf16(q38_evict_args a) { move_rows<Q38_KV_BF16>(a); }
+extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_WAVES) void q38_kv_evict_move_q8k(q38_evict_args a) { move_rows<Q38_KV_Q8>(a); }
+extern "C" __global__ __launch_bounds__(64 * Q38_EVICT_WAVES) void q38_kv_evict_move_mxfp4(q38_evict_args a) { move_rows<Q38_KV_MX4>(a); }

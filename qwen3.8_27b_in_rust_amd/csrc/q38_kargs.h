@@ -637,9 +637,10 @@ typedef struct {
  * (slot, kv head) of a sequence; it leaves, at moves + (blockIdx.y * 4 n_slots +
  * blockIdx.x) * 2 max_moves, the evicted positions below n_keep, and max_moves
  * further the kept ones from n_keep on, both rising, as many of each as counts
- * says.  The moves: grid (ceil(max_moves / Q38_EVICT_ROWS), 4 n_slots, n_seq),
- * 64 Q38_EVICT_ROWS threads. */
-#define Q38_EVICT_ROWS 8 /* a wave each */
+ * says.  The moves: grid (ceil(max_moves / rows) up to a multiple of 8, 4 n_slots, n_seq),
+ * 64 Q38_EVICT_WAVES threads, rows of a workgroup: a wave one, of 4-bit rows Q38_EVICT_MX4. */
+#define Q38_EVICT_WAVES 8
+#define Q38_EVICT_MX4 2
 typedef struct {
     char *kpool;
     char *vpool;

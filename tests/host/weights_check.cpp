@@ -322,7 +322,9 @@ int main() {
                 const auto a = arg<q38_evict_args>(g_launches[l]), m = arg<q38_evict_args>(g_launches[l + 1]);
                 REQUIRE(!memcmp(&a, &m, sizeof(a)) && g_launches[l].f == kSelect && g_launches[l].block == 1024 && g_launches[l].gx == 8);
                 REQUIRE(g_launches[l + 1].f == kMove && g_launches[l + 1].gy == 8 && g_launches[l + 1].gz == g_launches[l].gy);
-                REQUIRE((int)g_launches[l + 1].gx * Q38_EVICT_ROWS >= a.max_moves);
+                /* (an eighth of a list's workgroups to each XCD) */
+                const int rows = Q38_EVICT_WAVES * (kKvTypes[kv->type].ggml_type == Q38_GGML_MXFP4 ? Q38_EVICT_MX4 : 1);
+                REQUIRE((int)g_launches[l + 1].gx * rows >= a.max_moves && g_launches[l + 1].gx % 8 == 0);
                 const size_t lists = (size_t)g_launches[l].gy * 8;
                 REQUIRE(inside(a.counts, lists * 4) && inside(a.moves, lists * 2 * a.max_moves * 4));
                 REQUIRE((char *)a.moves >= (char *)a.counts + lists * 4);
