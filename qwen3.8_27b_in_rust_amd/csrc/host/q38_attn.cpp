@@ -207,7 +207,8 @@ struct q38_ctx {
     hipFunction_t f_evict_select = nullptr;
     hipFunction_t f_evict_move[kKvTypeCount] = {};
     /* [1]: a short context; [][1]: few queries */
-    hipFunction_t f_observe_stats[kKvTypeCount][2][2] = {}, f_observe_sums[kKvTypeCount][2][2] = {};
+    hipFunction_t f_observe_stats[kKvTypeCount][2][2] = {}, f_observe_sums[kKvTypeCount][2] = {};
+    hipFunction_t f_observe_add = nullptr;
     hipModule_t mod_rows_own[kKvTypeCount] = {}, mod_decode_own[kKvTypeCount] = {}; /* types with own_objects */
     hipFunction_t f_decode_typed[kKvTypeCount][2] = {}; /* from index 1 on; [1]: the pre step fused */
     hipFunction_t f_decode_typed_one[kKvTypeCount][2] = {};
@@ -550,6 +551,7 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
     Q38_HIP(hipModuleLoad(&ctx->mod_weigh, (dir + "/attn_weigh.hsaco").c_str()));
     Q38_HIP(hipModuleLoad(&ctx->mod_weights, (dir + "/kv_weights.hsaco").c_str()));
     Q38_HIP(hipModuleLoad(&ctx->mod_observe, (dir + "/attn_observe.hsaco").c_str()));
+    Q38_HIP(hipModuleGetFunction(&ctx->f_observe_add, ctx->mod_observe, "q38_observe_add"));
     Q38_HIP(hipModuleGetFunction(&ctx->f_weigh_merge, ctx->mod_weigh, "q38_attn_weigh_merge"));
     Q38_HIP(hipModuleGetFunction(&ctx->f_weights_copy, ctx->mod_weights, "q38_kv_weights_copy"));
     Q38_HIP(hipModuleGetFunction(&ctx->f_evict_select, ctx->mod_weights, "q38_kv_evict_select"));
@@ -576,7 +578,7 @@ int q38_ctx_create(q38_ctx **out, int device, const char *module_dir) {
         for (int v = 0; v < 4; ++v) {
             const std::string name = observe_name(i, v >> 1, v & 1);
             Q38_HIP(hipModuleGetFunction(&ctx->f_observe_stats[i][v >> 1][v & 1], ctx->mod_observe, ("q38_observe_stats_" + name).c_str()));
-            Q38_HIP(hipModuleGetFunction(&ctx->f_observe_sums[i][v >> 1][v & 1], ctx->mod_observe, ("q38_observe_sums_" + name).c_str()));
+            if (v < 2) Q38_HIP(hipModuleGetFunction(&ctx->f_observe_sums[i][v], ctx->mod_observe, ("q38_observe_sums_" + name).c_str()));
         }
     }
     const std::string p_proj = dir + "/proj.hsaco";
@@ -860,7 +862,7 @@ int q38_kernel_timer_start(q38_ctx *ctx, const char *kernel_name, int max_launch
             }
             for (int v = 0; i > 0 && v < 4; ++v) {
                 if (name == "q38_observe_stats_" + observe_name(i, v >> 1, v & 1)) f = ctx->f_observe_stats[i][v >> 1][v & 1];
-                if (name == "q38_observe_sums_" + observe_name(i, v >> 1, v & 1)) f = ctx->f_observe_sums[i][v >> 1][v & 1];
+                if (v < 2 && name == "q38_observe_sums_" + observe_name(i, 0, v)) f = ctx->f_observe_sums[i][v];
             }
             if (i > 0 && name == "q38_kv_evict_move_" + ty) f = ctx->f_evict_move[i];
         }
@@ -869,6 +871,7 @@ int q38_kernel_timer_start(q38_ctx *ctx, const char *kernel_name, int max_launch
                 if (name == norm_kernel_name(w, v)) f = ctx->f_norm[w][v];
         if (name == "q38_attn_weigh_merge") f = ctx->f_weigh_merge;
         if (name == "q38_kv_weights_copy") f = ctx->f_weights_copy;
+        if (name == "q38_observe_add") f = ctx->f_observe_add;
         if (name == "q38_kv_evict_select") f = ctx->f_evict_select;
         if (name == "q38_add_rms_norm_any") f = ctx->f_norm_any;
         if (name == "q38_dequantize_q8k") f = ctx->f_dequantize_q8k;
@@ -1399,33 +1402,48 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     a.n_groups = (n_tokens + Q38_OBSERVE_QUERIES - 1) / Q38_OBSERVE_QUERIES;
     if (a.n_groups > 65535) return fail("%d tokens: at most %d a call", n_tokens, 65535 * Q38_OBSERVE_QUERIES);
     if (check_not_capturing(kv, "a call whose workspace a later one may move")) return -1;
-    /* a workgroup a CU (64 splits at most, which are joined four lanes to a column), each of its waves with whole sets of
-     * pages: several at a time where half the CUs have that many, else one (us, several against one: 32 queries over 8K / 16K /
-     * 24K tokens of MXFP4 42.7 / 44.5 / 52.6 against 31.9 / 48.0 / 64.7, of bf16 44.0 / 49.4 / 60.9 against 33.0 / 52.0 /
-     * 68.2; one query 16.7 / 17.0 / 17.4 against 14.7 / 17.1 / 19.3) */
+    /* A workgroup a CU (64 splits at most, which are joined four lanes to a column).  Up to three pages a wave the
+     * statistics take one at a time and keep the scores for the sums; from there on, with scores of as many bytes as
+     * several passes over the keys, a wave takes several pages and the sums form the scores again (us, kept against
+     * formed again: 7 queries over 1000 / 8K / 24K / 32K tokens of bf16 11.3 / 13.4 / 25.2 / 30.2 against 24.6 / 24.7 /
+     * 33.9 / 38.3, of MXFP4 11.4 / 13.3 / 25.4 / 30.0 against 24.1 / 24.4 / 26.0 / 27.0; 32 over 8K / 24K / 32K of MXFP4
+     * 28.2 / 48.0 / 60.8 against 43.9 / 54.1 / 58.1; 1024 over 4K / 16K / 24K / 32K 311 / 856 / 1337 / 1810 against 901 /
+     * 1067 / 1206 / 1346). */
     const int pages = (int)((end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS);
     const int slots = std::min(std::max(ctx->cu_count / Q38_ATTN_KV_HEADS, 1), 64);
     const int held = kKvTypes[kv->type].ggml_type == Q38_GGML_Q8_K ? Q38_OBSERVE_PAGES_Q8 : Q38_OBSERVE_PAGES;
-    const int is_short = 2 * pages < slots * Q38_DECODE_TYPED_WAVES * held ? 1 : 0;
+    const int is_short = pages <= 3 * slots * Q38_DECODE_TYPED_WAVES ? 1 : 0;
     const int step = Q38_DECODE_TYPED_WAVES * (is_short ? 1 : held);
     const int few = a.n_groups == 1 ? 1 : 0;
     auto split_for = [&](int wanted) { return ((pages + wanted - 1) / wanted + step - 1) / step * step; };
-    /* the statistics of all groups at once */
-    a.split_pages = split_for(std::max(slots / a.n_groups, 1));
+    /* scores kept are those of as many groups at once as 128 MB hold, which the last level's cache does too (1024 queries
+     * over 4K tokens with 16 / 32 / 64 / 128 / 256 MB: 558 / 421 / 349 / 311 / 344); else the statistics of all groups at once */
+    const int groups = a.n_groups;
+    const size_t kept = is_short ? (size_t)pages * Q38_ATTN_KV_HEADS * Q38_OBSERVE_COLS * Q38_PAGE_TOKENS * sizeof(float) : 0;
+    const int batch = is_short ? (int)std::min<size_t>(groups, std::max<size_t>((128u << 20) / kept, 1)) : groups;
+    a.split_pages = split_for(std::max(slots / batch, 1));
     a.n_splits = (pages + a.split_pages - 1) / a.split_pages;
-    const size_t stats = (size_t)a.n_groups * Q38_ATTN_KV_HEADS * a.n_splits * Q38_OBSERVE_COLS * 2 * sizeof(float);
-    if (ctx->ensure_work(stats)) return -1;
+    const size_t stats = (size_t)batch * Q38_ATTN_KV_HEADS * a.n_splits * Q38_OBSERVE_COLS * 2 * sizeof(float); /* (of 16 bytes) */
+    if (ctx->ensure_work(stats + batch * kept)) return -1;
     a.kpool = reinterpret_cast<const char *>(kv->kslot(slot));
     a.weights = kv->weights_of(slot);
     a.page_row = kv->d_page_table + (size_t)seq * kv->pt_stride;
     a.q = d_q;
     a.part_ml = static_cast<float *>(ctx->work);
+    a.scores = a.part_ml + stats / sizeof(float);
     a.base_pos = base_pos;
     a.n_tokens = n_tokens;
     const unsigned block = 64 * Q38_DECODE_TYPED_WAVES;
-    if (ctx->launch(ctx->f_observe_stats[kv->type][is_short][few], a.n_splits, Q38_ATTN_KV_HEADS, a.n_groups, block, &a)) return -1;
+    for (a.group0 = 0; a.group0 < groups; a.group0 += batch) {
+        a.n_groups = std::min(batch, groups - a.group0);
+        if (ctx->launch(ctx->f_observe_stats[kv->type][is_short][few], a.n_splits, Q38_ATTN_KV_HEADS, a.n_groups, block, &a)) return -1;
+        if (is_short && ctx->launch(ctx->f_observe_add, (pages + Q38_DECODE_TYPED_WAVES - 1) / Q38_DECODE_TYPED_WAVES, Q38_ATTN_KV_HEADS, 1, block, &a))
+            return -1;
+    }
+    if (is_short) return 0;
+    a.group0 = 0;
     a.split_pages = split_for(slots);
-    return ctx->launch(ctx->f_observe_sums[kv->type][is_short][few], (pages + a.split_pages - 1) / a.split_pages, Q38_ATTN_KV_HEADS, 1, block, &a);
+    return ctx->launch(ctx->f_observe_sums[kv->type][few], (pages + a.split_pages - 1) / a.split_pages, Q38_ATTN_KV_HEADS, 1, block, &a);
 }
 
 int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n_tokens, const int32_t *n_keep,

@@ -4,11 +4,12 @@
  *
  * Query u (position base_pos + u) sees positions up to its own: token t of a kv
  * head takes W[t] += sum_u sum_h exp2(s_uht - M_uh) / L_uh over the group's heads
- * h.  M and L need every position first, so the scores are formed twice, on the
- * matrix unit both times: to keep 24 scores a query and token instead would write
- * and read more bytes than the keys have from 12 queries on.  The first launch
- * leaves each column's (a query's head) maximum and sum over a split of the
- * positions; the second joins the splits' and adds.
+ * h.  M and L need every position first: the first launch forms the scores and leaves
+ * each column's (a query's head) maximum and sum over a split of the positions, the
+ * second joins the splits' and adds.  A short context's scores are kept for it, 24 f32
+ * a query and token; over a longer one they would write and read several times the bytes that the
+ * keys have, and it forms them again on the matrix unit (q38_attn_observe in the host's
+ * code has both sides' times).
  *
  * S^T = K Q^T as in the decode (q38_decode_typed.h: a cached value is an operand
  * as it stands, a query is split into parts whose sum it is), but with 16 real
@@ -18,17 +19,17 @@
  * keep, and which sums over more than 16 queries hardly see (32 queries over 32K
  * tokens lie within 3e-7 of 64 bits; 7 over 1000 would within 6e-7, one within 2e-6).
  * A workgroup keeps the parts of 16 queries' 96 columns in LDS; a wave holds kPages
- * pages of keys as operands and reads each part once for all of them.  Groups of
- * queries come one after the other in a workgroup of the second launch, so that
- * every sum has one owner and a fixed order.
+ * pages of keys as operands and reads each part once for all of them (one page where it keeps
+ * scores).  Groups of queries come one after the other in a workgroup of the second
+ * launch, so that every sum has one owner and a fixed order.
  *
- * Measured: 32 queries over 32K tokens of MXFP4 in 25.9 us for the statistics and 32.7
- * for the sums.  The products of two parts are 25.8 GFLOP a launch, 20.5 us at the
- * 1260 TFLOP/s of a large library product: 79 and 63% of that rate (the keys, 19 MB,
- * would take 3); what is left is the vector unit's masks, exponentials and sums
- * over columns, 57 and 67 instructions a page and tile beside 16 products.  7 queries over 1000 tokens of
- * bf16 8.0 and 9.2: 32 workgroups, a wave a page or two, bound by the chain
- * queries - parts in LDS - keys - join.
+ * Measured: 32 queries over 32K tokens of MXFP4, formed twice, 25.9 us for the statistics
+ * and 32.7 for the sums.  The products of two parts are 25.8 GFLOP a launch, 20.5 us at
+ * the 1260 TFLOP/s of a large library product: 79 and 63% of that rate (the keys, 19
+ * MB, would take 3); what is left is the vector unit's masks, exponentials and sums
+ * over columns, 57 and 67 instructions a page and tile beside 16 products.  7 queries over
+ * 1000 tokens of bf16, scores kept, 8.2 and 4.0: 32 workgroups, a wave a page, bound by the
+ * chains queries - parts in LDS - keys - join and scores - join - sums.
  */
 #include "q38_decode_typed.h"
 
@@ -199,10 +200,17 @@ Q38_DEV Span span_of(const q38_observe_args &a) {
     return {begin, min(begin + a.split_pages, last + 1), last};
 }
 
+/* A short context's scores (log2 units, -inf where a column does not see): group, kv head and page by page, a tile
+ * as the lanes hold it. */
+Q38_DEV float *kept_scores(const q38_observe_args &a, int group, int j, int page, int tile, int lane) {
+    const int pages = ((a.base_pos + a.n_tokens - 1) >> 4) + 1;
+    return a.scores + (((((size_t)group * Q38_ATTN_KV_HEADS + j) * pages + page) * kTiles + tile) * 64 + lane) * 4;
+}
+
 template <int T, int kPages, int kParts>
 Q38_DEV void observe_stats(const q38_observe_args &a) {
     __shared__ __attribute__((aligned(16))) Queries<kParts> q;
-    const int j = blockIdx.y, group = blockIdx.z;
+    const int j = blockIdx.y, group = a.group0 + blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const Span sp = span_of(a);
     const int tiles = tiles_of(a, group);
@@ -235,6 +243,7 @@ Q38_DEV void observe_stats(const q38_observe_args &a) {
             const float base = none ? 0.0f : M[t];
             scores_of<T>(k, q.part[t], unscale[t], base, lane, s);
             if (masks) mask(s, page, min(last[t], 16 * sp.end - 1), g);
+            if constexpr (kPages == 1) q38_st4(kept_scores(a, blockIdx.z, j, page, t, lane), f32x4{s[0][0], s[0][1], s[0][2], s[0][3]} + base);
             float top = -INFINITY;
 #pragma unroll
             for (int p = 0; p < kPages; ++p) top = fmaxf(top, fmaxf(fmaxf(s[p][0], s[p][1]), fmaxf(s[p][2], s[p][3])));
@@ -276,15 +285,54 @@ Q38_DEV void observe_stats(const q38_observe_args &a) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
         sum += red[w][tid][0] == -INFINITY ? 0.0f : red[w][tid][1] * q38_exp2(red[w][tid][0] - top);
-    float *out = a.part_ml + ((((size_t)group * Q38_ATTN_KV_HEADS + j) * Q38_OBSERVE_COLS + tid) * a.n_splits + blockIdx.x) * 2;
+    float *out = a.part_ml + ((((size_t)blockIdx.z * Q38_ATTN_KV_HEADS + j) * Q38_OBSERVE_COLS + tid) * a.n_splits + blockIdx.x) * 2;
     out[0] = top;
     out[1] = sum;
+}
+
+/* A column's maximum, and one over its sum. */
+typedef float Stats[Q38_OBSERVE_COLS][2];
+
+/* at_group: the group's place in part_ml; u0: its first query. */
+Q38_DEV void join_stats(Stats &stat, const q38_observe_args &a, int at_group, int u0, int j, int tid) {
+            /* the splits' maxima and sums joined, four threads a column (a wave a column
+             * took 2 us longer a group) */
+            const int col = tid >> 2;
+            if (col < Q38_OBSERVE_COLS) {
+                constexpr int kEach = 64 / 4;
+                const float *ml = a.part_ml + (((size_t)at_group * Q38_ATTN_KV_HEADS + j) * Q38_OBSERVE_COLS + col) * a.n_splits * 2;
+                float m[kEach], l[kEach], top = -INFINITY, sum = 0.0f;
+    #pragma unroll
+                for (int n = 0; n < kEach; ++n) {
+                    const int at = 4 * n + (tid & 3);
+                    m[n] = -INFINITY;
+                    l[n] = 0.0f;
+                    if (at < a.n_splits) {
+                        m[n] = ml[2 * at];
+                        l[n] = ml[2 * at + 1];
+                    }
+                }
+    #pragma unroll
+                for (int n = 0; n < kEach; ++n) top = fmaxf(top, m[n]);
+                top = fmaxf(top, q38_dpp<0xB1>(top));
+                top = fmaxf(top, q38_dpp<0x4E>(top));
+                /* a split that the column sees nothing of has a maximum of -inf */
+    #pragma unroll
+                for (int n = 0; n < kEach; ++n) sum += m[n] != -INFINITY ? l[n] * q38_exp2(m[n] - top) : 0.0f;
+                sum += q38_dpp<0xB1>(sum);
+                sum += q38_dpp<0x4E>(sum);
+                const bool in = u0 + col / kGroup < a.n_tokens;
+                if ((tid & 3) == 0) {
+                    stat[col][0] = in ? top : 0.0f;
+                    stat[col][1] = in ? 1.0f / sum : 0.0f;
+                }
+            }
 }
 
 template <int T, int kPages, int kParts>
 Q38_DEV void observe_sums(const q38_observe_args &a) {
     __shared__ __attribute__((aligned(16))) Queries<kParts> q;
-    __shared__ float stat[Q38_OBSERVE_COLS][2]; /* a column's maximum, and one over its sum */
+    __shared__ Stats stat;
     const int j = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const Span sp = span_of(a);
@@ -294,38 +342,7 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
         if (16 * sp.begin > a.base_pos + min(u0 + Q38_OBSERVE_QUERIES, a.n_tokens) - 1) continue;
         __syncthreads(); /* the group before is done with q and stat */
         load_queries<T>(q, a, group, j, lane, wave);
-        /* the splits' maxima and sums joined, four threads a column (a wave a column
-         * took 2 us longer a group) */
-        const int col = tid >> 2;
-        if (col < Q38_OBSERVE_COLS) {
-            constexpr int kEach = 64 / 4;
-            const float *ml = a.part_ml + (((size_t)group * Q38_ATTN_KV_HEADS + j) * Q38_OBSERVE_COLS + col) * a.n_splits * 2;
-            float m[kEach], l[kEach], top = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int n = 0; n < kEach; ++n) {
-                const int at = 4 * n + (tid & 3);
-                m[n] = -INFINITY;
-                l[n] = 0.0f;
-                if (at < a.n_splits) {
-                    m[n] = ml[2 * at];
-                    l[n] = ml[2 * at + 1];
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < kEach; ++n) top = fmaxf(top, m[n]);
-            top = fmaxf(top, q38_dpp<0xB1>(top));
-            top = fmaxf(top, q38_dpp<0x4E>(top));
-            /* a split that the column sees nothing of has a maximum of -inf */
-#pragma unroll
-            for (int n = 0; n < kEach; ++n) sum += m[n] != -INFINITY ? l[n] * q38_exp2(m[n] - top) : 0.0f;
-            sum += q38_dpp<0xB1>(sum);
-            sum += q38_dpp<0x4E>(sum);
-            const bool in = u0 + col / kGroup < a.n_tokens;
-            if ((tid & 3) == 0) {
-                stat[col][0] = in ? top : 0.0f;
-                stat[col][1] = in ? 1.0f / sum : 0.0f;
-            }
-        }
+        join_stats(stat, a, group, u0, j, tid);
         __syncthreads();
         for (int page = sp.begin + wave; page < sp.end; page += kWaves * kPages) {
             Keys k[kPages];
@@ -377,25 +394,62 @@ Q38_DEV void observe_sums(const q38_observe_args &a) {
     }
 }
 
+/* The sums of a short context: a wave a page, from the scores that the statistics left. */
+Q38_DEV void observe_add(const q38_observe_args &a) {
+    __shared__ Stats stat;
+    const int j = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const int end = a.base_pos + a.n_tokens, pages = (end + 15) >> 4, page = blockIdx.x * kWaves + wave;
+    const bool live = page < pages;
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
+    for (int at = 0; at < a.n_groups; ++at) {
+        const int group = a.group0 + at, tiles = tiles_of(a, group);
+        f32x4 s[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) s[t] = q38_ld4(kept_scores(a, at, j, live ? page : 0, min(t, tiles - 1), lane));
+        __syncthreads(); /* the group before is done with stat */
+        join_stats(stat, a, at, group * Q38_OBSERVE_QUERIES, j, tid);
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            if (t >= tiles) continue;
+            const float top = stat[16 * t + c][0], inverse = stat[16 * t + c][1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __builtin_fmaf(q38_exp2(s[t][i] - top), inverse, w[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = q38_sum16(w[i]);
+    const int t0 = 16 * page + 4 * g;
+    if (c != 0 || t0 >= end) return;
+    float *sums = a.weights + (size_t)a.page_row[page] * Q38_WEIGHTS_PAGE + j * Q38_WEIGHTS_HEAD + 4 * g;
+    const f32x4 now = q38_ld4(sums) + w;
+    if (t0 + 4 <= end) {
+        q38_st4(sums, now);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (t0 + i < end) sums[i] = now[i];
+    }
+}
+
 }  // namespace
 
-#define Q38_OBSERVE_KERNEL(name, T, PAGES, PARTS)                                                                 \
+#define Q38_OBSERVE_STATS(name, T, PAGES, PARTS)                                                                 \
     extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_stats_##name(q38_observe_args a) {     \
         observe_stats<T, PAGES, PARTS>(a);                                                                       \
-    }                                                                                                            \
-    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_sums_##name(q38_observe_args a) {      \
-        observe_sums<T, PAGES, PARTS>(a);                                                                        \
     }
-#define Q38_OBSERVE_KERNELS(name, T)                      \
-    Q38_OBSERVE_KERNEL(name, T, kPagesOf<T>, 2)           \
-    Q38_OBSERVE_KERNEL(name##_short, T, 1, 2)
-/* few queries */
-#define Q38_OBSERVE_FEW(name, T)                          \
-    Q38_OBSERVE_KERNEL(name##_few, T, kPagesOf<T>, 3)     \
-    Q38_OBSERVE_KERNEL(name##_short_few, T, 1, 3)
-Q38_OBSERVE_KERNELS(f16, Q38_KV_F16)
-Q38_OBSERVE_KERNELS(bf16, Q38_KV_BF16)
-Q38_OBSERVE_FEW(bf16, Q38_KV_BF16)
-Q38_OBSERVE_KERNELS(q8k, Q38_KV_Q8)
-Q38_OBSERVE_KERNELS(mxfp4, Q38_KV_MX4)
-Q38_OBSERVE_FEW(mxfp4, Q38_KV_MX4)
+#define Q38_OBSERVE_SUMS(name, T, PARTS)                                                                         \
+    extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_sums_##name(q38_observe_args a) {      \
+        observe_sums<T, kPagesOf<T>, PARTS>(a);                                                                  \
+    }
+#define Q38_OBSERVE_KERNELS(name, suffix, T, PARTS)              \
+    Q38_OBSERVE_STATS(name##suffix, T, kPagesOf<T>, PARTS)       \
+    Q38_OBSERVE_STATS(name##_short##suffix, T, 1, PARTS)         \
+    Q38_OBSERVE_SUMS(name##suffix, T, PARTS)
+Q38_OBSERVE_KERNELS(f16, , Q38_KV_F16, 2)
+Q38_OBSERVE_KERNELS(bf16, , Q38_KV_BF16, 2)
+Q38_OBSERVE_KERNELS(bf16, _few, Q38_KV_BF16, 3)
+Q38_OBSERVE_KERNELS(q8k, , Q38_KV_Q8, 2)
+Q38_OBSERVE_KERNELS(mxfp4, , Q38_KV_MX4, 2)
+Q38_OBSERVE_KERNELS(mxfp4, _few, Q38_KV_MX4, 3)
+extern "C" __global__ __launch_bounds__(64 * kWaves) void q38_observe_add(q38_observe_args a) { observe_add(a); }

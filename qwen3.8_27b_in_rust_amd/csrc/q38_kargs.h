@@ -663,9 +663,10 @@ typedef struct {
  * of one kv head, Q38_OBSERVE_QUERIES queries a group.  Statistics: grid
  * (n_splits, 4, n_groups), 512 threads, the columns' maximum (log2 units) and sum
  * over a split's positions; sums: grid (splits of its own split_pages, 4), 512
- * threads. */
+ * threads; or, in a short context, the scores too and sums from them: grid
+ * (ceil(pages / 8), 4), 512 threads. */
 #define Q38_OBSERVE_QUERIES 16
-#define Q38_OBSERVE_PAGES 4 /* of keys that a wave holds, or one (a short context) */
+#define Q38_OBSERVE_PAGES 4 /* of keys that a wave holds, or one (scores kept) */
 #define Q38_OBSERVE_PAGES_Q8 3 /* of 8-bit rows, whose scales take registers too */
 #define Q38_OBSERVE_COLS (Q38_OBSERVE_QUERIES * Q38_ATTN_GROUP)
 typedef struct {
@@ -674,12 +675,13 @@ typedef struct {
     const int32_t *page_row; /* the sequence's page table */
     const float *q;          /* [n_tokens][24][256] */
     float *part_ml;          /* [n_groups][4][Q38_OBSERVE_COLS][n_splits][2] */
+    float *scores;           /* [n_groups][4][pages][6 tiles of 16 columns][64 lanes][4 tokens] */
     int32_t base_pos;
     int32_t n_tokens;
     int32_t split_pages;
     int32_t n_splits; /* of the statistics, 64 at most */
-    int32_t n_groups;
-    int32_t pad_;
+    int32_t n_groups; /* of this launch, */
+    int32_t group0;   /* from this one on */
 } q38_observe_args;
 
 #endif

@@ -71,14 +71,14 @@ int q38_scratch_address(int, void **ptr) {
 
 static hipFunction_t const kCopy = (hipFunction_t)0x1000, kSelect = (hipFunction_t)0x2000, kMove = (hipFunction_t)0x3000,
                            kStats = (hipFunction_t)0x4000, kSums = (hipFunction_t)0x5000, kWeigh = (hipFunction_t)0x6000,
-                           kWeighMerge = (hipFunction_t)0x7000, kRows = (hipFunction_t)0x8000;
+                           kWeighMerge = (hipFunction_t)0x7000, kRows = (hipFunction_t)0x8000, kAdd = (hipFunction_t)0x9000;
 static size_t arg_bytes(hipFunction_t f, int i) {
     if (f == kWeigh) return i ? sizeof(q38_weigh_args) : sizeof(q38_decode_typed_args);
     if (f == kWeighMerge) return i ? sizeof(q38_weigh_merge_args) : sizeof(q38_merge_args);
     if (i) return 0;
     if (f == kCopy) return sizeof(q38_kv_weights_args);
     if (f == kSelect || f == kMove) return sizeof(q38_evict_args);
-    if (f == kStats || f == kSums) return sizeof(q38_observe_args);
+    if (f == kStats || f == kSums || f == kAdd) return sizeof(q38_observe_args);
     return 0;
 }
 template <typename T>
@@ -125,11 +125,12 @@ struct Cache {
         ctx.f_weights_copy = kCopy;
         ctx.f_evict_select = kSelect;
         ctx.f_weigh_merge = kWeighMerge;
+        ctx.f_observe_add = kAdd;
         for (int i = 0; i < kKvTypeCount; ++i) {
             ctx.f_evict_move[i] = kMove;
             for (int v = 0; v < 2; ++v) {
                 ctx.f_observe_stats[i][v][0] = ctx.f_observe_stats[i][v][1] = kStats;
-                ctx.f_observe_sums[i][v][0] = ctx.f_observe_sums[i][v][1] = kSums;
+                ctx.f_observe_sums[i][v] = kSums;
                 ctx.f_weigh[i][v] = kWeigh;
             }
             for (q38_ctx::RowsKernel *k : {&ctx.f_kv_append[i], &ctx.f_kv_gather[i]}) k->many = k->few = kRows;
@@ -212,7 +213,7 @@ int main() {
     float *d_w = reinterpret_cast<float *>(0x50000000000ull);
     int32_t *d_t = reinterpret_cast<int32_t *>(0x60000000000ull);
     for (int type = 1; type < kKvTypeCount; ++type) {
-        Cache c(type, 2, 4000, 150, 4096);
+        Cache c(type, 2, 8000, 150, 25000);
         q38_kv *kv = c.kv;
         std::vector<int> ids;
         for (int i = 0; i < 150; ++i) {
@@ -288,15 +289,33 @@ int main() {
         /* a prompt's queries: every page of every group in one split of either launch, statistics inside the workspace */
         int big;
         REQUIRE(q38_seq_free(kv, ids.back()) == 0 && q38_seq_create(kv, &big) == 0);
-        for (int held : {16, 200, 4096}) {
+        for (int held : {16, 200, 4096, 24576, 24577}) {
             REQUIRE(q38_seq_reset(kv, big) == 0 && q38_seq_reserve(kv, big, held) == 0);
-            for (int n : {1, 16, 17, 160}) {
+            for (int n : {1, 16, 17, 160, 4096}) {
                 if (n > held) continue;
                 const float *q = reinterpret_cast<float *>(0x70000000000ull);
                 g_launches.clear();
-                REQUIRE(q38_attn_observe(kv, 3, big, held - n, n, q) == 0 && g_launches.size() == 2);
+                REQUIRE(q38_attn_observe(kv, 3, big, held - n, n, q) == 0 && g_launches.size() >= 2);
                 const auto a = arg<q38_observe_args>(g_launches[0]), s = arg<q38_observe_args>(g_launches[1]);
                 const int pages = (held + 15) / 16, groups = (n + 15) / 16;
+                if (g_launches[1].f == kAdd) {
+                    /* scores kept: every group in one batch, its statistics and scores inside the workspace */
+                    int next = 0;
+                    for (size_t l = 0; l < g_launches.size(); l += 2) {
+                        const auto x = arg<q38_observe_args>(g_launches[l]), y = arg<q38_observe_args>(g_launches[l + 1]);
+                        REQUIRE(!memcmp(&x, &y, sizeof(x)) && x.group0 == next && x.n_groups > 0 && x.n_tokens == n && x.base_pos == held - n);
+                        next += x.n_groups;
+                        REQUIRE(g_launches[l].f == kStats && g_launches[l].gy == 4 && (int)g_launches[l].gz == x.n_groups && (int)g_launches[l].gx == x.n_splits);
+                        REQUIRE(x.n_splits <= 64 && (x.n_splits - 1) * x.split_pages < pages && x.n_splits * x.split_pages >= pages);
+                        REQUIRE(g_launches[l + 1].f == kAdd && (int)g_launches[l + 1].gx == (pages + 7) / 8 && g_launches[l + 1].gy == 4 && g_launches[l + 1].gz == 1);
+                        const size_t stats = (size_t)x.n_groups * 4 * Q38_OBSERVE_COLS * x.n_splits * 8;
+                        REQUIRE(inside(x.part_ml, stats) && (char *)x.scores >= (char *)x.part_ml + stats && (uintptr_t)x.scores % 16 == 0);
+                        REQUIRE(inside(x.scores, (size_t)x.n_groups * 4 * pages * Q38_OBSERVE_COLS * 16 * 4));
+                        REQUIRE(x.page_row == kv->d_page_table + (size_t)big * kv->pt_stride && x.weights == kv->weights_of(0));
+                    }
+                    REQUIRE(next == groups);
+                    continue;
+                }
                 REQUIRE(g_launches[0].f == kStats && g_launches[0].gy == 4 && (int)g_launches[0].gz == groups && a.n_groups == groups);
                 REQUIRE((int)g_launches[0].gx == a.n_splits && a.n_splits <= 64 && (a.n_splits - 1) * a.split_pages < pages && a.n_splits * a.split_pages >= pages);
                 REQUIRE(g_launches[1].f == kSums && g_launches[1].gy == 4 && g_launches[1].gz == 1 && s.n_splits == a.n_splits);

@@ -280,6 +280,29 @@ def test_observe(pkg, ctx, ty, base, n):
         assert np.array_equal(_bits(c.weights(s, P + 5)[0]), _bits(got))
 
 
+@pytest.mark.parametrize("ty,P,n", [(ty, P, n) for ty in sorted(TYPES) for P, n in ((24576, 2), (24577, 1), (24600, 19))] +
+                         [("bf16", 4800, 300), ("q8_k", 4800, 300)])
+def test_observe_long_and_many(pkg, ctx, ty, P, n):
+    """Contexts on both sides of the one from which scores are formed twice, and more groups of queries than are kept at once."""
+    rng = np.random.default_rng(P + n)
+    K, Q = _rows(rng, P), _q(rng, n)
+    with Cache(pkg, ctx, ty, [P]) as c:
+        s = c.seqs[0]
+        c.kv.write(3, s, 0, P, ctx.array(K), ctx.array(K))
+        c.kv.attn_observe(3, s, P - n, n, ctx.array(Q))
+        got, _ = c.weights(s, P)
+        k = stored(K, ty)
+        want, bound = np.zeros((P, 4)), np.zeros((P, 4))
+        for u in range(n):
+            w, e = weights_of(Q[u], k[:P - n + u + 1], OBSERVE[ty])
+            want[:P - n + u + 1] += w
+            bound[:P - n + u + 1] += e
+        _held(got, want, bound + 7 * n * U * want)
+        c.kv.weights_put(3, [s], [0], [P])
+        c.kv.attn_observe(3, s, P - n, n, ctx.array(Q))
+        assert np.array_equal(_bits(c.weights(s, P)[0]), _bits(got))
+
+
 @typed
 def test_observe_equals_decode_steps(pkg, ctx, ty):
     """A long context with large and small queries: the sums of one call against those of decode steps."""

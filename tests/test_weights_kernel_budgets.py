@@ -19,8 +19,9 @@ KERNELS = {
     "attn_decode_mxfp4": ([f"q38_attn_decode_mxfp4{p}" for p in ("", "_pre", "_one", "_pre_one")], 256),
     "kv_rows_mxfp4": ([f"q38_kv_{c}_mxfp4{s}" for c in ("append", "gather") for s in ("", "_few")], 64),
     "attn_weigh": ([f"q38_attn_weigh_{t}{p}" for t in TYPES for p in ("", "_pre")] + ["q38_attn_weigh_merge"], 256),
-    "attn_observe": ([f"q38_observe_{c}_{t}{s}" for c in ("stats", "sums") for t in TYPES for s in ("", "_short")] +
-                     [f"q38_observe_{c}_{t}{s}_few" for c in ("stats", "sums") for t in ("bf16", "mxfp4") for s in ("", "_short")], 256),
+    "attn_observe": ([f"q38_observe_{c}_{t}" for c in ("stats", "sums") for t in TYPES + ("bf16_few", "mxfp4_few")] +
+                     [f"q38_observe_stats_{t}" for t in [t + "_short" for t in TYPES] + ["bf16_short_few", "mxfp4_short_few"]] +
+                     ["q38_observe_add"], 256),
     "kv_weights": (["q38_kv_weights_copy", "q38_kv_evict_select"] + [f"q38_kv_evict_move_{t}" for t in TYPES], 128),
 }
 
