@@ -248,6 +248,66 @@ def test_a_stored_row_starts_at_zero(pkg, ctx):
         assert not w[90:].any() and np.array_equal(t[90:].reshape(-1), np.arange(28, 68)) and np.array_equal(w[:90], mark[:90])
 
 
+@typed
+@pytest.mark.parametrize("P", [2049, 4096])
+def test_decode_of_one_long_split(pkg, ctx, ty, P):
+    """A split of more tokens than its workgroup's threads take at once adds its sums in the decode launch."""
+    rng = np.random.default_rng(P)
+    K, Q = _rows(rng, P), _q(rng)
+    with Cache(pkg, ctx, ty, [P]) as c, decode_split(ctx, 4096):
+        s, o = c.seqs[0], ctx.empty((24, 256))
+        c.kv.write(3, s, 0, P - 1, ctx.array(K), ctx.array(K))
+        last = ctx.array(K[-1:])
+        c.kv.attn_decode(3, [s], [P - 1], ctx.array(Q), o, k_new=last, v_new=last)
+        got, t = c.weights(s, P)
+        want, bound = weights_of(Q[0], stored(K, ty))
+        _held(got, want, bound)
+        assert np.array_equal(t, np.repeat(np.arange(P)[:, None], 4, 1))
+
+
+def test_two_caches_of_one_context(pkg, ctx):
+    """Calls on two tracking caches in turn, with one workspace between them, give what each gives by itself, bit for bit."""
+    rng = np.random.default_rng(3)
+    lengths, n = {"mxfp4": 700, "bf16": 300}, 20
+    K = {ty: _rows(rng, P) for ty, P in lengths.items()}
+    Q = {ty: _q(rng, n) for ty in lengths}
+
+    def steps(c, ty, out):
+        """One call of the run after the other."""
+        s, P, q = c.seqs[0], lengths[ty], ctx.array(Q[ty])
+        c.kv.write(3, s, 0, P, ctx.array(K[ty]), ctx.array(K[ty]))
+        yield
+        c.kv.attn_observe(3, s, P - n, n, q)
+        yield
+        o = ctx.empty((24, 256))
+        held = P
+        for u in range(6):
+            new = ctx.array(K[ty][u:u + 1])
+            c.kv.attn_decode(3, [s], [held], q.offset(u * 6144), o, k_new=new, v_new=new)
+            yield
+            out.append(_bits(o.download()))
+            held += 1
+            if u == 2:
+                c.kv.evict([s], [held], [200], [16])
+                held = 200
+                yield
+        out.extend([_bits(c.weights(s, held)[0]), c.weights(s, held)[1]] + [_bits(x) for x in c.rows(s, held)])
+
+    alone, together = {}, {}
+    for ty in lengths:
+        with Cache(pkg, ctx, ty, [lengths[ty]]) as c:
+            for _ in steps(c, ty, alone.setdefault(ty, [])):
+                pass
+    with Cache(pkg, ctx, "mxfp4", [700]) as c, Cache(pkg, ctx, "bf16", [300]) as d:
+        runs = [steps(c, "mxfp4", together.setdefault("mxfp4", [])), steps(d, "bf16", together.setdefault("bf16", []))]
+        while runs:
+            runs = [r for r in runs if next(r, "done") != "done"]
+    for ty in lengths:
+        assert len(alone[ty]) == len(together[ty]) == 10
+        for x, y in zip(alone[ty], together[ty]):
+            assert np.array_equal(x, y)
+
+
 # ------------------------------------------------------------------ a prompt's queries
 
 
