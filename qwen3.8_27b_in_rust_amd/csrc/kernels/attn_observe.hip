@@ -250,7 +250,7 @@ Q38_DEV void observe_stats(const q38_observe_args &a) {
             if (__any(top > (none ? -INFINITY : kRefSlack))) {
                 const float by = none ? (top == -INFINITY ? 0.0f : top) : fmaxf(top, 0.0f);
                 if (!none || top != -INFINITY) M[t] = base + by;
-                L[t] *= q38_exp2(-by); /* (nothing where there is no reference yet) */
+                L[t] *= none ? 0.0f : q38_exp2(-by); /* (a first reference below -128 has no finite power: 0 times it is none) */
 #pragma unroll
                 for (int p = 0; p < kPages; ++p)
 #pragma unroll
