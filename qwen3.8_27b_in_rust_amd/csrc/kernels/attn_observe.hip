@@ -155,6 +155,9 @@ Q38_DEV void scores_of(const Keys (&k)[kPages], const Step (&part)[kParts][8], f
     asm volatile("" : "+v"(lane));
     constexpr int kSums = kInBf16<T> ? 1 : 2;
     const float first = kInBf16<T> ? -base : 0.0f;
+    /* 8-bit rows: a query's unit below 1 before the row's scale and one above after it, as their product may pass f32's
+     * end where the score does not */
+    const float below = fminf(unscale, 1.0f), above = fmaxf(unscale, 1.0f);
     f32x4 c[kPages][kSums];
 #pragma unroll
     for (int p = 0; p < kPages; ++p)
@@ -176,7 +179,7 @@ Q38_DEV void scores_of(const Keys (&k)[kPages], const Step (&part)[kParts][8], f
                 s[p][i] = c[p][0][i];
             } else {
                 const float x = __builtin_fmaf(c[p][kSums - 1][i], 1.0f / kLowUnit<T>, c[p][0][i]);
-                s[p][i] = __builtin_fmaf(x, T == Q38_KV_Q8 ? unscale * k[p].scale[i] : unscale, -base);
+                s[p][i] = T == Q38_KV_Q8 ? __builtin_fmaf(x * below * k[p].scale[i], above, -base) : __builtin_fmaf(x, unscale, -base);
             }
         }
 }

@@ -101,3 +101,31 @@ def test_first_look_at_very_low_scores(pkg, ctx, ty):
             # equal scores: six heads' weights of 1 / P
             got = _observed(pkg, ctx, ty, K, Q)
             assert np.all(np.abs(got.astype(np.float64) - 6.0 / P) <= 6.0 / P * (P + 40) * U), (P, low, got)
+
+
+def _far_sizes(case, P, n):
+    """Scores of ordinary size from queries near an end of the f32 range: their powers of two and the rows' scales, multiplied
+    in one order or another, need not be within it."""
+    rng = np.random.default_rng(P + n)
+    K, Q = _rows(rng, P), rng.uniform(-2e38, 2e38, (n, 24, 256)).astype(np.float32)
+    if case == "small_keys":
+        return K * np.float32(1e-36), Q  # scores of some hundred
+    # large keys, but where the queries are; or the other way round
+    K *= 1e7
+    K[:, ::256] = 0.0
+    Q[:, :, 1:] = 0.0
+    if case == "small_queries":
+        K[:, ::256] = 1e38 * np.sign(rng.standard_normal((P, 4)))
+        Q[:, :, 0] = rng.uniform(-1e-37, 1e-37, (n, 24))
+    return K, Q
+
+
+far_sizes = pytest.mark.parametrize("case", ["zero_products", "small_keys", "small_queries"])
+
+
+@far_sizes
+@pytest.mark.parametrize("P,n", [(SHORT, 3), (LONG, 2)])
+def test_observe_queries_and_scales_of_far_sizes(pkg, ctx, case, P, n):
+    K, Q = _far_sizes(case, P, n)
+    want, bound = _want("q8_k", K, Q, OBSERVE["q8_k"])
+    _held(_observed(pkg, ctx, "q8_k", K, Q), want, bound)
