@@ -177,7 +177,7 @@ Q38_DEV uint32_t pack16(uint16_t lo, uint16_t hi) { return (uint32_t)hi << 16 | 
  * values.  valid: tokens of the page that count (16 but for the sequence's
  * last page); first: nothing is summed yet. */
 template <int T, bool kWeigh = false>
-Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64], float unscale, int valid, bool first,
+Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64], float unscale, float above, int valid, bool first,
                        int lane, float *scores = nullptr) {
     const int c = lane & 15, g = lane >> 4;
     f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
@@ -212,7 +212,7 @@ Q38_DEV void page_step(State &st, const Page<T> &p, const q38_u32x4 (*q)[8][64],
         const float x = s0[i] + s1[i];
         const float y = kInBf16<T> ? x : x * unscale;
         s[i] = y + row_ror8(y);
-        if (T == Q38_KV_Q8) s[i] *= ks[i];
+        if (T == Q38_KV_Q8) s[i] = s[i] * ks[i] * above;
         if (valid < 16 && 4 * g + i >= valid) {
             s[i] = -INFINITY;
             vs[i] = 0.0f;
@@ -792,7 +792,10 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
     const int c = lane & 15, g = lane >> 4;
 
     if (wave < n_pages) {
-        const float unscale = q_unscale[c & 7] * (c < 8 ? 1.0f : 1.0f / kLowUnit<T>); /* the column's */
+        /* the column's unit; 8-bit rows: one below 1 before the row's scale and one above after it (a query near f32's
+         * end over small keys has products with its unit past that end, where the scores are not) */
+        const float unit = q_unscale[c & 7], above = fmaxf(unit, 1.0f);
+        const float unscale = (T == Q38_KV_Q8 ? fminf(unit, 1.0f) : unit) * (c < 8 ? 1.0f : 1.0f / kLowUnit<T>);
         State st;
         st.ref = -INFINITY;
         st.l = 0.0f;
@@ -833,7 +836,7 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
                         valid = t_end - t_begin - Q38_PAGE_TOKENS * at;
                         if (has_pos && a.k_new != nullptr) put_new_token<T>(buf[u][0], new_rows, valid - 1, lane);
                     }
-                    page_step<T, kWeigh>(st, buf[u][0], q_frag, unscale, valid, at == wave, lane, scores);
+                    page_step<T, kWeigh>(st, buf[u][0], q_frag, unscale, above, valid, at == wave, lane, scores);
                     fetch(buf[u][0], at + kWaves * kDepth);
                 }
             }

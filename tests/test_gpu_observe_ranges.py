@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 from parity import decode_split
 from test_gpu_weights import DECODE, OBSERVE, Cache, U, _held, _q, _rows, stored, typed, weights_of
+from typed_rows import attend
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +130,21 @@ def test_observe_queries_and_scales_of_far_sizes(pkg, ctx, case, P, n):
     K, Q = _far_sizes(case, P, n)
     want, bound = _want("q8_k", K, Q, OBSERVE["q8_k"])
     _held(_observed(pkg, ctx, "q8_k", K, Q), want, bound)
+
+
+@far_sizes
+def test_decode_queries_and_scales_of_far_sizes(pkg, ctx, case):
+    """Outputs and sums of a decode call."""
+    K, Q = _far_sizes(case, SHORT, 1)
+    V = _rows(np.random.default_rng(1), SHORT)
+    want, bound = _want("q8_k", K, Q, DECODE)
+    out, off = attend(Q[0], stored(K, "q8_k"), stored(V, "q8_k"))
+    with Cache(pkg, ctx, "q8_k", [SHORT]) as c:
+        c.kv.write(3, c.seqs[0], 0, SHORT, ctx.array(K), ctx.array(V))
+        o = ctx.empty((24, 256))
+        for tracks in (True, False):
+            c.kv.track_weights(tracks)
+            c.kv.attn_decode(3, c.seqs, [SHORT - 1], ctx.array(Q), o)
+            assert np.all(np.abs(o.download() - out) <= off)
+            if tracks:
+                _held(c.weights(c.seqs[0], SHORT)[0], want, bound)
