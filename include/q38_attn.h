@@ -231,6 +231,10 @@ int q38_kv_weights_get(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids,
  * the cache, give causally to all positions up to their own.  All of a prompt's
  * queries, or its last ones, as the caller wants them to count.  It cannot be captured. */
 int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens, const float *d_q);
+/* What q38_attn_observe keeps of a query over BF16 and MXFP4 rows: 3 bf16 parts (the default), all
+ * of its bits as in a decode, or 2, for a third fewer products: 16 bits, which leave up to 2^-16 of
+ * sum |q k| / 16 of a score, and so of a weight.  Over F16 and Q8_K rows it keeps 22 bits either way. */
+int q38_set_observe_parts(q38_ctx *ctx, int parts);
 
 /* Of the n_tokens[b] tokens that sequence seq_ids[b] holds (positions 0 ..
  * n_tokens[b] - 1, written in every layer), n_keep[b] stay, in each layer and kv

@@ -62,6 +62,7 @@ _SIGNATURES = {
     "q38_sync": (c_int, [_P]),
     "q38_device_info": (c_int, [_P, POINTER(c_int), POINTER(c_int), POINTER(c_int), c_char_p, c_size_t]),
     "q38_set_decode_split": (c_int, [_P, c_int]),
+    "q38_set_observe_parts": (c_int, [_P, c_int]),
     "q38_alloc": (c_int, [_P, c_size_t, POINTER(c_void_p)]),
     "q38_free": (c_int, [_P, _P]),
     "q38_upload": (c_int, [_P, _P, _P, c_size_t]),
@@ -265,6 +266,10 @@ class Context:
     def set_decode_split(self, tokens: int) -> None:
         """Context tokens per decode workgroup (multiple of 16), 0 = automatic."""
         _check(lib().q38_set_decode_split(self.handle, int(tokens)), "q38_set_decode_split")
+
+    def set_observe_parts(self, parts: int) -> None:
+        """Parts of an observed query over BF16 and MXFP4 rows: 3 keep all of its bits, 2 keep 16."""
+        _check(lib().q38_set_observe_parts(self.handle, int(parts)), "q38_set_observe_parts")
 
     def stream(self) -> int:
         return lib().q38_ctx_stream(self.handle)

@@ -140,11 +140,11 @@ constexpr KvType kKvTypes[] = {
     {Q38_GGML_MXFP4, Q38_KV_PAGE_MX4, "mxfp4", true},
 };
 constexpr int kKvTypeCount = (int)(sizeof(kKvTypes) / sizeof(kKvTypes[0]));
-/* q38_attn_observe's kernels over rows of a type, for a short context and for few queries (bf16 operands, which take
- * a third part of theirs then). */
-std::string observe_name(int type, int short_context, int few) {
+/* q38_attn_observe's kernels over rows of a type, for a short context and with queries in three parts (of bf16 operands;
+ * the others' are whole in two). */
+std::string observe_name(int type, int short_context, int three) {
     const int ty = kKvTypes[type].ggml_type;
-    const bool third = few && (ty == Q38_GGML_BF16 || ty == Q38_GGML_MXFP4);
+    const bool third = three && (ty == Q38_GGML_BF16 || ty == Q38_GGML_MXFP4);
     return std::string(kKvTypes[type].suffix) + (short_context ? "_short" : "") + (third ? "_few" : "");
 }
 /* q38_add_rms_norm's kernels that hold a row in registers: 256 or 1024
@@ -206,7 +206,7 @@ struct q38_ctx {
     hipFunction_t f_weights_copy = nullptr;
     hipFunction_t f_evict_select = nullptr;
     hipFunction_t f_evict_move[kKvTypeCount] = {};
-    /* [1]: a short context; [][1]: few queries */
+    /* [1]: a short context; [][1]: queries in three parts */
     hipFunction_t f_observe_stats[kKvTypeCount][2][2] = {}, f_observe_sums[kKvTypeCount][2] = {};
     hipFunction_t f_observe_add = nullptr;
     hipModule_t mod_rows_own[kKvTypeCount] = {}, mod_decode_own[kKvTypeCount] = {}; /* types with own_objects */
@@ -244,6 +244,7 @@ struct q38_ctx {
     int decode_block = 64 * Q38_DECODE_WAVES; /* threads of a decode workgroup (the kernel's launch bound) */
     int gdn_decode_block = 512;               /* threads of a q38_gdn_decode workgroup (its launch bound) */
     int split_tokens = 0; /* context tokens per decode workgroup; 0: chosen per launch */
+    int observe_parts = 3; /* of an observed query over bf16 operands */
     int clock_khz = 0;
     int lds_bytes = 0;
     int lds_per_cu = 0;
@@ -681,6 +682,13 @@ int q38_set_decode_split(q38_ctx *ctx, int tokens) {
         return fail("split of %d tokens: 0, or a multiple of %d in %d..%d", tokens, Q38_PAGE_TOKENS, Q38_PAGE_TOKENS,
                     Q38_MAX_SPLIT_TOKENS);
     ctx->split_tokens = tokens;
+    return 0;
+}
+
+int q38_set_observe_parts(q38_ctx *ctx, int parts) {
+    if (ctx == nullptr) return fail("ctx is NULL");
+    if (parts != 2 && parts != 3) return fail("%d parts of a query: 2 or 3", parts);
+    ctx->observe_parts = parts;
     return 0;
 }
 
@@ -1405,19 +1413,21 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     /* A workgroup a CU (64 splits at most, which are joined four lanes to a column).  Up to three pages a wave the
      * statistics take one at a time and keep the scores for the sums; from there on, with scores of as many bytes as
      * several passes over the keys, a wave takes several pages and the sums form the scores again (us, kept against
-     * formed again: 7 queries over 1000 / 8K / 24K / 32K tokens of bf16 11.3 / 13.4 / 25.2 / 30.2 against 24.6 / 24.7 /
-     * 33.9 / 38.3, of MXFP4 11.4 / 13.3 / 25.4 / 30.0 against 24.1 / 24.4 / 26.0 / 27.0; 32 over 8K / 24K / 32K of MXFP4
-     * 28.2 / 48.0 / 60.8 against 43.9 / 54.1 / 58.1; 1024 over 4K / 16K / 24K / 32K 311 / 856 / 1337 / 1810 against 901 /
-     * 1067 / 1206 / 1346). */
+     * formed again, queries in three parts: 7 queries over 1000 / 8K / 24K / 32K tokens of bf16 11.4 / 13.6 / 25.3 / 30.4
+     * against 24.4 / 24.9 / 33.8 / 38.4, of MXFP4 11.3 / 13.4 / 25.4 / 30.0 against 24.0 / 24.4 / 26.0 / 27.2, of Q8_K 11.7 /
+     * 13.9 / 24.1 / 28.9 against 21.4 / 21.9 / 24.8 / 34.7; 32 over 8K / 24K / 32K of MXFP4 31.3 / 54.5 / 70.1 against 54.8 /
+     * 67.6 / 70.3; 1024 over 4K / 16K / 24K / 32K of bf16 362 / 1028 / 1606 / 2146 against 1206 / 1528 / 1749 / 1963).  Where the
+     * sides cross depends on the type and the queries too, from 24K tokens (1024 over Q8_K 1450 against 1380) to past 32K (7
+     * and 32 over bf16). */
     const int pages = (int)((end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS);
     const int slots = std::min(std::max(ctx->cu_count / Q38_ATTN_KV_HEADS, 1), 64);
     const int held = kKvTypes[kv->type].ggml_type == Q38_GGML_Q8_K ? Q38_OBSERVE_PAGES_Q8 : Q38_OBSERVE_PAGES;
     const int is_short = pages <= 3 * slots * Q38_DECODE_TYPED_WAVES ? 1 : 0;
     const int step = Q38_DECODE_TYPED_WAVES * (is_short ? 1 : held);
-    const int few = a.n_groups == 1 ? 1 : 0;
+    const int three = ctx->observe_parts == 3 ? 1 : 0;
     auto split_for = [&](int wanted) { return ((pages + wanted - 1) / wanted + step - 1) / step * step; };
     /* scores kept are those of as many groups at once as 128 MB hold, which the last level's cache does too (1024 queries
-     * over 4K tokens with 16 / 32 / 64 / 128 / 256 MB: 558 / 421 / 349 / 311 / 344); else the statistics of all groups at once */
+     * in two parts over 4K tokens with 16 / 32 / 64 / 128 / 256 MB: 558 / 421 / 349 / 311 / 344); else the statistics of all groups at once */
     const int groups = a.n_groups;
     const size_t kept = is_short ? (size_t)pages * Q38_ATTN_KV_HEADS * Q38_OBSERVE_COLS * Q38_PAGE_TOKENS * sizeof(float) : 0;
     const int batch = is_short ? (int)std::min<size_t>(groups, std::max<size_t>((128u << 20) / kept, 1)) : groups;
@@ -1436,14 +1446,14 @@ int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
     const unsigned block = 64 * Q38_DECODE_TYPED_WAVES;
     for (a.group0 = 0; a.group0 < groups; a.group0 += batch) {
         a.n_groups = std::min(batch, groups - a.group0);
-        if (ctx->launch(ctx->f_observe_stats[kv->type][is_short][few], a.n_splits, Q38_ATTN_KV_HEADS, a.n_groups, block, &a)) return -1;
+        if (ctx->launch(ctx->f_observe_stats[kv->type][is_short][three], a.n_splits, Q38_ATTN_KV_HEADS, a.n_groups, block, &a)) return -1;
         if (is_short && ctx->launch(ctx->f_observe_add, (pages + Q38_DECODE_TYPED_WAVES - 1) / Q38_DECODE_TYPED_WAVES, Q38_ATTN_KV_HEADS, 1, block, &a))
             return -1;
     }
     if (is_short) return 0;
     a.group0 = 0;
     a.split_pages = split_for(slots);
-    return ctx->launch(ctx->f_observe_sums[kv->type][few], (pages + a.split_pages - 1) / a.split_pages, Q38_ATTN_KV_HEADS, 1, block, &a);
+    return ctx->launch(ctx->f_observe_sums[kv->type][three], (pages + a.split_pages - 1) / a.split_pages, Q38_ATTN_KV_HEADS, 1, block, &a);
 }
 
 int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n_tokens, const int32_t *n_keep,

@@ -14,21 +14,22 @@
  * S^T = K Q^T as in the decode (q38_decode_typed.h: a cached value is an operand
  * as it stands, a query is split into parts whose sum it is), but with 16 real
  * columns a product.  f16 operands take a query's two parts (22 bits), bf16 ones
- * three (24) for up to 16 queries and two for more: rounded to nearest they leave
- * 2^-16 of it at most, as the prefill's do, which half as many products again would
- * keep, and which sums over more than 16 queries hardly see (32 queries over 32K
- * tokens lie within 3e-7 of 64 bits; 7 over 1000 would within 6e-7, one within 2e-6).
+ * three, which are all of its 24 bits; two of them, rounded to nearest, leave 2^-16
+ * of a query, and over scores of 60 some 3e-4 of a weight: only where the caller asks
+ * for them (q38_set_observe_parts).
  * A workgroup keeps the parts of 16 queries' 96 columns in LDS; a wave holds kPages
  * pages of keys as operands and reads each part once for all of them (one page where it keeps
  * scores).  Groups of queries come one after the other in a workgroup of the second
  * launch, so that every sum has one owner and a fixed order.
  *
- * Measured: 32 queries over 32K tokens of MXFP4, formed twice, 25.9 us for the statistics
- * and 32.7 for the sums.  The products of two parts are 25.8 GFLOP a launch, 20.5 us at
- * the 1260 TFLOP/s of a large library product: 79 and 63% of that rate (the keys, 19
- * MB, would take 3); what is left is the vector unit's masks, exponentials and sums
- * over columns, 57 and 67 instructions a page and tile beside 16 products.  7 queries over
- * 1000 tokens of bf16, scores kept, 8.2 and 4.0: 32 workgroups, a wave a page, bound by the
+ * Measured: 32 queries over 32K tokens of MXFP4, formed twice, 34.1 us for the statistics
+ * and 43.5 for the sums (26.6 and 33.4 with two parts).  The products of three parts are 38.7
+ * GFLOP a launch, which keep the matrix unit busy for 3.775e7 cycles, 15 us on 1024 SIMDs: 45
+ * and 35% (the keys, 19 MB, would take 3).  The rest is the vector unit's masks, exponentials and
+ * sums over columns, 68 and 82 instructions a page and tile beside 24 products, and the
+ * parts' way from LDS: the branches at each tile keep one tile's products from
+ * running beside the exponentials of the one before.  7 queries over
+ * 1000 tokens of bf16, scores kept, 8.1 and 3.5: 32 workgroups, a wave a page, bound by the
  * chains queries - parts in LDS - keys - join and scores - join - sums.
  */
 #include "q38_decode_typed.h"
