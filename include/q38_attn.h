@@ -214,10 +214,15 @@ int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
 int q38_kv_track_weights(q38_kv *kv, int enable);
 /* Tokens of the sequence that evictions have taken out so far. */
 int q38_seq_evicted(q38_kv *kv, int seq, int *n_tokens);
+/* A sequence handed on from another cache: n_tokens, q38_seq_evicted's there, and n_keep, its last
+ * eviction's, as if its evictions had been made here.  For a sequence that has evicted none, once
+ * its rows, sums and own positions are stored (q38_kv_gather and q38_kv_weights_get there,
+ * q38_kv_write and q38_kv_weights_put with d_tokens here). */
+int q38_seq_set_evicted(q38_kv *kv, int seq, int n_tokens, int n_keep);
 
 /* Sums and own positions of a ragged batch of reserved positions, packed in
  * order in rows [rows][4 kv heads] as q38_kv_gather's, to hand a sequence on
- * with them or to look at them.  put: d_weights NULL sets zeros, d_tokens NULL
+ * with them (and q38_seq_set_evicted) or to look at them.  put: d_weights NULL sets zeros, d_tokens NULL
  * what a row stored there has, position + evicted tokens; a sequence once a
  * call.  get: either may be NULL, not both. */
 int q38_kv_weights_put(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,

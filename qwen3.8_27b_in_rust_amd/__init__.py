@@ -83,6 +83,7 @@ _SIGNATURES = {
     "q38_kv_gather": (c_int, [_P, c_int, c_int, _I32P, _I32P, _I32P, c_int, _P, _P]),
     "q38_kv_track_weights": (c_int, [_P, c_int]),
     "q38_seq_evicted": (c_int, [_P, c_int, POINTER(c_int)]),
+    "q38_seq_set_evicted": (c_int, [_P, c_int, c_int, c_int]),
     "q38_kv_weights_put": (c_int, [_P, c_int, c_int, _I32P, _I32P, _I32P, _P, _P]),
     "q38_kv_weights_get": (c_int, [_P, c_int, c_int, _I32P, _I32P, _I32P, _P, _P]),
     "q38_attn_observe": (c_int, [_P, c_int, c_int, c_int, c_int, _P]),
@@ -480,6 +481,10 @@ class KVCache:
         n = c_int()
         _check(lib().q38_seq_evicted(self.handle, seq, ctypes.byref(n)), "q38_seq_evicted")
         return n.value
+
+    def seq_set_evicted(self, seq, n_tokens, n_keep) -> None:
+        """A handed-on sequence's evicted tokens so far, and how many its last eviction kept."""
+        _check(lib().q38_seq_set_evicted(self.handle, seq, n_tokens, n_keep), "q38_seq_set_evicted")
 
     def weights_put(self, layer, seq_ids, pos0, n_tokens, weights=None, tokens=None):
         """Sums (None: zeros) and own positions (None: the rows' places) of a ragged batch, rows of 4 kv heads."""

@@ -1316,6 +1316,9 @@ int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
 
 /* ------------------------------------------- sums of attention weights, eviction */
 
+/* tokens that a sequence with evictions may have read */
+constexpr int32_t kMaxRead = 1 << 30;
+
 static int check_tracks(const q38_kv *kv) {
     if (kv == nullptr) return fail("kv is NULL");
     if (!kv->tracks) return fail("the cache does not track weights (q38_kv_track_weights)");
@@ -1361,6 +1364,19 @@ int q38_seq_evicted(q38_kv *kv, int seq, int *n_tokens) {
     if (kv == nullptr || n_tokens == nullptr) return fail("NULL argument");
     if (kv->check_seq(seq)) return -1;
     *n_tokens = kv->evicted_of(seq);
+    return 0;
+}
+
+int q38_seq_set_evicted(q38_kv *kv, int seq, int n_tokens, int n_keep) {
+    if (check_tracks(kv)) return -1;
+    if (kv->check_seq(seq)) return -1;
+    if (n_tokens < 0 || n_keep < 0) return fail("negative count");
+    if (n_tokens > kMaxRead) return fail("sequence %d has read more than 2^30 tokens", seq);
+    if (n_tokens == 0 && n_keep > 0) return fail("an eviction that takes no tokens out keeps %d of them", n_keep);
+    if (n_keep > kv->seq_pages[seq] * Q38_PAGE_TOKENS) return fail("sequence %d: %d tokens are not reserved", seq, n_keep);
+    if (kv->evicted[seq].tokens > 0) return fail("sequence %d has evicted tokens", seq);
+    kv->evicted[seq].tokens = n_tokens;
+    kv->evicted[seq].kept = n_keep;
     return 0;
 }
 
@@ -1476,7 +1492,7 @@ int q38_kv_evict(q38_kv *kv, int n_seq, const int32_t *seq_ids, const int32_t *n
             return fail("sequence %d holds %d tokens since its last eviction, not %d", s, kv->evicted[s].kept, n_tokens[b]);
         if (n_keep[b] > n_tokens[b]) return fail("sequence %d: %d tokens to keep of %d", s, n_keep[b], n_tokens[b]);
         if (n_recent[b] > n_keep[b]) return fail("sequence %d: %d recent tokens to keep among %d", s, n_recent[b], n_keep[b]);
-        if ((long)kv->evicted[s].tokens + n_tokens[b] > (1L << 30)) return fail("sequence %d has read more than 2^30 tokens", s);
+        if ((long)kv->evicted[s].tokens + n_tokens[b] > kMaxRead) return fail("sequence %d has read more than 2^30 tokens", s);
         max_moves = std::max<long>(max_moves, std::min(n_keep[b], n_tokens[b] - n_keep[b]));
     }
     if (check_not_capturing(kv, "an eviction")) return -1;
