@@ -196,7 +196,9 @@ int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
  * q38_kv_write and q38_attn_prefill, which take cache positions as ever;
  * q38_kv_append refuses a sequence that has evicted tokens.  Rows that stay keep
  * the turn that they were stored with.  Positions below the last eviction's n_keep are
- * in no order: rows are stored from n_keep on (others fail with -1), and
+ * in no order: rows are stored from n_keep on, decode calls without a new row and
+ * prefills without rows go on from n_keep - 1 at least, past all that were kept
+ * (others fail with -1), and
  * q38_seq_truncate goes back to n_keep or to 0, not between.
  * q38_seq_reset, a truncate to 0 and q38_seq_set_pages begin anew, with none
  * evicted. */
@@ -234,7 +236,9 @@ int q38_kv_weights_get(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids,
  * that the queries d_q [n_tokens][24][256] (post-norm, post-RoPE, 16-byte
  * aligned) of positions base_pos .. base_pos + n_tokens - 1, whose rows are in
  * the cache, give causally to all positions up to their own.  All of a prompt's
- * queries, or its last ones, as the caller wants them to count.  It cannot be captured. */
+ * queries, or its last ones, as the caller wants them to count.  Of a sequence that has
+ * evicted tokens a query below the last eviction's n_keep - 1 counts by place: for the tokens at
+ * positions up to its own, whichever these are in each kv head.  It cannot be captured. */
 int q38_attn_observe(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens, const float *d_q);
 /* What q38_attn_observe keeps of a query over BF16 and MXFP4 rows: 3 bf16 parts (the default), all
  * of its bits as in a decode, or 2, for a third fewer products: 16 bits, which leave up to 2^-16 of

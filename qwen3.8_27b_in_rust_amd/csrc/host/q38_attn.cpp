@@ -357,7 +357,8 @@ struct q38_kv {
     float *weights_of(int slot) const { return weights + (size_t)slot * slot_sums(); }
     int32_t *tokens_of(int slot) const { return reinterpret_cast<int32_t *>(weights_of(slot)) + Q38_PAGE_TOKENS; }
     int32_t evicted_of(int seq) const { return tracks ? evicted[seq].tokens : 0; }
-    /* Rows are stored past what the last eviction has left. */
+    /* Rows are stored past what the last eviction has left, and attended to up to `pos` where that takes in all of it. */
+    int check_read(int seq, long pos) const { return check_store(seq, pos + 1); }
     int check_store(int seq, long pos) const {
         if (tracks && pos < evicted[seq].kept)
             return fail("sequence %d: positions before %d have been in no order since the last eviction", seq, evicted[seq].kept);
@@ -1877,6 +1878,8 @@ int validate_decode(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, co
             pages_needed += std::max(0, need - kv->seq_pages[s]);
         } else if (need > kv->seq_pages[s]) {
             return fail("sequence %d: position %d is not reserved", s, positions[b]);
+        } else if (kv->check_read(s, positions[b])) {
+            return -1;
         }
     }
     if (pages_needed > (long)kv->free_pages.size())
@@ -2468,7 +2471,7 @@ int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
                     kv->pt_stride * Q38_PAGE_TOKENS);
     const long need = (end + Q38_PAGE_TOKENS - 1) / Q38_PAGE_TOKENS - kv->seq_pages[seq];
     if (d_k == nullptr && need > 0) return fail("positions %d..%ld are not reserved", base_pos, end - 1);
-    if (d_k != nullptr && kv->check_store(seq, base_pos)) return -1;
+    if (d_k != nullptr ? kv->check_store(seq, base_pos) : kv->check_read(seq, base_pos)) return -1;
     if (need > (long)kv->free_pages.size())
         return fail("KV pool exhausted: need %ld pages, %zu free", need, kv->free_pages.size());
     q38_ctx *ctx = kv->ctx;

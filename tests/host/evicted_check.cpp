@@ -172,9 +172,38 @@ static void handed_on(int type) {
     REQUIRE(q38_seq_free(c.kv, a) == 0 && c.seq(10) == a && c.gone(a) == 0);
 }
 
+/* Positions below what the last eviction kept: nothing is attended to by place there. */
+static void reads_in_no_order(int type) {
+    Cache c(type);
+    REQUIRE(q38_kv_track_weights(c.kv, 1) == 0);
+    const int a = c.seq(100), b = c.seq(100);
+    c.evict(a, 100, 40);
+    const int32_t both[2] = {b, a}, at[2] = {5, 38}, last[2] = {5, 39};
+    c.refused([&] { return q38_attn_decode(c.kv, 3, 2, both, at, d, nullptr, nullptr, nullptr, d); }, "before 40 have been in no order");
+    c.refused([&] { return q38_attn_prefill(c.kv, 3, a, 38, 1, d, nullptr, nullptr, nullptr, d); }, "before 40 have been in no order");
+    c.refused([&] { return q38_attn_prefill(c.kv, 3, a, 0, 45, d, nullptr, nullptr, nullptr, d); }, "in no order");
+    /* all that were kept are an order's end */
+    REQUIRE(q38_attn_decode(c.kv, 3, 2, both, last, d, nullptr, nullptr, nullptr, d) == 0);
+    REQUIRE(q38_attn_prefill(c.kv, 3, a, 39, 5, d, nullptr, nullptr, nullptr, d) == 0);
+    q38_decode_call call = {};
+    call.layer = 3;
+    call.d_q = d;
+    call.d_out = d;
+    q38_decode_graph *g = nullptr;
+    c.refused([&] { return q38_decode_graph_create(c.kv, 2, both, at, 1, &call, &g); }, "in no order");
+    REQUIRE(q38_decode_graph_create(c.kv, 2, both, last, 1, &call, &g) == 0);
+    c.refused([&] { return q38_decode_graph_set_positions(g, at); }, "in no order");
+    REQUIRE(q38_decode_graph_launch(g) == 0 && g_replays > 0);
+    REQUIRE(q38_decode_graph_destroy(g) == 0);
+    /* a cache that tracks nothing has an order everywhere */
+    REQUIRE(q38_seq_reset(c.kv, a) == 0 && q38_seq_reserve(c.kv, a, 100) == 0);
+    REQUIRE(q38_attn_decode(c.kv, 3, 2, both, at, d, nullptr, nullptr, nullptr, d) == 0);
+}
+
 int main() {
     for (int type : {1, 4}) {
         handed_on(type);
+        reads_in_no_order(type);
     }
     printf("evicted ok\n");
     return 0;
