@@ -225,8 +225,8 @@ int q38_seq_set_evicted(q38_kv *kv, int seq, int n_tokens, int n_keep);
 /* Sums and own positions of a ragged batch of reserved positions, packed in
  * order in rows [rows][4 kv heads] as q38_kv_gather's, to hand a sequence on
  * with them (and q38_seq_set_evicted) or to look at them.  put: d_weights NULL sets zeros, d_tokens NULL
- * what a row stored there has, position + evicted tokens; a sequence once a
- * call.  get: either may be NULL, not both. */
+ * what a row stored there has, position + evicted tokens (fails with -1 below the last eviction's
+ * n_keep, where that is not the token's own); a sequence once a call.  get: either may be NULL, not both. */
 int q38_kv_weights_put(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,
                        const int32_t *n_tokens, const float *d_weights, const int32_t *d_tokens);
 int q38_kv_weights_get(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, const int32_t *pos0,

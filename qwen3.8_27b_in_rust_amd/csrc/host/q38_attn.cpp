@@ -1392,6 +1392,8 @@ int q38_kv_weights_put(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids,
     for (int b = 0; b < n_seq; ++b) {
         if (seen[seq_ids[b]]) return fail("sequence %d appears twice", seq_ids[b]);
         seen[seq_ids[b]] = 1;
+        /* a place tells a token's own position only past the last eviction's */
+        if (d_tokens == nullptr && n_tokens[b] > 0 && kv->check_store(seq_ids[b], pos0[b])) return -1;
     }
     return launch_weights(kv, slot, true, n_seq, seq_ids, pos0, n_tokens, const_cast<float *>(d_weights),
                           const_cast<int32_t *>(d_tokens));

@@ -200,8 +200,27 @@ static void reads_in_no_order(int type) {
     REQUIRE(q38_attn_decode(c.kv, 3, 2, both, at, d, nullptr, nullptr, nullptr, d) == 0);
 }
 
+/* Sums put back without own positions: those of positions in no order are nothing that a place tells. */
+static void sums_in_no_order(int type) {
+    Cache c(type);
+    REQUIRE(q38_kv_track_weights(c.kv, 1) == 0);
+    const int a = c.seq(100), b = c.seq(100);
+    c.evict(a, 100, 40);
+    REQUIRE(q38_seq_reserve(c.kv, a, 60) == 0);
+    const int32_t both[2] = {b, a}, at[2] = {0, 39}, next[2] = {0, 40}, n[2] = {30, 3}, one[2] = {30, 0};
+    int32_t *own = reinterpret_cast<int32_t *>(d);
+    for (const float *sums : {(const float *)nullptr, (const float *)d})
+        c.refused([&] { return q38_kv_weights_put(c.kv, 3, 2, both, at, n, sums, nullptr); }, "before 40 have been in no order");
+    /* with them, past them, and none of them */
+    REQUIRE(q38_kv_weights_put(c.kv, 3, 2, both, at, n, nullptr, own) == 0);
+    REQUIRE(q38_kv_weights_put(c.kv, 3, 2, both, at, n, d, own) == 0);
+    REQUIRE(q38_kv_weights_put(c.kv, 3, 2, both, next, n, d, nullptr) == 0);
+    REQUIRE(q38_kv_weights_put(c.kv, 3, 2, both, at, one, d, nullptr) == 0);
+}
+
 int main() {
     for (int type : {1, 4}) {
+        sums_in_no_order(type);
         handed_on(type);
         reads_in_no_order(type);
     }
