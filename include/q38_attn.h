@@ -211,7 +211,8 @@ int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
  * starts at 0 (in a decode call that appends it, at the weight it gives itself).
  * A score that is not finite spoils its kv head's sums.  Such a call needs 24 f32 scores a
  * token in its workspace.  A graph is recorded with tracking on or off, and its
- * positions are set anew after an eviction.  The sums' memory is kept, tracking or
+ * positions are set anew after an eviction, or once their pages were given back (a launch
+ * fails with -1 until then).  The sums' memory is kept, tracking or
  * not, until the cache is destroyed.  A change of tracking cannot be captured. */
 int q38_kv_track_weights(q38_kv *kv, int enable);
 /* Tokens of the sequence that evictions have taken out so far. */

@@ -2086,6 +2086,22 @@ struct q38_decode_graph {
         return 0;
     }
 
+    /* Whether a replay over a tracking cache may still go to the positions last set: an eviction moves rows and gives
+     * pages back, and a new beginning may come to as many evicted tokens again. */
+    int check_positions() const {
+        bool appends = false;
+        for (const Call &k : calls) appends |= k.appends;
+        for (int b = 0; b < n_seq && !calls.empty(); ++b) {
+            const int s = seq_ids[b];
+            if (kv->check_seq(s)) return -1;
+            if (evicted[b] != kv->evicted_of(s)) return fail("sequence %d has evicted tokens since the graph's positions were set", s);
+            if (appends ? kv->check_store(s, positions[b]) : kv->check_read(s, positions[b])) return -1;
+            if (positions[b] >= kv->seq_pages[s] * Q38_PAGE_TOKENS)
+                return fail("sequence %d: position %d is not reserved any more", s, positions[b]);
+        }
+        return 0;
+    }
+
     void note_evicted() {
         for (int b = 0; b < n_seq; ++b) evicted[b] = kv->evicted_of(seq_ids[b]);
     }
@@ -2300,9 +2316,7 @@ int q38_decode_graph_launch(q38_decode_graph *g) {
     if (g == nullptr) return fail("graph is NULL");
     if (g->exec == nullptr) return fail("the graph is not instantiated (q38_decode_graph_end)");
     if (g->tracks != g->kv->tracks) return fail("the cache's tracking of weights has changed since the graph was begun");
-    for (int b = 0; b < g->n_seq; ++b)
-        if (g->evicted[b] != g->kv->evicted_of(g->seq_ids[b]))
-            return fail("sequence %d has evicted tokens since the graph's positions were set", g->seq_ids[b]);
+    if (g->tracks && g->check_positions()) return -1;
     Q38_HIP(hipGraphLaunch(g->exec, g->kv->ctx->stream));
     return 0;
 }

@@ -218,8 +218,61 @@ static void sums_in_no_order(int type) {
     REQUIRE(q38_kv_weights_put(c.kv, 3, 2, both, at, one, d, nullptr) == 0);
 }
 
+/* Graphs whose positions an eviction, or what came after it, has taken away. */
+static void graphs_of_positions_gone(int type) {
+    Cache c(type);
+    REQUIRE(q38_kv_track_weights(c.kv, 1) == 0);
+    const int32_t a = c.seq(100);
+    q38_decode_call call = {};
+    call.layer = 3;
+    call.d_q = call.d_k_new = call.d_v_new = d;
+    call.d_out = d;
+    q38_decode_graph *g = nullptr;
+    auto launch = [&] { return q38_decode_graph_launch(g); };
+    /* an eviction of nothing gives back the page that the graph's next token is for */
+    int32_t at = 112;
+    REQUIRE(q38_decode_graph_create(c.kv, 1, &a, &at, 1, &call, &g) == 0 && launch() == 0);
+    c.evict(a, 112, 112);
+    REQUIRE(c.gone(a) == 0);
+    c.refused(launch, "position 112 is not reserved any more");
+    REQUIRE(q38_decode_graph_set_positions(g, &at) == 0 && launch() == 0);
+    /* as many evicted as before, of which more were kept */
+    at = 40;
+    c.evict(a, 100, 40);
+    c.refused(launch, "evicted tokens since");
+    REQUIRE(q38_decode_graph_set_positions(g, &at) == 0 && launch() == 0);
+    REQUIRE(q38_seq_reset(c.kv, a) == 0 && q38_seq_reserve(c.kv, a, 120) == 0);
+    c.refused(launch, "evicted tokens since");
+    c.evict(a, 120, 60);
+    REQUIRE(c.gone(a) == 60);
+    c.refused(launch, "before 60 have been in no order");
+    at = 60;
+    REQUIRE(q38_decode_graph_set_positions(g, &at) == 0 && launch() == 0);
+    /* a sequence that is no more, and another in its place */
+    REQUIRE(q38_seq_free(c.kv, a) == 0);
+    c.refused(launch, "does not exist");
+    REQUIRE(c.seq(16) == a);
+    c.refused(launch, "evicted tokens since");
+    REQUIRE(q38_decode_graph_destroy(g) == 0);
+    /* calls without a new row */
+    call.d_k_new = call.d_v_new = nullptr;
+    REQUIRE(q38_seq_reserve(c.kv, a, 100) == 0);
+    at = 30;
+    REQUIRE(q38_decode_graph_create(c.kv, 1, &a, &at, 1, &call, &g) == 0 && launch() == 0);
+    REQUIRE(q38_seq_truncate(c.kv, a, 16) == 0);
+    c.refused(launch, "position 30 is not reserved any more");
+    REQUIRE(q38_decode_graph_destroy(g) == 0);
+    /* a graph without decode calls has no positions */
+    q38_linear_weights w = {d, d, d, d};
+    REQUIRE(q38_seq_reserve(c.kv, a, 100) == 0 && q38_decode_graph_begin(c.kv, 1, &a, &at, &g) == 0);
+    REQUIRE(q38_decode_graph_add_linear_core(g, 1, &w, d, d, d, d, d, d, d) == 0 && q38_decode_graph_end(g) == 0);
+    c.evict(a, 100, 10);
+    REQUIRE(launch() == 0 && q38_decode_graph_destroy(g) == 0);
+}
+
 int main() {
     for (int type : {1, 4}) {
+        graphs_of_positions_gone(type);
         sums_in_no_order(type);
         handed_on(type);
         reads_in_no_order(type);
