@@ -11,7 +11,6 @@ __graft_entry__.py), or call the library through any FFI directly.
 """
 from __future__ import annotations
 
-import array
 import ctypes
 import os
 import struct
@@ -180,16 +179,12 @@ _PACK = [struct.Struct("%di" % n).pack for n in range(65)]
 
 def _i32(seq) -> bytes:
     """Host integers as the int32 array that a call reads (and does not keep)."""
+    n = len(seq)
     try:
-        return _PACK[len(seq)](*seq)
-    except IndexError:  # more of them
-        try:
-            return array.array("i", seq).tobytes()
-        except (TypeError, OverflowError):
-            pass
+        return _PACK[n](*seq) if n < len(_PACK) else struct.pack("%di" % n, *seq)
     except struct.error:
         pass
-    return bytes((c_int32 * len(seq))(*map(int, seq)))  # values that convert to int
+    return bytes((c_int32 * n)(*map(int, seq)))  # values that convert to int
 
 
 class DeviceArray:
