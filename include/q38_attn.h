@@ -194,7 +194,8 @@ int q38_kv_gather(q38_kv *kv, int layer, int n_seq, const int32_t *seq_ids, cons
  * q38_full_core, q38_full_core_noalloc and the graphs turn q and k at p + e by
  * themselves; q38_attn_pre takes p + e as its pos0, before q38_attn_decode,
  * q38_kv_write and q38_attn_prefill, which take cache positions as ever;
- * q38_kv_append refuses a sequence that has evicted tokens.  Rows that stay keep
+ * q38_kv_append refuses a sequence that has evicted tokens.  A position is turned by as
+ * the nearest f32 number (from 2^24 on not each has its own).  Rows that stay keep
  * the turn that they were stored with.  Positions below the last eviction's n_keep are
  * in no order: rows are stored from n_keep on, decode calls without a new row and
  * prefills without rows go on from n_keep - 1 at least, past all that were kept

@@ -299,38 +299,38 @@ typedef float Stats[Q38_OBSERVE_COLS][2];
 
 /* at_group: the group's place in part_ml; u0: its first query. */
 Q38_DEV void join_stats(Stats &stat, const q38_observe_args &a, int at_group, int u0, int j, int tid) {
-            /* the splits' maxima and sums joined, four threads a column (a wave a column
-             * took 2 us longer a group) */
-            const int col = tid >> 2;
-            if (col < Q38_OBSERVE_COLS) {
-                constexpr int kEach = 64 / 4;
-                const float *ml = a.part_ml + (((size_t)at_group * Q38_ATTN_KV_HEADS + j) * Q38_OBSERVE_COLS + col) * a.n_splits * 2;
-                float m[kEach], l[kEach], top = -INFINITY, sum = 0.0f;
-    #pragma unroll
-                for (int n = 0; n < kEach; ++n) {
-                    const int at = 4 * n + (tid & 3);
-                    m[n] = -INFINITY;
-                    l[n] = 0.0f;
-                    if (at < a.n_splits) {
-                        m[n] = ml[2 * at];
-                        l[n] = ml[2 * at + 1];
-                    }
-                }
-    #pragma unroll
-                for (int n = 0; n < kEach; ++n) top = fmaxf(top, m[n]);
-                top = fmaxf(top, q38_dpp<0xB1>(top));
-                top = fmaxf(top, q38_dpp<0x4E>(top));
-                /* a split that the column sees nothing of has a maximum of -inf */
-    #pragma unroll
-                for (int n = 0; n < kEach; ++n) sum += m[n] != -INFINITY ? l[n] * q38_exp2(m[n] - top) : 0.0f;
-                sum += q38_dpp<0xB1>(sum);
-                sum += q38_dpp<0x4E>(sum);
-                const bool in = u0 + col / kGroup < a.n_tokens;
-                if ((tid & 3) == 0) {
-                    stat[col][0] = in ? top : 0.0f;
-                    stat[col][1] = in ? 1.0f / sum : 0.0f;
-                }
+    /* the splits' maxima and sums joined, four threads a column (a wave a column
+     * took 2 us longer a group) */
+    const int col = tid >> 2;
+    if (col < Q38_OBSERVE_COLS) {
+        constexpr int kEach = 64 / 4;
+        const float *ml = a.part_ml + (((size_t)at_group * Q38_ATTN_KV_HEADS + j) * Q38_OBSERVE_COLS + col) * a.n_splits * 2;
+        float m[kEach], l[kEach], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int at = 4 * n + (tid & 3);
+            m[n] = -INFINITY;
+            l[n] = 0.0f;
+            if (at < a.n_splits) {
+                m[n] = ml[2 * at];
+                l[n] = ml[2 * at + 1];
             }
+        }
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) top = fmaxf(top, m[n]);
+        top = fmaxf(top, q38_dpp<0xB1>(top));
+        top = fmaxf(top, q38_dpp<0x4E>(top));
+        /* a split that the column sees nothing of has a maximum of -inf */
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) sum += m[n] != -INFINITY ? l[n] * q38_exp2(m[n] - top) : 0.0f;
+        sum += q38_dpp<0xB1>(sum);
+        sum += q38_dpp<0x4E>(sum);
+        const bool in = u0 + col / kGroup < a.n_tokens;
+        if ((tid & 3) == 0) {
+            stat[col][0] = in ? top : 0.0f;
+            stat[col][1] = in ? 1.0f / sum : 0.0f;
+        }
+    }
 }
 
 template <int T, int kPages, int kParts>

@@ -10,7 +10,7 @@
  * reads and writes would lie in one another's way.
  *
  * Measured: a layer of 32K tokens to 8K, bf16: lists 22.3 us (four workgroups, one a kv head;
- * 16 layers' are 64 beside each other, in the same time), 24.6K rows moved in
+ * 16 layers' are 64 beside each other, in 24), 24.6K rows moved in
  * 24-30, for 81 MB read and 35 written past L2, 3.9-4.8 TB/s.  (The rows have 25 MB: their bytes
  * lie in nine of ten lines of the pages they come from.)  Eight sequences of 250 to
  * 4003 tokens of Q8_K to 60% of them 11.5 and 13.4.

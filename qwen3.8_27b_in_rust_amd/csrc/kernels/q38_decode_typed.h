@@ -73,8 +73,8 @@ Q38_DEV q38_u32x2 ld_block8(__amdgpu_buffer_rsrc_t r, int at) {
 
 /* A page's scores, lane (c, g)'s four tokens of column c: columns past the six heads lie
  * past the range, where nothing is stored (a branch instead of it would leave the count of outstanding accesses
- * open, and every wait for the page's values would wait for this store as well: 128K tokens of MXFP4 42.4 us
- * against 39).  MXFP4's are written through L2 (32K tokens 15.3 us against 16.4, and 128K 38.5 against 38.9);
+ * open, and every wait for the page's values would wait for this store as well: 128K tokens of MXFP4, one layer again and
+ * again, 42.4 us against 38.9).  MXFP4's are written through L2 (32K tokens 15.3 us against 16.4, and 128K 38.5 against 38.9);
  * other rows' stay there for a while (bf16 27.3 against 28.0 and 100 in both, Q8_K 19.1 against 18.7 and 56.8
  * against 57.5). */
 template <int T>
@@ -880,19 +880,19 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
         } else {
             float m[kWaves], f[kWaves];
             f32x4 o[kWaves];
-    #pragma unroll
+#pragma unroll
             for (int w = 0; w < kWaves; ++w) {
                 m[w] = w < n_pages ? red_m[wave][w] : -INFINITY;
                 o[w] = q38_ld4(&red_o[w][wave][4 * lane]);
                 M = fmaxf(M, m[w]);
             }
-    #pragma unroll
+#pragma unroll
             for (int w = 0; w < kWaves; ++w) {
                 f[w] = q38_exp2(m[w] - M);
                 /* a wave without pages has left nothing there */
                 L += w < n_pages ? red_l[wave][w] * f[w] : 0.0f;
                 const float fu = f[w] * red_unit[wave][w];
-    #pragma unroll
+#pragma unroll
                 for (int e = 0; e < 4; ++e) O[e] = w < n_pages ? __builtin_fmaf(fu, o[w][e], O[e]) : O[e];
             }
         }
@@ -900,7 +900,7 @@ Q38_DEV void decode_typed(const Args &a, const Sums &sums = Sums()) {
             f32x4 r = O / L;
             if (a.gate != nullptr) {
                 const f32x4 gate = q38_ld4(a.gate + ((size_t)b * Q38_ATTN_HEADS + h) * a.gate_head_stride + 4 * lane);
-    #pragma unroll
+#pragma unroll
                 for (int e = 0; e < 4; ++e) r[e] *= q38_sigmoid(gate[e]);
             }
             q38_st4(a.out + (size_t)b * Q38_ATTN_Q_DIM + at, r);
