@@ -77,6 +77,20 @@ namespace {
                                           __FILE__, __LINE__);                          \
     } while (0)
 
+/* Memory of a context's device, whichever one is current: another context's, or the caller's own choice, which stays. */
+template <typename T>
+hipError_t malloc_on(int device, T **p, size_t bytes) {
+    int now = device;
+    const bool other = hipGetDevice(&now) == hipSuccess && now != device;
+    if (other) {
+        const hipError_t e = hipSetDevice(device);
+        if (e != hipSuccess) return e;
+    }
+    const hipError_t e = hipMalloc(p, bytes);
+    if (other) (void)hipSetDevice(now);
+    return e;
+}
+
 std::string library_dir() {
     Dl_info info;
     if (dladdr(reinterpret_cast<void *>(&library_dir), &info) == 0 || info.dli_fname == nullptr)
@@ -270,7 +284,7 @@ struct q38_ctx {
         }
         const int want = std::max(n_seq, 64);
         const size_t bytes = (size_t)want * Q38_GDN_ARRIVALS * sizeof(int32_t);
-        Q38_HIP(hipMalloc(&arrivals, bytes));
+        Q38_HIP(malloc_on(device, &arrivals, bytes));
         Q38_HIP(hipMemsetAsync(arrivals, 0, bytes, stream));
         arrival_seqs = want;
         return 0;
@@ -286,7 +300,7 @@ struct q38_ctx {
             work_bytes = 0;
         }
         size_t want = std::max(bytes, (size_t)1 << 20);
-        Q38_HIP(hipMalloc(&work, want));
+        Q38_HIP(malloc_on(device, &work, want));
         work_bytes = want;
         return 0;
     }
@@ -706,7 +720,7 @@ int q38_device_info(q38_ctx *ctx, int *cu_count, int *clock_khz, int *lds_bytes,
 int q38_alloc(q38_ctx *ctx, size_t bytes, void **d_ptr) {
     if (ctx == nullptr || d_ptr == nullptr) return fail("NULL argument");
     *d_ptr = nullptr;
-    Q38_HIP(hipMalloc(d_ptr, bytes ? bytes : 4));
+    Q38_HIP(malloc_on(ctx->device, d_ptr, bytes ? bytes : 4));
     return 0;
 }
 
@@ -1344,7 +1358,7 @@ int q38_kv_track_weights(q38_kv *kv, int enable) {
     }
     if (kv->type == 0) return fail("a cache of F32 rows tracks no weights: F16, BF16, Q8_K or MXFP4 rows do");
     const size_t bytes = kv->slot_sums() * kv->n_slots * sizeof(float);
-    if (kv->weights == nullptr && hipMalloc(&kv->weights, bytes) != hipSuccess) {
+    if (kv->weights == nullptr && malloc_on(kv->ctx->device, &kv->weights, bytes) != hipSuccess) {
         (void)hipGetLastError();
         kv->weights = nullptr;
         return fail("cannot allocate %zu bytes for the sums of weights", bytes);
@@ -2055,7 +2069,7 @@ struct q38_decode_graph {
                 work_bytes = 0;
             }
             const size_t want = std::max(need, (size_t)1 << 20);
-            Q38_HIP(hipMalloc(&work, want));
+            Q38_HIP(malloc_on(kv->ctx->device, &work, want));
             work_bytes = want;
         }
         return 0;
@@ -2525,7 +2539,7 @@ int q38_attn_prefill(q38_kv *kv, int layer, int seq, int base_pos, int n_tokens,
         const int cap = (int)std::min<long>(max_blocks, std::max<long>(a.n_kblocks, 2L * im->cap));
         const size_t block_bytes = Q38_PREFILL_IMAGE_BYTES;
         void *buf = nullptr;
-        if (hipMalloc(&buf, (size_t)Q38_ATTN_KV_HEADS * cap * block_bytes) != hipSuccess) {
+        if (malloc_on(ctx->device, &buf, (size_t)Q38_ATTN_KV_HEADS * cap * block_bytes) != hipSuccess) {
             (void)hipGetLastError();
             im = nullptr;
         } else {

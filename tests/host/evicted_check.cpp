@@ -20,8 +20,19 @@ static hipError_t check_launch(hipFunction_t f, unsigned, unsigned, unsigned, un
     g_launches.push_back(f);
     return hipSuccess;
 }
+static int g_device = 0;
+static std::vector<int> g_malloc_devices; /* that were current at each allocation */
+static hipError_t check_get_device(int *device) {
+    *device = g_device;
+    return hipSuccess;
+}
+static hipError_t check_set_device(int device) {
+    g_device = device;
+    return hipSuccess;
+}
 template <typename T>
 static hipError_t check_malloc(T **p, size_t bytes) {
+    g_malloc_devices.push_back(g_device);
     *p = reinterpret_cast<T *>(g_next);
     g_next += (bytes + 0xFFFFFFF) & ~(size_t)0xFFFFFFF;
     return hipSuccess;
@@ -55,6 +66,8 @@ static hipError_t check_graph_launch(hipGraphExec_t, hipStream_t) {
 static hipError_t check_graph_destroy(hipGraph_t) { return hipSuccess; }
 static hipError_t check_exec_destroy(hipGraphExec_t) { return hipSuccess; }
 #define hipMalloc check_malloc
+#define hipGetDevice check_get_device
+#define hipSetDevice check_set_device
 #define hipFree check_free
 #define hipMemsetAsync check_set
 #define hipStreamIsCapturing check_capturing
@@ -270,8 +283,39 @@ static void graphs_of_positions_gone(int type) {
     REQUIRE(launch() == 0 && q38_decode_graph_destroy(g) == 0);
 }
 
+/* A context of one device while another is current: what its calls allocate is its own. */
+static void two_devices(int type) {
+    Cache c(type);
+    c.ctx.device = 1;
+    auto own = [&](auto call) {
+        const size_t before = g_malloc_devices.size();
+        REQUIRE(call() == 0 && g_malloc_devices.size() > before && g_device == 0);
+        for (size_t i = before; i < g_malloc_devices.size(); ++i) REQUIRE(g_malloc_devices[i] == 1);
+    };
+    void *p = nullptr;
+    own([&] { return q38_alloc(&c.ctx, 100, &p); });
+    own([&] { return q38_kv_track_weights(c.kv, 1); });
+    const int32_t a = c.seq(500), at = 499, n = 500, keep = 250, none = 0;
+    auto fresh = [&] { c.ctx.work = nullptr, c.ctx.work_bytes = 0; };
+    own([&] { return q38_attn_decode(c.kv, 3, 1, &a, &at, d, nullptr, nullptr, nullptr, d); });
+    fresh();
+    own([&] { return q38_attn_observe(c.kv, 3, a, 480, 20, d); });
+    fresh();
+    own([&] { return q38_attn_prefill(c.kv, 3, a, 480, 20, d, nullptr, nullptr, nullptr, d); });
+    fresh();
+    own([&] { return q38_kv_evict(c.kv, 1, &a, &n, &keep, &none); });
+    q38_decode_call call = {};
+    call.layer = 3;
+    call.d_q = call.d_k_new = call.d_v_new = d;
+    call.d_out = d;
+    q38_decode_graph *g = nullptr;
+    own([&] { return q38_decode_graph_create(c.kv, 1, &a, &keep, 1, &call, &g); });
+    REQUIRE(q38_decode_graph_destroy(g) == 0);
+}
+
 int main() {
     for (int type : {1, 4}) {
+        two_devices(type);
         graphs_of_positions_gone(type);
         sums_in_no_order(type);
         handed_on(type);
